@@ -1,0 +1,1131 @@
+// Attention of drafted tokens over the paged cache: every sequence brings a tree of tokens, each of which sees the cached
+// keys in front of the tree and its own ancestors in it.
+//
+// For query head h of drafted token i of a sequence with `base` cached keys: score_t = (q_h . K_t[kv(h)]) * scale over the
+// cached keys t < base (with a window W: t > pos_i - W) and the drafted keys t = base + j with bit j of mask_i set;
+// p = softmax, o_h = sum_t p_t V_t[kv(h)]; a row that sees no key gives zeros.  The drafted tokens' own keys and values lie
+// in the cache already, row j at position base + j, in the order of the batch.
+//
+// A row of work is (token, head of the group); the rows of a sequence and a kv head share its keys, so the time to beat
+// is one pass over the live pages.  As in attention_stream.cu the pages of all (sequence, kv head, tile of rows) form one
+// list of units, CTA c takes the stretch [c T / G, (c + 1) T / G), and what several CTAs saw pieces of is added up by
+// attention_tree_merge_kernel, in CTA order.  Everything the cut depends on is read from the device, so a captured launch
+// serves whatever lengths the description holds at its replay.
+//
+// Two kernels.  attention_tree_tc_kernel: bfloat16, heads of 64 or 128, on tcgen05 (below).  attention_tree_simple_kernel:
+// any head size up to 256, float32 or bfloat16, on the CUDA cores in float32 throughout.
+//
+// The tcgen05 kernel.  A CTA has two halves, each with a warp that issues MMAs, eight softmax warps (two threads per row),
+// two buffers of scores and an accumulator in tensor memory: S = Q K^T (128 rows x 64 keys), P to shared memory, O += P V.
+//   ROWS2 = false (at most 128 rows per sequence and kv head): both halves hold the same rows and take every other page,
+//     so that one page's softmax runs under the other's loads and MMAs; their sums are joined at the end of a run;
+//   ROWS2 = true: the halves hold 128 rows each and share every page, which then is fetched once for 256 rows.
+// One thread of warp 0 feeds rings of K and V pages by TMA, and the queries of the run that comes next.
+//
+// The products with masked keys: P is zero there, but zero times an infinity or a NaN is not, and a page that is masked for
+// some row may hold either (rows behind the sequence's end, a drafted branch that overflowed).  So the V page of a masked
+// tile is looked through; rows of V that are not finite are zeroed in shared memory, and what they give to the rows that do
+// see them is added by hand.
+//
+// Every mbarrier wait is bounded: on expiry a code goes to the status word; the softmax warps then walk through the rest of
+// their barriers without work, so that all leave together.
+#include <math.h>
+
+#include "tc_common.cuh"
+
+#define TR_KEYS 64
+#define TR_MAX_SEQS 4096
+#define TR_SOFTMAX_WARPS 8
+#define TR_THREADS (32 + 2 * 32 + 2 * TR_SOFTMAX_WARPS * 32)
+
+struct TreeParams {
+  const int* token_pos;                    // [tokens]
+  const unsigned long long* mask; int words;   // [tokens][words]
+  const int* seq_start; const int* seq_len;    // [seqs + 1], [seqs]
+  const int* block_table; int bt_stride, bt_width;
+  const void* q; int ldq;
+  const void* k_cache; const void* v_cache;
+  void* out; int ldo;
+  float* part_o;                           // [G][2][rows per tile][head_dim]: pieces, unnormalised
+  float2* part_ml;                         // [G][2][rows per tile]: their (maximum, sum)
+  struct TreeCut* cut;                     // [G]: what each CTA's stretch begins in
+  int* status;
+  int n_tokens, n_seqs, n_q, n_kv, gs, head_dim, window, n_pages, rows_per_tile;
+  float scale;
+};
+
+// What CTA c's stretch begins in, for the merge.
+struct TreeCut {
+  long long item_begin, total;             // the item's first unit; units in all
+  int b, kvh, rt, n_pages;
+};
+
+struct TreeSeq {                           // a sequence's share of the list
+  int row0, n_new, base, len, first, n_pages, n_tiles;
+};
+__device__ __forceinline__ TreeSeq tree_seq(const TreeParams& P, int b) {
+  TreeSeq s;
+  s.row0 = min(max(P.seq_start[b], 0), P.n_tokens);
+  s.n_new = min(max(P.seq_start[b + 1], s.row0), P.n_tokens) - s.row0;
+  s.len = max(P.seq_len[b], 0);
+  s.base = max(s.len - s.n_new, 0);
+  const int pages = max(min((int)(((long long)s.len + TR_KEYS - 1) / TR_KEYS), P.bt_width), 1);
+  const int lo = (P.window > 0 && s.base - P.window + 1 > 0) ? s.base - P.window + 1 : 0;
+  s.first = min(lo / TR_KEYS, pages - 1);
+  s.n_pages = pages - s.first;
+  s.n_tiles = (int)(((long long)s.n_new * P.gs + P.rows_per_tile - 1) / P.rows_per_tile);
+  return s;
+}
+__device__ __forceinline__ long long tree_begin(int c, int G, long long T) { return (long long)c * T / G; }
+
+// A stretch of pages of one (sequence, kv head, tile of rows).
+struct TreeRun {
+  TreeSeq s;
+  int b, kvh, rt, page0, n;
+  bool from_start, to_end, holds_u0;
+};
+
+struct TreeCursor {
+  long long u, u0, u1;
+  int b, item, off;
+  TreeSeq s;
+  __device__ __forceinline__ void begin(const TreeParams& P, long long u0_, long long u1_, int b_, int item_, int off_) {
+    u = u0 = u0_; u1 = u1_; b = b_; item = item_; off = off_;
+    if (u < u1) s = tree_seq(P, b);
+  }
+  __device__ __forceinline__ bool next(const TreeParams& P, TreeRun& r) {
+    if (u >= u1) return false;
+    r.s = s; r.b = b;
+    r.kvh = item / s.n_tiles; r.rt = item % s.n_tiles;
+    r.page0 = s.first + off;
+    r.n = (int)min((long long)(s.n_pages - off), u1 - u);
+    r.from_start = off == 0;
+    r.to_end = off + r.n == s.n_pages;
+    r.holds_u0 = u == u0;
+    u += r.n; off += r.n;
+    if (off == s.n_pages) {
+      off = 0;
+      if (++item == s.n_tiles * P.n_kv) {
+        item = 0;
+        do { b++; if (b < P.n_seqs) s = tree_seq(P, b); } while (b < P.n_seqs && s.n_tiles == 0);
+      }
+    }
+    return true;
+  }
+};
+
+// Where CTA c begins; every thread of the block calls it.  `sums` holds a running sum per sequence for the while.
+struct TreeStart { long long u0, u1; int b, item, off; };
+__device__ __forceinline__ TreeStart tree_start(const TreeParams& P, long long* sums) {
+  const int n_threads = blockDim.x, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  for (int b = threadIdx.x; b < P.n_seqs; b += n_threads) {
+    const TreeSeq s = tree_seq(P, b);
+    sums[b + 1] = (long long)s.n_pages * s.n_tiles * P.n_kv;
+  }
+  if (threadIdx.x == 0) sums[0] = 0;
+  __syncthreads();
+  if (warp == 0) {
+    long long carry = 0;
+    for (int base = 0; base < P.n_seqs; base += 32) {
+      const int i = base + lane;
+      long long v = i < P.n_seqs ? sums[i + 1] : 0;
+#pragma unroll
+      for (int d = 1; d < 32; d <<= 1) {
+        const long long n = __shfl_up_sync(0xffffffffu, v, d);
+        if (lane >= d) v += n;
+      }
+      if (i < P.n_seqs) sums[i + 1] = v + carry;
+      carry += __shfl_sync(0xffffffffu, v, 31);
+    }
+  }
+  __syncthreads();
+  TreeStart t;
+  const long long T = sums[P.n_seqs];
+  const int c = blockIdx.x, G = gridDim.x;
+  t.u0 = tree_begin(c, G, T); t.u1 = tree_begin(c + 1, G, T);
+  t.b = t.item = t.off = 0;
+  if (t.u0 < t.u1) {
+    int lo = 0, hi = P.n_seqs - 1;                // the last sequence that begins at or before u0 and is not empty
+    while (lo < hi) {
+      const int mid = (lo + hi + 1) >> 1;
+      if (sums[mid] <= t.u0) lo = mid; else hi = mid - 1;
+    }
+    const TreeSeq s = tree_seq(P, lo);
+    const long long r = t.u0 - sums[lo];
+    t.b = lo; t.item = (int)(r / s.n_pages); t.off = (int)(r % s.n_pages);
+    if (threadIdx.x == 0) {
+      TreeCut cut;
+      cut.item_begin = t.u0 - t.off; cut.total = T;
+      cut.b = lo; cut.kvh = t.item / s.n_tiles; cut.rt = t.item % s.n_tiles; cut.n_pages = s.n_pages;
+      P.cut[c] = cut;
+    }
+  } else if (threadIdx.x == 0) {
+    P.cut[c].total = T; P.cut[c].n_pages = 0;
+  }
+  return t;
+}
+
+// Which of the 64 keys from position `key0` on a drafted token sees.
+__device__ __forceinline__ unsigned long long tree_visible(const TreeParams& P, const TreeSeq& s, int token, int lo, int key0,
+                                                           bool page_ok) {
+  if (!page_ok) return 0;
+  const unsigned long long all = ~0ull;
+  unsigned long long cached = 0;
+  const int to_base = s.base - key0;               // cached keys from here on
+  if (to_base >= 64) cached = all;
+  else if (to_base > 0) cached = (1ull << to_base) - 1;
+  const int to_lo = lo - key0;
+  if (to_lo >= 64) cached = 0;
+  else if (to_lo > 0) cached &= all << to_lo;
+  unsigned long long nodes = 0;
+  if (to_base < 64) {                              // drafted keys in this page: node 0 lies at bit to_base
+    const unsigned long long* m = P.mask + (size_t)token * P.words;
+    const int n = min(s.n_new, 64 * P.words);
+    auto word = [&](int w) -> unsigned long long {
+      if (64 * w >= n) return 0;
+      const unsigned long long v = __ldcg(m + w);
+      return n - 64 * w >= 64 ? v : v & ((1ull << (n - 64 * w)) - 1);
+    };
+    if (to_base > 0) nodes = word(0) << to_base;
+    else {
+      const int o = -to_base, w = o >> 6, sh = o & 63;
+      nodes = word(w) >> sh;
+      if (sh) nodes |= word(w + 1) << (64 - sh);
+    }
+  }
+  unsigned long long v = cached | nodes;
+  const int left = s.len - key0;                   // nothing behind the sequence's end
+  if (left < 64) v &= left > 0 ? (1ull << left) - 1 : 0;
+  return v;
+}
+
+// ================================================================ tcgen05
+template <int HD, bool ROWS2>
+struct TreeSmem {
+  static constexpr int STAGES = HD == 64 ? 8 : 4;       // (even: with alternating halves a stage is always the same half's)
+  static constexpr int QB = ROWS2 ? 1 : 2;              // queries of the next run beside those of this one
+  alignas(1024) bf16 q[2][128 * HD];                    // ROWS2: per half; else: of two runs
+  alignas(1024) bf16 k[STAGES][TR_KEYS * HD];           // [HD/64][64 keys][64 dims]
+  alignas(1024) bf16 v[STAGES][TR_KEYS * HD];
+  alignas(1024) bf16 p[2][128 * TR_KEYS];               // per half; at the end of a run: the rows' sums and maxima
+  uint64_t q_full[QB], q_empty[QB], k_full[STAGES], v_full[STAGES];
+  uint64_t s_full[2][STAGES], pv_full[2][STAGES], p_full[2];
+  unsigned long long bad[2];
+  int row_of[32];                                       // cache row of a tile's page, from the K to the V request
+  uint32_t tmem_base;
+  int o_ready[2];
+  int abort_flag;
+};
+
+__device__ __forceinline__ float tr_max3(float a, float b, float c) {
+  float r;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
+}
+__device__ __forceinline__ float tr_exp2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+__device__ __forceinline__ void tr_bar(int id, int n) { asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(n) : "memory"); }
+__device__ __forceinline__ bool tr_bar_or(int id, int n, bool mine) {
+  uint32_t r;
+  asm volatile(
+      "{\n\t.reg .pred p, q;\n\t"
+      "setp.ne.u32 q, %3, 0;\n\t"
+      "barrier.cta.red.or.pred p, %1, %2, q;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(r) : "r"(id), "r"(n), "r"((uint32_t)mine) : "memory");
+  return r != 0;
+}
+__device__ __forceinline__ float tmem_ld1f(uint32_t taddr) {
+  uint32_t r;
+  asm volatile("tcgen05.ld.sync.aligned.32x32b.x1.b32 {%0}, [%1];" : "=r"(r) : "r"(taddr));
+  tmem_ld_wait();
+  return __uint_as_float(r);
+}
+
+#define TR_FAIL(code) { atomicCAS(P.status, 0, code); S.abort_flag = 1; }
+
+template <int HD, bool ROWS2>
+__global__ void __launch_bounds__(TR_THREADS, 1)
+attention_tree_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k,
+                         const __grid_constant__ CUtensorMap map_v, const TreeParams P) {
+  extern __shared__ __align__(1024) uint8_t smem_raw[];
+  using Smem = TreeSmem<HD, ROWS2>;
+  constexpr int STAGES = Smem::STAGES, QB = Smem::QB, DB = HD / 64;
+  constexpr uint32_t COL_PV = 128;
+  static_assert(sizeof(Smem) <= 227 * 1024, "shared memory of an SM");
+  Smem& S = *reinterpret_cast<Smem*>(smem_raw);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  if (smem_u32(smem_raw) & 1023) {                      // (the swizzled tiles need it)
+    if (threadIdx.x == 0) atomicCAS(P.status, 0, 510);
+    return;
+  }
+  volatile int* abort_flag = &S.abort_flag;
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < QB; i++) { mbar_init(&S.q_full[i], 1); mbar_init(&S.q_empty[i], 2); }
+    for (int s = 0; s < STAGES; s++) {
+      mbar_init(&S.k_full[s], 1); mbar_init(&S.v_full[s], 1);
+      for (int h = 0; h < 2; h++) { mbar_init(&S.s_full[h][s], 1); mbar_init(&S.pv_full[h][s], 1); }
+    }
+    for (int h = 0; h < 2; h++) { mbar_init(&S.p_full[h], TR_SOFTMAX_WARPS); S.bad[h] = 0; S.o_ready[h] = 0; }
+    S.abort_flag = 0;
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  if (warp == 1) {
+    tmem_alloc(&S.tmem_base, 512);
+    tmem_relinquish();
+  }
+  pdl_wait();                                           // everything below may read what the kernel before this one wrote
+  const TreeStart start = tree_start(P, reinterpret_cast<long long*>(S.k));
+  fence_async_shared();                                 // the sums lie where TMA will write
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem_base = S.tmem_base;
+  const int gs = P.gs;
+  const int half_tokens = 128 / gs;                     // tokens of a half's 128 rows
+  TreeCursor cur;
+  cur.begin(P, start.u0, start.u1, start.b, start.item, start.off);
+  TreeRun run;
+  auto half_ntok = [&](const TreeRun& r, int h) {       // tokens of the run's tile that half h holds
+    const int t0 = ROWS2 ? (2 * r.rt + h) * half_tokens : r.rt * half_tokens;
+    return min(max(r.s.n_new - t0, 0), half_tokens);
+  };
+
+  if (warp == 0) {
+    // ---------------------------------------------------------------- producer
+    if (lane == 0 && start.u0 < start.u1) {
+      asm volatile("prefetch.tensormap [%0];" ::"l"(&map_q) : "memory");
+      asm volatile("prefetch.tensormap [%0];" ::"l"(&map_k) : "memory");
+      asm volatile("prefetch.tensormap [%0];" ::"l"(&map_v) : "memory");
+      const uint32_t n_units = (uint32_t)(start.u1 - start.u0);
+      TreeCursor cq = cur;
+      TreeRun rq;
+      bool more_q = cq.next(P, rq);
+      bool have = cur.next(P, run);
+      int tile = 0, nq = 0;
+      uint32_t jk = 0, jv = 0;
+      const int* bt = P.block_table + (size_t)run.b * P.bt_stride;
+      int pg = __ldcg(bt + run.page0);
+      auto freed = [&](uint64_t (*bars)[STAGES], uint32_t j) -> bool {   // tile j - STAGES has been read
+        const uint32_t par = ((j / STAGES) - 1) & 1;
+        if (ROWS2) return mbar_test_wait(&bars[0][j % STAGES], par) && mbar_test_wait(&bars[1][j % STAGES], par);
+        return mbar_test_wait(&bars[j & 1][j % STAGES], par);
+      };
+      uint32_t idle = 0;
+      bool ok = true;
+      while ((more_q || jv < n_units) && ok) {
+        bool moved = false;
+        if (more_q && (nq < QB || mbar_test_wait(&S.q_empty[nq % QB], ((nq / QB) - 1) & 1))) {
+          uint64_t* bar = &S.q_full[nq % QB];
+          const uint32_t box = (uint32_t)half_tokens * gs * HD * sizeof(bf16);
+          const bool second = ROWS2 && half_ntok(rq, 1) > 0;
+          mbar_expect_tx(bar, second ? 2 * box : box);
+          const int tok0 = rq.s.row0 + rq.rt * half_tokens * (ROWS2 ? 2 : 1);
+          for (int db = 0; db < DB; db++) {
+            tma_load_3d(&map_q, S.q[ROWS2 ? 0 : nq % QB] + db * 128 * 64, bar, db * 64, rq.kvh * gs, tok0);
+            if (second) tma_load_3d(&map_q, S.q[1] + db * 128 * 64, bar, db * 64, rq.kvh * gs, tok0 + half_tokens);
+          }
+          nq++;
+          more_q = cq.next(P, rq);
+          moved = true;
+        }
+        if (have && (jk < STAGES || freed(S.s_full, jk))) {
+          const int s = jk % STAGES;
+          // (a page number outside the pool: some page's rows are fetched and nobody sees them)
+          const int row = (int)(((long long)((unsigned)pg < (unsigned)P.n_pages ? pg : 0) * P.n_kv + run.kvh) * TR_KEYS);
+          S.row_of[jk & 31] = row;
+          mbar_expect_tx(&S.k_full[s], TR_KEYS * HD * sizeof(bf16));
+          for (int db = 0; db < DB; db++) tma_load_2d(&map_k, S.k[s] + db * TR_KEYS * 64, &S.k_full[s], db * 64, row);
+          jk++;
+          if (++tile == run.n) {
+            tile = 0;
+            have = cur.next(P, run);
+            bt = P.block_table + (size_t)run.b * P.bt_stride;
+          }
+          if (have) pg = __ldcg(bt + run.page0 + tile);
+          moved = true;
+        }
+        if (jv < jk && (jv < STAGES || freed(S.pv_full, jv))) {
+          const int s = jv % STAGES, row = S.row_of[jv & 31];
+          mbar_expect_tx(&S.v_full[s], TR_KEYS * HD * sizeof(bf16));
+          for (int db = 0; db < DB; db++) tma_load_2d(&map_v, S.v[s] + db * TR_KEYS * 64, &S.v_full[s], db * 64, row);
+          jv++;
+          moved = true;
+        }
+        if (moved) { idle = 0; continue; }
+        __nanosleep(32);
+        if (++idle >= 4u * TC_SPIN_LIMIT || ((idle & 1023u) == 0 && *abort_flag)) { TR_FAIL(501); ok = false; }
+      }
+      pdl_trigger();
+      if (!ok) {
+        for (int i = 0; i < 2000; i++) __nanosleep(1000);   // let copies already issued land
+      }
+    }
+  } else if (warp <= 2) {
+    // ---------------------------------------------------------------- MMA issuer of half `warp - 1`
+    const int h = warp - 1;
+    const uint32_t idesc_s = instr_desc_bf16(TR_KEYS), idesc_pv = instr_desc_bf16(HD, true);
+    const uint32_t tmem_h = tmem_base + h * 256, p_addr = smem_u32(S.p[h]);
+    bool ok = true;
+    // This half's tiles as one sequence over the runs, the scores one tile ahead of the products with V: what is known of
+    // the tile whose P V is still to come
+    bool pend = false, pend_first = false, pend_active = false;
+    uint32_t pend_it = 0, pend_i = 0;
+    uint32_t it = 0, i = 0;                              // tiles of the stretch, of this half
+    auto values = [&]() {                                // P V of the pending tile
+      const int s = pend_it % STAGES;
+      if (!__all_sync(0xffffffffu, mbar_wait(&S.v_full[s], (pend_it / STAGES) & 1, abort_flag))) { if (lane == 0) TR_FAIL(506); ok = false; return; }
+      if (!__all_sync(0xffffffffu, mbar_wait(&S.p_full[h], pend_i & 1, abort_flag))) { if (lane == 0) TR_FAIL(505); ok = false; return; }
+      if (!pend_active) {                                // no rows of this half: the page is free
+        if (lane == 0) mbar_arrive(&S.pv_full[h][s]);
+        __syncwarp();
+        return;
+      }
+      tc_fence_after();
+      const uint32_t v_addr = smem_u32(S.v[s]);
+      const bool fresh = pend_first && *(volatile int*)&S.o_ready[h] == 0;
+      if (elect_one()) {
+#pragma unroll
+        for (int kk = 0; kk < 4; kk++)
+          umma_bf16(tmem_h + COL_PV, smem_desc_sw128(p_addr + kk * 32),
+                    smem_desc_sw128_mn(v_addr + kk * 16 * 128, TR_KEYS * 128), idesc_pv, (fresh && kk == 0) ? 0u : 1u);
+        umma_commit(&S.pv_full[h][s]);
+      }
+      __syncwarp();
+    };
+    for (int r = 0; ok && cur.next(P, run); r++) {
+      const bool active = !ROWS2 || half_ntok(run, h) > 0;
+      if (!__all_sync(0xffffffffu, mbar_wait(&S.q_full[r % QB], (r / QB) & 1, abort_flag))) { if (lane == 0) TR_FAIL(502); ok = false; break; }
+      const uint32_t q_addr = smem_u32(S.q[ROWS2 ? h : r % QB]);
+      bool first = true;
+      const uint32_t it_end = it + run.n;
+      for (; it < it_end && ok; it++) {
+        if (!ROWS2 && (int)(it & 1) != h) continue;
+        const int s = it % STAGES;
+        if (!__all_sync(0xffffffffu, mbar_wait(&S.k_full[s], (it / STAGES) & 1, abort_flag))) { if (lane == 0) TR_FAIL(503); ok = false; break; }
+        if (active) {
+          tc_fence_after();
+          const uint32_t k_addr = smem_u32(S.k[s]);
+          if (elect_one()) {
+#pragma unroll
+            for (int db = 0; db < DB; db++)
+#pragma unroll
+              for (int kk = 0; kk < 4; kk++)
+                umma_bf16(tmem_h + (i & 1) * TR_KEYS, smem_desc_sw128(q_addr + db * 128 * 128 + kk * 32),
+                          smem_desc_sw128(k_addr + db * TR_KEYS * 128 + kk * 32), idesc_s, (db | kk) ? 1u : 0u);
+            umma_commit(&S.s_full[h][s]);
+          }
+          __syncwarp();
+        } else {
+          if (lane == 0) mbar_arrive(&S.s_full[h][s]);
+          __syncwarp();
+        }
+        if (pend) values();
+        pend = true; pend_first = first; pend_active = active; pend_it = it; pend_i = i;
+        first = false;
+        i++;
+      }
+      it = it_end;
+      if (ok) {                                          // the run's scores are issued: its queries are free behind them
+        if (elect_one()) umma_commit(&S.q_empty[r % QB]);
+        __syncwarp();
+      }
+    }
+    if (ok && pend) values();
+  } else {
+    // ---------------------------------------------------------------- softmax (eight warps per half)
+    const int sw = warp - 3, h = sw / TR_SOFTMAX_WARPS;
+    const int quarter = warp & 3;                        // tensor-memory lanes this warp may read
+    const int half = (sw % TR_SOFTMAX_WARPS) >> 2;       // 0: keys 0..31 and the lower dims; 1: the others
+    const int row = quarter * 32 + lane;
+    const int tok = row / gs, head = row % gs;
+    const uint32_t lane_base = tmem_base + ((uint32_t)(quarter * 32) << 16);
+    const uint32_t lane_addr = lane_base + h * 256;
+    constexpr int OD = HD / 2;
+    const uint32_t o_addr = lane_addr + COL_PV + half * OD;
+    const float to_log2 = P.scale * 1.4426950408889634f;
+    const int tile_bar = ROWS2 ? 1 : 1 + h, tile_threads = ROWS2 ? 2 * TR_SOFTMAX_WARPS * 32 : TR_SOFTMAX_WARPS * 32;
+    const int tile_tid = ROWS2 ? threadIdx.x - 96 : threadIdx.x - 96 - h * TR_SOFTMAX_WARPS * 32;
+    unsigned long long* bad_word = &S.bad[ROWS2 ? 0 : h];
+    bool ok = true;
+    uint32_t it = 0, i = 0;
+    while (cur.next(P, run)) {
+      const TreeSeq& sq = run.s;
+      const int ntok = half_ntok(run, h);
+      const bool active = ntok > 0;
+      const bool valid = tok < ntok;
+      const bool warp_active = quarter * 32 < ntok * gs;
+      const int tok0 = sq.row0 + (ROWS2 ? 2 * run.rt + h : run.rt) * half_tokens;
+      const int token = tok0 + (valid ? tok : 0);
+      int lo = 0, lo_max = 0;
+      if (P.window > 0) {
+        lo = valid ? max(P.token_pos[token] - P.window + 1, 0) : 0;
+        // the furthest edge of the tile's rows (all rows of both halves: the halves decide alike)
+        const int t0 = sq.row0 + run.rt * half_tokens * (ROWS2 ? 2 : 1);
+        const int t1 = min(t0 + half_tokens * (ROWS2 ? 2 : 1), sq.row0 + sq.n_new);
+        for (int t = t0 + lane; t < t1; t += 32) lo_max = max(lo_max, P.token_pos[t] - P.window + 1);
+        lo_max = __reduce_max_sync(0xffffffffu, lo_max);
+      }
+      const int* bt = P.block_table + (size_t)run.b * P.bt_stride;
+      const uint32_t it_end = it + run.n;
+      const uint32_t it_first = it;
+      float m_ref = -INFINITY, l = 0.f;
+      uint32_t last = 0;
+      bool any_tile = false;
+      if (!ROWS2 && (int)(it & 1) != h) it++;
+      int pg_next = it < it_end ? __ldcg(bt + run.page0 + (int)(it - it_first)) : 0;
+      for (; it < it_end; it += ROWS2 ? 1 : 2) {
+        const int s = it % STAGES, b = i & 1;
+        const int page = run.page0 + (int)(it - it_first), key0 = page * TR_KEYS;
+        const int pg = pg_next;
+        if (it + (ROWS2 ? 1 : 2) < it_end) pg_next = __ldcg(bt + page + (ROWS2 ? 1 : 2));
+        const bool page_ok = (unsigned)pg < (unsigned)P.n_pages;
+        const bool needs_mask = key0 + TR_KEYS > sq.base || key0 < lo_max || !page_ok;
+        if (ok && !__all_sync(0xffffffffu, mbar_wait(&S.s_full[h][s], (it / STAGES) & 1, abort_flag))) {
+          if (lane == 0) TR_FAIL(509);
+          ok = false;
+        }
+        unsigned long long vis = ~0ull, bad = 0;
+        if (needs_mask) {
+          vis = valid ? tree_visible(P, sq, token, lo, key0, page_ok) : 0;
+          // values that are not finite (see the top of this file)
+          bool mine = false;
+          if (ok && !__all_sync(0xffffffffu, mbar_wait(&S.v_full[s], (it / STAGES) & 1, abort_flag))) {
+            if (lane == 0) TR_FAIL(507);
+            ok = false;
+          }
+          const int key = tile_tid & 63, part = tile_tid >> 6, n_parts = tile_threads >> 6;
+          uint4* vrow = reinterpret_cast<uint4*>(S.v[s]) + key * 8;      // 8 chunks of 16 bytes a row and block of 64 dims
+          if (ok) {
+            for (int c = part; c < HD / 8; c += n_parts) {
+              const uint4 x = vrow[(c >> 3) * (TR_KEYS * 8) + (c & 7)];
+#pragma unroll
+              for (int e = 0; e < 4; e++) {
+                const uint32_t w = e == 0 ? x.x : e == 1 ? x.y : e == 2 ? x.z : x.w;
+                mine = mine || (w & 0x7f80u) == 0x7f80u || (w & 0x7f800000u) == 0x7f800000u;
+              }
+            }
+          }
+          if (tr_bar_or(tile_bar, tile_threads, mine)) {
+            if (mine) atomicOr(bad_word, 1ull << key);
+            tr_bar(tile_bar, tile_threads);
+            bad = *(volatile unsigned long long*)bad_word;
+            if ((bad >> key) & 1)
+              for (int c = part; c < HD / 8; c += n_parts) vrow[(c >> 3) * (TR_KEYS * 8) + (c & 7)] = make_uint4(0, 0, 0, 0);
+            fence_async_shared();
+            tr_bar(tile_bar, tile_threads);
+            if (tile_tid == 0) *(volatile unsigned long long*)bad_word = 0;
+          }
+        }
+        const bool first = !any_tile;
+        any_tile = true;
+        last = it;
+        // P V of this half's tile before has read P and is in O.  Warps without rows wait for it too: were they to run
+        // ahead, their word for this tile would be counted as one for the tile before
+        auto wait_before = [&]() {
+          const uint32_t before = it - (ROWS2 ? 1 : 2);
+          if (ok && !__all_sync(0xffffffffu, mbar_wait(&S.pv_full[h][before % STAGES], (before / STAGES) & 1, abort_flag))) {
+            if (lane == 0) TR_FAIL(508);
+            ok = false;
+          }
+        };
+        if (ok && active && warp_active) {
+          tc_fence_after();
+          float sc[32], sd[32];                          // this thread's half of the keys, and the other half
+          tmem_ld32f(lane_addr + b * TR_KEYS + half * 32, sc);
+          tmem_ld32f(lane_addr + b * TR_KEYS + (half ^ 1) * 32, sd);
+          tmem_ld_wait();
+          float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+          if (needs_mask) {
+            const uint32_t vs = (uint32_t)(vis >> (half * 32)), vt = (uint32_t)(vis >> ((half ^ 1) * 32));
+#pragma unroll
+            for (int e = 0; e < 32; e++) {
+              sc[e] = (vs >> e) & 1 ? sc[e] : -INFINITY;
+              sd[e] = (vt >> e) & 1 ? sd[e] : -INFINITY;
+              mx[e & 3] = tr_max3(mx[e & 3], sc[e], sd[e]);
+            }
+          } else {
+#pragma unroll
+            for (int e = 0; e < 32; e++) mx[e & 3] = tr_max3(mx[e & 3], sc[e], sd[e]);
+          }
+          const float tile_max = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * to_log2;     // scale > 0
+          // the reference moves only when the row's maximum has outgrown it by more than 8 (a factor 256); both threads
+          // of a row see the same numbers and decide alike
+          const bool grow = tile_max > m_ref + 8.0f;
+          const float corr = grow ? tr_exp2(m_ref - tile_max) : 1.0f;
+          if (grow) m_ref = tile_max;
+          const float m_use = (m_ref == -INFINITY) ? 0.f : m_ref;
+          uint32_t packed[16];
+          float sum0 = 0.f, sum1 = 0.f;
+#pragma unroll
+          for (int e = 0; e < 32; e += 2) {
+            const float p0 = tr_exp2(fmaf(sc[e], to_log2, -m_use));
+            const float p1 = tr_exp2(fmaf(sc[e + 1], to_log2, -m_use));
+            // to bfloat16 by dropping the low mantissa bits; the sums run over the same shortened values, so the common
+            // part of the shortening divides out and what stays is as wide as round-to-nearest's error
+            const uint32_t u = __byte_perm(__float_as_uint(p0), __float_as_uint(p1), 0x7632);
+            sum0 += __uint_as_float(u << 16);
+            sum1 += __uint_as_float(u & 0xffff0000u);
+            packed[e >> 1] = u;
+          }
+          if (!first) {
+            wait_before();
+            if (ok && __any_sync(0xffffffffu, grow)) {
+              tc_fence_after();
+#pragma unroll
+              for (int c = 0; c < OD; c += 32) {
+                uint32_t r[32];
+                tmem_ld32(o_addr + c, r);
+                tmem_ld_wait();
+#pragma unroll
+                for (int e = 0; e < 32; e++) r[e] = __float_as_uint(__uint_as_float(r[e]) * corr);
+                tmem_st32(o_addr + c, r);
+              }
+              tmem_st_wait();
+            }
+          }
+          l = l * corr + (sum0 + sum1);
+          if (bad && ok) {                               // what values that are not finite give to the rows that see them
+            tc_fence_after();
+            for (int c = 0; c < OD; c += 32) {
+              uint32_t r[32];
+              if (!first) { tmem_ld32(o_addr + c, r); tmem_ld_wait(); }
+              else {
+#pragma unroll
+                for (int e = 0; e < 32; e++) r[e] = 0;
+              }
+              for (int k = 0; k < 64; k++) {
+                if (!((bad >> k) & 1)) continue;
+                const float x = tmem_ld1f(lane_addr + b * TR_KEYS + k);
+                const bool sees = (vis >> k) & 1;
+                const float p = tr_exp2(fmaf(x, to_log2, -m_use));
+                const bf16* vp = reinterpret_cast<const bf16*>(P.v_cache) +
+                                 (((size_t)(page_ok ? pg : 0) * P.n_kv + run.kvh) * TR_KEYS + k) * HD + half * OD + c;
+#pragma unroll
+                for (int e = 0; e < 32; e++)
+                  if (sees) r[e] = __float_as_uint(fmaf(p, ld_fresh(vp + e), __uint_as_float(r[e])));
+              }
+              tmem_st32(o_addr + c, r);
+            }
+            tmem_st_wait();
+          }
+          if (ok) {
+            uint8_t* prow = reinterpret_cast<uint8_t*>(S.p[h]) + row * 128;
+#pragma unroll
+            for (int c = 0; c < 4; c++) {
+              const int chunk = half * 4 + c;
+              *reinterpret_cast<uint4*>(prow + ((chunk ^ (row & 7)) << 4)) =
+                  make_uint4(packed[4 * c], packed[4 * c + 1], packed[4 * c + 2], packed[4 * c + 3]);
+            }
+          }
+        } else if (!first) {
+          wait_before();
+        }
+        if (first && sw % TR_SOFTMAX_WARPS == 0 && lane == 0) S.o_ready[h] = bad != 0;   // (`bad` is the same in all of them)
+        fence_async_shared();
+        tc_fence_before();
+        __syncwarp();
+        if (ok && lane == 0) mbar_arrive(&S.p_full[h]);
+        i++;
+      }
+      it = it_end;
+      // ---- the run is over
+      if (ok && any_tile && !__all_sync(0xffffffffu, mbar_wait(&S.pv_full[h][last % STAGES], (last / STAGES) & 1, abort_flag))) {
+        if (lane == 0) TR_FAIL(508);
+        ok = false;
+      }
+      tc_fence_after();
+      float* l_buf = reinterpret_cast<float*>(S.p[h]);   // [2][128] sums, [128] maxima (P is no longer read)
+      l_buf[half * 128 + row] = l;
+      if (half == 0) l_buf[256 + row] = m_ref;
+      const bool whole = run.from_start && run.to_end;
+      const int slot = 2 * blockIdx.x + (run.holds_u0 ? 0 : 1);
+      bf16* out_row = reinterpret_cast<bf16*>(P.out) + (size_t)token * P.ldo + (size_t)(run.kvh * gs + head) * HD;
+      if (ROWS2) {
+        tr_bar(2 + h, TR_SOFTMAX_WARPS * 32);
+        if (ok && !*abort_flag && warp_active) {
+          const float L = l_buf[row] + l_buf[128 + row];
+          const float inv = L > 0.f ? 1.0f / L : (L == 0.f ? 0.f : L);   // (a sum that is no number stays one)
+          float* po = P.part_o + ((size_t)slot * 256 + h * 128 + row) * HD + half * OD;
+#pragma unroll
+          for (int c = 0; c < OD; c += 32) {
+            float o[32];
+            tmem_ld32f(o_addr + c, o);                   // (all lanes take part; only valid rows store)
+            tmem_ld_wait();
+            if (valid && whole) {
+#pragma unroll
+              for (int e = 0; e < 32; e += 8) {
+                uint4 w;
+                uint32_t* wp = reinterpret_cast<uint32_t*>(&w);
+#pragma unroll
+                for (int x = 0; x < 4; x++) {
+                  __nv_bfloat162 a = __floats2bfloat162_rn(L == 0.f ? 0.f : o[e + 2 * x] * inv, L == 0.f ? 0.f : o[e + 2 * x + 1] * inv);
+                  wp[x] = *reinterpret_cast<uint32_t*>(&a);
+                }
+                *reinterpret_cast<uint4*>(out_row + half * OD + c + e) = w;
+              }
+            } else if (valid) {
+#pragma unroll
+              for (int e = 0; e < 32; e += 4)
+                *reinterpret_cast<float4*>(po + c + e) = make_float4(o[e], o[e + 1], o[e + 2], o[e + 3]);
+            }
+          }
+          if (valid && !whole && half == 0) P.part_ml[(size_t)slot * 256 + h * 128 + row] = make_float2(m_ref, L);
+        }
+        tc_fence_before();
+        tr_bar(2 + h, TR_SOFTMAX_WARPS * 32);            // the buffer is P again
+      } else {
+        // both halves hold the same rows: a quarter of the dims for each of a row's four threads
+        tc_fence_before();
+        tr_bar(3, 2 * TR_SOFTMAX_WARPS * 32);
+        tc_fence_after();
+        if (ok && !*abort_flag && warp_active) {
+          const float* a = reinterpret_cast<const float*>(S.p[0]);
+          const float* c = reinterpret_cast<const float*>(S.p[1]);
+          const float m0 = a[256 + row], m1 = c[256 + row];
+          const float M = fmaxf(m0, m1), Mu = M == -INFINITY ? 0.f : M;
+          const float f0 = tr_exp2(m0 - Mu), f1 = tr_exp2(m1 - Mu);
+          const float L = f0 * (a[row] + a[128 + row]) + f1 * (c[row] + c[128 + row]);
+          const float inv = L > 0.f ? 1.0f / L : (L == 0.f ? 0.f : L);
+          // a half that had no page in this run left its accumulator alone
+          const bool has0 = run.n > 1 || (it_first & 1) == 0, has1 = run.n > 1 || (it_first & 1) == 1;
+          constexpr int QD = HD / 4;
+          const int d0 = (2 * h + half) * QD;
+          float o[QD];
+#pragma unroll
+          for (int x = 0; x < QD; x += 16) {
+            uint32_t r0[16], r1[16];
+            if (has0) { tmem_ld16(lane_base + COL_PV + d0 + x, r0); }
+            if (has1) { tmem_ld16(lane_base + 256 + COL_PV + d0 + x, r1); }
+            tmem_ld_wait();
+#pragma unroll
+            for (int e = 0; e < 16; e++) {
+              // (a half that saw no key of the row has nothing but zeros to give, whatever lies in them)
+              float y = 0.f;
+              if (has0 && m0 != -INFINITY) y = f0 * __uint_as_float(r0[e]);
+              if (has1 && m1 != -INFINITY) y = fmaf(f1, __uint_as_float(r1[e]), y);
+              o[x + e] = y;
+            }
+          }
+          if (valid && whole) {
+#pragma unroll
+            for (int e = 0; e < QD; e += 8) {
+              uint4 w;
+              uint32_t* wp = reinterpret_cast<uint32_t*>(&w);
+#pragma unroll
+              for (int x = 0; x < 4; x++) {
+                __nv_bfloat162 z = __floats2bfloat162_rn(L == 0.f ? 0.f : o[e + 2 * x] * inv, L == 0.f ? 0.f : o[e + 2 * x + 1] * inv);
+                wp[x] = *reinterpret_cast<uint32_t*>(&z);
+              }
+              *reinterpret_cast<uint4*>(out_row + d0 + e) = w;
+            }
+          } else if (valid) {
+            float* po = P.part_o + ((size_t)slot * 128 + row) * HD + d0;
+#pragma unroll
+            for (int e = 0; e < QD; e += 4)
+              *reinterpret_cast<float4*>(po + e) = make_float4(o[e], o[e + 1], o[e + 2], o[e + 3]);
+            if (d0 == 0) P.part_ml[(size_t)slot * 128 + row] = make_float2(M, L);
+          }
+        }
+        tc_fence_before();
+        tr_bar(3, 2 * TR_SOFTMAX_WARPS * 32);
+      }
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 1) {
+    tc_fence_after();
+    tmem_dealloc(tmem_base, 512);
+  }
+}
+
+// ================================================================ any head size, CUDA cores
+// 256 threads take 32 rows of a (sequence, kv head) through pages of 64 keys held in shared memory as float32.  Thread
+// (ty, tx) owns rows 2 ty and 2 ty + 1: the scores of keys tx, tx + 16, .., and the output dims 4 (tx + 16 j) .. + 3; the
+// running maximum and sum of a row are kept by its sixteen threads alike.  Everything is float32, exponentials included.
+#define TG_THREADS 256
+#define TG_ROWS 32
+
+template <typename T, int NC>
+__global__ void __launch_bounds__(TG_THREADS)
+attention_tree_simple_kernel(const TreeParams P) {
+  extern __shared__ __align__(16) float tg_smem[];
+  const int hd = P.head_dim, hp = (hd + 3) & ~3, pitch = hp + 4;
+  float* qs = tg_smem;                             // [32][pitch]
+  float* ks = qs + TG_ROWS * pitch;                // [64][pitch]
+  float* vs = ks + TR_KEYS * pitch;                // [64][hp]
+  float* ps = vs + TR_KEYS * hp;                   // [32][64]
+  pdl_wait();
+  const TreeStart start = tree_start(P, reinterpret_cast<long long*>(tg_smem));
+  __syncthreads();
+  const int tid = threadIdx.x, ty = tid >> 4, tx = tid & 15;
+  const float scale_log2 = P.scale * 1.4426950408889634f;
+  TreeCursor cur;
+  cur.begin(P, start.u0, start.u1, start.b, start.item, start.off);
+  TreeRun run;
+  while (cur.next(P, run)) {
+    const TreeSeq& sq = run.s;
+    const int r0 = run.rt * TG_ROWS, n_rows = min(sq.n_new * P.gs - r0, TG_ROWS);
+    __syncthreads();                               // (the run before may still be reading)
+    for (int e = tid; e < TG_ROWS * hp; e += TG_THREADS) {
+      const int r = e / hp, d = e % hp;
+      float x = 0.f;
+      if (r < n_rows && d < hd)
+        x = ld_fresh(reinterpret_cast<const T*>(P.q) + (size_t)(sq.row0 + (r0 + r) / P.gs) * P.ldq +
+                     (size_t)(run.kvh * P.gs + (r0 + r) % P.gs) * hd + d);
+      qs[r * pitch + d] = x;
+    }
+    int token[2], lo[2], lo_max = 0;
+    bool valid[2];
+    float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
+    float4 acc[2][NC];
+#pragma unroll
+    for (int e = 0; e < 2; e++) {
+      const int r = 2 * ty + e;
+      valid[e] = r < n_rows;
+      token[e] = sq.row0 + (valid[e] ? (r0 + r) / P.gs : 0);
+      lo[e] = (P.window > 0 && valid[e]) ? max(P.token_pos[token[e]] - P.window + 1, 0) : 0;
+      lo_max = max(lo_max, lo[e]);
+#pragma unroll
+      for (int j = 0; j < NC; j++) acc[e][j] = make_float4(0.f, 0.f, 0.f, 0.f);
+    }
+    for (int i = 0; i < run.n; i++) {
+      const int page = run.page0 + i, key0 = page * TR_KEYS;
+      const int pg = P.block_table[(size_t)run.b * P.bt_stride + page];
+      const bool page_ok = (unsigned)pg < (unsigned)P.n_pages;
+      __syncthreads();                             // the page before is read (and the queries are in place)
+      bool odd = false;
+      if (page_ok) {
+        const size_t off = ((size_t)pg * P.n_kv + run.kvh) * TR_KEYS * hd;
+        const T* kp = reinterpret_cast<const T*>(P.k_cache) + off;
+        const T* vp = reinterpret_cast<const T*>(P.v_cache) + off;
+        if (sizeof(T) == 4 && hd == hp && (((uintptr_t)kp | (uintptr_t)vp) & 15) == 0) {
+          const int c4 = hp >> 2;
+          for (int e = tid; e < TR_KEYS * c4; e += TG_THREADS) {
+            const int r = e / c4, c = e % c4;
+            const float4 a = ld_fresh(reinterpret_cast<const float4*>(kp) + e);
+            const float4 b = ld_fresh(reinterpret_cast<const float4*>(vp) + e);
+            *reinterpret_cast<float4*>(ks + r * pitch + 4 * c) = a;
+            *reinterpret_cast<float4*>(vs + r * hp + 4 * c) = b;
+            odd = odd || !(isfinite(b.x) && isfinite(b.y) && isfinite(b.z) && isfinite(b.w));
+          }
+        } else {
+          for (int e = tid; e < TR_KEYS * hp; e += TG_THREADS) {
+            const int r = e / hp, d = e % hp;
+            const float a = d < hd ? ld_fresh(kp + (size_t)r * hd + d) : 0.f;
+            const float b = d < hd ? ld_fresh(vp + (size_t)r * hd + d) : 0.f;
+            ks[r * pitch + d] = a;
+            vs[r * hp + d] = b;
+            odd = odd || !isfinite(b);
+          }
+        }
+      }
+      odd = __syncthreads_or(odd);
+      if (!page_ok) continue;                      // (nobody sees a page outside the pool)
+      // scores
+      float s[2][4];
+#pragma unroll
+      for (int e = 0; e < 2; e++)
+#pragma unroll
+        for (int j = 0; j < 4; j++) s[e][j] = 0.f;
+      const float* q0 = qs + 2 * ty * pitch;
+      const float* k0 = ks + tx * pitch;
+      for (int d = 0; d < hp; d += 4) {
+        const float4 a = *reinterpret_cast<const float4*>(q0 + d), b = *reinterpret_cast<const float4*>(q0 + pitch + d);
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+          const float4 x = *reinterpret_cast<const float4*>(k0 + 16 * j * pitch + d);
+          s[0][j] = fmaf(a.x, x.x, s[0][j]); s[0][j] = fmaf(a.y, x.y, s[0][j]);
+          s[0][j] = fmaf(a.z, x.z, s[0][j]); s[0][j] = fmaf(a.w, x.w, s[0][j]);
+          s[1][j] = fmaf(b.x, x.x, s[1][j]); s[1][j] = fmaf(b.y, x.y, s[1][j]);
+          s[1][j] = fmaf(b.z, x.z, s[1][j]); s[1][j] = fmaf(b.w, x.w, s[1][j]);
+        }
+      }
+      unsigned long long vis[2] = {~0ull, ~0ull};
+      const bool masked = key0 + TR_KEYS > sq.base || key0 < lo_max;
+#pragma unroll
+      for (int e = 0; e < 2; e++) {
+        if (masked) vis[e] = valid[e] ? tree_visible(P, sq, token[e], lo[e], key0, true) : 0;
+        float mx = -INFINITY;
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+          s[e][j] = (vis[e] >> (tx + 16 * j)) & 1 ? s[e][j] * scale_log2 : -INFINITY;
+          mx = fmaxf(mx, s[e][j]);
+        }
+#pragma unroll
+        for (int d = 1; d < 16; d <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, d));
+        const float m_new = fmaxf(m[e], mx), m_use = m_new == -INFINITY ? 0.f : m_new;
+        const float corr = exp2f(m[e] - m_use);
+        m[e] = m_new;
+        float sum = 0.f;
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+          const float p = exp2f(s[e][j] - m_use);
+          sum += p;
+          ps[(2 * ty + e) * TR_KEYS + tx + 16 * j] = p;
+        }
+#pragma unroll
+        for (int d = 1; d < 16; d <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
+        l[e] = fmaf(l[e], corr, sum);
+#pragma unroll
+        for (int j = 0; j < NC; j++) { acc[e][j].x *= corr; acc[e][j].y *= corr; acc[e][j].z *= corr; acc[e][j].w *= corr; }
+      }
+      __syncwarp();                                // a row's probabilities come from its own warp
+      const float* p0 = ps + 2 * ty * TR_KEYS;
+      auto add = [&](int k, bool see0, bool see1) {
+        const float a = p0[k], b = p0[TR_KEYS + k];
+#pragma unroll
+        for (int j = 0; j < NC; j++) {
+          const int d = 4 * (tx + 16 * j);
+          if (NC * 64 == hp || d < hp) {
+            const float4 x = *reinterpret_cast<const float4*>(vs + k * hp + d);
+            if (see0) {
+              acc[0][j].x = fmaf(a, x.x, acc[0][j].x); acc[0][j].y = fmaf(a, x.y, acc[0][j].y);
+              acc[0][j].z = fmaf(a, x.z, acc[0][j].z); acc[0][j].w = fmaf(a, x.w, acc[0][j].w);
+            }
+            if (see1) {
+              acc[1][j].x = fmaf(b, x.x, acc[1][j].x); acc[1][j].y = fmaf(b, x.y, acc[1][j].y);
+              acc[1][j].z = fmaf(b, x.z, acc[1][j].z); acc[1][j].w = fmaf(b, x.w, acc[1][j].w);
+            }
+          }
+        }
+      };
+      if (odd && masked) {                         // zero times an infinity is not zero: masked keys are left out
+        for (int k = 0; k < TR_KEYS; k++) add(k, (vis[0] >> k) & 1, (vis[1] >> k) & 1);
+      } else {
+#pragma unroll 4
+        for (int k = 0; k < TR_KEYS; k++) add(k, true, true);
+      }
+    }
+    const bool whole = run.from_start && run.to_end;
+    const int slot = 2 * blockIdx.x + (run.holds_u0 ? 0 : 1);
+#pragma unroll
+    for (int e = 0; e < 2; e++) {
+      if (!valid[e]) continue;
+      const int r = 2 * ty + e;
+      const float inv = l[e] == 0.f ? 0.f : 1.0f / l[e];
+      T* op = reinterpret_cast<T*>(P.out) + (size_t)token[e] * P.ldo + (size_t)(run.kvh * P.gs + (r0 + r) % P.gs) * hd;
+      float* po = P.part_o + ((size_t)slot * TG_ROWS + r) * hp;
+#pragma unroll
+      for (int j = 0; j < NC; j++) {
+        const int d = 4 * (tx + 16 * j);
+        const float y[4] = {acc[e][j].x, acc[e][j].y, acc[e][j].z, acc[e][j].w};
+        if (whole) {
+#pragma unroll
+          for (int x = 0; x < 4; x++)
+            if (d + x < hd) op[d + x] = from_float<T>(l[e] == 0.f ? 0.f : y[x] * inv);
+        } else if (d < hp) {
+          *reinterpret_cast<float4*>(po + d) = acc[e][j];
+        }
+      }
+      if (!whole && tx == 0) P.part_ml[(size_t)slot * TG_ROWS + r] = make_float2(m[e], l[e]);
+    }
+  }
+}
+
+// ================================================================ the pieces of what several CTAs saw
+// Block (c, y): rows 8 y .. 8 y + 7 of the item that the cut between CTAs c and c + 1 goes through, where it is the first
+// one to do so.  A warp takes a row; its lanes first fetch the pieces' maxima and sums.
+template <typename T>
+__global__ void __launch_bounds__(256)
+attention_tree_merge_kernel(const TreeParams P, int G, int slot_half, int half_rows) {
+  __shared__ float w_s[8][32];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  pdl_wait();
+  const int c = blockIdx.x + 1;
+  const TreeCut cut = P.cut[c];
+  if (cut.n_pages == 0) return;
+  const long long T_ = cut.total, u0 = tree_begin(c, G, T_), ib = cut.item_begin, ie = ib + cut.n_pages;
+  int first = c - 1;                               // the last CTA before c that has anything (a short list leaves some idle)
+  while (first > 0 && tree_begin(first, G, T_) == u0) first--;
+  const long long ub = tree_begin(first, G, T_);
+  if (u0 == ib || ub > ib) return;
+  const TreeSeq sq = tree_seq(P, cut.b);
+  const int r = blockIdx.y * 8 + warp, flat = cut.rt * P.rows_per_tile + r;
+  if (r >= P.rows_per_tile || flat >= sq.n_new * P.gs) return;
+  const int hd = P.head_dim, hp = (hd + 3) & ~3;
+  const int slot_rows = (P.rows_per_tile / half_rows) * slot_half, srow = (r / half_rows) * slot_half + r % half_rows;
+  const int slot_of_first = ub == ib ? 0 : 1;
+  int n = 1;                                       // pieces: CTAs first .. first + n - 1
+  while (first + n < G && tree_begin(first + n, G, T_) < ie) n++;
+  auto slot_row = [&](int i) { return ((size_t)(2 * (first + i) + (i == 0 ? slot_of_first : 0))) * slot_rows + srow; };
+  auto empty = [&](int i) { return i > 0 && tree_begin(first + i, G, T_) == tree_begin(first + i + 1, G, T_); };
+  float M = -INFINITY;
+  for (int i = lane; i < n; i += 32)
+    if (!empty(i)) M = fmaxf(M, __ldcg(&P.part_ml[slot_row(i)].x));
+  M = warp_max(M);
+  const float Mu = M == -INFINITY ? 0.f : M;
+  float L = 0.f;
+  float4 acc[2];
+  acc[0] = acc[1] = make_float4(0.f, 0.f, 0.f, 0.f);
+  for (int i0 = 0; i0 < n; i0 += 32) {
+    const int i = i0 + lane;
+    float w = 0.f, part = 0.f;
+    if (i < n && !empty(i)) {
+      const float2 ml = __ldcg(&P.part_ml[slot_row(i)]);
+      w = exp2f(ml.x - Mu);
+      part = w * ml.y;
+    }
+    L += warp_sum(part);
+    __syncwarp();
+    w_s[warp][lane] = w;
+    __syncwarp();
+    const int k1 = min(32, n - i0);
+#pragma unroll 4
+    for (int k = 0; k < k1; k++) {
+      const float wk = w_s[warp][k];
+      if (wk == 0.f) continue;                     // (no key seen: the piece may hold anything)
+      const float* po = P.part_o + slot_row(i0 + k) * hp;
+#pragma unroll
+      for (int j = 0; j < 2; j++) {
+        const int d = 4 * (lane + 32 * j);
+        if (d < hp) {
+          const float4 x = __ldcg(reinterpret_cast<const float4*>(po + d));
+          acc[j].x = fmaf(wk, x.x, acc[j].x); acc[j].y = fmaf(wk, x.y, acc[j].y);
+          acc[j].z = fmaf(wk, x.z, acc[j].z); acc[j].w = fmaf(wk, x.w, acc[j].w);
+        }
+      }
+    }
+  }
+  const float inv = L == 0.f ? 0.f : 1.0f / L;
+  T* op = reinterpret_cast<T*>(P.out) + (size_t)(sq.row0 + flat / P.gs) * P.ldo +
+          (size_t)(cut.kvh * P.gs + flat % P.gs) * hd;
+#pragma unroll
+  for (int j = 0; j < 2; j++) {
+    const int d = 4 * (lane + 32 * j);
+    const float y[4] = {acc[j].x, acc[j].y, acc[j].z, acc[j].w};
+#pragma unroll
+    for (int x = 0; x < 4; x++)
+      if (d + x < hd) op[d + x] = from_float<T>(L == 0.f ? 0.f : y[x] * inv);
+  }
+}
+
+// ---------------------------------------------------------------- host side
+static int tree_map(CUtensorMap* map, const void* base, int rank, const cuuint64_t* dims, const cuuint64_t* strides,
+                    const cuuint32_t* box) {
+  EncodeTiledFn fn = encode_fn();
+  if (!fn) return STRATUM_ERR_LIMIT;
+  cuuint32_t estr[3] = {1, 1, 1};
+  CUresult r = fn(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, rank, const_cast<void*>(base), dims, strides, box, estr,
+                  CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                  CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  return r == CUDA_SUCCESS ? 0 : STRATUM_ERR_SHAPE;
+}
+
+// Whether this device's function attributes are set (they are a device's own).
+static bool first_on_device(unsigned long long* done) {
+  int dev = 0;
+  cudaGetDevice(&dev);
+  const unsigned long long bit = 1ull << (dev & 63);
+  const bool first = !(*done & bit);
+  *done |= bit;
+  return first;
+}
+
+template <int HD, bool ROWS2>
+static int launch_tree_tc(const CUtensorMap& mq, const CUtensorMap& mk, const CUtensorMap& mv, const TreeParams& P, int G,
+                          cudaStream_t stream) {
+  const size_t smem = sizeof(TreeSmem<HD, ROWS2>);
+  auto kern = attention_tree_tc_kernel<HD, ROWS2>;
+  static unsigned long long done = 0;
+  if (first_on_device(&done)) {
+    cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+    if (e != cudaSuccess) { done = 0; return (int)e; }
+  }
+  return launch_pdl(kern, dim3(G), dim3(TR_THREADS), smem, stream, mq, mk, mv, P);
+}
+
+static size_t simple_smem(int head_dim, int n_seqs) {
+  const int hp = (head_dim + 3) & ~3;
+  const size_t tiles = ((size_t)(TG_ROWS + TR_KEYS) * (hp + 4) + (size_t)TR_KEYS * hp + (size_t)TG_ROWS * TR_KEYS) * sizeof(float);
+  const size_t sums = (size_t)(n_seqs + 1) * sizeof(long long);
+  return tiles > sums ? tiles : sums;
+}
+
+template <typename T, int NC>
+static int launch_tree_simple(const TreeParams& P, int G, cudaStream_t stream) {
+  const size_t smem = simple_smem(P.head_dim, P.n_seqs);
+  auto kern = attention_tree_simple_kernel<T, NC>;
+  static unsigned long long done = 0;
+  if (first_on_device(&done)) {
+    cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, 227 * 1024);
+    if (e != cudaSuccess) { done = 0; return (int)e; }
+  }
+  return launch_pdl(kern, dim3(G), dim3(TG_THREADS), smem, stream, P);
+}
+
+// CTAs of a launch (the scratch has two slots of rows for each): tensor: the tcgen05 kernel, else the CUDA-core kernel, of
+// which as many share an SM as their shared memory allows.
+STRATUM_EXPORT int stratum_attention_tree_ctas(int tensor, int head_dim) {
+  if (tensor) return sm_count();
+  const int per_sm = (int)((size_t)(227 * 1024) / (simple_smem(head_dim, 0) + 1024));
+  return sm_count() * (per_sm < 1 ? 1 : per_sm > 4 ? 4 : per_sm);
+}
+
+// Scratch: part_o float32 [G][2][slot rows][head_dim rounded up to 4], part_ml float32 [G][2][slot rows][2], cut 32 bytes
+// a CTA.  Slot rows: 32 (tensor = 0), 128, or 256 (rows2).
+STRATUM_EXPORT int stratum_attention_tree(const void* q, int ldq, const void* k_cache, const void* v_cache, long long n_pages,
+                                          int dtype, const int* token_pos, const void* mask, int words,
+                                          const int* seq_start, const int* seq_len, const int* block_table, int bt_stride,
+                                          int bt_width, void* out, int ldo, int n_tokens, int n_seqs, int n_q, int n_kv,
+                                          int head_dim, int page_tokens, int window, float scale, int tensor, int rows2,
+                                          float* part_o, void* part_ml, void* cut, int* status, cudaStream_t stream) {
+  if (n_tokens <= 0 || n_seqs <= 0) return 0;
+  if (dtype != STRATUM_DT_F32 && dtype != STRATUM_DT_BF16) return STRATUM_ERR_DTYPE;
+  if (n_kv < 1 || n_q < 1 || n_q % n_kv != 0 || page_tokens != TR_KEYS || head_dim < 1 || head_dim > 256) return STRATUM_ERR_SHAPE;
+  if (words < 1 || bt_width < 1 || window < 0 || n_pages < 1) return STRATUM_ERR_SHAPE;
+  if (n_seqs > TR_MAX_SEQS || n_pages * n_kv * TR_KEYS > 0x7fffffffLL) return STRATUM_ERR_LIMIT;
+  const int gs = n_q / n_kv;
+  if ((long long)n_tokens * gs > 0x7fffffffLL) return STRATUM_ERR_LIMIT;
+  if (!part_o || !part_ml || !cut || !status) return STRATUM_ERR_ALIGN;
+  TreeParams P;
+  P.token_pos = token_pos; P.mask = (const unsigned long long*)mask; P.words = words;
+  P.seq_start = seq_start; P.seq_len = seq_len;
+  P.block_table = block_table; P.bt_stride = bt_stride; P.bt_width = bt_width;
+  P.q = q; P.ldq = ldq; P.k_cache = k_cache; P.v_cache = v_cache; P.out = out; P.ldo = ldo;
+  P.part_o = part_o; P.part_ml = (float2*)part_ml; P.cut = (TreeCut*)cut; P.status = status;
+  P.n_tokens = n_tokens; P.n_seqs = n_seqs; P.n_q = n_q; P.n_kv = n_kv; P.gs = gs; P.head_dim = head_dim;
+  P.window = window; P.n_pages = (int)n_pages; P.scale = scale;
+  const int G = stratum_attention_tree_ctas(tensor, head_dim);
+  int st, slot_half, half_rows;
+  if (tensor) {
+    if (dtype != STRATUM_DT_BF16 || (head_dim != 64 && head_dim != 128) || gs > 128 || !(scale > 0.f)) return STRATUM_ERR_SHAPE;
+    if (ldq % 8 != 0 || ldo % 8 != 0) return STRATUM_ERR_ALIGN;
+    if (((uintptr_t)q | (uintptr_t)k_cache | (uintptr_t)v_cache | (uintptr_t)out) & 15) return STRATUM_ERR_ALIGN;
+    const int half_tokens = 128 / gs;
+    slot_half = 128; half_rows = half_tokens * gs;
+    P.rows_per_tile = half_rows * (rows2 ? 2 : 1);
+    CUtensorMap mq, mk, mv;
+    {  // q as [tokens][n_q heads][head_dim]; a box is 64 dims x gs heads x half_tokens tokens: rows token * gs + head
+      cuuint64_t dims[3] = {(cuuint64_t)head_dim, (cuuint64_t)n_q, (cuuint64_t)n_tokens};
+      cuuint64_t strides[2] = {(cuuint64_t)head_dim * sizeof(bf16), (cuuint64_t)ldq * sizeof(bf16)};
+      cuuint32_t box[3] = {64, (cuuint32_t)gs, (cuuint32_t)half_tokens};
+      if ((st = tree_map(&mq, q, 3, dims, strides, box)) != 0) return st;
+    }
+    {  // the cache as [pages * n_kv * 64 rows][head_dim]; a box is 64 dims x 64 keys
+      cuuint64_t dims[2] = {(cuuint64_t)head_dim, (cuuint64_t)n_pages * n_kv * TR_KEYS};
+      cuuint64_t strides[1] = {(cuuint64_t)head_dim * sizeof(bf16)};
+      cuuint32_t box[2] = {64, TR_KEYS};
+      if ((st = tree_map(&mk, k_cache, 2, dims, strides, box)) != 0) return st;
+      if ((st = tree_map(&mv, v_cache, 2, dims, strides, box)) != 0) return st;
+    }
+    if (head_dim == 64) st = rows2 ? launch_tree_tc<64, true>(mq, mk, mv, P, G, stream) : launch_tree_tc<64, false>(mq, mk, mv, P, G, stream);
+    else st = rows2 ? launch_tree_tc<128, true>(mq, mk, mv, P, G, stream) : launch_tree_tc<128, false>(mq, mk, mv, P, G, stream);
+  } else {
+    slot_half = half_rows = P.rows_per_tile = TG_ROWS;
+    if (dtype == STRATUM_DT_F32)
+      st = head_dim <= 64 ? launch_tree_simple<float, 1>(P, G, stream)
+         : head_dim <= 128 ? launch_tree_simple<float, 2>(P, G, stream) : launch_tree_simple<float, 4>(P, G, stream);
+    else
+      st = head_dim <= 64 ? launch_tree_simple<bf16, 1>(P, G, stream)
+         : head_dim <= 128 ? launch_tree_simple<bf16, 2>(P, G, stream) : launch_tree_simple<bf16, 4>(P, G, stream);
+  }
+  if (st != 0 || G < 2) return st;
+  const dim3 grid(G - 1, (P.rows_per_tile + 7) / 8);
+  return dtype == STRATUM_DT_F32 ? launch_pdl(attention_tree_merge_kernel<float>, grid, dim3(256), 0, stream, P, G, slot_half, half_rows)
+                                 : launch_pdl(attention_tree_merge_kernel<bf16>, grid, dim3(256), 0, stream, P, G, slot_half, half_rows);
+}

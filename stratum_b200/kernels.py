@@ -495,6 +495,7 @@ def check_status() -> None:
         _status_word.zero_()
         where = {101: "the TMA producer waiting for a free stage", 102: "the MMA warp waiting for a free accumulator",
                  103: "the MMA warp waiting for a loaded stage", 104: "the epilogue waiting for an accumulator",
+                 **{c: "the attention of drafted tokens" for c in (501, 502, 503, 505, 506, 507, 508, 509, 510)},
                  431: "the resident decode step's ring (a free stage)", 432: "the resident decode step's ring (a filled stage)",
                  **{c: "a block of the resident decode step waiting for the others" for c in (401, 402, 403, 405, 411, 421)}}
         raise KernelError(f"a device-side wait ran out in {where.get(code, f'code {code}')}; results are invalid")
@@ -1658,6 +1659,100 @@ def attention_stream(qkv: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Te
              _ptr(status_word()),
              _stream()), "attention_stream")
     count_launches(1)
+
+
+# ------------------------------------------------------------------ drafted tokens
+def _one_device(what: str, *tensors: Optional[torch.Tensor]) -> None:
+    """All on the current device, which is also the one this process's launches go to (see _stream, status_word)."""
+    here = torch.cuda.current_device() if torch.cuda.is_available() else None
+    for t in tensors:
+        if t is None:
+            continue
+        if not t.is_cuda:
+            raise KernelError(f"{what}: tensors must live on a CUDA device (no CPU path exists)")
+        if t.device.index != here:
+            raise KernelError(f"{what}: a tensor lives on {t.device}, the current device is cuda:{here}")
+    if _device_index is not None and _device_index != here:
+        raise KernelError(f"{what}: this process launches on cuda:{_device_index}, the current device is cuda:{here}")
+
+
+def _shaped(t: torch.Tensor, name: str, dtype, shape=None) -> None:
+    if t.dtype != dtype:
+        raise KernelError(f"{name} must be {dtype}, is {t.dtype}")
+    if not t.is_contiguous():
+        raise KernelError(f"{name} must be contiguous")
+    if shape is not None and t.shape != shape:
+        raise KernelError(f"{name} must have the shape {shape}, has {tuple(t.shape)}")
+
+
+_tree_ctas: dict = {}
+TREE_MAX_SEQS = 4096
+
+
+def attention_tree(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, token_pos: torch.Tensor,
+                   tree_mask: torch.Tensor, seq_start: torch.Tensor, seq_len: torch.Tensor, block_table: torch.Tensor,
+                   out: torch.Tensor, n_q: int, n_kv: int, head_dim: int, page_tokens: int, window: int, scale: float,
+                   max_new: int) -> None:
+    """Attention of drafted tokens, a tree of them per sequence, over the paged cache (csrc/attention_tree.cu).
+
+    q [tokens, >= n_q * head_dim] (query heads first), out [tokens, >= n_q * head_dim], the caches [pages, n_kv, 64,
+    head_dim], all float32 or all bfloat16.  Sequence s has the rows seq_start[s] .. seq_start[s + 1] - 1 (int32 [seqs +
+    1]) and seq_len[s] cached keys (int32 [seqs]), its drafted ones among them: row j's key and value lie at position
+    seq_len[s] - rows + j.  tree_mask (int64 [tokens, words]): bit j of word w says that the token sees row 64 w + j of
+    its sequence (itself among them, if it is to).  In front of the drafted rows a token sees every cached key or, with a
+    window, those at positions above token_pos - window; token_pos is not below the position of the sequence's first
+    drafted row, and the window does not touch what the mask says.  A token that sees nothing gets zeros; rows behind the
+    last sequence are left as they were; a page number outside the pool holds keys that nobody sees.
+    max_new: drafted tokens of the sequence that has most (how the work is cut, not what comes out).
+
+    bfloat16 heads of 64 or 128 on tcgen05, with probabilities rounded to bfloat16 as the value product's operand has to
+    be; float32 and every other head size up to 256 on the CUDA cores in float32."""
+    dt = q.dtype
+    code = dtype_code(dt)
+    _one_device("attention_tree", q, k_cache, v_cache, token_pos, tree_mask, seq_start, seq_len, block_table, out)
+    _shaped(k_cache, "k_cache", dt); _shaped(v_cache, "v_cache", dt, k_cache.shape)
+    if k_cache.dim() != 4 or tuple(k_cache.shape[1:]) != (n_kv, page_tokens, head_dim) or n_q < 1 or n_q % max(n_kv, 1):
+        raise KernelError("attention_tree: the caches are [pages, n_kv, page_tokens, head_dim], n_q a multiple of n_kv")
+    T, B = q.shape[0], seq_len.numel()
+    for t, name in ((q, "q"), (out, "out")):
+        if t.dim() != 2 or t.dtype != dt or t.shape[0] != T or t.shape[1] < n_q * head_dim or t.stride(1) != 1 \
+                or (T > 1 and t.stride(0) < n_q * head_dim):
+            raise KernelError(f"attention_tree: {name} must be [tokens, >= n_q * head_dim] of the cache's dtype, rows contiguous")
+    _shaped(token_pos, "token_pos", torch.int32, (T,)); _shaped(seq_len, "seq_len", torch.int32, (B,))
+    _shaped(seq_start, "seq_start", torch.int32, (B + 1,)); _shaped(tree_mask, "tree_mask", torch.int64)
+    _shaped(block_table, "block_table", torch.int32)
+    if tree_mask.dim() != 2 or tree_mask.shape[0] != T or (T > 0 and tree_mask.shape[1] < 1):
+        raise KernelError("attention_tree: tree_mask is [tokens, words]")
+    if block_table.dim() != 2 or block_table.shape[0] != B or (B > 0 and block_table.shape[1] < 1):
+        raise KernelError("attention_tree: block_table is [sequences, pages]")
+    if window < 0 or max_new < 0:
+        raise KernelError("attention_tree: window and max_new are not negative")
+    if T == 0 or B == 0:
+        return
+    group = n_q // n_kv
+    tensor = (dt == torch.bfloat16 and head_dim in (64, 128) and group <= 128 and scale > 0 and q.stride(0) % 8 == 0
+              and out.stride(0) % 8 == 0 and not (q.data_ptr() | out.data_ptr() | k_cache.data_ptr() | v_cache.data_ptr()) & 15)
+    # more rows than a half of a CTA holds: both halves share every page (else they take pages in turn)
+    rows2 = max_new * group > 128
+    key = (tensor, head_dim)
+    ctas = _tree_ctas.get(key)
+    if ctas is None:
+        ctas = _tree_ctas[key] = int(build.load("attention_tree").stratum_attention_tree_ctas(int(tensor), head_dim))
+    slots = 2 * ctas * (32 if not tensor else 256 if rows2 else 128)
+    # (scratch of this call's own: calls on several streams, and captured ones, do not meet in it)
+    scratch = torch.empty(slots * ((head_dim + 3) // 4 * 4 + 2) + 8 * ctas, dtype=torch.float32, device=q.device)
+    at = scratch.data_ptr()
+    part_ml = at + 4 * slots * ((head_dim + 3) // 4 * 4)
+    f = _fn("attention_tree", "stratum_attention_tree",
+            [c_void_p, c_int, c_void_p, c_void_p, ctypes.c_longlong, c_int, c_void_p, c_void_p, c_int, c_void_p, c_void_p,
+             c_void_p, c_int, c_int, c_void_p, c_int, c_int, c_int, c_int, c_int, c_int, c_int, c_int, c_float, c_int, c_int,
+             c_void_p, c_void_p, c_void_p, c_void_p, c_void_p])
+    _check(f(q.data_ptr(), q.stride(0), k_cache.data_ptr(), v_cache.data_ptr(), k_cache.shape[0], code,
+             token_pos.data_ptr(), tree_mask.data_ptr(), tree_mask.shape[1], seq_start.data_ptr(), seq_len.data_ptr(),
+             block_table.data_ptr(), block_table.stride(0), block_table.shape[1], out.data_ptr(), out.stride(0), T, B, n_q,
+             n_kv, head_dim, page_tokens, window, scale, int(tensor), int(rows2), at, part_ml, part_ml + 8 * slots,
+             status_word().data_ptr(), _stream()), "attention_tree")
+    count_launches(1)          # the merge kernel
 
 
 # ------------------------------------------------------------------ a decode step's layers as one kernel
