@@ -15,11 +15,14 @@
 // Two kernels.  attention_tree_tc_kernel: bfloat16, heads of 64 or 128, on tcgen05 (below).  attention_tree_simple_kernel:
 // any head size up to 256, float32 or bfloat16, on the CUDA cores in float32 throughout.
 //
-// The tcgen05 kernel.  A CTA has two halves, each with a warp that issues MMAs, eight softmax warps (two threads per row),
-// two buffers of scores and an accumulator in tensor memory: S = Q K^T (128 rows x 64 keys), P to shared memory, O += P V.
+// The tcgen05 kernel.  A CTA has two halves, each with a warp that issues MMAs, four softmax warps (a thread per row),
+// two buffers of scores and an accumulator in tensor memory: S = Q K^T (128 rows x 64 keys), P = exp(S - ref), O += P V.
 //   ROWS2 = false (at most 128 rows per sequence and kv head): both halves hold the same rows and take every other page,
 //     so that one page's softmax runs under the other's loads and MMAs; their sums are joined at the end of a run;
 //   ROWS2 = true: the halves hold 128 rows each and share every page, which then is fetched once for 256 rows.
+// P goes back into tensor memory, over the scores it came from, and is the first operand of P V there: with P in shared
+// memory its writing and its reading by the MMAs took a third of what shared memory moves per tile, and every tile had to
+// wait for the one before to be read (91 us against XX for one sequence of 32,700 tokens and 61 drafted ones).
 // One thread of warp 0 feeds rings of K and V pages by TMA, and the queries of the run that comes next.
 //
 // The products with masked keys: P is zero there, but zero times an infinity or a NaN is not, and a page that is masked for
@@ -35,7 +38,7 @@
 
 #define TR_KEYS 64
 #define TR_MAX_SEQS 4096
-#define TR_SOFTMAX_WARPS 8
+#define TR_SOFTMAX_WARPS 4                  // per half, a thread a row
 #define TR_THREADS (32 + 2 * 32 + 2 * TR_SOFTMAX_WARPS * 32)
 
 struct TreeParams {
@@ -86,22 +89,22 @@ struct TreeRun {
 };
 
 struct TreeCursor {
-  long long u, u0, u1;
+  int u, n_units;                          // units behind us, units of the stretch
   int b, item, off;
   TreeSeq s;
-  __device__ __forceinline__ void begin(const TreeParams& P, long long u0_, long long u1_, int b_, int item_, int off_) {
-    u = u0 = u0_; u1 = u1_; b = b_; item = item_; off = off_;
-    if (u < u1) s = tree_seq(P, b);
+  __device__ __forceinline__ void begin(const TreeParams& P, int n_units_, int b_, int item_, int off_) {
+    u = 0; n_units = n_units_; b = b_; item = item_; off = off_;
+    if (u < n_units) s = tree_seq(P, b);
   }
   __device__ __forceinline__ bool next(const TreeParams& P, TreeRun& r) {
-    if (u >= u1) return false;
+    if (u >= n_units) return false;
     r.s = s; r.b = b;
     r.kvh = item / s.n_tiles; r.rt = item % s.n_tiles;
     r.page0 = s.first + off;
-    r.n = (int)min((long long)(s.n_pages - off), u1 - u);
+    r.n = min(s.n_pages - off, n_units - u);
     r.from_start = off == 0;
     r.to_end = off + r.n == s.n_pages;
-    r.holds_u0 = u == u0;
+    r.holds_u0 = u == 0;
     u += r.n; off += r.n;
     if (off == s.n_pages) {
       off = 0;
@@ -114,8 +117,23 @@ struct TreeCursor {
   }
 };
 
+// A warp's walk over the runs of its CTA's stretch, kept in shared memory: in registers it would push the tile loops' values
+// out to local memory, which has next to no L1 beside the rings (a prompt-sized tree took 100 us with them there, of which
+// most was waiting for those loads).
+struct TreeWalk {
+  TreeCursor cur;
+  TreeRun run;
+  int more;
+};
+__device__ __forceinline__ bool tree_advance(const TreeParams& P, TreeWalk& w, int lane) {
+  __syncwarp();
+  if (lane == 0) w.more = w.cur.next(P, w.run);
+  __syncwarp();
+  return w.more != 0;
+}
+
 // Where CTA c begins; every thread of the block calls it.  `sums` holds a running sum per sequence for the while.
-struct TreeStart { long long u0, u1; int b, item, off; };
+struct TreeStart { int n_units, b, item, off; };
 __device__ __forceinline__ TreeStart tree_start(const TreeParams& P, long long* sums) {
   const int n_threads = blockDim.x, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   for (int b = threadIdx.x; b < P.n_seqs; b += n_threads) {
@@ -142,20 +160,21 @@ __device__ __forceinline__ TreeStart tree_start(const TreeParams& P, long long* 
   TreeStart t;
   const long long T = sums[P.n_seqs];
   const int c = blockIdx.x, G = gridDim.x;
-  t.u0 = tree_begin(c, G, T); t.u1 = tree_begin(c + 1, G, T);
+  const long long u0 = tree_begin(c, G, T);
+  t.n_units = (int)(tree_begin(c + 1, G, T) - u0);
   t.b = t.item = t.off = 0;
-  if (t.u0 < t.u1) {
+  if (t.n_units > 0) {
     int lo = 0, hi = P.n_seqs - 1;                // the last sequence that begins at or before u0 and is not empty
     while (lo < hi) {
       const int mid = (lo + hi + 1) >> 1;
-      if (sums[mid] <= t.u0) lo = mid; else hi = mid - 1;
+      if (sums[mid] <= u0) lo = mid; else hi = mid - 1;
     }
     const TreeSeq s = tree_seq(P, lo);
-    const long long r = t.u0 - sums[lo];
+    const long long r = u0 - sums[lo];
     t.b = lo; t.item = (int)(r / s.n_pages); t.off = (int)(r % s.n_pages);
     if (threadIdx.x == 0) {
       TreeCut cut;
-      cut.item_begin = t.u0 - t.off; cut.total = T;
+      cut.item_begin = u0 - t.off; cut.total = T;
       cut.b = lo; cut.kvh = t.item / s.n_tiles; cut.rt = t.item % s.n_tiles; cut.n_pages = s.n_pages;
       P.cut[c] = cut;
     }
@@ -202,15 +221,16 @@ __device__ __forceinline__ unsigned long long tree_visible(const TreeParams& P, 
 // ================================================================ tcgen05
 template <int HD, bool ROWS2>
 struct TreeSmem {
-  static constexpr int STAGES = HD == 64 ? 8 : 4;       // (even: with alternating halves a stage is always the same half's)
+  static constexpr int STAGES = HD == 64 ? 10 : ROWS2 ? 5 : 4;   // (even where the halves alternate: a stage is then always the same half's)
   static constexpr int QB = ROWS2 ? 1 : 2;              // queries of the next run beside those of this one
   alignas(1024) bf16 q[2][128 * HD];                    // ROWS2: per half; else: of two runs
   alignas(1024) bf16 k[STAGES][TR_KEYS * HD];           // [HD/64][64 keys][64 dims]
   alignas(1024) bf16 v[STAGES][TR_KEYS * HD];
-  alignas(1024) bf16 p[2][128 * TR_KEYS];               // per half; at the end of a run: the rows' sums and maxima
+  float2 ml[2][ROWS2 ? 1 : 128];                                    // a row's maximum and sum in either half, at the end of a run
   uint64_t q_full[QB], q_empty[QB], k_full[STAGES], v_full[STAGES];
-  uint64_t s_full[2][STAGES], pv_full[2][STAGES], p_full[2];
+  uint64_t s_full[2][STAGES], pv_full[2][STAGES], p_full[2][2];
   unsigned long long bad[2];
+  TreeWalk walk[2 + 2 + 2 * TR_SOFTMAX_WARPS];          // queries, pages, MMA warps, softmax warps
   int row_of[32];                                       // cache row of a tile's page, from the K to the V request
   uint32_t tmem_base;
   int o_ready[2];
@@ -238,6 +258,11 @@ __device__ __forceinline__ bool tr_bar_or(int id, int n, bool mine) {
       : "=r"(r) : "r"(id), "r"(n), "r"((uint32_t)mine) : "memory");
   return r != 0;
 }
+// two outputs as bfloat16; zeros where the row's sum L is zero (it saw no key)
+__device__ __forceinline__ uint32_t tr_pack(float L, float a, float b) {
+  const __nv_bfloat162 v = __floats2bfloat162_rn(L == 0.f ? 0.f : a, L == 0.f ? 0.f : b);
+  return *reinterpret_cast<const uint32_t*>(&v);
+}
 __device__ __forceinline__ float tmem_ld1f(uint32_t taddr) {
   uint32_t r;
   asm volatile("tcgen05.ld.sync.aligned.32x32b.x1.b32 {%0}, [%1];" : "=r"(r) : "r"(taddr));
@@ -245,7 +270,74 @@ __device__ __forceinline__ float tmem_ld1f(uint32_t taddr) {
   return __uint_as_float(r);
 }
 
+// D += A B with A (128 rows x 16 bfloat16) in tensor memory: two values of k to a column
+__device__ __forceinline__ void umma_bf16_ts(uint32_t tmem_d, uint32_t tmem_a, uint64_t desc_b, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}"
+      ::"r"(tmem_d), "r"(tmem_a), "l"(desc_b), "r"(idesc), "r"(accumulate) : "memory");
+}
+
 #define TR_FAIL(code) { atomicCAS(P.status, 0, code); S.abort_flag = 1; }
+
+// The two parts that only masked tiles need are functions of their own, so that the loop over the other tiles keeps its
+// registers.
+
+// The keys of a page of values (in shared memory) that hold anything not finite; their rows are zeroed.  The `n` threads of
+// barrier `id` come here together, numbered by `tid`.
+template <int HD>
+__device__ __noinline__ unsigned long long tree_look_through(uint4* v, unsigned long long* word, int id, int n, int tid, bool ok) {
+  const int key = tid & 63, part = tid >> 6, n_parts = n >> 6;
+  uint4* row = v + key * 8;                              // 8 chunks of 16 bytes a key and block of 64 dims
+  bool mine = false;
+  if (ok) {
+    for (int c = part; c < HD / 8; c += n_parts) {
+      const uint4 x = row[(c >> 3) * (TR_KEYS * 8) + (c & 7)];
+#pragma unroll
+      for (int e = 0; e < 4; e++) {
+        const uint32_t w = e == 0 ? x.x : e == 1 ? x.y : e == 2 ? x.z : x.w;
+        mine = mine || (w & 0x7f80u) == 0x7f80u || (w & 0x7f800000u) == 0x7f800000u;
+      }
+    }
+  }
+  if (!tr_bar_or(id, n, mine)) return 0;
+  if (mine) atomicOr(word, 1ull << key);
+  tr_bar(id, n);
+  const unsigned long long bad = *(volatile unsigned long long*)word;
+  if ((bad >> key) & 1)
+    for (int c = part; c < HD / 8; c += n_parts) row[(c >> 3) * (TR_KEYS * 8) + (c & 7)] = make_uint4(0, 0, 0, 0);
+  fence_async_shared();
+  tr_bar(id, n);
+  if (tid == 0) *(volatile unsigned long long*)word = 0;
+  return bad;
+}
+
+// Adds what the keys in `bad` give to this thread's row of the output in tensor memory (or to zeros where it holds nothing
+// yet).  v: the page's values in the cache.
+template <int HD>
+__device__ __noinline__ void tree_add_bad(unsigned long long bad, unsigned long long vis, uint32_t s_addr, uint32_t o_addr,
+                                          float to_log2, float m_use, const bf16* v, bool fresh) {
+  for (int c = 0; c < HD; c += 32) {
+    uint32_t r[32];
+    tmem_ld32(o_addr + c, r);
+    tmem_ld_wait();
+    if (fresh) {
+#pragma unroll
+      for (int e = 0; e < 32; e++) r[e] = 0;
+    }
+    for (int k = 0; k < 64; k++) {
+      if (!((bad >> k) & 1)) continue;
+      const float p = tr_exp2(fmaf(tmem_ld1f(s_addr + k), to_log2, -m_use));
+      const bool sees = (vis >> k) & 1;
+#pragma unroll
+      for (int e = 0; e < 32; e++)
+        if (sees) r[e] = __float_as_uint(fmaf(p, ld_fresh(v + (size_t)k * HD + c + e), __uint_as_float(r[e])));
+    }
+    tmem_st32(o_addr + c, r);
+  }
+  tmem_st_wait();
+}
 
 template <int HD, bool ROWS2>
 __global__ void __launch_bounds__(TR_THREADS, 1)
@@ -269,7 +361,10 @@ attention_tree_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
       mbar_init(&S.k_full[s], 1); mbar_init(&S.v_full[s], 1);
       for (int h = 0; h < 2; h++) { mbar_init(&S.s_full[h][s], 1); mbar_init(&S.pv_full[h][s], 1); }
     }
-    for (int h = 0; h < 2; h++) { mbar_init(&S.p_full[h], TR_SOFTMAX_WARPS); S.bad[h] = 0; S.o_ready[h] = 0; }
+    for (int h = 0; h < 2; h++) {
+      mbar_init(&S.p_full[h][0], TR_SOFTMAX_WARPS); mbar_init(&S.p_full[h][1], TR_SOFTMAX_WARPS);
+      S.bad[h] = 0; S.o_ready[h] = 0;
+    }
     S.abort_flag = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
@@ -286,9 +381,13 @@ attention_tree_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
   const uint32_t tmem_base = S.tmem_base;
   const int gs = P.gs;
   const int half_tokens = 128 / gs;                     // tokens of a half's 128 rows
-  TreeCursor cur;
-  cur.begin(P, start.u0, start.u1, start.b, start.item, start.off);
-  TreeRun run;
+  TreeWalk& walk = S.walk[warp + 1];                    // (warp 0: [1]; [0] is its walk over the queries)
+  const TreeRun& run = walk.run;
+  if (lane == 0) {
+    walk.cur.begin(P, start.n_units, start.b, start.item, start.off);
+    if (warp == 0) S.walk[0].cur = walk.cur;
+  }
+  __syncwarp();
   auto half_ntok = [&](const TreeRun& r, int h) {       // tokens of the run's tile that half h holds
     const int t0 = ROWS2 ? (2 * r.rt + h) * half_tokens : r.rt * half_tokens;
     return min(max(r.s.n_new - t0, 0), half_tokens);
@@ -296,15 +395,15 @@ attention_tree_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
 
   if (warp == 0) {
     // ---------------------------------------------------------------- producer
-    if (lane == 0 && start.u0 < start.u1) {
+    if (lane == 0 && start.n_units > 0) {
       asm volatile("prefetch.tensormap [%0];" ::"l"(&map_q) : "memory");
       asm volatile("prefetch.tensormap [%0];" ::"l"(&map_k) : "memory");
       asm volatile("prefetch.tensormap [%0];" ::"l"(&map_v) : "memory");
-      const uint32_t n_units = (uint32_t)(start.u1 - start.u0);
-      TreeCursor cq = cur;
-      TreeRun rq;
+      const uint32_t n_units = (uint32_t)start.n_units;
+      TreeCursor& cq = S.walk[0].cur;
+      TreeRun& rq = S.walk[0].run;
       bool more_q = cq.next(P, rq);
-      bool have = cur.next(P, run);
+      bool have = walk.cur.next(P, walk.run);
       int tile = 0, nq = 0;
       uint32_t jk = 0, jv = 0;
       const int* bt = P.block_table + (size_t)run.b * P.bt_stride;
@@ -342,7 +441,7 @@ attention_tree_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
           jk++;
           if (++tile == run.n) {
             tile = 0;
-            have = cur.next(P, run);
+            have = walk.cur.next(P, walk.run);
             bt = P.block_table + (size_t)run.b * P.bt_stride;
           }
           if (have) pg = __ldcg(bt + run.page0 + tile);
@@ -368,7 +467,7 @@ attention_tree_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
     // ---------------------------------------------------------------- MMA issuer of half `warp - 1`
     const int h = warp - 1;
     const uint32_t idesc_s = instr_desc_bf16(TR_KEYS), idesc_pv = instr_desc_bf16(HD, true);
-    const uint32_t tmem_h = tmem_base + h * 256, p_addr = smem_u32(S.p[h]);
+    const uint32_t tmem_h = tmem_base + h * 256;
     bool ok = true;
     // This half's tiles as one sequence over the runs, the scores one tile ahead of the products with V: what is known of
     // the tile whose P V is still to come
@@ -378,44 +477,47 @@ attention_tree_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
     auto values = [&]() {                                // P V of the pending tile
       const int s = pend_it % STAGES;
       if (!__all_sync(0xffffffffu, mbar_wait(&S.v_full[s], (pend_it / STAGES) & 1, abort_flag))) { if (lane == 0) TR_FAIL(506); ok = false; return; }
-      if (!__all_sync(0xffffffffu, mbar_wait(&S.p_full[h], pend_i & 1, abort_flag))) { if (lane == 0) TR_FAIL(505); ok = false; return; }
+      if (!__all_sync(0xffffffffu, mbar_wait(&S.p_full[h][pend_i & 1], (pend_i >> 1) & 1, abort_flag))) { if (lane == 0) TR_FAIL(505); ok = false; return; }
       if (!pend_active) {                                // no rows of this half: the page is free
         if (lane == 0) mbar_arrive(&S.pv_full[h][s]);
         __syncwarp();
         return;
       }
       tc_fence_after();
-      const uint32_t v_addr = smem_u32(S.v[s]);
+      const uint64_t vd = smem_desc_sw128_mn(smem_u32(S.v[s]), TR_KEYS * 128);
+      const uint32_t p_addr = tmem_h + (pend_i & 1) * TR_KEYS;
       const bool fresh = pend_first && *(volatile int*)&S.o_ready[h] == 0;
       if (elect_one()) {
 #pragma unroll
-        for (int kk = 0; kk < 4; kk++)
-          umma_bf16(tmem_h + COL_PV, smem_desc_sw128(p_addr + kk * 32),
-                    smem_desc_sw128_mn(v_addr + kk * 16 * 128, TR_KEYS * 128), idesc_pv, (fresh && kk == 0) ? 0u : 1u);
+        for (int kk = 0; kk < 4; kk++)                   // 16 keys a step: 8 columns of P, 16 rows of V (in units of 16 bytes)
+          umma_bf16_ts(tmem_h + COL_PV, p_addr + kk * 8, vd + (uint64_t)(kk * 16 * 128 / 16), idesc_pv, (fresh && kk == 0) ? 0u : 1u);
         umma_commit(&S.pv_full[h][s]);
       }
       __syncwarp();
     };
-    for (int r = 0; ok && cur.next(P, run); r++) {
+    for (int r = 0; ok && tree_advance(P, walk, lane); r++) {
       const bool active = !ROWS2 || half_ntok(run, h) > 0;
       if (!__all_sync(0xffffffffu, mbar_wait(&S.q_full[r % QB], (r / QB) & 1, abort_flag))) { if (lane == 0) TR_FAIL(502); ok = false; break; }
-      const uint32_t q_addr = smem_u32(S.q[ROWS2 ? h : r % QB]);
+      const uint64_t qd = smem_desc_sw128(smem_u32(S.q[ROWS2 ? h : r % QB]));
       bool first = true;
       const uint32_t it_end = it + run.n;
       for (; it < it_end && ok; it++) {
         if (!ROWS2 && (int)(it & 1) != h) continue;
         const int s = it % STAGES;
+        const uint32_t before2 = it - 2 * (ROWS2 ? 1 : 2);
         if (!__all_sync(0xffffffffu, mbar_wait(&S.k_full[s], (it / STAGES) & 1, abort_flag))) { if (lane == 0) TR_FAIL(503); ok = false; break; }
         if (active) {
+          // the buffer holds P of two tiles ago: its product with V has been issued, and is over
+          if (i >= 2 && !__all_sync(0xffffffffu, mbar_wait(&S.pv_full[h][before2 % STAGES], (before2 / STAGES) & 1, abort_flag))) { if (lane == 0) TR_FAIL(504); ok = false; break; }
           tc_fence_after();
-          const uint32_t k_addr = smem_u32(S.k[s]);
+          const uint64_t kd = smem_desc_sw128(smem_u32(S.k[s]));
           if (elect_one()) {
 #pragma unroll
             for (int db = 0; db < DB; db++)
 #pragma unroll
-              for (int kk = 0; kk < 4; kk++)
-                umma_bf16(tmem_h + (i & 1) * TR_KEYS, smem_desc_sw128(q_addr + db * 128 * 128 + kk * 32),
-                          smem_desc_sw128(k_addr + db * TR_KEYS * 128 + kk * 32), idesc_s, (db | kk) ? 1u : 0u);
+              for (int kk = 0; kk < 4; kk++)             // (descriptors count in units of 16 bytes)
+                umma_bf16(tmem_h + (i & 1) * TR_KEYS, qd + (uint64_t)((db * 128 * 128 + kk * 32) / 16),
+                          kd + (uint64_t)((db * TR_KEYS * 128 + kk * 32) / 16), idesc_s, (db | kk) ? 1u : 0u);
             umma_commit(&S.s_full[h][s]);
           }
           __syncwarp();
@@ -436,30 +538,26 @@ attention_tree_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
     }
     if (ok && pend) values();
   } else {
-    // ---------------------------------------------------------------- softmax (eight warps per half)
-    const int sw = warp - 3, h = sw / TR_SOFTMAX_WARPS;
+    // ---------------------------------------------------------------- softmax (four warps per half, a thread a row)
+    const int h = (warp - 3) / TR_SOFTMAX_WARPS;
     const int quarter = warp & 3;                        // tensor-memory lanes this warp may read
-    const int half = (sw % TR_SOFTMAX_WARPS) >> 2;       // 0: keys 0..31 and the lower dims; 1: the others
     const int row = quarter * 32 + lane;
     const int tok = row / gs, head = row % gs;
     const uint32_t lane_base = tmem_base + ((uint32_t)(quarter * 32) << 16);
     const uint32_t lane_addr = lane_base + h * 256;
-    constexpr int OD = HD / 2;
-    const uint32_t o_addr = lane_addr + COL_PV + half * OD;
+    const uint32_t o_addr = lane_addr + COL_PV;
     const float to_log2 = P.scale * 1.4426950408889634f;
+    constexpr int STEP = ROWS2 ? 1 : 2;                  // from a tile of this half to the next
     const int tile_bar = ROWS2 ? 1 : 1 + h, tile_threads = ROWS2 ? 2 * TR_SOFTMAX_WARPS * 32 : TR_SOFTMAX_WARPS * 32;
     const int tile_tid = ROWS2 ? threadIdx.x - 96 : threadIdx.x - 96 - h * TR_SOFTMAX_WARPS * 32;
-    unsigned long long* bad_word = &S.bad[ROWS2 ? 0 : h];
     bool ok = true;
     uint32_t it = 0, i = 0;
-    while (cur.next(P, run)) {
+    while (tree_advance(P, walk, lane)) {
       const TreeSeq& sq = run.s;
       const int ntok = half_ntok(run, h);
-      const bool active = ntok > 0;
       const bool valid = tok < ntok;
       const bool warp_active = quarter * 32 < ntok * gs;
-      const int tok0 = sq.row0 + (ROWS2 ? 2 * run.rt + h : run.rt) * half_tokens;
-      const int token = tok0 + (valid ? tok : 0);
+      const int token = sq.row0 + (ROWS2 ? 2 * run.rt + h : run.rt) * half_tokens + (valid ? tok : 0);
       int lo = 0, lo_max = 0;
       if (P.window > 0) {
         lo = valid ? max(P.token_pos[token] - P.window + 1, 0) : 0;
@@ -469,189 +567,133 @@ attention_tree_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
         for (int t = t0 + lane; t < t1; t += 32) lo_max = max(lo_max, P.token_pos[t] - P.window + 1);
         lo_max = __reduce_max_sync(0xffffffffu, lo_max);
       }
-      const int* bt = P.block_table + (size_t)run.b * P.bt_stride;
-      const uint32_t it_end = it + run.n;
-      const uint32_t it_first = it;
-      float m_ref = -INFINITY, l = 0.f;
-      uint32_t last = 0;
-      bool any_tile = false;
+      const uint32_t it_first = it, it_end = it + run.n;
       if (!ROWS2 && (int)(it & 1) != h) it++;
-      int pg_next = it < it_end ? __ldcg(bt + run.page0 + (int)(it - it_first)) : 0;
-      for (; it < it_end; it += ROWS2 ? 1 : 2) {
+      const uint32_t it_mine = it;                       // this half's first tile of the run (it_end or beyond: none)
+      const int* bt = P.block_table + (size_t)run.b * P.bt_stride + run.page0 - (int)it_first;   // [it]: the tile's page
+      int pg_next = it < it_end ? __ldcg(bt + (int)it) : 0;
+      float m_ref = -INFINITY, l = 0.f;
+      for (; it < it_end; it += STEP) {
         const int s = it % STAGES, b = i & 1;
-        const int page = run.page0 + (int)(it - it_first), key0 = page * TR_KEYS;
+        const int key0 = (run.page0 + (int)(it - it_first)) * TR_KEYS;
         const int pg = pg_next;
-        if (it + (ROWS2 ? 1 : 2) < it_end) pg_next = __ldcg(bt + page + (ROWS2 ? 1 : 2));
+        if (it + STEP < it_end) pg_next = __ldcg(bt + (int)it + STEP);
         const bool page_ok = (unsigned)pg < (unsigned)P.n_pages;
         const bool needs_mask = key0 + TR_KEYS > sq.base || key0 < lo_max || !page_ok;
+        const bool first = it == it_mine;
         if (ok && !__all_sync(0xffffffffu, mbar_wait(&S.s_full[h][s], (it / STAGES) & 1, abort_flag))) {
           if (lane == 0) TR_FAIL(509);
           ok = false;
         }
-        unsigned long long vis = ~0ull, bad = 0;
+        unsigned long long vis = 0, bad = 0;
         if (needs_mask) {
-          vis = valid ? tree_visible(P, sq, token, lo, key0, page_ok) : 0;
-          // values that are not finite (see the top of this file)
-          bool mine = false;
+          if (valid) vis = tree_visible(P, sq, token, lo, key0, page_ok);
           if (ok && !__all_sync(0xffffffffu, mbar_wait(&S.v_full[s], (it / STAGES) & 1, abort_flag))) {
             if (lane == 0) TR_FAIL(507);
             ok = false;
           }
-          const int key = tile_tid & 63, part = tile_tid >> 6, n_parts = tile_threads >> 6;
-          uint4* vrow = reinterpret_cast<uint4*>(S.v[s]) + key * 8;      // 8 chunks of 16 bytes a row and block of 64 dims
-          if (ok) {
-            for (int c = part; c < HD / 8; c += n_parts) {
-              const uint4 x = vrow[(c >> 3) * (TR_KEYS * 8) + (c & 7)];
-#pragma unroll
-              for (int e = 0; e < 4; e++) {
-                const uint32_t w = e == 0 ? x.x : e == 1 ? x.y : e == 2 ? x.z : x.w;
-                mine = mine || (w & 0x7f80u) == 0x7f80u || (w & 0x7f800000u) == 0x7f800000u;
-              }
-            }
-          }
-          if (tr_bar_or(tile_bar, tile_threads, mine)) {
-            if (mine) atomicOr(bad_word, 1ull << key);
-            tr_bar(tile_bar, tile_threads);
-            bad = *(volatile unsigned long long*)bad_word;
-            if ((bad >> key) & 1)
-              for (int c = part; c < HD / 8; c += n_parts) vrow[(c >> 3) * (TR_KEYS * 8) + (c & 7)] = make_uint4(0, 0, 0, 0);
-            fence_async_shared();
-            tr_bar(tile_bar, tile_threads);
-            if (tile_tid == 0) *(volatile unsigned long long*)bad_word = 0;
-          }
+          bad = tree_look_through<HD>(reinterpret_cast<uint4*>(S.v[s]), &S.bad[ROWS2 ? 0 : h], tile_bar, tile_threads, tile_tid, ok);
         }
-        const bool first = !any_tile;
-        any_tile = true;
-        last = it;
-        // P V of this half's tile before has read P and is in O.  Warps without rows wait for it too: were they to run
-        // ahead, their word for this tile would be counted as one for the tile before
+        // P V of this half's tile before is in O
         auto wait_before = [&]() {
-          const uint32_t before = it - (ROWS2 ? 1 : 2);
+          const uint32_t before = it - STEP;
           if (ok && !__all_sync(0xffffffffu, mbar_wait(&S.pv_full[h][before % STAGES], (before / STAGES) & 1, abort_flag))) {
             if (lane == 0) TR_FAIL(508);
             ok = false;
           }
         };
-        if (ok && active && warp_active) {
+        if (ok && warp_active) {
           tc_fence_after();
-          float sc[32], sd[32];                          // this thread's half of the keys, and the other half
-          tmem_ld32f(lane_addr + b * TR_KEYS + half * 32, sc);
-          tmem_ld32f(lane_addr + b * TR_KEYS + (half ^ 1) * 32, sd);
-          tmem_ld_wait();
-          float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+          float sc[TR_KEYS];
+          {
+            uint32_t (&r)[TR_KEYS] = reinterpret_cast<uint32_t (&)[TR_KEYS]>(sc);
+            tmem_ld32(lane_addr + b * TR_KEYS, reinterpret_cast<uint32_t (&)[32]>(r[0]));
+            tmem_ld32(lane_addr + b * TR_KEYS + 32, reinterpret_cast<uint32_t (&)[32]>(r[32]));
+            tmem_ld_wait();
+          }
           if (needs_mask) {
-            const uint32_t vs = (uint32_t)(vis >> (half * 32)), vt = (uint32_t)(vis >> ((half ^ 1) * 32));
+            const uint32_t v0 = (uint32_t)vis, v1 = (uint32_t)(vis >> 32);
 #pragma unroll
             for (int e = 0; e < 32; e++) {
-              sc[e] = (vs >> e) & 1 ? sc[e] : -INFINITY;
-              sd[e] = (vt >> e) & 1 ? sd[e] : -INFINITY;
-              mx[e & 3] = tr_max3(mx[e & 3], sc[e], sd[e]);
+              sc[e] = (v0 >> e) & 1 ? sc[e] : -INFINITY;
+              sc[32 + e] = (v1 >> e) & 1 ? sc[32 + e] : -INFINITY;
             }
-          } else {
-#pragma unroll
-            for (int e = 0; e < 32; e++) mx[e & 3] = tr_max3(mx[e & 3], sc[e], sd[e]);
           }
+          // (four running maxima: one chain would cost more time than everything else a thread does per tile)
+          float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+          for (int e = 0; e < TR_KEYS; e += 8)
+#pragma unroll
+            for (int x = 0; x < 4; x++) mx[x] = tr_max3(mx[x], sc[e + 2 * x], sc[e + 2 * x + 1]);
           const float tile_max = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * to_log2;     // scale > 0
-          // the reference moves only when the row's maximum has outgrown it by more than 8 (a factor 256); both threads
-          // of a row see the same numbers and decide alike
+          // the reference moves only when the row's maximum has outgrown it by more than 8 (a factor 256)
           const bool grow = tile_max > m_ref + 8.0f;
           const float corr = grow ? tr_exp2(m_ref - tile_max) : 1.0f;
           if (grow) m_ref = tile_max;
           const float m_use = (m_ref == -INFINITY) ? 0.f : m_ref;
-          uint32_t packed[16];
-          float sum0 = 0.f, sum1 = 0.f;
+          uint32_t packed[TR_KEYS / 2];
+          float sum[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-          for (int e = 0; e < 32; e += 2) {
+          for (int e = 0; e < TR_KEYS; e += 2) {
             const float p0 = tr_exp2(fmaf(sc[e], to_log2, -m_use));
             const float p1 = tr_exp2(fmaf(sc[e + 1], to_log2, -m_use));
             // to bfloat16 by dropping the low mantissa bits; the sums run over the same shortened values, so the common
             // part of the shortening divides out and what stays is as wide as round-to-nearest's error
             const uint32_t u = __byte_perm(__float_as_uint(p0), __float_as_uint(p1), 0x7632);
-            sum0 += __uint_as_float(u << 16);
-            sum1 += __uint_as_float(u & 0xffff0000u);
+            sum[e & 2] += __uint_as_float(u << 16);
+            sum[(e & 2) + 1] += __uint_as_float(u & 0xffff0000u);
             packed[e >> 1] = u;
           }
-          if (!first) {
-            wait_before();
-            if (ok && __any_sync(0xffffffffu, grow)) {
-              tc_fence_after();
-#pragma unroll
-              for (int c = 0; c < OD; c += 32) {
-                uint32_t r[32];
-                tmem_ld32(o_addr + c, r);
-                tmem_ld_wait();
-#pragma unroll
-                for (int e = 0; e < 32; e++) r[e] = __float_as_uint(__uint_as_float(r[e]) * corr);
-                tmem_st32(o_addr + c, r);
-              }
-              tmem_st_wait();
-            }
-          }
-          l = l * corr + (sum0 + sum1);
-          if (bad && ok) {                               // what values that are not finite give to the rows that see them
+          const bool move = __any_sync(0xffffffffu, grow);
+          if (!first && (move || bad)) wait_before();
+          if (ok && !first && move) {
             tc_fence_after();
-            for (int c = 0; c < OD; c += 32) {
+#pragma unroll 1
+            for (int c = 0; c < HD; c += 32) {
               uint32_t r[32];
-              if (!first) { tmem_ld32(o_addr + c, r); tmem_ld_wait(); }
-              else {
+              tmem_ld32(o_addr + c, r);
+              tmem_ld_wait();
 #pragma unroll
-                for (int e = 0; e < 32; e++) r[e] = 0;
-              }
-              for (int k = 0; k < 64; k++) {
-                if (!((bad >> k) & 1)) continue;
-                const float x = tmem_ld1f(lane_addr + b * TR_KEYS + k);
-                const bool sees = (vis >> k) & 1;
-                const float p = tr_exp2(fmaf(x, to_log2, -m_use));
-                const bf16* vp = reinterpret_cast<const bf16*>(P.v_cache) +
-                                 (((size_t)(page_ok ? pg : 0) * P.n_kv + run.kvh) * TR_KEYS + k) * HD + half * OD + c;
-#pragma unroll
-                for (int e = 0; e < 32; e++)
-                  if (sees) r[e] = __float_as_uint(fmaf(p, ld_fresh(vp + e), __uint_as_float(r[e])));
-              }
+              for (int e = 0; e < 32; e++) r[e] = __float_as_uint(__uint_as_float(r[e]) * corr);
               tmem_st32(o_addr + c, r);
             }
+          }
+          l = fmaf(l, corr, (sum[0] + sum[1]) + (sum[2] + sum[3]));
+          if (bad && ok) {                               // what values that are not finite give to the rows that see them
+            tc_fence_after();
             tmem_st_wait();
+            tree_add_bad<HD>(bad, vis, lane_addr + b * TR_KEYS, o_addr, to_log2, m_use,
+                             reinterpret_cast<const bf16*>(P.v_cache) +
+                                 ((size_t)(page_ok ? pg : 0) * P.n_kv + run.kvh) * TR_KEYS * HD, first);
           }
-          if (ok) {
-            uint8_t* prow = reinterpret_cast<uint8_t*>(S.p[h]) + row * 128;
-#pragma unroll
-            for (int c = 0; c < 4; c++) {
-              const int chunk = half * 4 + c;
-              *reinterpret_cast<uint4*>(prow + ((chunk ^ (row & 7)) << 4)) =
-                  make_uint4(packed[4 * c], packed[4 * c + 1], packed[4 * c + 2], packed[4 * c + 3]);
-            }
-          }
-        } else if (!first) {
-          wait_before();
+          tmem_st32(lane_addr + b * TR_KEYS, packed);    // over the scores
+          tmem_st_wait();
         }
-        if (first && sw % TR_SOFTMAX_WARPS == 0 && lane == 0) S.o_ready[h] = bad != 0;   // (`bad` is the same in all of them)
-        fence_async_shared();
+        if (first && quarter == 0 && lane == 0) S.o_ready[h] = bad != 0;   // (`bad` is the same in all of them)
         tc_fence_before();
         __syncwarp();
-        if (ok && lane == 0) mbar_arrive(&S.p_full[h]);
+        if (ok && lane == 0) mbar_arrive(&S.p_full[h][b]);
         i++;
       }
-      it = it_end;
       // ---- the run is over
-      if (ok && any_tile && !__all_sync(0xffffffffu, mbar_wait(&S.pv_full[h][last % STAGES], (last / STAGES) & 1, abort_flag))) {
-        if (lane == 0) TR_FAIL(508);
-        ok = false;
+      if (it_mine < it_end) {
+        const uint32_t last = it - STEP;
+        if (ok && !__all_sync(0xffffffffu, mbar_wait(&S.pv_full[h][last % STAGES], (last / STAGES) & 1, abort_flag))) {
+          if (lane == 0) TR_FAIL(508);
+          ok = false;
+        }
       }
-      tc_fence_after();
-      float* l_buf = reinterpret_cast<float*>(S.p[h]);   // [2][128] sums, [128] maxima (P is no longer read)
-      l_buf[half * 128 + row] = l;
-      if (half == 0) l_buf[256 + row] = m_ref;
+      it = it_end;
       const bool whole = run.from_start && run.to_end;
       const int slot = 2 * blockIdx.x + (run.holds_u0 ? 0 : 1);
       bf16* out_row = reinterpret_cast<bf16*>(P.out) + (size_t)token * P.ldo + (size_t)(run.kvh * gs + head) * HD;
+      tc_fence_after();
       if (ROWS2) {
-        tr_bar(2 + h, TR_SOFTMAX_WARPS * 32);
         if (ok && !*abort_flag && warp_active) {
-          const float L = l_buf[row] + l_buf[128 + row];
-          const float inv = L > 0.f ? 1.0f / L : (L == 0.f ? 0.f : L);   // (a sum that is no number stays one)
-          float* po = P.part_o + ((size_t)slot * 256 + h * 128 + row) * HD + half * OD;
-#pragma unroll
-          for (int c = 0; c < OD; c += 32) {
+          const float inv = 1.0f / l;
+          float* po = P.part_o + ((size_t)slot * 256 + h * 128 + row) * HD;
+#pragma unroll 1
+          for (int c = 0; c < HD; c += 32) {
             float o[32];
             tmem_ld32f(o_addr + c, o);                   // (all lanes take part; only valid rows store)
             tmem_ld_wait();
@@ -661,11 +703,8 @@ attention_tree_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
                 uint4 w;
                 uint32_t* wp = reinterpret_cast<uint32_t*>(&w);
 #pragma unroll
-                for (int x = 0; x < 4; x++) {
-                  __nv_bfloat162 a = __floats2bfloat162_rn(L == 0.f ? 0.f : o[e + 2 * x] * inv, L == 0.f ? 0.f : o[e + 2 * x + 1] * inv);
-                  wp[x] = *reinterpret_cast<uint32_t*>(&a);
-                }
-                *reinterpret_cast<uint4*>(out_row + half * OD + c + e) = w;
+                for (int x = 0; x < 4; x++) wp[x] = tr_pack(l, o[e + 2 * x] * inv, o[e + 2 * x + 1] * inv);
+                *reinterpret_cast<uint4*>(out_row + c + e) = w;
               }
             } else if (valid) {
 #pragma unroll
@@ -673,62 +712,62 @@ attention_tree_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
                 *reinterpret_cast<float4*>(po + c + e) = make_float4(o[e], o[e + 1], o[e + 2], o[e + 3]);
             }
           }
-          if (valid && !whole && half == 0) P.part_ml[(size_t)slot * 256 + h * 128 + row] = make_float2(m_ref, L);
+          if (valid && !whole) P.part_ml[(size_t)slot * 256 + h * 128 + row] = make_float2(m_ref, l);
         }
         tc_fence_before();
-        tr_bar(2 + h, TR_SOFTMAX_WARPS * 32);            // the buffer is P again
       } else {
-        // both halves hold the same rows: a quarter of the dims for each of a row's four threads
+        // both halves hold the same rows: half of the dims for each of a row's two threads
+        S.ml[h][row] = make_float2(m_ref, l);
         tc_fence_before();
         tr_bar(3, 2 * TR_SOFTMAX_WARPS * 32);
         tc_fence_after();
         if (ok && !*abort_flag && warp_active) {
-          const float* a = reinterpret_cast<const float*>(S.p[0]);
-          const float* c = reinterpret_cast<const float*>(S.p[1]);
-          const float m0 = a[256 + row], m1 = c[256 + row];
-          const float M = fmaxf(m0, m1), Mu = M == -INFINITY ? 0.f : M;
-          const float f0 = tr_exp2(m0 - Mu), f1 = tr_exp2(m1 - Mu);
-          const float L = f0 * (a[row] + a[128 + row]) + f1 * (c[row] + c[128 + row]);
-          const float inv = L > 0.f ? 1.0f / L : (L == 0.f ? 0.f : L);
-          // a half that had no page in this run left its accumulator alone
+          const float2 a0 = S.ml[0][row], a1 = S.ml[1][row];
+          const float M = fmaxf(a0.x, a1.x), Mu = M == -INFINITY ? 0.f : M;
+          const float f0 = tr_exp2(a0.x - Mu), f1 = tr_exp2(a1.x - Mu);
+          const float L = f0 * a0.y + f1 * a1.y, inv = 1.0f / L;
+          // a half that had no page in this run left its accumulator alone; one that saw no key of the row has nothing to
+          // give, whatever lies in it
           const bool has0 = run.n > 1 || (it_first & 1) == 0, has1 = run.n > 1 || (it_first & 1) == 1;
-          constexpr int QD = HD / 4;
-          const int d0 = (2 * h + half) * QD;
-          float o[QD];
+          float* po = P.part_o + ((size_t)slot * 128 + row) * HD;
+#pragma unroll 1
+          for (int c = h * (HD / 2); c < (h + 1) * (HD / 2); c += 32) {
+            float o[32];
+            uint32_t r[32];
 #pragma unroll
-          for (int x = 0; x < QD; x += 16) {
-            uint32_t r0[16], r1[16];
-            if (has0) { tmem_ld16(lane_base + COL_PV + d0 + x, r0); }
-            if (has1) { tmem_ld16(lane_base + 256 + COL_PV + d0 + x, r1); }
-            tmem_ld_wait();
+            for (int e = 0; e < 32; e++) o[e] = 0.f;
+            if (has0) {
+              tmem_ld32(lane_base + COL_PV + c, r);
+              tmem_ld_wait();
+              if (a0.x != -INFINITY) {
 #pragma unroll
-            for (int e = 0; e < 16; e++) {
-              // (a half that saw no key of the row has nothing but zeros to give, whatever lies in them)
-              float y = 0.f;
-              if (has0 && m0 != -INFINITY) y = f0 * __uint_as_float(r0[e]);
-              if (has1 && m1 != -INFINITY) y = fmaf(f1, __uint_as_float(r1[e]), y);
-              o[x + e] = y;
-            }
-          }
-          if (valid && whole) {
-#pragma unroll
-            for (int e = 0; e < QD; e += 8) {
-              uint4 w;
-              uint32_t* wp = reinterpret_cast<uint32_t*>(&w);
-#pragma unroll
-              for (int x = 0; x < 4; x++) {
-                __nv_bfloat162 z = __floats2bfloat162_rn(L == 0.f ? 0.f : o[e + 2 * x] * inv, L == 0.f ? 0.f : o[e + 2 * x + 1] * inv);
-                wp[x] = *reinterpret_cast<uint32_t*>(&z);
+                for (int e = 0; e < 32; e++) o[e] = f0 * __uint_as_float(r[e]);
               }
-              *reinterpret_cast<uint4*>(out_row + d0 + e) = w;
             }
-          } else if (valid) {
-            float* po = P.part_o + ((size_t)slot * 128 + row) * HD + d0;
+            if (has1) {
+              tmem_ld32(lane_base + 256 + COL_PV + c, r);
+              tmem_ld_wait();
+              if (a1.x != -INFINITY) {
 #pragma unroll
-            for (int e = 0; e < QD; e += 4)
-              *reinterpret_cast<float4*>(po + e) = make_float4(o[e], o[e + 1], o[e + 2], o[e + 3]);
-            if (d0 == 0) P.part_ml[(size_t)slot * 128 + row] = make_float2(M, L);
+                for (int e = 0; e < 32; e++) o[e] = fmaf(f1, __uint_as_float(r[e]), o[e]);
+              }
+            }
+            if (valid && whole) {
+#pragma unroll
+              for (int e = 0; e < 32; e += 8) {
+                uint4 w;
+                uint32_t* wp = reinterpret_cast<uint32_t*>(&w);
+#pragma unroll
+                for (int x = 0; x < 4; x++) wp[x] = tr_pack(L, o[e + 2 * x] * inv, o[e + 2 * x + 1] * inv);
+                *reinterpret_cast<uint4*>(out_row + c + e) = w;
+              }
+            } else if (valid) {
+#pragma unroll
+              for (int e = 0; e < 32; e += 4)
+                *reinterpret_cast<float4*>(po + c + e) = make_float4(o[e], o[e + 1], o[e + 2], o[e + 3]);
+            }
           }
+          if (valid && !whole && h == 0) P.part_ml[(size_t)slot * 128 + row] = make_float2(M, L);
         }
         tc_fence_before();
         tr_bar(3, 2 * TR_SOFTMAX_WARPS * 32);
@@ -765,7 +804,7 @@ attention_tree_simple_kernel(const TreeParams P) {
   const int tid = threadIdx.x, ty = tid >> 4, tx = tid & 15;
   const float scale_log2 = P.scale * 1.4426950408889634f;
   TreeCursor cur;
-  cur.begin(P, start.u0, start.u1, start.b, start.item, start.off);
+  cur.begin(P, start.n_units, start.b, start.item, start.off);
   TreeRun run;
   while (cur.next(P, run)) {
     const TreeSeq& sq = run.s;

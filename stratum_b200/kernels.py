@@ -495,7 +495,7 @@ def check_status() -> None:
         _status_word.zero_()
         where = {101: "the TMA producer waiting for a free stage", 102: "the MMA warp waiting for a free accumulator",
                  103: "the MMA warp waiting for a loaded stage", 104: "the epilogue waiting for an accumulator",
-                 **{c: "the attention of drafted tokens" for c in (501, 502, 503, 505, 506, 507, 508, 509, 510)},
+                 **{c: "the attention of drafted tokens" for c in (501, 502, 503, 504, 505, 506, 507, 508, 509, 510)},
                  431: "the resident decode step's ring (a free stage)", 432: "the resident decode step's ring (a filled stage)",
                  **{c: "a block of the resident decode step waiting for the others" for c in (401, 402, 403, 405, 411, 421)}}
         raise KernelError(f"a device-side wait ran out in {where.get(code, f'code {code}')}; results are invalid")
