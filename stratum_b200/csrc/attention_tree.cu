@@ -59,8 +59,9 @@ struct TreeParams {
 
 // What CTA c's stretch begins in, for the merge.
 struct TreeCut {
-  long long item_begin, total;             // the item's first unit; units in all
-  int b, kvh, rt, n_pages;
+  long long u0, item_begin;                // the stretch's first unit, the first unit of the item that holds it
+  int n_pages, kvh;                        // units of the item (0: the stretch is empty); its kv head,
+  int flat0, n_rows;                       // its first row (token of the batch * gs + head), its rows
 };
 
 struct TreeSeq {                           // a sequence's share of the list
@@ -173,13 +174,16 @@ __device__ __forceinline__ TreeStart tree_start(const TreeParams& P, long long* 
     const long long r = u0 - sums[lo];
     t.b = lo; t.item = (int)(r / s.n_pages); t.off = (int)(r % s.n_pages);
     if (threadIdx.x == 0) {
+      const int rt = t.item % s.n_tiles;
       TreeCut cut;
-      cut.item_begin = u0 - t.off; cut.total = T;
-      cut.b = lo; cut.kvh = t.item / s.n_tiles; cut.rt = t.item % s.n_tiles; cut.n_pages = s.n_pages;
+      cut.u0 = u0; cut.item_begin = u0 - t.off;
+      cut.n_pages = s.n_pages; cut.kvh = t.item / s.n_tiles;
+      cut.flat0 = s.row0 * P.gs + rt * P.rows_per_tile;
+      cut.n_rows = min(s.n_new * P.gs - rt * P.rows_per_tile, P.rows_per_tile);
       P.cut[c] = cut;
     }
   } else if (threadIdx.x == 0) {
-    P.cut[c].total = T; P.cut[c].n_pages = 0;
+    P.cut[c].u0 = u0; P.cut[c].n_pages = 0;
   }
   return t;
 }
@@ -783,34 +787,63 @@ attention_tree_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
 }
 
 // ================================================================ any head size, CUDA cores
-// 256 threads take 32 rows of a (sequence, kv head) through pages of 64 keys held in shared memory as float32.  Thread
-// (ty, tx) owns rows 2 ty and 2 ty + 1: the scores of keys tx, tx + 16, .., and the output dims 4 (tx + 16 j) .. + 3; the
+// 256 threads take 16 R rows of a (sequence, kv head) through pages of 64 keys held in shared memory as float32.  Thread
+// (ty, tx) owns rows R ty .. R ty + R - 1: the scores of keys tx, tx + 16, .., and the output dims 4 (tx + 16 j) .. + 3; the
 // running maximum and sum of a row are kept by its sixteen threads alike.  Everything is float32, exponentials included.
+// R = 4 (a tree of more than 32 rows) reads shared memory three times for every sixteen multiplications that two rows'
+// threads would read it for five times, and shared memory is what bounds this kernel.  float32 pages come by cp.async: the
+// next keys while this page's values are summed, the next values while the next scores are computed.
 #define TG_THREADS 256
-#define TG_ROWS 32
 
-template <typename T, int NC>
+__device__ __forceinline__ void cp_async16(void* dst, const void* src) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(dst)), "l"(src) : "memory");
+}
+__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N> __device__ __forceinline__ void cp_async_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
+
+template <typename T, int NC, int R>
 __global__ void __launch_bounds__(TG_THREADS)
 attention_tree_simple_kernel(const TreeParams P) {
   extern __shared__ __align__(16) float tg_smem[];
+  constexpr int ROWS = 16 * R, PK = TR_KEYS + 4;
   const int hd = P.head_dim, hp = (hd + 3) & ~3, pitch = hp + 4;
-  float* qs = tg_smem;                             // [32][pitch]
-  float* ks = qs + TG_ROWS * pitch;                // [64][pitch]
+  float* qs = tg_smem;                             // [ROWS][pitch]
+  float* ks = qs + ROWS * pitch;                   // [64][pitch]
   float* vs = ks + TR_KEYS * pitch;                // [64][hp]
-  float* ps = vs + TR_KEYS * hp;                   // [32][64]
+  float* ps = vs + TR_KEYS * hp;                   // [ROWS][PK]
   pdl_wait();
   const TreeStart start = tree_start(P, reinterpret_cast<long long*>(tg_smem));
-  __syncthreads();
   const int tid = threadIdx.x, ty = tid >> 4, tx = tid & 15;
   const float scale_log2 = P.scale * 1.4426950408889634f;
+  const bool direct = sizeof(T) == 4 && hd == hp && (((uintptr_t)P.k_cache | (uintptr_t)P.v_cache) & 15) == 0;
+  // a page's keys (or values) into rows of `to` that lie `step` apart; nothing of a page outside the pool
+  auto fetch = [&](const void* cache, int pg, int kvh, float* to, int step) {
+    if ((unsigned)pg < (unsigned)P.n_pages) {
+      const T* from = reinterpret_cast<const T*>(cache) + ((size_t)pg * P.n_kv + kvh) * TR_KEYS * hd;
+      if (direct) {
+        const int c4 = hp >> 2;
+        for (int e = tid; e < TR_KEYS * c4; e += TG_THREADS) cp_async16(to + (e / c4) * step + 4 * (e % c4), reinterpret_cast<const float4*>(from) + e);
+      } else {
+        for (int e = tid; e < TR_KEYS * hp; e += TG_THREADS) {
+          const int r = e / hp, d = e % hp;
+          to[r * step + d] = d < hd ? ld_fresh(from + (size_t)r * hd + d) : 0.f;
+        }
+      }
+    }
+    cp_async_commit();
+  };
   TreeCursor cur;
   cur.begin(P, start.n_units, start.b, start.item, start.off);
   TreeRun run;
   while (cur.next(P, run)) {
     const TreeSeq& sq = run.s;
-    const int r0 = run.rt * TG_ROWS, n_rows = min(sq.n_new * P.gs - r0, TG_ROWS);
-    __syncthreads();                               // (the run before may still be reading)
-    for (int e = tid; e < TG_ROWS * hp; e += TG_THREADS) {
+    const int r0 = run.rt * ROWS, n_rows = min(sq.n_new * P.gs - r0, ROWS);
+    const int* bt = P.block_table + (size_t)run.b * P.bt_stride + run.page0;
+    __syncthreads();                               // (the run before, or the start, may still be reading)
+    int pg = bt[0];
+    fetch(P.k_cache, pg, run.kvh, ks, pitch);
+    fetch(P.v_cache, pg, run.kvh, vs, hp);
+    for (int e = tid; e < ROWS * hp; e += TG_THREADS) {
       const int r = e / hp, d = e % hp;
       float x = 0.f;
       if (r < n_rows && d < hd)
@@ -818,13 +851,15 @@ attention_tree_simple_kernel(const TreeParams P) {
                      (size_t)(run.kvh * P.gs + (r0 + r) % P.gs) * hd + d);
       qs[r * pitch + d] = x;
     }
-    int token[2], lo[2], lo_max = 0;
-    bool valid[2];
-    float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
-    float4 acc[2][NC];
+    const bool busy = 2 * R * (tid >> 5) < n_rows;   // (warps without rows load and wait with the others)
+    int token[R], lo[R], lo_max = 0;
+    bool valid[R];
+    float m[R], l[R];
+    float4 acc[R][NC];
 #pragma unroll
-    for (int e = 0; e < 2; e++) {
-      const int r = 2 * ty + e;
+    for (int e = 0; e < R; e++) {
+      const int r = R * ty + e;
+      m[e] = -INFINITY; l[e] = 0.f;
       valid[e] = r < n_rows;
       token[e] = sq.row0 + (valid[e] ? (r0 + r) / P.gs : 0);
       lo[e] = (P.window > 0 && valid[e]) ? max(P.token_pos[token[e]] - P.window + 1, 0) : 0;
@@ -833,62 +868,44 @@ attention_tree_simple_kernel(const TreeParams P) {
       for (int j = 0; j < NC; j++) acc[e][j] = make_float4(0.f, 0.f, 0.f, 0.f);
     }
     for (int i = 0; i < run.n; i++) {
-      const int page = run.page0 + i, key0 = page * TR_KEYS;
-      const int pg = P.block_table[(size_t)run.b * P.bt_stride + page];
+      const int key0 = (run.page0 + i) * TR_KEYS;
       const bool page_ok = (unsigned)pg < (unsigned)P.n_pages;
-      __syncthreads();                             // the page before is read (and the queries are in place)
-      bool odd = false;
-      if (page_ok) {
-        const size_t off = ((size_t)pg * P.n_kv + run.kvh) * TR_KEYS * hd;
-        const T* kp = reinterpret_cast<const T*>(P.k_cache) + off;
-        const T* vp = reinterpret_cast<const T*>(P.v_cache) + off;
-        if (sizeof(T) == 4 && hd == hp && (((uintptr_t)kp | (uintptr_t)vp) & 15) == 0) {
-          const int c4 = hp >> 2;
-          for (int e = tid; e < TR_KEYS * c4; e += TG_THREADS) {
-            const int r = e / c4, c = e % c4;
-            const float4 a = ld_fresh(reinterpret_cast<const float4*>(kp) + e);
-            const float4 b = ld_fresh(reinterpret_cast<const float4*>(vp) + e);
-            *reinterpret_cast<float4*>(ks + r * pitch + 4 * c) = a;
-            *reinterpret_cast<float4*>(vs + r * hp + 4 * c) = b;
-            odd = odd || !(isfinite(b.x) && isfinite(b.y) && isfinite(b.z) && isfinite(b.w));
-          }
-        } else {
-          for (int e = tid; e < TR_KEYS * hp; e += TG_THREADS) {
-            const int r = e / hp, d = e % hp;
-            const float a = d < hd ? ld_fresh(kp + (size_t)r * hd + d) : 0.f;
-            const float b = d < hd ? ld_fresh(vp + (size_t)r * hd + d) : 0.f;
-            ks[r * pitch + d] = a;
-            vs[r * hp + d] = b;
-            odd = odd || !isfinite(b);
-          }
-        }
-      }
-      odd = __syncthreads_or(odd);
-      if (!page_ok) continue;                      // (nobody sees a page outside the pool)
-      // scores
-      float s[2][4];
+      const int pg_next = i + 1 < run.n ? bt[i + 1] : -1;
+      cp_async_wait<1>();                          // this page's keys are here (its values may be on their way)
+      __syncthreads();
+      float s[R][4];
 #pragma unroll
-      for (int e = 0; e < 2; e++)
+      for (int e = 0; e < R; e++)
 #pragma unroll
         for (int j = 0; j < 4; j++) s[e][j] = 0.f;
-      const float* q0 = qs + 2 * ty * pitch;
-      const float* k0 = ks + tx * pitch;
-      for (int d = 0; d < hp; d += 4) {
-        const float4 a = *reinterpret_cast<const float4*>(q0 + d), b = *reinterpret_cast<const float4*>(q0 + pitch + d);
+      if (page_ok && busy) {
+        const float* q0 = qs + R * ty * pitch;
+        const float* k0 = ks + tx * pitch;
+#pragma unroll 2
+        for (int d = 0; d < hp; d += 4) {
+          float4 a[R];
 #pragma unroll
-        for (int j = 0; j < 4; j++) {
-          const float4 x = *reinterpret_cast<const float4*>(k0 + 16 * j * pitch + d);
-          s[0][j] = fmaf(a.x, x.x, s[0][j]); s[0][j] = fmaf(a.y, x.y, s[0][j]);
-          s[0][j] = fmaf(a.z, x.z, s[0][j]); s[0][j] = fmaf(a.w, x.w, s[0][j]);
-          s[1][j] = fmaf(b.x, x.x, s[1][j]); s[1][j] = fmaf(b.y, x.y, s[1][j]);
-          s[1][j] = fmaf(b.z, x.z, s[1][j]); s[1][j] = fmaf(b.w, x.w, s[1][j]);
+          for (int e = 0; e < R; e++) a[e] = *reinterpret_cast<const float4*>(q0 + e * pitch + d);
+#pragma unroll
+          for (int j = 0; j < 4; j++) {
+            const float4 x = *reinterpret_cast<const float4*>(k0 + 16 * j * pitch + d);
+#pragma unroll
+            for (int e = 0; e < R; e++) {
+              s[e][j] = fmaf(a[e].x, x.x, s[e][j]); s[e][j] = fmaf(a[e].y, x.y, s[e][j]);
+              s[e][j] = fmaf(a[e].z, x.z, s[e][j]); s[e][j] = fmaf(a[e].w, x.w, s[e][j]);
+            }
+          }
         }
       }
-      unsigned long long vis[2] = {~0ull, ~0ull};
-      const bool masked = key0 + TR_KEYS > sq.base || key0 < lo_max;
+      __syncthreads();                             // the keys are read
+      if (i + 1 < run.n) fetch(P.k_cache, pg_next, run.kvh, ks, pitch); else cp_async_commit();
+      unsigned long long vis[R];
+      const bool masked = key0 + TR_KEYS > sq.base || key0 < lo_max || !page_ok;
 #pragma unroll
-      for (int e = 0; e < 2; e++) {
-        if (masked) vis[e] = valid[e] ? tree_visible(P, sq, token[e], lo[e], key0, true) : 0;
+      for (int e = 0; e < R; e++) {
+        vis[e] = ~0ull;
+        if (!busy) continue;
+        if (masked) vis[e] = valid[e] ? tree_visible(P, sq, token[e], lo[e], key0, page_ok) : 0;
         float mx = -INFINITY;
 #pragma unroll
         for (int j = 0; j < 4; j++) {
@@ -905,7 +922,7 @@ attention_tree_simple_kernel(const TreeParams P) {
         for (int j = 0; j < 4; j++) {
           const float p = exp2f(s[e][j] - m_use);
           sum += p;
-          ps[(2 * ty + e) * TR_KEYS + tx + 16 * j] = p;
+          ps[(R * ty + e) * PK + tx + 16 * j] = p;
         }
 #pragma unroll
         for (int d = 1; d < 16; d <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
@@ -913,42 +930,67 @@ attention_tree_simple_kernel(const TreeParams P) {
 #pragma unroll
         for (int j = 0; j < NC; j++) { acc[e][j].x *= corr; acc[e][j].y *= corr; acc[e][j].z *= corr; acc[e][j].w *= corr; }
       }
-      __syncwarp();                                // a row's probabilities come from its own warp
-      const float* p0 = ps + 2 * ty * TR_KEYS;
-      auto add = [&](int k, bool see0, bool see1) {
-        const float a = p0[k], b = p0[TR_KEYS + k];
+      cp_async_wait<1>();                          // its values too
+      __syncthreads();
+      bool odd = false;
+      if (__syncthreads_or(masked)) {              // zero times an infinity is not zero: are there any among the values?
+        if (page_ok)
+          for (int e = tid; e < TR_KEYS * hp; e += TG_THREADS) odd = odd || !isfinite(vs[e]);
+        odd = __syncthreads_or(odd);
+      }
+      const float* p0 = ps + R * ty * PK;          // (a row's probabilities come from its own warp)
+      if (!page_ok || !busy) {
+      } else if (odd) {                            // then masked keys are left out, one by one
+        for (int k = 0; k < TR_KEYS; k++) {
 #pragma unroll
-        for (int j = 0; j < NC; j++) {
-          const int d = 4 * (tx + 16 * j);
-          if (NC * 64 == hp || d < hp) {
+          for (int j = 0; j < NC; j++) {
+            const int d = 4 * (tx + 16 * j);
+            if (d >= hp) continue;
             const float4 x = *reinterpret_cast<const float4*>(vs + k * hp + d);
-            if (see0) {
-              acc[0][j].x = fmaf(a, x.x, acc[0][j].x); acc[0][j].y = fmaf(a, x.y, acc[0][j].y);
-              acc[0][j].z = fmaf(a, x.z, acc[0][j].z); acc[0][j].w = fmaf(a, x.w, acc[0][j].w);
-            }
-            if (see1) {
-              acc[1][j].x = fmaf(b, x.x, acc[1][j].x); acc[1][j].y = fmaf(b, x.y, acc[1][j].y);
-              acc[1][j].z = fmaf(b, x.z, acc[1][j].z); acc[1][j].w = fmaf(b, x.w, acc[1][j].w);
+#pragma unroll
+            for (int e = 0; e < R; e++) {
+              if (!((vis[e] >> k) & 1)) continue;
+              const float p = p0[e * PK + k];
+              acc[e][j].x = fmaf(p, x.x, acc[e][j].x); acc[e][j].y = fmaf(p, x.y, acc[e][j].y);
+              acc[e][j].z = fmaf(p, x.z, acc[e][j].z); acc[e][j].w = fmaf(p, x.w, acc[e][j].w);
             }
           }
         }
-      };
-      if (odd && masked) {                         // zero times an infinity is not zero: masked keys are left out
-        for (int k = 0; k < TR_KEYS; k++) add(k, (vis[0] >> k) & 1, (vis[1] >> k) & 1);
       } else {
-#pragma unroll 4
-        for (int k = 0; k < TR_KEYS; k++) add(k, true, true);
+#pragma unroll 1
+        for (int k = 0; k < TR_KEYS; k += 4) {
+          float4 p[R];
+#pragma unroll
+          for (int e = 0; e < R; e++) p[e] = *reinterpret_cast<const float4*>(p0 + e * PK + k);
+#pragma unroll
+          for (int kk = 0; kk < 4; kk++)
+#pragma unroll
+            for (int j = 0; j < NC; j++) {
+              const int d = 4 * (tx + 16 * j);
+              if (NC * 64 != hp && d >= hp) continue;
+              const float4 x = *reinterpret_cast<const float4*>(vs + (k + kk) * hp + d);
+#pragma unroll
+              for (int e = 0; e < R; e++) {
+                const float w = kk == 0 ? p[e].x : kk == 1 ? p[e].y : kk == 2 ? p[e].z : p[e].w;
+                acc[e][j].x = fmaf(w, x.x, acc[e][j].x); acc[e][j].y = fmaf(w, x.y, acc[e][j].y);
+                acc[e][j].z = fmaf(w, x.z, acc[e][j].z); acc[e][j].w = fmaf(w, x.w, acc[e][j].w);
+              }
+            }
+        }
       }
+      __syncthreads();                             // the values are read
+      pg = pg_next;
+      if (i + 1 < run.n) fetch(P.v_cache, pg, run.kvh, vs, hp); else cp_async_commit();
     }
     const bool whole = run.from_start && run.to_end;
     const int slot = 2 * blockIdx.x + (run.holds_u0 ? 0 : 1);
 #pragma unroll
-    for (int e = 0; e < 2; e++) {
+    for (int e = 0; e < R; e++) {
       if (!valid[e]) continue;
-      const int r = 2 * ty + e;
-      const float inv = l[e] == 0.f ? 0.f : 1.0f / l[e];
+      const int r = R * ty + e;
+      const float inv = 1.0f / l[e];
       T* op = reinterpret_cast<T*>(P.out) + (size_t)token[e] * P.ldo + (size_t)(run.kvh * P.gs + (r0 + r) % P.gs) * hd;
-      float* po = P.part_o + ((size_t)slot * TG_ROWS + r) * hp;
+      float* po = P.part_o + ((size_t)slot * ROWS + r) * hp;
 #pragma unroll
       for (int j = 0; j < NC; j++) {
         const int d = 4 * (tx + 16 * j);
@@ -961,85 +1003,110 @@ attention_tree_simple_kernel(const TreeParams P) {
           *reinterpret_cast<float4*>(po + d) = acc[e][j];
         }
       }
-      if (!whole && tx == 0) P.part_ml[(size_t)slot * TG_ROWS + r] = make_float2(m[e], l[e]);
+      if (!whole && tx == 0) P.part_ml[(size_t)slot * ROWS + r] = make_float2(m[e], l[e]);
     }
   }
+  cp_async_wait<0>();
 }
 
 // ================================================================ the pieces of what several CTAs saw
-// Block (c, y): rows 8 y .. 8 y + 7 of the item that the cut between CTAs c and c + 1 goes through, where it is the first
-// one to do so.  A warp takes a row; its lanes first fetch the pieces' maxima and sums.
-template <typename T>
+// Block (c, y): rows 32 y .. 32 y + 31 of the item that the cut between CTAs c and c + 1 goes through, where it is the first
+// one to do so; a warp takes four rows at a time, so that the pieces of all four are on their way together.  The lanes look
+// up where the stretches begin and fetch the pieces' maxima and sums.
+#define TM_ROWS 4
+template <typename T, int NJ>
 __global__ void __launch_bounds__(256)
 attention_tree_merge_kernel(const TreeParams P, int G, int slot_half, int half_rows) {
-  __shared__ float w_s[8][32];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   pdl_wait();
   const int c = blockIdx.x + 1;
   const TreeCut cut = P.cut[c];
-  if (cut.n_pages == 0) return;
-  const long long T_ = cut.total, u0 = tree_begin(c, G, T_), ib = cut.item_begin, ie = ib + cut.n_pages;
-  int first = c - 1;                               // the last CTA before c that has anything (a short list leaves some idle)
-  while (first > 0 && tree_begin(first, G, T_) == u0) first--;
-  const long long ub = tree_begin(first, G, T_);
-  if (u0 == ib || ub > ib) return;
-  const TreeSeq sq = tree_seq(P, cut.b);
-  const int r = blockIdx.y * 8 + warp, flat = cut.rt * P.rows_per_tile + r;
-  if (r >= P.rows_per_tile || flat >= sq.n_new * P.gs) return;
+  const long long u0 = cut.u0, ib = cut.item_begin, ie = ib + cut.n_pages;
+  if (cut.n_pages == 0 || u0 == ib) return;
+  // the last CTA before c that has anything (a short list leaves some idle)
+  int first = -1;
+  long long ub = 0;
+  for (int i0 = c - 1; first < 0 && i0 >= 0; i0 -= 32) {
+    const long long u = i0 - lane >= 0 ? P.cut[i0 - lane].u0 : u0;
+    const unsigned have = __ballot_sync(0xffffffffu, u < u0);
+    if (have) { const int l = __ffs(have) - 1; first = i0 - l; ub = __shfl_sync(0xffffffffu, u, l); }
+  }
+  if (first < 0 || ub > ib) return;
+  const int r0 = (blockIdx.y * 8 + warp) * TM_ROWS;
+  if (r0 >= cut.n_rows) return;
   const int hd = P.head_dim, hp = (hd + 3) & ~3;
-  const int slot_rows = (P.rows_per_tile / half_rows) * slot_half, srow = (r / half_rows) * slot_half + r % half_rows;
-  const int slot_of_first = ub == ib ? 0 : 1;
-  int n = 1;                                       // pieces: CTAs first .. first + n - 1
-  while (first + n < G && tree_begin(first + n, G, T_) < ie) n++;
-  auto slot_row = [&](int i) { return ((size_t)(2 * (first + i) + (i == 0 ? slot_of_first : 0))) * slot_rows + srow; };
-  auto empty = [&](int i) { return i > 0 && tree_begin(first + i, G, T_) == tree_begin(first + i + 1, G, T_); };
-  float M = -INFINITY;
-  for (int i = lane; i < n; i += 32)
-    if (!empty(i)) M = fmaxf(M, __ldcg(&P.part_ml[slot_row(i)].x));
-  M = warp_max(M);
-  const float Mu = M == -INFINITY ? 0.f : M;
-  float L = 0.f;
-  float4 acc[2];
-  acc[0] = acc[1] = make_float4(0.f, 0.f, 0.f, 0.f);
-  for (int i0 = 0; i0 < n; i0 += 32) {
-    const int i = i0 + lane;
-    float w = 0.f, part = 0.f;
-    if (i < n && !empty(i)) {
-      const float2 ml = __ldcg(&P.part_ml[slot_row(i)]);
-      w = exp2f(ml.x - Mu);
-      part = w * ml.y;
-    }
-    L += warp_sum(part);
-    __syncwarp();
-    w_s[warp][lane] = w;
-    __syncwarp();
-    const int k1 = min(32, n - i0);
-#pragma unroll 4
-    for (int k = 0; k < k1; k++) {
-      const float wk = w_s[warp][k];
-      if (wk == 0.f) continue;                     // (no key seen: the piece may hold anything)
-      const float* po = P.part_o + slot_row(i0 + k) * hp;
+  const int slot_rows = (P.rows_per_tile / half_rows) * slot_half, n = min(TM_ROWS, cut.n_rows - r0);
+  int srow[TM_ROWS];
 #pragma unroll
-      for (int j = 0; j < 2; j++) {
-        const int d = 4 * (lane + 32 * j);
-        if (d < hp) {
-          const float4 x = __ldcg(reinterpret_cast<const float4*>(po + d));
-          acc[j].x = fmaf(wk, x.x, acc[j].x); acc[j].y = fmaf(wk, x.y, acc[j].y);
-          acc[j].z = fmaf(wk, x.z, acc[j].z); acc[j].w = fmaf(wk, x.w, acc[j].w);
+  for (int x = 0; x < TM_ROWS; x++) {
+    const int r = min(r0 + x, cut.n_rows - 1);
+    srow[x] = (r / half_rows) * slot_half + r % half_rows;
+  }
+  float M[TM_ROWS], L[TM_ROWS];
+  float4 acc[TM_ROWS][NJ];
+#pragma unroll
+  for (int x = 0; x < TM_ROWS; x++) {
+    M[x] = -INFINITY; L[x] = 0.f;
+#pragma unroll
+    for (int j = 0; j < NJ; j++) acc[x][j] = make_float4(0.f, 0.f, 0.f, 0.f);
+  }
+  // 32 stretches at a time, from `first` on; an item of few pages is over within the first of them
+  for (int i0 = first; i0 < G; i0 += 32) {
+    const int i = i0 + lane;
+    const long long u = i < G ? P.cut[i].u0 : ie;
+    const bool any = i < G && (i == first || (u < ie && P.cut[i].n_pages > 0));
+    const unsigned have = __ballot_sync(0xffffffffu, any);
+    const bool over = __any_sync(0xffffffffu, u >= ie);
+    if (!have) {                                   // (a short list leaves stretches of idle CTAs between its pieces)
+      if (over) break;
+      continue;
+    }
+    const size_t slot = (size_t)(2 * i + ((i == first && ub != ib) ? 1 : 0)) * slot_rows;
+    float w[TM_ROWS];
+#pragma unroll
+    for (int x = 0; x < TM_ROWS; x++) {
+      const float2 ml = any ? __ldcg(&P.part_ml[slot + srow[x]]) : make_float2(-INFINITY, 0.f);
+      const float m = fmaxf(M[x], warp_max(ml.x)), mu = m == -INFINITY ? 0.f : m;
+      const float corr = exp2f(M[x] - mu);
+      w[x] = exp2f(ml.x - mu);
+      L[x] = fmaf(L[x], corr, warp_sum(w[x] * ml.y));
+      M[x] = m;
+#pragma unroll
+      for (int j = 0; j < NJ; j++) { acc[x][j].x *= corr; acc[x][j].y *= corr; acc[x][j].z *= corr; acc[x][j].w *= corr; }
+    }
+    for (unsigned left = have; left; left &= left - 1) {
+      const int l = __ffs(left) - 1;
+      const size_t piece = (size_t)(2 * (i0 + l) + ((i0 + l == first && ub != ib) ? 1 : 0)) * slot_rows;
+#pragma unroll
+      for (int x = 0; x < TM_ROWS; x++) {
+        const float wk = __shfl_sync(0xffffffffu, w[x], l);
+#pragma unroll
+        for (int j = 0; j < NJ; j++) {
+          const int d = 4 * (lane + 32 * j);
+          if (wk != 0.f && d < hp) {               // (no key seen: the piece may hold anything)
+            const float4 v = __ldcg(reinterpret_cast<const float4*>(P.part_o + (piece + srow[x]) * hp + d));
+            acc[x][j].x = fmaf(wk, v.x, acc[x][j].x); acc[x][j].y = fmaf(wk, v.y, acc[x][j].y);
+            acc[x][j].z = fmaf(wk, v.z, acc[x][j].z); acc[x][j].w = fmaf(wk, v.w, acc[x][j].w);
+          }
         }
       }
     }
+    if (over) break;
   }
-  const float inv = L == 0.f ? 0.f : 1.0f / L;
-  T* op = reinterpret_cast<T*>(P.out) + (size_t)(sq.row0 + flat / P.gs) * P.ldo +
-          (size_t)(cut.kvh * P.gs + flat % P.gs) * hd;
 #pragma unroll
-  for (int j = 0; j < 2; j++) {
-    const int d = 4 * (lane + 32 * j);
-    const float y[4] = {acc[j].x, acc[j].y, acc[j].z, acc[j].w};
+  for (int x = 0; x < TM_ROWS; x++) {
+    if (x >= n) break;
+    const int flat = cut.flat0 + r0 + x;
+    const float inv = 1.0f / L[x];
+    T* op = reinterpret_cast<T*>(P.out) + (size_t)(flat / P.gs) * P.ldo + (size_t)(cut.kvh * P.gs + flat % P.gs) * hd;
 #pragma unroll
-    for (int x = 0; x < 4; x++)
-      if (d + x < hd) op[d + x] = from_float<T>(L == 0.f ? 0.f : y[x] * inv);
+    for (int j = 0; j < NJ; j++) {
+      const int d = 4 * (lane + 32 * j);
+      const float y[4] = {acc[x][j].x, acc[x][j].y, acc[x][j].z, acc[x][j].w};
+#pragma unroll
+      for (int e = 0; e < 4; e++)
+        if (d + e < hd) op[d + e] = from_float<T>(L[x] == 0.f ? 0.f : y[e] * inv);
+    }
   }
 }
 
@@ -1078,17 +1145,17 @@ static int launch_tree_tc(const CUtensorMap& mq, const CUtensorMap& mk, const CU
   return launch_pdl(kern, dim3(G), dim3(TR_THREADS), smem, stream, mq, mk, mv, P);
 }
 
-static size_t simple_smem(int head_dim, int n_seqs) {
+static size_t simple_smem(int head_dim, int rows, int n_seqs) {
   const int hp = (head_dim + 3) & ~3;
-  const size_t tiles = ((size_t)(TG_ROWS + TR_KEYS) * (hp + 4) + (size_t)TR_KEYS * hp + (size_t)TG_ROWS * TR_KEYS) * sizeof(float);
+  const size_t tiles = ((size_t)(rows + TR_KEYS) * (hp + 4) + (size_t)TR_KEYS * hp + (size_t)rows * (TR_KEYS + 4)) * sizeof(float);
   const size_t sums = (size_t)(n_seqs + 1) * sizeof(long long);
   return tiles > sums ? tiles : sums;
 }
 
-template <typename T, int NC>
+template <typename T, int NC, int R>
 static int launch_tree_simple(const TreeParams& P, int G, cudaStream_t stream) {
-  const size_t smem = simple_smem(P.head_dim, P.n_seqs);
-  auto kern = attention_tree_simple_kernel<T, NC>;
+  const size_t smem = simple_smem(P.head_dim, 16 * R, P.n_seqs);
+  auto kern = attention_tree_simple_kernel<T, NC, R>;
   static unsigned long long done = 0;
   if (first_on_device(&done)) {
     cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, 227 * 1024);
@@ -1096,22 +1163,34 @@ static int launch_tree_simple(const TreeParams& P, int G, cudaStream_t stream) {
   }
   return launch_pdl(kern, dim3(G), dim3(TG_THREADS), smem, stream, P);
 }
+template <typename T>
+static int launch_tree_simple_of(const TreeParams& P, int G, cudaStream_t stream) {
+  if (P.rows_per_tile == 32)
+    return P.head_dim <= 64 ? launch_tree_simple<T, 1, 2>(P, G, stream)
+         : P.head_dim <= 128 ? launch_tree_simple<T, 2, 2>(P, G, stream) : launch_tree_simple<T, 4, 2>(P, G, stream);
+  return P.head_dim <= 64 ? launch_tree_simple<T, 1, 4>(P, G, stream)
+       : P.head_dim <= 128 ? launch_tree_simple<T, 2, 4>(P, G, stream) : launch_tree_simple<T, 4, 4>(P, G, stream);
+}
 
-// CTAs of a launch (the scratch has two slots of rows for each): tensor: the tcgen05 kernel, else the CUDA-core kernel, of
-// which as many share an SM as their shared memory allows.
-STRATUM_EXPORT int stratum_attention_tree_ctas(int tensor, int head_dim) {
+// Slot rows of a launch's scratch: tensor: the tcgen05 kernel, of 128 rows a half; else the CUDA-core kernel, of 32 or 64
+// rows.  many: a tree has more rows than the smaller one of the two holds.
+STRATUM_EXPORT int stratum_attention_tree_slot_rows(int tensor, int many) { return tensor ? (many ? 256 : 128) : (many ? 64 : 32); }
+
+// CTAs of a launch (the scratch has two slots of rows for each): of the CUDA-core kernel as many share an SM as their
+// shared memory allows.
+STRATUM_EXPORT int stratum_attention_tree_ctas(int tensor, int many, int head_dim) {
   if (tensor) return sm_count();
-  const int per_sm = (int)((size_t)(227 * 1024) / (simple_smem(head_dim, 0) + 1024));
+  const int per_sm = (int)((size_t)(227 * 1024) / (simple_smem(head_dim, many ? 64 : 32, 0) + 1024));
   return sm_count() * (per_sm < 1 ? 1 : per_sm > 4 ? 4 : per_sm);
 }
 
 // Scratch: part_o float32 [G][2][slot rows][head_dim rounded up to 4], part_ml float32 [G][2][slot rows][2], cut 32 bytes
-// a CTA.  Slot rows: 32 (tensor = 0), 128, or 256 (rows2).
+// a CTA.
 STRATUM_EXPORT int stratum_attention_tree(const void* q, int ldq, const void* k_cache, const void* v_cache, long long n_pages,
                                           int dtype, const int* token_pos, const void* mask, int words,
                                           const int* seq_start, const int* seq_len, const int* block_table, int bt_stride,
                                           int bt_width, void* out, int ldo, int n_tokens, int n_seqs, int n_q, int n_kv,
-                                          int head_dim, int page_tokens, int window, float scale, int tensor, int rows2,
+                                          int head_dim, int page_tokens, int window, float scale, int tensor, int many,
                                           float* part_o, void* part_ml, void* cut, int* status, cudaStream_t stream) {
   if (n_tokens <= 0 || n_seqs <= 0) return 0;
   if (dtype != STRATUM_DT_F32 && dtype != STRATUM_DT_BF16) return STRATUM_ERR_DTYPE;
@@ -1129,7 +1208,7 @@ STRATUM_EXPORT int stratum_attention_tree(const void* q, int ldq, const void* k_
   P.part_o = part_o; P.part_ml = (float2*)part_ml; P.cut = (TreeCut*)cut; P.status = status;
   P.n_tokens = n_tokens; P.n_seqs = n_seqs; P.n_q = n_q; P.n_kv = n_kv; P.gs = gs; P.head_dim = head_dim;
   P.window = window; P.n_pages = (int)n_pages; P.scale = scale;
-  const int G = stratum_attention_tree_ctas(tensor, head_dim);
+  const int G = stratum_attention_tree_ctas(tensor, many, head_dim);
   int st, slot_half, half_rows;
   if (tensor) {
     if (dtype != STRATUM_DT_BF16 || (head_dim != 64 && head_dim != 128) || gs > 128 || !(scale > 0.f)) return STRATUM_ERR_SHAPE;
@@ -1137,7 +1216,7 @@ STRATUM_EXPORT int stratum_attention_tree(const void* q, int ldq, const void* k_
     if (((uintptr_t)q | (uintptr_t)k_cache | (uintptr_t)v_cache | (uintptr_t)out) & 15) return STRATUM_ERR_ALIGN;
     const int half_tokens = 128 / gs;
     slot_half = 128; half_rows = half_tokens * gs;
-    P.rows_per_tile = half_rows * (rows2 ? 2 : 1);
+    P.rows_per_tile = half_rows * (many ? 2 : 1);
     CUtensorMap mq, mk, mv;
     {  // q as [tokens][n_q heads][head_dim]; a box is 64 dims x gs heads x half_tokens tokens: rows token * gs + head
       cuuint64_t dims[3] = {(cuuint64_t)head_dim, (cuuint64_t)n_q, (cuuint64_t)n_tokens};
@@ -1152,19 +1231,17 @@ STRATUM_EXPORT int stratum_attention_tree(const void* q, int ldq, const void* k_
       if ((st = tree_map(&mk, k_cache, 2, dims, strides, box)) != 0) return st;
       if ((st = tree_map(&mv, v_cache, 2, dims, strides, box)) != 0) return st;
     }
-    if (head_dim == 64) st = rows2 ? launch_tree_tc<64, true>(mq, mk, mv, P, G, stream) : launch_tree_tc<64, false>(mq, mk, mv, P, G, stream);
-    else st = rows2 ? launch_tree_tc<128, true>(mq, mk, mv, P, G, stream) : launch_tree_tc<128, false>(mq, mk, mv, P, G, stream);
+    if (head_dim == 64) st = many ? launch_tree_tc<64, true>(mq, mk, mv, P, G, stream) : launch_tree_tc<64, false>(mq, mk, mv, P, G, stream);
+    else st = many ? launch_tree_tc<128, true>(mq, mk, mv, P, G, stream) : launch_tree_tc<128, false>(mq, mk, mv, P, G, stream);
   } else {
-    slot_half = half_rows = P.rows_per_tile = TG_ROWS;
-    if (dtype == STRATUM_DT_F32)
-      st = head_dim <= 64 ? launch_tree_simple<float, 1>(P, G, stream)
-         : head_dim <= 128 ? launch_tree_simple<float, 2>(P, G, stream) : launch_tree_simple<float, 4>(P, G, stream);
-    else
-      st = head_dim <= 64 ? launch_tree_simple<bf16, 1>(P, G, stream)
-         : head_dim <= 128 ? launch_tree_simple<bf16, 2>(P, G, stream) : launch_tree_simple<bf16, 4>(P, G, stream);
+    slot_half = half_rows = P.rows_per_tile = many ? 64 : 32;
+    st = dtype == STRATUM_DT_F32 ? launch_tree_simple_of<float>(P, G, stream) : launch_tree_simple_of<bf16>(P, G, stream);
   }
   if (st != 0 || G < 2) return st;
-  const dim3 grid(G - 1, (P.rows_per_tile + 7) / 8);
-  return dtype == STRATUM_DT_F32 ? launch_pdl(attention_tree_merge_kernel<float>, grid, dim3(256), 0, stream, P, G, slot_half, half_rows)
-                                 : launch_pdl(attention_tree_merge_kernel<bf16>, grid, dim3(256), 0, stream, P, G, slot_half, half_rows);
+  const dim3 grid(G - 1, (P.rows_per_tile + 8 * TM_ROWS - 1) / (8 * TM_ROWS)), block(256);
+  if (dtype == STRATUM_DT_F32)
+    return head_dim <= 128 ? launch_pdl(attention_tree_merge_kernel<float, 1>, grid, block, 0, stream, P, G, slot_half, half_rows)
+                           : launch_pdl(attention_tree_merge_kernel<float, 2>, grid, block, 0, stream, P, G, slot_half, half_rows);
+  return head_dim <= 128 ? launch_pdl(attention_tree_merge_kernel<bf16, 1>, grid, block, 0, stream, P, G, slot_half, half_rows)
+                         : launch_pdl(attention_tree_merge_kernel<bf16, 2>, grid, block, 0, stream, P, G, slot_half, half_rows);
 }

@@ -1685,8 +1685,7 @@ def _shaped(t: torch.Tensor, name: str, dtype, shape=None) -> None:
         raise KernelError(f"{name} must have the shape {shape}, has {tuple(t.shape)}")
 
 
-_tree_ctas: dict = {}
-TREE_MAX_SEQS = 4096
+_tree_plans: dict = {}         # (tensor cores, many rows, head size) -> CTAs, scratch rows of a CTA's slot
 
 
 def attention_tree(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, token_pos: torch.Tensor,
@@ -1732,13 +1731,16 @@ def attention_tree(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor
     group = n_q // n_kv
     tensor = (dt == torch.bfloat16 and head_dim in (64, 128) and group <= 128 and scale > 0 and q.stride(0) % 8 == 0
               and out.stride(0) % 8 == 0 and not (q.data_ptr() | out.data_ptr() | k_cache.data_ptr() | v_cache.data_ptr()) & 15)
-    # more rows than a half of a CTA holds: both halves share every page (else they take pages in turn)
-    rows2 = max_new * group > 128
-    key = (tensor, head_dim)
-    ctas = _tree_ctas.get(key)
-    if ctas is None:
-        ctas = _tree_ctas[key] = int(build.load("attention_tree").stratum_attention_tree_ctas(int(tensor), head_dim))
-    slots = 2 * ctas * (32 if not tensor else 256 if rows2 else 128)
+    # more rows than a half of a CTA holds: both halves share every page (else they take pages in turn); on the CUDA cores:
+    # tiles of 64 rows
+    many = max_new * group > (128 if tensor else 32)
+    key = (tensor, many, head_dim)
+    plan = _tree_plans.get(key)
+    if plan is None:
+        lib = build.load("attention_tree")
+        plan = _tree_plans[key] = (int(lib.stratum_attention_tree_ctas(int(tensor), int(many), head_dim)),
+                                   int(lib.stratum_attention_tree_slot_rows(int(tensor), int(many))))
+    ctas, slots = plan[0], 2 * plan[0] * plan[1]
     # (scratch of this call's own: calls on several streams, and captured ones, do not meet in it)
     scratch = torch.empty(slots * ((head_dim + 3) // 4 * 4 + 2) + 8 * ctas, dtype=torch.float32, device=q.device)
     at = scratch.data_ptr()
@@ -1750,7 +1752,7 @@ def attention_tree(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor
     _check(f(q.data_ptr(), q.stride(0), k_cache.data_ptr(), v_cache.data_ptr(), k_cache.shape[0], code,
              token_pos.data_ptr(), tree_mask.data_ptr(), tree_mask.shape[1], seq_start.data_ptr(), seq_len.data_ptr(),
              block_table.data_ptr(), block_table.stride(0), block_table.shape[1], out.data_ptr(), out.stride(0), T, B, n_q,
-             n_kv, head_dim, page_tokens, window, scale, int(tensor), int(rows2), at, part_ml, part_ml + 8 * slots,
+             n_kv, head_dim, page_tokens, window, scale, int(tensor), int(many), at, part_ml, part_ml + 8 * slots,
              status_word().data_ptr(), _stream()), "attention_tree")
     count_launches(1)          # the merge kernel
 
