@@ -58,7 +58,7 @@ struct TreeParams {
 };
 
 // What CTA c's stretch begins in, for the merge.
-struct TreeCut {
+struct alignas(16) TreeCut {
   long long u0, item_begin;                // the stretch's first unit, the first unit of the item that holds it
   int n_pages, kvh;                        // units of the item (0: the stretch is empty); its kv head,
   int flat0, n_rows;                       // its first row (token of the batch * gs + head), its rows
@@ -69,9 +69,9 @@ struct TreeSeq {                           // a sequence's share of the list
 };
 __device__ __forceinline__ TreeSeq tree_seq(const TreeParams& P, int b) {
   TreeSeq s;
-  s.row0 = min(max(P.seq_start[b], 0), P.n_tokens);
-  s.n_new = min(max(P.seq_start[b + 1], s.row0), P.n_tokens) - s.row0;
-  s.len = max(P.seq_len[b], 0);
+  s.row0 = min(max(__ldcg(P.seq_start + b), 0), P.n_tokens);
+  s.n_new = min(max(__ldcg(P.seq_start + b + 1), s.row0), P.n_tokens) - s.row0;
+  s.len = max(__ldcg(P.seq_len + b), 0);
   s.base = max(s.len - s.n_new, 0);
   const int pages = max(min((int)(((long long)s.len + TR_KEYS - 1) / TR_KEYS), P.bt_width), 1);
   const int lo = (P.window > 0 && s.base - P.window + 1 > 0) ? s.base - P.window + 1 : 0;
@@ -564,11 +564,11 @@ attention_tree_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
       const int token = sq.row0 + (ROWS2 ? 2 * run.rt + h : run.rt) * half_tokens + (valid ? tok : 0);
       int lo = 0, lo_max = 0;
       if (P.window > 0) {
-        lo = valid ? max(P.token_pos[token] - P.window + 1, 0) : 0;
+        lo = valid ? max(__ldcg(P.token_pos + token) - P.window + 1, 0) : 0;
         // the furthest edge of the tile's rows (all rows of both halves: the halves decide alike)
         const int t0 = sq.row0 + run.rt * half_tokens * (ROWS2 ? 2 : 1);
         const int t1 = min(t0 + half_tokens * (ROWS2 ? 2 : 1), sq.row0 + sq.n_new);
-        for (int t = t0 + lane; t < t1; t += 32) lo_max = max(lo_max, P.token_pos[t] - P.window + 1);
+        for (int t = t0 + lane; t < t1; t += 32) lo_max = max(lo_max, __ldcg(P.token_pos + t) - P.window + 1);
         lo_max = __reduce_max_sync(0xffffffffu, lo_max);
       }
       const uint32_t it_first = it, it_end = it + run.n;
@@ -840,7 +840,7 @@ attention_tree_simple_kernel(const TreeParams P) {
     const int r0 = run.rt * ROWS, n_rows = min(sq.n_new * P.gs - r0, ROWS);
     const int* bt = P.block_table + (size_t)run.b * P.bt_stride + run.page0;
     __syncthreads();                               // (the run before, or the start, may still be reading)
-    int pg = bt[0];
+    int pg = __ldcg(bt);
     fetch(P.k_cache, pg, run.kvh, ks, pitch);
     fetch(P.v_cache, pg, run.kvh, vs, hp);
     for (int e = tid; e < ROWS * hp; e += TG_THREADS) {
@@ -862,7 +862,7 @@ attention_tree_simple_kernel(const TreeParams P) {
       m[e] = -INFINITY; l[e] = 0.f;
       valid[e] = r < n_rows;
       token[e] = sq.row0 + (valid[e] ? (r0 + r) / P.gs : 0);
-      lo[e] = (P.window > 0 && valid[e]) ? max(P.token_pos[token[e]] - P.window + 1, 0) : 0;
+      lo[e] = (P.window > 0 && valid[e]) ? max(__ldcg(P.token_pos + token[e]) - P.window + 1, 0) : 0;
       lo_max = max(lo_max, lo[e]);
 #pragma unroll
       for (int j = 0; j < NC; j++) acc[e][j] = make_float4(0.f, 0.f, 0.f, 0.f);
@@ -870,7 +870,7 @@ attention_tree_simple_kernel(const TreeParams P) {
     for (int i = 0; i < run.n; i++) {
       const int key0 = (run.page0 + i) * TR_KEYS;
       const bool page_ok = (unsigned)pg < (unsigned)P.n_pages;
-      const int pg_next = i + 1 < run.n ? bt[i + 1] : -1;
+      const int pg_next = i + 1 < run.n ? __ldcg(bt + i + 1) : -1;
       cp_async_wait<1>();                          // this page's keys are here (its values may be on their way)
       __syncthreads();
       float s[R][4];
@@ -1020,14 +1020,17 @@ attention_tree_merge_kernel(const TreeParams P, int G, int slot_half, int half_r
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   pdl_wait();
   const int c = blockIdx.x + 1;
-  const TreeCut cut = P.cut[c];
+  // (all of this was written by the kernel before, and is read past L1)
+  const int4 cut_lo = __ldcg(reinterpret_cast<const int4*>(P.cut + c)), cut_hi = __ldcg(reinterpret_cast<const int4*>(P.cut + c) + 1);
+  TreeCut cut;
+  reinterpret_cast<int4*>(&cut)[0] = cut_lo; reinterpret_cast<int4*>(&cut)[1] = cut_hi;
   const long long u0 = cut.u0, ib = cut.item_begin, ie = ib + cut.n_pages;
   if (cut.n_pages == 0 || u0 == ib) return;
   // the last CTA before c that has anything (a short list leaves some idle)
   int first = -1;
   long long ub = 0;
   for (int i0 = c - 1; first < 0 && i0 >= 0; i0 -= 32) {
-    const long long u = i0 - lane >= 0 ? P.cut[i0 - lane].u0 : u0;
+    const long long u = i0 - lane >= 0 ? __ldcg(&P.cut[i0 - lane].u0) : u0;
     const unsigned have = __ballot_sync(0xffffffffu, u < u0);
     if (have) { const int l = __ffs(have) - 1; first = i0 - l; ub = __shfl_sync(0xffffffffu, u, l); }
   }
@@ -1053,8 +1056,8 @@ attention_tree_merge_kernel(const TreeParams P, int G, int slot_half, int half_r
   // 32 stretches at a time, from `first` on; an item of few pages is over within the first of them
   for (int i0 = first; i0 < G; i0 += 32) {
     const int i = i0 + lane;
-    const long long u = i < G ? P.cut[i].u0 : ie;
-    const bool any = i < G && (i == first || (u < ie && P.cut[i].n_pages > 0));
+    const long long u = i < G ? __ldcg(&P.cut[i].u0) : ie;
+    const bool any = i < G && (i == first || (u < ie && __ldcg(&P.cut[i].n_pages) > 0));
     const unsigned have = __ballot_sync(0xffffffffu, any);
     const bool over = __any_sync(0xffffffffu, u >= ie);
     if (!have) {                                   // (a short list leaves stretches of idle CTAs between its pieces)

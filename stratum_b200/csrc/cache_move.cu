@@ -1,0 +1,183 @@
+// What a paged cache does besides growing: whole pages are copied (a sequence begins as a copy of another one), and the
+// rows of the drafted tokens that were kept move together behind the tokens in front of them.  Both work on a group's keys
+// and values in all its layers in one launch, and move bytes: any element type.
+//
+// A page of a layer is one stretch of n_kv * 64 * head_dim elements, a token's row of a (page, head) one of head_dim.
+#include "common.cuh"
+
+static int sms() {
+  static int n = 0;
+  if (!n) {
+    int dev = 0;
+    cudaGetDevice(&dev);
+    cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev);
+    if (n <= 0) n = 148;
+  }
+  return n;
+}
+
+// ================================================================ pages
+// The pairs travel with the launch.  Pages are cut into pieces of CM_PIECE bytes; a block takes every (grid)th piece, each
+// thread 16 bytes (or 4, or 1, where the sizes ask for that) at a time, four on their way together.
+#define CM_PAIRS 480
+#define CM_THREADS 256
+struct PagePairs { int src[CM_PAIRS], dst[CM_PAIRS]; };
+
+template <typename V>
+__global__ void __launch_bounds__(CM_THREADS)
+copy_pages_kernel(uint8_t* a, uint8_t* b, long long pages, long long bytes_a, long long bytes_b, int layers, int n_pairs,
+                  const __grid_constant__ PagePairs pairs) {
+  pdl_wait();
+  constexpr int UNROLL = 8, PIECE = CM_THREADS * UNROLL;           // in units of V
+  const long long va = bytes_a / sizeof(V), vb = bytes_b / sizeof(V);
+  const long long pa = (va + PIECE - 1) / PIECE, pb = (vb + PIECE - 1) / PIECE, per_page = pa + pb;
+  const long long total = per_page * layers * n_pairs;
+  for (long long w = blockIdx.x; w < total; w += gridDim.x) {
+    const long long page = w / per_page;
+    const int layer = (int)(page / n_pairs), pair = (int)(page % n_pairs);
+    long long piece = w % per_page;
+    const bool second = piece >= pa;
+    if (second) piece -= pa;
+    const long long n = second ? vb : va;
+    V* base = reinterpret_cast<V*>(second ? b : a) + layer * pages * n;
+    const V* from = base + pairs.src[pair] * n;
+    V* to = base + pairs.dst[pair] * n;
+    const long long i0 = piece * PIECE + threadIdx.x;
+    V x[UNROLL];
+#pragma unroll
+    for (int j = 0; j < UNROLL; j++) if (i0 + j * CM_THREADS < n) x[j] = __ldcg(from + i0 + j * CM_THREADS);
+#pragma unroll
+    for (int j = 0; j < UNROLL; j++) if (i0 + j * CM_THREADS < n) to[i0 + j * CM_THREADS] = x[j];
+  }
+}
+
+// a, b: [layers][pages][bytes_a | bytes_b], b may be null (bytes_b 0).  Pages src[i] -> dst[i]; no page is written that
+// another pair reads or writes (the caller has looked).
+STRATUM_EXPORT int stratum_copy_pages(void* a, void* b, long long pages, long long bytes_a, long long bytes_b, int layers,
+                                      const int* src, const int* dst, int n_pairs, cudaStream_t stream) {
+  if (n_pairs <= 0 || layers <= 0) return 0;
+  if (n_pairs > CM_PAIRS) return STRATUM_ERR_LIMIT;
+  if (!a || bytes_a <= 0 || bytes_b < 0 || (bytes_b > 0 && !b)) return STRATUM_ERR_SHAPE;
+  PagePairs pairs;
+  for (int i = 0; i < n_pairs; i++) {
+    if (src[i] < 0 || src[i] >= pages || dst[i] < 0 || dst[i] >= pages) return STRATUM_ERR_LIMIT;
+    pairs.src[i] = src[i]; pairs.dst[i] = dst[i];
+  }
+  for (int i = n_pairs; i < CM_PAIRS; i++) pairs.src[i] = pairs.dst[i] = 0;
+  const unsigned long long all = (unsigned long long)(uintptr_t)a | (uintptr_t)b | (unsigned long long)bytes_a | (unsigned long long)bytes_b;
+  const int unit = (all & 15) == 0 ? 16 : (all & 3) == 0 ? 4 : 1;
+  const long long piece = (long long)unit * CM_THREADS * 8;
+  const long long total = ((bytes_a + piece - 1) / piece + (bytes_b + piece - 1) / piece) * layers * n_pairs;
+  const long long most = (long long)sms() * 8;
+  const dim3 grid((unsigned)(total < most ? total : most));
+  uint8_t* pa = (uint8_t*)a;
+  uint8_t* pb = (uint8_t*)b;
+  if (unit == 16) return launch_pdl(copy_pages_kernel<uint4>, grid, dim3(CM_THREADS), 0, stream, pa, pb, pages, bytes_a, bytes_b, layers, n_pairs, pairs);
+  if (unit == 4) return launch_pdl(copy_pages_kernel<uint32_t>, grid, dim3(CM_THREADS), 0, stream, pa, pb, pages, bytes_a, bytes_b, layers, n_pairs, pairs);
+  return launch_pdl(copy_pages_kernel<uint8_t>, grid, dim3(CM_THREADS), 0, stream, pa, pb, pages, bytes_a, bytes_b, layers, n_pairs, pairs);
+}
+
+// ================================================================ kept rows
+// Sequence s has seq_len[s] keys of which the last n = seq_start[s + 1] - seq_start[s] are drafted ones; path[seq_start[s] + j],
+// j = 1 .. kept[s], says which of them is kept in the j-th place.  Row base + path[j] of every layer, head, keys and values
+// goes to base + j.  The path rises and path[j] >= j (nodes stand behind their parents), so rows move towards the front
+// only and, taken in ascending stretches of which each is read before it is written, none is written that is still to be read.
+//
+// A warp owns a (sequence, layer, head, keys or values) and moves its rows CR_ROWS at a time; what it moves is its own, so
+// nothing waits for other warps.
+#define CR_THREADS 256
+#define CR_ROWS 8
+
+template <typename V>
+__global__ void __launch_bounds__(CR_THREADS)
+keep_rows_kernel(uint8_t* k, uint8_t* v, long long pages, int heads_k, int heads_v, int bytes_k, int bytes_v, int layers,
+                 int page_tokens, const int* block_table, int bt_stride, int bt_width, const int* seq_start, const int* seq_len,
+                 const int* path, const int* kept, int n_tokens, int per_seq) {
+  pdl_wait();
+  const int lane = threadIdx.x & 31;
+  const int s = blockIdx.x / per_seq;
+  int w = (blockIdx.x % per_seq) * (CR_THREADS / 32) + (threadIdx.x >> 5);          // layer, then keys' heads and values' heads
+  if (w >= layers * (heads_k + heads_v)) return;
+  const int layer = w / (heads_k + heads_v);
+  w %= heads_k + heads_v;
+  const bool second = w >= heads_k;
+  const int head = second ? w - heads_k : w, heads = second ? heads_v : heads_k;
+  const int units = (second ? bytes_v : bytes_k) / (int)sizeof(V);                  // of a row
+  const int a = min(max(__ldcg(seq_start + s), 0), n_tokens), n = min(max(__ldcg(seq_start + s + 1), a), n_tokens) - a;
+  const int base = __ldcg(seq_len + s) - n;
+  const int last = min(__ldcg(kept + s), n - 1);
+  if (last < 1 || base < 0) return;
+  V* all = reinterpret_cast<V*>(second ? v : k) + (long long)layer * pages * heads * page_tokens * units;
+  const int* bt = block_table + (long long)s * bt_stride;
+  // where position p of this head lies, or null
+  auto at = [&](int p) -> V* {
+    const int i = p / page_tokens;
+    if (i >= bt_width) return nullptr;
+    const int pg = __ldcg(bt + i);
+    if (pg < 0 || pg >= pages) return nullptr;
+    return all + (((long long)pg * heads + head) * page_tokens + p % page_tokens) * units;
+  };
+  int before = 0;                                  // the path's entry in front; one that does not rise ends it
+  for (int j0 = 1; j0 <= last; j0 += 32) {
+    const int j = j0 + lane;
+    int node = j <= last ? __ldcg(path + a + j) : -1;
+    int prev = __shfl_up_sync(0xffffffffu, node, 1);
+    if (lane == 0) prev = before;
+    const unsigned wrong = __ballot_sync(0xffffffffu, j > last || node <= prev || node >= n);
+    const int count = wrong ? __ffs(wrong) - 1 : 32;
+    before = __shfl_sync(0xffffffffu, node, 31);
+    V* from = nullptr;
+    V* to = nullptr;
+    if (lane < count && node != j) { from = at(base + node); to = at(base + j); }
+    if (!from || !to) from = to = nullptr;
+    const unsigned moves = __ballot_sync(0xffffffffu, from != nullptr);
+    for (unsigned left = moves; left;) {
+      // up to CR_ROWS rows of the path, in its order: read, then written
+      int l[CR_ROWS], m = 0;
+#pragma unroll
+      for (int x = 0; x < CR_ROWS; x++) {
+        l[x] = left ? __ffs(left) - 1 : 0;
+        if (left) { m = x + 1; left &= left - 1; }
+      }
+      for (int i0 = 0; i0 < units; i0 += 32) {
+        V x[CR_ROWS];
+#pragma unroll
+        for (int r = 0; r < CR_ROWS; r++) {
+          const V* f = reinterpret_cast<const V*>(__shfl_sync(0xffffffffu, (unsigned long long)from, l[r]));
+          if (r < m && i0 + lane < units) x[r] = __ldcg(f + i0 + lane);
+        }
+        __syncwarp();
+#pragma unroll
+        for (int r = 0; r < CR_ROWS; r++) {
+          V* t = reinterpret_cast<V*>(__shfl_sync(0xffffffffu, (unsigned long long)to, l[r]));
+          if (r < m && i0 + lane < units) t[i0 + lane] = x[r];
+        }
+        __syncwarp();
+      }
+    }
+    if (count < 32) return;
+  }
+}
+
+// k: [layers][pages][heads_k][page_tokens][bytes_k], v likewise (null: heads_v 0).
+STRATUM_EXPORT int stratum_keep_rows(void* k, void* v, long long pages, int heads_k, int heads_v, int bytes_k, int bytes_v,
+                                     int layers, int page_tokens, const int* block_table, int bt_stride, int bt_width,
+                                     const int* seq_start, const int* seq_len, const int* path, const int* kept, int n_tokens,
+                                     int n_seqs, cudaStream_t stream) {
+  if (n_seqs <= 0 || layers <= 0 || n_tokens <= 0) return 0;
+  if (!k || heads_k < 1 || bytes_k < 1 || heads_v < 0 || (heads_v > 0 && (!v || bytes_v < 1)) || page_tokens < 1 || bt_width < 1)
+    return STRATUM_ERR_SHAPE;
+  const long long warps = (long long)layers * (heads_k + heads_v), per_seq = (warps + CR_THREADS / 32 - 1) / (CR_THREADS / 32);
+  if (warps > 0x7fffffffLL || per_seq * n_seqs > 0x7fffffffLL) return STRATUM_ERR_LIMIT;
+  const unsigned long long all = (unsigned long long)(uintptr_t)k | (uintptr_t)v | (unsigned)bytes_k | (unsigned)bytes_v;
+  const dim3 grid((unsigned)(per_seq * n_seqs)), block(CR_THREADS);
+  uint8_t* pk = (uint8_t*)k;
+  uint8_t* pv = (uint8_t*)v;
+#define KEEP(V)                                                                                                              \
+  launch_pdl(keep_rows_kernel<V>, grid, block, 0, stream, pk, pv, pages, heads_k, heads_v, bytes_k, bytes_v, layers, page_tokens, \
+             block_table, bt_stride, bt_width, seq_start, seq_len, path, kept, n_tokens, (int)per_seq)
+  if ((all & 15) == 0) return KEEP(uint4);
+  if ((all & 3) == 0) return KEEP(uint32_t);
+  return KEEP(uint8_t);
+#undef KEEP
+}

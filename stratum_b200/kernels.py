@@ -1757,6 +1757,157 @@ def attention_tree(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor
     count_launches(1)          # the merge kernel
 
 
+def _rows_of(t: torch.Tensor, name: str, rows: Optional[int] = None) -> None:
+    """A float32 matrix with contiguous rows (any distance between them)."""
+    if t.dtype != torch.float32 or t.dim() != 2:
+        raise KernelError(f"{name} must be a float32 matrix, is {t.dtype} with {t.dim()} dimensions")
+    if (t.shape[1] > 1 and t.stride(1) != 1) or (t.shape[0] > 1 and t.stride(0) < t.shape[1]):
+        raise KernelError(f"{name}: rows must be contiguous and not overlap")
+    if rows is not None and t.shape[0] != rows:
+        raise KernelError(f"{name} must have {rows} rows, has {t.shape[0]}")
+
+
+def token_probs(logits: torch.Tensor, temperature: torch.Tensor, out: torch.Tensor) -> None:
+    """out[r] = softmax(logits[r] / temperature[r]); temperature <= 0 (or no number): one at the largest logit, the lowest
+    index among equals.  logits and out float32 [rows, vocab] (rows contiguous; out may be logits itself), temperature
+    float32 [rows].  A logit that is no number counts as -inf, infinite ones share the row, a row of nothing but -inf
+    gives zeros."""
+    _one_device("token_probs", logits, temperature, out)
+    _rows_of(logits, "logits"); _rows_of(out, "out", logits.shape[0])
+    R, V = logits.shape
+    if out.shape[1] != V:
+        raise KernelError("token_probs: out and logits disagree")
+    _shaped(temperature, "temperature", torch.float32, (R,))
+    if R == 0 or V == 0:
+        return
+    same = out.data_ptr() == logits.data_ptr() and (R == 1 or out.stride(0) == logits.stride(0))
+    if not same:
+        a, b = logits.data_ptr(), out.data_ptr()
+        if a < b + 4 * ((R - 1) * out.stride(0) + V) and b < a + 4 * ((R - 1) * logits.stride(0) + V):
+            raise KernelError("token_probs: out is logits itself or memory of its own")
+    f = _fn("draft_verify", "stratum_token_probs",
+            [c_void_p, ctypes.c_longlong, c_void_p, c_void_p, ctypes.c_longlong, c_int, c_int, c_void_p])
+    _check(f(logits.data_ptr(), logits.stride(0), temperature.data_ptr(), out.data_ptr(), out.stride(0), R, V, _stream()),
+           "token_probs")
+
+
+VERIFY_MAX_NODES = 1024            # of a sequence
+
+
+def verify_drafts(target: torch.Tensor, draft: Optional[torch.Tensor], tokens: torch.Tensor, parents: torch.Tensor,
+                  seq_start: torch.Tensor, uniform: torch.Tensor, path: torch.Tensor, n_kept: torch.Tensor,
+                  next_ids: torch.Tensor) -> None:
+    """Walk every sequence's tree of drafted tokens (csrc/draft_verify.cu): which are kept, and the token behind them.
+
+    Sequence s's nodes are the rows seq_start[s] .. seq_start[s + 1] - 1 (int32 [seqs + 1]); the first is the token it went
+    on with, the others are drafts with tokens[row] (int32; an id outside the vocabulary is never kept) behind the node
+    parents[row] of their sequence (int32, counted from the sequence's first row and smaller than their own number).
+    target[row] (float32 [rows, vocab]): the target's probabilities behind the node.  draft[row]: the distribution its
+    children were drawn from, each for itself; None: they were looked up.  uniform (float32 [rows], in [0, 1)): a number per
+    draft for its own trial; the first node's is for the draw of the next token.  The kept tokens and the next one are then
+    distributed as the target's own.
+
+    path (int32 [rows]): in place j behind seq_start[s] the number of the node kept j-th, 0 (the first node) in front, -1
+    behind the last.  n_kept (int32 [seqs]): drafts kept; next_ids (int32 [seqs]): the next token (0 where the target's row
+    has no weight, -1 for a sequence without nodes).  Rows behind the last sequence are left as they were.  At most
+    VERIFY_MAX_NODES nodes of a sequence are looked at."""
+    _one_device("verify_drafts", target, draft, tokens, parents, seq_start, uniform, path, n_kept, next_ids)
+    _rows_of(target, "target")
+    T, V = target.shape
+    if draft is not None:
+        _rows_of(draft, "draft", T)
+        if draft.shape[1] != V:
+            raise KernelError("verify_drafts: draft and target disagree")
+    B = n_kept.numel()
+    for t, name in ((tokens, "tokens"), (parents, "parents"), (path, "path")):
+        _shaped(t, name, torch.int32, (T,))
+    _shaped(uniform, "uniform", torch.float32, (T,)); _shaped(seq_start, "seq_start", torch.int32, (B + 1,))
+    _shaped(n_kept, "n_kept", torch.int32, (B,)); _shaped(next_ids, "next_ids", torch.int32, (B,))
+    if V < 1:
+        raise KernelError("verify_drafts: an empty vocabulary")
+    if T > B * VERIFY_MAX_NODES:
+        raise KernelError(f"verify_drafts: {T} rows are more than {VERIFY_MAX_NODES} for each of {B} sequences")
+    if B == 0:
+        return
+    f = _fn("draft_verify", "stratum_verify_drafts",
+            [c_void_p, ctypes.c_longlong, c_void_p, ctypes.c_longlong, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p,
+             c_void_p, c_void_p, c_int, c_int, c_int, c_void_p])
+    _check(f(target.data_ptr(), target.stride(0), None if draft is None else draft.data_ptr(),
+             0 if draft is None else draft.stride(0), tokens.data_ptr(), parents.data_ptr(), seq_start.data_ptr(),
+             uniform.data_ptr(), path.data_ptr(), n_kept.data_ptr(), next_ids.data_ptr(), T, B, V, _stream()), "verify_drafts")
+
+
+def _storage(k: torch.Tensor, v: Optional[torch.Tensor], what: str) -> None:
+    """A group's keys and values [layers, pages, heads, page_tokens, size] (values with heads and a size of their own)."""
+    for t, name in ((k, "k"), (v, "v")):
+        if t is None:
+            continue
+        if t.dim() != 5 or not t.is_contiguous() or t.numel() == 0:
+            raise KernelError(f"{what}: {name} must be contiguous [layers, pages, heads, page_tokens, size]")
+    if v is not None and (v.shape[:2] != k.shape[:2] or v.shape[3] != k.shape[3]):
+        raise KernelError(f"{what}: k and v have layers, pages and page_tokens in common")
+
+
+def keep_rows(k: torch.Tensor, v: Optional[torch.Tensor], block_table: torch.Tensor, seq_start: torch.Tensor,
+              seq_len: torch.Tensor, path: torch.Tensor, n_kept: torch.Tensor) -> None:
+    """The cached rows of the drafted tokens that were kept move together, in every layer and head: sequence s's drafted
+    rows lie at positions seq_len[s] - rows ..., rows = seq_start[s + 1] - seq_start[s], and the row of node
+    path[seq_start[s] + j], j = 1 .. n_kept[s], goes to place j of them (path and n_kept as verify_drafts writes them: a
+    path that does not rise ends there).  k, v [layers, pages, heads, page_tokens, size] of any element type (v None: keys
+    alone), block_table int32 [seqs, pages]; a page number outside the pool is passed over."""
+    _one_device("keep_rows", k, v, block_table, seq_start, seq_len, path, n_kept)
+    _storage(k, v, "keep_rows")
+    B, T = n_kept.numel(), path.numel()
+    _shaped(block_table, "block_table", torch.int32); _shaped(path, "path", torch.int32, (T,))
+    _shaped(seq_start, "seq_start", torch.int32, (B + 1,)); _shaped(seq_len, "seq_len", torch.int32, (B,))
+    _shaped(n_kept, "n_kept", torch.int32, (B,))
+    if block_table.dim() != 2 or block_table.shape[0] != B or (B > 0 and block_table.shape[1] < 1):
+        raise KernelError("keep_rows: block_table is [sequences, pages]")
+    if B == 0 or T == 0:
+        return
+    L, pages, heads, page_tokens, size = k.shape
+    f = _fn("cache_move", "stratum_keep_rows",
+            [c_void_p, c_void_p, ctypes.c_longlong, c_int, c_int, c_int, c_int, c_int, c_int, c_void_p, c_int, c_int, c_void_p,
+             c_void_p, c_void_p, c_void_p, c_int, c_int, c_void_p])
+    _check(f(k.data_ptr(), None if v is None else v.data_ptr(), pages, heads, 0 if v is None else v.shape[2],
+             size * k.element_size(), 0 if v is None else v.shape[4] * v.element_size(), L, page_tokens,
+             block_table.data_ptr(), block_table.stride(0), block_table.shape[1], seq_start.data_ptr(), seq_len.data_ptr(),
+             path.data_ptr(), n_kept.data_ptr(), T, B, _stream()), "keep_rows")
+
+
+COPY_PAGES_MAX = 480               # pairs of a launch
+
+
+def copy_pages(k: torch.Tensor, v: Optional[torch.Tensor], src, dst) -> None:
+    """Page dst[i] becomes a copy of page src[i] in every layer, keys and values; src and dst are host lists of page numbers
+    that travel with the launch.  k [layers, pages, ...], v [layers, pages, ...] or None: contiguous, of any element type.  No page is
+    written twice, or written and read in one call (refused before anything runs)."""
+    _one_device("copy_pages", k, v)
+    src, dst = [int(p) for p in src], [int(p) for p in dst]
+    for t, name in ((k, "k"), (v, "v")):
+        if t is not None and (t.dim() < 2 or not t.is_contiguous() or t.numel() == 0):
+            raise KernelError(f"copy_pages: {name} must be contiguous [layers, pages, ...]")
+    if v is not None and v.shape[:2] != k.shape[:2]:
+        raise KernelError("copy_pages: k and v have layers and pages in common")
+    L, pages = k.shape[:2]
+    if len(src) != len(dst):
+        raise KernelError("copy_pages: one destination for every source")
+    if any(not 0 <= p < pages for p in src) or any(not 0 <= p < pages for p in dst):
+        raise KernelError(f"copy_pages: a page outside 0 .. {pages - 1}")
+    written = set(dst)
+    if len(written) != len(dst) or written & set(src):
+        raise KernelError("copy_pages: a page is written twice, or written and read")
+    sizes = [0 if t is None else t.stride(1) * t.element_size() for t in (k, v)]
+    f = _fn("cache_move", "stratum_copy_pages",
+            [c_void_p, c_void_p, ctypes.c_longlong, ctypes.c_longlong, ctypes.c_longlong, c_int, c_void_p, c_void_p, c_int,
+             c_void_p])
+    for i in range(0, len(src), COPY_PAGES_MAX):
+        a, b = src[i:i + COPY_PAGES_MAX], dst[i:i + COPY_PAGES_MAX]
+        n = len(a)
+        _check(f(k.data_ptr(), None if v is None else v.data_ptr(), pages, sizes[0], sizes[1], L, (c_int * n)(*a),
+                 (c_int * n)(*b), n, _stream()), "copy_pages")
+
+
 # ------------------------------------------------------------------ a decode step's layers as one kernel
 DECODE_LAYERS_MAX, DECODE_LAYERS_MAX_ROWS, DECODE_LAYERS_MAX_BLOCKS = 96, 16, 160
 DECODE_LAYERS_ABSENT = 0              # arrivals its meetings wait for in vain (for a test of the bounded wait)
