@@ -802,10 +802,14 @@ __device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commi
 template <int N> __device__ __forceinline__ void cp_async_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
 
 template <typename T, int NC, int R>
-__global__ void __launch_bounds__(TG_THREADS)
+__global__ void __launch_bounds__(TG_THREADS, NC == 1 ? (R == 2 ? 3 : 2) : NC == 2 ? (R == 2 ? 2 : 1) : 1)
 attention_tree_simple_kernel(const TreeParams P) {
   extern __shared__ __align__(16) float tg_smem[];
   constexpr int ROWS = 16 * R, PK = TR_KEYS + 4;
+  // what concerns the run and its rows lies in shared memory, as the registers are the products'
+  __shared__ TreeWalk walk;
+  __shared__ unsigned long long row_vis[ROWS];     // which keys of a masked page a row sees
+  __shared__ int row_token[ROWS], row_lo[ROWS], edge;
   const int hd = P.head_dim, hp = (hd + 3) & ~3, pitch = hp + 4;
   float* qs = tg_smem;                             // [ROWS][pitch]
   float* ks = qs + ROWS * pitch;                   // [64][pitch]
@@ -832,14 +836,15 @@ attention_tree_simple_kernel(const TreeParams P) {
     }
     cp_async_commit();
   };
-  TreeCursor cur;
-  cur.begin(P, start.n_units, start.b, start.item, start.off);
-  TreeRun run;
-  while (cur.next(P, run)) {
-    const TreeSeq& sq = run.s;
-    const int r0 = run.rt * ROWS, n_rows = min(sq.n_new * P.gs - r0, ROWS);
-    const int* bt = P.block_table + (size_t)run.b * P.bt_stride + run.page0;
+  if (tid == 0) walk.cur.begin(P, start.n_units, start.b, start.item, start.off);
+  const TreeRun& run = walk.run;
+  for (;;) {
     __syncthreads();                               // (the run before, or the start, may still be reading)
+    if (tid == 0) { walk.more = walk.cur.next(P, walk.run); edge = 0; }
+    __syncthreads();
+    if (!walk.more) break;
+    const int r0 = run.rt * ROWS, n_rows = min(run.s.n_new * P.gs - r0, ROWS);
+    const int* bt = P.block_table + (size_t)run.b * P.bt_stride + run.page0;
     int pg = __ldcg(bt);
     fetch(P.k_cache, pg, run.kvh, ks, pitch);
     fetch(P.v_cache, pg, run.kvh, vs, hp);
@@ -847,23 +852,22 @@ attention_tree_simple_kernel(const TreeParams P) {
       const int r = e / hp, d = e % hp;
       float x = 0.f;
       if (r < n_rows && d < hd)
-        x = ld_fresh(reinterpret_cast<const T*>(P.q) + (size_t)(sq.row0 + (r0 + r) / P.gs) * P.ldq +
+        x = ld_fresh(reinterpret_cast<const T*>(P.q) + (size_t)(run.s.row0 + (r0 + r) / P.gs) * P.ldq +
                      (size_t)(run.kvh * P.gs + (r0 + r) % P.gs) * hd + d);
       qs[r * pitch + d] = x;
     }
+    if (tid < ROWS) {
+      const int token = tid < n_rows ? run.s.row0 + (r0 + tid) / P.gs : -1;
+      const int lo = (P.window > 0 && token >= 0) ? max(__ldcg(P.token_pos + token) - P.window + 1, 0) : 0;
+      row_token[tid] = token; row_lo[tid] = lo;
+      if (lo > 0) atomicMax(&edge, lo);
+    }
     const bool busy = 2 * R * (tid >> 5) < n_rows;   // (warps without rows load and wait with the others)
-    int token[R], lo[R], lo_max = 0;
-    bool valid[R];
     float m[R], l[R];
     float4 acc[R][NC];
 #pragma unroll
     for (int e = 0; e < R; e++) {
-      const int r = R * ty + e;
       m[e] = -INFINITY; l[e] = 0.f;
-      valid[e] = r < n_rows;
-      token[e] = sq.row0 + (valid[e] ? (r0 + r) / P.gs : 0);
-      lo[e] = (P.window > 0 && valid[e]) ? max(__ldcg(P.token_pos + token[e]) - P.window + 1, 0) : 0;
-      lo_max = max(lo_max, lo[e]);
 #pragma unroll
       for (int j = 0; j < NC; j++) acc[e][j] = make_float4(0.f, 0.f, 0.f, 0.f);
     }
@@ -873,6 +877,9 @@ attention_tree_simple_kernel(const TreeParams P) {
       const int pg_next = i + 1 < run.n ? __ldcg(bt + i + 1) : -1;
       cp_async_wait<1>();                          // this page's keys are here (its values may be on their way)
       __syncthreads();
+      const bool masked = key0 + TR_KEYS > run.s.base || key0 < edge || !page_ok;
+      if (masked && tid < ROWS)
+        row_vis[tid] = row_token[tid] >= 0 ? tree_visible(P, run.s, row_token[tid], row_lo[tid], key0, page_ok) : 0;
       float s[R][4];
 #pragma unroll
       for (int e = 0; e < R; e++)
@@ -899,17 +906,14 @@ attention_tree_simple_kernel(const TreeParams P) {
       }
       __syncthreads();                             // the keys are read
       if (i + 1 < run.n) fetch(P.k_cache, pg_next, run.kvh, ks, pitch); else cp_async_commit();
-      unsigned long long vis[R];
-      const bool masked = key0 + TR_KEYS > sq.base || key0 < lo_max || !page_ok;
 #pragma unroll
       for (int e = 0; e < R; e++) {
-        vis[e] = ~0ull;
         if (!busy) continue;
-        if (masked) vis[e] = valid[e] ? tree_visible(P, sq, token[e], lo[e], key0, page_ok) : 0;
         float mx = -INFINITY;
+        const unsigned long long vis = masked ? row_vis[R * ty + e] >> tx : ~0ull;
 #pragma unroll
         for (int j = 0; j < 4; j++) {
-          s[e][j] = (vis[e] >> (tx + 16 * j)) & 1 ? s[e][j] * scale_log2 : -INFINITY;
+          s[e][j] = (vis >> (16 * j)) & 1 ? s[e][j] * scale_log2 : -INFINITY;
           mx = fmaxf(mx, s[e][j]);
         }
 #pragma unroll
@@ -933,7 +937,7 @@ attention_tree_simple_kernel(const TreeParams P) {
       cp_async_wait<1>();                          // its values too
       __syncthreads();
       bool odd = false;
-      if (__syncthreads_or(masked)) {              // zero times an infinity is not zero: are there any among the values?
+      if (masked) {                                // zero times an infinity is not zero: are there any among the values?
         if (page_ok)
           for (int e = tid; e < TR_KEYS * hp; e += TG_THREADS) odd = odd || !isfinite(vs[e]);
         odd = __syncthreads_or(odd);
@@ -949,7 +953,7 @@ attention_tree_simple_kernel(const TreeParams P) {
             const float4 x = *reinterpret_cast<const float4*>(vs + k * hp + d);
 #pragma unroll
             for (int e = 0; e < R; e++) {
-              if (!((vis[e] >> k) & 1)) continue;
+              if (!((row_vis[R * ty + e] >> k) & 1)) continue;
               const float p = p0[e * PK + k];
               acc[e][j].x = fmaf(p, x.x, acc[e][j].x); acc[e][j].y = fmaf(p, x.y, acc[e][j].y);
               acc[e][j].z = fmaf(p, x.z, acc[e][j].z); acc[e][j].w = fmaf(p, x.w, acc[e][j].w);
@@ -986,10 +990,10 @@ attention_tree_simple_kernel(const TreeParams P) {
     const int slot = 2 * blockIdx.x + (run.holds_u0 ? 0 : 1);
 #pragma unroll
     for (int e = 0; e < R; e++) {
-      if (!valid[e]) continue;
       const int r = R * ty + e;
+      if (r >= n_rows) continue;
       const float inv = 1.0f / l[e];
-      T* op = reinterpret_cast<T*>(P.out) + (size_t)token[e] * P.ldo + (size_t)(run.kvh * P.gs + (r0 + r) % P.gs) * hd;
+      T* op = reinterpret_cast<T*>(P.out) + (size_t)row_token[r] * P.ldo + (size_t)(run.kvh * P.gs + (r0 + r) % P.gs) * hd;
       float* po = P.part_o + ((size_t)slot * ROWS + r) * hp;
 #pragma unroll
       for (int j = 0; j < NC; j++) {
@@ -1161,7 +1165,7 @@ static int launch_tree_simple(const TreeParams& P, int G, cudaStream_t stream) {
   auto kern = attention_tree_simple_kernel<T, NC, R>;
   static unsigned long long done = 0;
   if (first_on_device(&done)) {
-    cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, 227 * 1024);
+    cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, 220 * 1024);
     if (e != cudaSuccess) { done = 0; return (int)e; }
   }
   return launch_pdl(kern, dim3(G), dim3(TG_THREADS), smem, stream, P);
@@ -1179,12 +1183,12 @@ static int launch_tree_simple_of(const TreeParams& P, int G, cudaStream_t stream
 // rows.  many: a tree has more rows than the smaller one of the two holds.
 STRATUM_EXPORT int stratum_attention_tree_slot_rows(int tensor, int many) { return tensor ? (many ? 256 : 128) : (many ? 64 : 32); }
 
-// CTAs of a launch (the scratch has two slots of rows for each): of the CUDA-core kernel as many share an SM as their
-// shared memory allows.
+// CTAs of a launch (the scratch has two slots of rows for each): one per SM, or of the CUDA-core kernel as many as find room.
 STRATUM_EXPORT int stratum_attention_tree_ctas(int tensor, int many, int head_dim) {
   if (tensor) return sm_count();
-  const int per_sm = (int)((size_t)(227 * 1024) / (simple_smem(head_dim, many ? 64 : 32, 0) + 1024));
-  return sm_count() * (per_sm < 1 ? 1 : per_sm > 4 ? 4 : per_sm);
+  const int most = head_dim <= 64 ? (many ? 2 : 3) : head_dim <= 128 ? (many ? 1 : 2) : 1;     // (by registers: see the kernel)
+  const int room = (int)((size_t)(227 * 1024) / (simple_smem(head_dim, many ? 64 : 32, 0) + 3072));
+  return sm_count() * (room < 1 ? 1 : room < most ? room : most);
 }
 
 // Scratch: part_o float32 [G][2][slot rows][head_dim rounded up to 4], part_ml float32 [G][2][slot rows][2], cut 32 bytes
