@@ -39,7 +39,8 @@
 #define TR_KEYS 64
 #define TR_MAX_SEQS 4096
 #define TR_SOFTMAX_WARPS 4                  // per half, a thread a row
-#define TR_THREADS (32 + 2 * 32 + 2 * TR_SOFTMAX_WARPS * 32)
+#define TR_THREADS (32 + 2 * 32 + 2 * TR_SOFTMAX_WARPS * 32 + 32)
+#define TR_RUNS 4
 
 struct TreeParams {
   const int* token_pos;                    // [tokens]
@@ -59,9 +60,10 @@ struct TreeParams {
 
 // What CTA c's stretch begins in, for the merge.
 struct alignas(16) TreeCut {
-  long long u0, item_begin;                // the stretch's first unit, the first unit of the item that holds it
-  int n_pages, kvh;                        // units of the item (0: the stretch is empty); its kv head,
+  long long u0, item_begin, total;         // the stretch's first unit, the first unit of the item that holds it, units in all
+  int n_pages, kvh;                        // pages of the item (0: the stretch begins in none of its pages); its kv head,
   int flat0, n_rows;                       // its first row (token of the batch * gs + head), its rows
+  int pad[2];
 };
 
 struct TreeSeq {                           // a sequence's share of the list
@@ -80,66 +82,62 @@ __device__ __forceinline__ TreeSeq tree_seq(const TreeParams& P, int b) {
   s.n_tiles = (int)(((long long)s.n_new * P.gs + P.rows_per_tile - 1) / P.rows_per_tile);
   return s;
 }
-__device__ __forceinline__ long long tree_begin(int c, int G, long long T) { return (long long)c * T / G; }
+// The list of units: every item (sequence, kv head, tile of rows) has one for each of its pages and TREE_ITEM_UNITS more
+// behind them, for what an item costs besides its pages.  (Without them a CTA whose stretch was made of short sequences took
+// 80 us where the others took 46.)  A short list is cut among fewer CTAs, TREE_LEAST_UNITS to each: what a piece of one page
+// saves in its own time, adding up its pieces costs again.
+#define TREE_ITEM_UNITS 3
+#define TREE_LEAST_UNITS 4
+__device__ __forceinline__ int tree_ctas(long long T, int G) {
+  const long long n = (T + TREE_LEAST_UNITS - 1) / TREE_LEAST_UNITS;
+  return n < 1 ? 1 : n < G ? (int)n : G;
+}
+__device__ __forceinline__ long long tree_begin(int c, int ctas, long long T) { return c >= ctas ? T : (long long)c * T / ctas; }
 
-// A stretch of pages of one (sequence, kv head, tile of rows).
+// A stretch of pages of one item.
 struct TreeRun {
   TreeSeq s;
-  int b, kvh, rt, page0, n;
+  int b, kvh, rt, page0, n;                // n = 0: there are no more
+  int edge;                                // the furthest window edge of the tile's rows
   bool from_start, to_end, holds_u0;
 };
 
 struct TreeCursor {
-  int u, n_units;                          // units behind us, units of the stretch
+  int left;                                // units of the stretch that are still ahead
   int b, item, off;
+  bool moved;
   TreeSeq s;
-  __device__ __forceinline__ void begin(const TreeParams& P, int n_units_, int b_, int item_, int off_) {
-    u = 0; n_units = n_units_; b = b_; item = item_; off = off_;
-    if (u < n_units) s = tree_seq(P, b);
+  __device__ __forceinline__ void step(const TreeParams& P, int n) {
+    moved = true;
+    off += n; left -= n;
+    if (off < s.n_pages + TREE_ITEM_UNITS) return;
+    off = 0;
+    if (++item < s.n_tiles * P.n_kv) return;
+    item = 0;
+    do { b++; if (b < P.n_seqs) s = tree_seq(P, b); } while (b < P.n_seqs && s.n_tiles == 0);
   }
-  __device__ __forceinline__ bool next(const TreeParams& P, TreeRun& r) {
-    if (u >= n_units) return false;
+  __device__ __forceinline__ void next(const TreeParams& P, TreeRun& r) {
+    if (left > 0 && off >= s.n_pages) step(P, min(s.n_pages + TREE_ITEM_UNITS - off, left));
+    if (left <= 0) { r.n = 0; return; }
+    const int n = min(s.n_pages - off, left);
     r.s = s; r.b = b;
     r.kvh = item / s.n_tiles; r.rt = item % s.n_tiles;
     r.page0 = s.first + off;
-    r.n = min(s.n_pages - off, n_units - u);
+    r.n = n;
+    r.edge = 0;
     r.from_start = off == 0;
-    r.to_end = off + r.n == s.n_pages;
-    r.holds_u0 = u == 0;
-    u += r.n; off += r.n;
-    if (off == s.n_pages) {
-      off = 0;
-      if (++item == s.n_tiles * P.n_kv) {
-        item = 0;
-        do { b++; if (b < P.n_seqs) s = tree_seq(P, b); } while (b < P.n_seqs && s.n_tiles == 0);
-      }
-    }
-    return true;
+    r.to_end = off + n == s.n_pages;
+    r.holds_u0 = !moved;
+    step(P, n);
   }
 };
 
-// A warp's walk over the runs of its CTA's stretch, kept in shared memory: in registers it would push the tile loops' values
-// out to local memory, which has next to no L1 beside the rings (a prompt-sized tree took 100 us with them there, of which
-// most was waiting for those loads).
-struct TreeWalk {
-  TreeCursor cur;
-  TreeRun run;
-  int more;
-};
-__device__ __forceinline__ bool tree_advance(const TreeParams& P, TreeWalk& w, int lane) {
-  __syncwarp();
-  if (lane == 0) w.more = w.cur.next(P, w.run);
-  __syncwarp();
-  return w.more != 0;
-}
-
 // Where CTA c begins; every thread of the block calls it.  `sums` holds a running sum per sequence for the while.
-struct TreeStart { int n_units, b, item, off; };
-__device__ __forceinline__ TreeStart tree_start(const TreeParams& P, long long* sums) {
+__device__ __forceinline__ TreeCursor tree_start(const TreeParams& P, long long* sums) {
   const int n_threads = blockDim.x, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   for (int b = threadIdx.x; b < P.n_seqs; b += n_threads) {
     const TreeSeq s = tree_seq(P, b);
-    sums[b + 1] = (long long)s.n_pages * s.n_tiles * P.n_kv;
+    sums[b + 1] = (long long)(s.n_pages + TREE_ITEM_UNITS) * s.n_tiles * P.n_kv;
   }
   if (threadIdx.x == 0) sums[0] = 0;
   __syncthreads();
@@ -158,39 +156,40 @@ __device__ __forceinline__ TreeStart tree_start(const TreeParams& P, long long* 
     }
   }
   __syncthreads();
-  TreeStart t;
+  TreeCursor t;
   const long long T = sums[P.n_seqs];
-  const int c = blockIdx.x, G = gridDim.x;
-  const long long u0 = tree_begin(c, G, T);
-  t.n_units = (int)(tree_begin(c + 1, G, T) - u0);
+  const int c = blockIdx.x, ctas = tree_ctas(T, gridDim.x);
+  const long long u0 = tree_begin(c, ctas, T);
+  t.left = (int)(tree_begin(c + 1, ctas, T) - u0);
   t.b = t.item = t.off = 0;
-  if (t.n_units > 0) {
+  t.moved = false;
+  TreeCut cut;
+  cut.u0 = u0; cut.item_begin = 0; cut.total = T; cut.n_pages = cut.kvh = cut.flat0 = cut.n_rows = 0;
+  if (t.left > 0) {
     int lo = 0, hi = P.n_seqs - 1;                // the last sequence that begins at or before u0 and is not empty
     while (lo < hi) {
       const int mid = (lo + hi + 1) >> 1;
       if (sums[mid] <= u0) lo = mid; else hi = mid - 1;
     }
-    const TreeSeq s = tree_seq(P, lo);
+    t.s = tree_seq(P, lo);
     const long long r = u0 - sums[lo];
-    t.b = lo; t.item = (int)(r / s.n_pages); t.off = (int)(r % s.n_pages);
-    if (threadIdx.x == 0) {
-      const int rt = t.item % s.n_tiles;
-      TreeCut cut;
-      cut.u0 = u0; cut.item_begin = u0 - t.off;
-      cut.n_pages = s.n_pages; cut.kvh = t.item / s.n_tiles;
-      cut.flat0 = s.row0 * P.gs + rt * P.rows_per_tile;
-      cut.n_rows = min(s.n_new * P.gs - rt * P.rows_per_tile, P.rows_per_tile);
-      P.cut[c] = cut;
+    const int per = t.s.n_pages + TREE_ITEM_UNITS;
+    t.b = lo; t.item = (int)(r / per); t.off = (int)(r % per);
+    if (t.off < t.s.n_pages) {
+      const int rt = t.item % t.s.n_tiles;
+      cut.item_begin = u0 - t.off;
+      cut.n_pages = t.s.n_pages; cut.kvh = t.item / t.s.n_tiles;
+      cut.flat0 = t.s.row0 * P.gs + rt * P.rows_per_tile;
+      cut.n_rows = min(t.s.n_new * P.gs - rt * P.rows_per_tile, P.rows_per_tile);
     }
-  } else if (threadIdx.x == 0) {
-    P.cut[c].u0 = u0; P.cut[c].n_pages = 0;
   }
+  if (threadIdx.x == 0) P.cut[c] = cut;
   return t;
 }
 
-// Which of the 64 keys from position `key0` on a drafted token sees.
+// Which of the 64 keys from position `key0` on a drafted token sees; word0: the first word of its mask.
 __device__ __forceinline__ unsigned long long tree_visible(const TreeParams& P, const TreeSeq& s, int token, int lo, int key0,
-                                                           bool page_ok) {
+                                                           bool page_ok, unsigned long long word0) {
   if (!page_ok) return 0;
   const unsigned long long all = ~0ull;
   unsigned long long cached = 0;
@@ -206,7 +205,7 @@ __device__ __forceinline__ unsigned long long tree_visible(const TreeParams& P, 
     const int n = min(s.n_new, 64 * P.words);
     auto word = [&](int w) -> unsigned long long {
       if (64 * w >= n) return 0;
-      const unsigned long long v = __ldcg(m + w);
+      const unsigned long long v = w == 0 ? word0 : __ldcg(m + w);
       return n - 64 * w >= 64 ? v : v & ((1ull << (n - 64 * w)) - 1);
     };
     if (to_base > 0) nodes = word(0) << to_base;
@@ -233,8 +232,10 @@ struct TreeSmem {
   float2 ml[2][ROWS2 ? 1 : 128];                                    // a row's maximum and sum in either half, at the end of a run
   uint64_t q_full[QB], q_empty[QB], k_full[STAGES], v_full[STAGES];
   uint64_t s_full[2][STAGES], pv_full[2][STAGES], p_full[2][2];
-  unsigned long long bad[2];
-  TreeWalk walk[2 + 2 + 2 * TR_SOFTMAX_WARPS];          // queries, pages, MMA warps, softmax warps
+  unsigned long long bad[2][2];
+  TreeRun runs[TR_RUNS];                                // the runs ahead, from the warp that walks the list
+  uint64_t run_full[TR_RUNS], run_empty[TR_RUNS];
+  uint64_t tile_meet[2], run_meet;                      // softmax warps wait for one another (bounded, as every wait)
   int row_of[32];                                       // cache row of a tile's page, from the K to the V request
   uint32_t tmem_base;
   int o_ready[2];
@@ -251,16 +252,11 @@ __device__ __forceinline__ float tr_exp2(float x) {
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
-__device__ __forceinline__ void tr_bar(int id, int n) { asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(n) : "memory"); }
-__device__ __forceinline__ bool tr_bar_or(int id, int n, bool mine) {
-  uint32_t r;
-  asm volatile(
-      "{\n\t.reg .pred p, q;\n\t"
-      "setp.ne.u32 q, %3, 0;\n\t"
-      "barrier.cta.red.or.pred p, %1, %2, q;\n\t"
-      "selp.u32 %0, 1, 0, p;\n\t}"
-      : "=r"(r) : "r"(id), "r"(n), "r"((uint32_t)mine) : "memory");
-  return r != 0;
+// The warps that `bar` counts wait for one another: false if one of them has given up.
+__device__ __forceinline__ bool tr_meet(uint64_t* bar, uint32_t phase, volatile int* abort_flag) {
+  __syncwarp();
+  if ((threadIdx.x & 31) == 0) mbar_arrive(bar);
+  return __all_sync(0xffffffffu, mbar_wait(bar, phase & 1, abort_flag));
 }
 // two outputs as bfloat16; zeros where the row's sum L is zero (it saw no key)
 __device__ __forceinline__ uint32_t tr_pack(float L, float a, float b) {
@@ -288,32 +284,34 @@ __device__ __forceinline__ void umma_bf16_ts(uint32_t tmem_d, uint32_t tmem_a, u
 // The two parts that only masked tiles need are functions of their own, so that the loop over the other tiles keeps its
 // registers.
 
-// The keys of a page of values (in shared memory) that hold anything not finite; their rows are zeroed.  The `n` threads of
-// barrier `id` come here together, numbered by `tid`.
+// The keys of a page of values (in shared memory) that hold anything not finite; their rows are zeroed.  The `n` threads that
+// meet at `bar` come here together, numbered by `tid`; `words` are two, used in turn (the other one is cleared for the next
+// time, by when everybody has seen it).  They meet once, and once more where there are such keys.  Whoever waits in vain
+// sets the flag.
 template <int HD>
-__device__ __noinline__ unsigned long long tree_look_through(uint4* v, unsigned long long* word, int id, int n, int tid, bool ok) {
+__device__ __noinline__ unsigned long long tree_look_through(uint4* v, unsigned long long* words, int n, int tid, uint64_t* bar,
+                                                             uint32_t phase, uint32_t turn, volatile int* abort_flag) {
   const int key = tid & 63, part = tid >> 6, n_parts = n >> 6;
-  uint4* row = v + key * 8;                              // 8 chunks of 16 bytes a key and block of 64 dims
+  uint4* row = v + key * 8;                              // 8 chunks of 16 bytes a key and block of 64 dims, visited from another
+  auto chunk = [&](int c) { return (c >> 3) * (TR_KEYS * 8) + ((c + key) & 7); };        // one on by each key: all banks
   bool mine = false;
-  if (ok) {
-    for (int c = part; c < HD / 8; c += n_parts) {
-      const uint4 x = row[(c >> 3) * (TR_KEYS * 8) + (c & 7)];
+  for (int c = part; c < HD / 8; c += n_parts) {
+    const uint4 x = row[chunk(c)];
 #pragma unroll
-      for (int e = 0; e < 4; e++) {
-        const uint32_t w = e == 0 ? x.x : e == 1 ? x.y : e == 2 ? x.z : x.w;
-        mine = mine || (w & 0x7f80u) == 0x7f80u || (w & 0x7f800000u) == 0x7f800000u;
-      }
+    for (int e = 0; e < 4; e++) {
+      const uint32_t w = e == 0 ? x.x : e == 1 ? x.y : e == 2 ? x.z : x.w;
+      mine = mine || (w & 0x7f80u) == 0x7f80u || (w & 0x7f800000u) == 0x7f800000u;
     }
   }
-  if (!tr_bar_or(id, n, mine)) return 0;
-  if (mine) atomicOr(word, 1ull << key);
-  tr_bar(id, n);
-  const unsigned long long bad = *(volatile unsigned long long*)word;
+  if (mine) atomicOr(&words[turn & 1], 1ull << key);
+  if (tid == 0) *(volatile unsigned long long*)&words[(turn & 1) ^ 1] = 0;
+  if (!tr_meet(bar, phase, abort_flag)) { *abort_flag = 1; return 0; }
+  const unsigned long long bad = *(volatile unsigned long long*)&words[turn & 1];
+  if (!bad) return 0;
   if ((bad >> key) & 1)
-    for (int c = part; c < HD / 8; c += n_parts) row[(c >> 3) * (TR_KEYS * 8) + (c & 7)] = make_uint4(0, 0, 0, 0);
+    for (int c = part; c < HD / 8; c += n_parts) row[chunk(c)] = make_uint4(0, 0, 0, 0);
   fence_async_shared();
-  tr_bar(id, n);
-  if (tid == 0) *(volatile unsigned long long*)word = 0;
+  if (!tr_meet(bar, phase + 1, abort_flag)) *abort_flag = 1;
   return bad;
 }
 
@@ -367,8 +365,11 @@ attention_tree_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
     }
     for (int h = 0; h < 2; h++) {
       mbar_init(&S.p_full[h][0], TR_SOFTMAX_WARPS); mbar_init(&S.p_full[h][1], TR_SOFTMAX_WARPS);
-      S.bad[h] = 0; S.o_ready[h] = 0;
+      S.bad[h][0] = S.bad[h][1] = 0; S.o_ready[h] = 0;
+      mbar_init(&S.tile_meet[h], ROWS2 ? 2 * TR_SOFTMAX_WARPS : TR_SOFTMAX_WARPS);
     }
+    for (int i = 0; i < TR_RUNS; i++) { mbar_init(&S.run_full[i], 1); mbar_init(&S.run_empty[i], 3 + 2 * TR_SOFTMAX_WARPS); }
+    mbar_init(&S.run_meet, 2 * TR_SOFTMAX_WARPS);
     S.abort_flag = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
@@ -377,7 +378,7 @@ attention_tree_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
     tmem_relinquish();
   }
   pdl_wait();                                           // everything below may read what the kernel before this one wrote
-  const TreeStart start = tree_start(P, reinterpret_cast<long long*>(S.k));
+  TreeCursor cur = tree_start(P, reinterpret_cast<long long*>(S.k));
   fence_async_shared();                                 // the sums lie where TMA will write
   tc_fence_before();
   __syncthreads();
@@ -385,13 +386,6 @@ attention_tree_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
   const uint32_t tmem_base = S.tmem_base;
   const int gs = P.gs;
   const int half_tokens = 128 / gs;                     // tokens of a half's 128 rows
-  TreeWalk& walk = S.walk[warp + 1];                    // (warp 0: [1]; [0] is its walk over the queries)
-  const TreeRun& run = walk.run;
-  if (lane == 0) {
-    walk.cur.begin(P, start.n_units, start.b, start.item, start.off);
-    if (warp == 0) S.walk[0].cur = walk.cur;
-  }
-  __syncwarp();
   auto half_ntok = [&](const TreeRun& r, int h) {       // tokens of the run's tile that half h holds
     const int t0 = ROWS2 ? (2 * r.rt + h) * half_tokens : r.rt * half_tokens;
     return min(max(r.s.n_new - t0, 0), half_tokens);
@@ -399,19 +393,15 @@ attention_tree_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
 
   if (warp == 0) {
     // ---------------------------------------------------------------- producer
-    if (lane == 0 && start.n_units > 0) {
+    if (lane == 0) {
       asm volatile("prefetch.tensormap [%0];" ::"l"(&map_q) : "memory");
       asm volatile("prefetch.tensormap [%0];" ::"l"(&map_k) : "memory");
       asm volatile("prefetch.tensormap [%0];" ::"l"(&map_v) : "memory");
-      const uint32_t n_units = (uint32_t)start.n_units;
-      TreeCursor& cq = S.walk[0].cur;
-      TreeRun& rq = S.walk[0].run;
-      bool more_q = cq.next(P, rq);
-      bool have = walk.cur.next(P, walk.run);
-      int tile = 0, nq = 0;
+      // runs whose queries, whose keys have been asked for, whose place in the ring has been given back
+      int nq = 0, nr = 0, given = 0;
+      bool more_q = true, more_k = true, in_run = false;
+      int tile = 0, pg = 0;
       uint32_t jk = 0, jv = 0;
-      const int* bt = P.block_table + (size_t)run.b * P.bt_stride;
-      int pg = __ldcg(bt + run.page0);
       auto freed = [&](uint64_t (*bars)[STAGES], uint32_t j) -> bool {   // tile j - STAGES has been read
         const uint32_t par = ((j / STAGES) - 1) & 1;
         if (ROWS2) return mbar_test_wait(&bars[0][j % STAGES], par) && mbar_test_wait(&bars[1][j % STAGES], par);
@@ -419,23 +409,38 @@ attention_tree_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
       };
       uint32_t idle = 0;
       bool ok = true;
-      while ((more_q || jv < n_units) && ok) {
+      while ((more_q || more_k || jv < jk) && ok) {
         bool moved = false;
-        if (more_q && (nq < QB || mbar_test_wait(&S.q_empty[nq % QB], ((nq / QB) - 1) & 1))) {
-          uint64_t* bar = &S.q_full[nq % QB];
-          const uint32_t box = (uint32_t)half_tokens * gs * HD * sizeof(bf16);
-          const bool second = ROWS2 && half_ntok(rq, 1) > 0;
-          mbar_expect_tx(bar, second ? 2 * box : box);
-          const int tok0 = rq.s.row0 + rq.rt * half_tokens * (ROWS2 ? 2 : 1);
-          for (int db = 0; db < DB; db++) {
-            tma_load_3d(&map_q, S.q[ROWS2 ? 0 : nq % QB] + db * 128 * 64, bar, db * 64, rq.kvh * gs, tok0);
-            if (second) tma_load_3d(&map_q, S.q[1] + db * 128 * 64, bar, db * 64, rq.kvh * gs, tok0 + half_tokens);
+        if (more_q && mbar_test_wait(&S.run_full[nq % TR_RUNS], (nq / TR_RUNS) & 1)) {
+          const TreeRun& rq = S.runs[nq % TR_RUNS];
+          if (rq.n == 0) {
+            more_q = false;
+            moved = true;
+          } else if (nq < QB || mbar_test_wait(&S.q_empty[nq % QB], ((nq / QB) - 1) & 1)) {
+            uint64_t* bar = &S.q_full[nq % QB];
+            const uint32_t box = (uint32_t)half_tokens * gs * HD * sizeof(bf16);
+            const bool second = ROWS2 && half_ntok(rq, 1) > 0;
+            mbar_expect_tx(bar, second ? 2 * box : box);
+            const int tok0 = rq.s.row0 + rq.rt * half_tokens * (ROWS2 ? 2 : 1);
+            for (int db = 0; db < DB; db++) {
+              tma_load_3d(&map_q, S.q[ROWS2 ? 0 : nq % QB] + db * 128 * 64, bar, db * 64, rq.kvh * gs, tok0);
+              if (second) tma_load_3d(&map_q, S.q[1] + db * 128 * 64, bar, db * 64, rq.kvh * gs, tok0 + half_tokens);
+            }
+            nq++;
+            moved = true;
           }
-          nq++;
-          more_q = cq.next(P, rq);
+        }
+        if (more_k && !in_run && mbar_test_wait(&S.run_full[nr % TR_RUNS], (nr / TR_RUNS) & 1)) {
+          const TreeRun& run = S.runs[nr % TR_RUNS];
+          if (run.n == 0) more_k = false;
+          else {
+            in_run = true; tile = 0;
+            pg = __ldcg(P.block_table + (size_t)run.b * P.bt_stride + run.page0);
+          }
           moved = true;
         }
-        if (have && (jk < STAGES || freed(S.s_full, jk))) {
+        if (in_run && (jk < STAGES || freed(S.s_full, jk))) {
+          const TreeRun& run = S.runs[nr % TR_RUNS];
           const int s = jk % STAGES;
           // (a page number outside the pool: some page's rows are fetched and nobody sees them)
           const int row = (int)(((long long)((unsigned)pg < (unsigned)P.n_pages ? pg : 0) * P.n_kv + run.kvh) * TR_KEYS);
@@ -443,14 +448,11 @@ attention_tree_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
           mbar_expect_tx(&S.k_full[s], TR_KEYS * HD * sizeof(bf16));
           for (int db = 0; db < DB; db++) tma_load_2d(&map_k, S.k[s] + db * TR_KEYS * 64, &S.k_full[s], db * 64, row);
           jk++;
-          if (++tile == run.n) {
-            tile = 0;
-            have = walk.cur.next(P, walk.run);
-            bt = P.block_table + (size_t)run.b * P.bt_stride;
-          }
-          if (have) pg = __ldcg(bt + run.page0 + tile);
+          if (++tile == run.n) { in_run = false; nr++; }
+          else pg = __ldcg(P.block_table + (size_t)run.b * P.bt_stride + run.page0 + tile);
           moved = true;
         }
+        if (given < nq && given < nr) { mbar_arrive(&S.run_empty[given % TR_RUNS]); given++; }
         if (jv < jk && (jv < STAGES || freed(S.pv_full, jv))) {
           const int s = jv % STAGES, row = S.row_of[jv & 31];
           mbar_expect_tx(&S.v_full[s], TR_KEYS * HD * sizeof(bf16));
@@ -499,7 +501,10 @@ attention_tree_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
       }
       __syncwarp();
     };
-    for (int r = 0; ok && tree_advance(P, walk, lane); r++) {
+    for (int r = 0; ok; r++) {
+      if (!__all_sync(0xffffffffu, mbar_wait(&S.run_full[r % TR_RUNS], (r / TR_RUNS) & 1, abort_flag))) { if (lane == 0) TR_FAIL(511); ok = false; break; }
+      const TreeRun& run = S.runs[r % TR_RUNS];
+      if (run.n == 0) break;
       const bool active = !ROWS2 || half_ntok(run, h) > 0;
       if (!__all_sync(0xffffffffu, mbar_wait(&S.q_full[r % QB], (r / QB) & 1, abort_flag))) { if (lane == 0) TR_FAIL(502); ok = false; break; }
       const uint64_t qd = smem_desc_sw128(smem_u32(S.q[ROWS2 ? h : r % QB]));
@@ -538,10 +543,11 @@ attention_tree_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
       if (ok) {                                          // the run's scores are issued: its queries are free behind them
         if (elect_one()) umma_commit(&S.q_empty[r % QB]);
         __syncwarp();
+        if (lane == 0) mbar_arrive(&S.run_empty[r % TR_RUNS]);
       }
     }
     if (ok && pend) values();
-  } else {
+  } else if (warp < 3 + 2 * TR_SOFTMAX_WARPS) {
     // ---------------------------------------------------------------- softmax (four warps per half, a thread a row)
     const int h = (warp - 3) / TR_SOFTMAX_WARPS;
     const int quarter = warp & 3;                        // tensor-memory lanes this warp may read
@@ -552,25 +558,23 @@ attention_tree_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
     const uint32_t o_addr = lane_addr + COL_PV;
     const float to_log2 = P.scale * 1.4426950408889634f;
     constexpr int STEP = ROWS2 ? 1 : 2;                  // from a tile of this half to the next
-    const int tile_bar = ROWS2 ? 1 : 1 + h, tile_threads = ROWS2 ? 2 * TR_SOFTMAX_WARPS * 32 : TR_SOFTMAX_WARPS * 32;
+    const int tile_threads = ROWS2 ? 2 * TR_SOFTMAX_WARPS * 32 : TR_SOFTMAX_WARPS * 32;
     const int tile_tid = ROWS2 ? threadIdx.x - 96 : threadIdx.x - 96 - h * TR_SOFTMAX_WARPS * 32;
     bool ok = true;
-    uint32_t it = 0, i = 0;
-    while (tree_advance(P, walk, lane)) {
+    uint32_t it = 0, i = 0, tile_phase = 0, run_phase = 0, turn = 0;
+#define TR_WAIT(bar, parity, code) \
+  if (!__all_sync(0xffffffffu, mbar_wait(bar, parity, abort_flag))) { if (lane == 0) TR_FAIL(code); ok = false; break; }
+    for (int r = 0; ok; r++) {
+      TR_WAIT(&S.run_full[r % TR_RUNS], (r / TR_RUNS) & 1, 511)
+      const TreeRun& run = S.runs[r % TR_RUNS];
+      if (run.n == 0) break;
       const TreeSeq& sq = run.s;
       const int ntok = half_ntok(run, h);
       const bool valid = tok < ntok;
       const bool warp_active = quarter * 32 < ntok * gs;
       const int token = sq.row0 + (ROWS2 ? 2 * run.rt + h : run.rt) * half_tokens + (valid ? tok : 0);
-      int lo = 0, lo_max = 0;
-      if (P.window > 0) {
-        lo = valid ? max(__ldcg(P.token_pos + token) - P.window + 1, 0) : 0;
-        // the furthest edge of the tile's rows (all rows of both halves: the halves decide alike)
-        const int t0 = sq.row0 + run.rt * half_tokens * (ROWS2 ? 2 : 1);
-        const int t1 = min(t0 + half_tokens * (ROWS2 ? 2 : 1), sq.row0 + sq.n_new);
-        for (int t = t0 + lane; t < t1; t += 32) lo_max = max(lo_max, __ldcg(P.token_pos + t) - P.window + 1);
-        lo_max = __reduce_max_sync(0xffffffffu, lo_max);
-      }
+      const int lo = (P.window > 0 && valid) ? max(__ldcg(P.token_pos + token) - P.window + 1, 0) : 0;
+      const unsigned long long word0 = valid ? __ldcg(P.mask + (size_t)token * P.words) : 0;      // (for the last page or two)
       const uint32_t it_first = it, it_end = it + run.n;
       if (!ROWS2 && (int)(it & 1) != h) it++;
       const uint32_t it_mine = it;                       // this half's first tile of the run (it_end or beyond: none)
@@ -583,30 +587,20 @@ attention_tree_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
         const int pg = pg_next;
         if (it + STEP < it_end) pg_next = __ldcg(bt + (int)it + STEP);
         const bool page_ok = (unsigned)pg < (unsigned)P.n_pages;
-        const bool needs_mask = key0 + TR_KEYS > sq.base || key0 < lo_max || !page_ok;
+        const bool needs_mask = key0 + TR_KEYS > sq.base || key0 < run.edge || !page_ok;
         const bool first = it == it_mine;
-        if (ok && !__all_sync(0xffffffffu, mbar_wait(&S.s_full[h][s], (it / STAGES) & 1, abort_flag))) {
-          if (lane == 0) TR_FAIL(509);
-          ok = false;
-        }
+        TR_WAIT(&S.s_full[h][s], (it / STAGES) & 1, 509)
         unsigned long long vis = 0, bad = 0;
         if (needs_mask) {
-          if (valid) vis = tree_visible(P, sq, token, lo, key0, page_ok);
-          if (ok && !__all_sync(0xffffffffu, mbar_wait(&S.v_full[s], (it / STAGES) & 1, abort_flag))) {
-            if (lane == 0) TR_FAIL(507);
-            ok = false;
-          }
-          bad = tree_look_through<HD>(reinterpret_cast<uint4*>(S.v[s]), &S.bad[ROWS2 ? 0 : h], tile_bar, tile_threads, tile_tid, ok);
+          if (valid) vis = tree_visible(P, sq, token, lo, key0, page_ok, word0);
+          TR_WAIT(&S.v_full[s], (it / STAGES) & 1, 507)
+          bad = tree_look_through<HD>(reinterpret_cast<uint4*>(S.v[s]), S.bad[ROWS2 ? 0 : h], tile_threads, tile_tid,
+                                      &S.tile_meet[ROWS2 ? 0 : h], tile_phase, turn, abort_flag);
+          turn++;
+          tile_phase += bad ? 2 : 1;
+          if (*abort_flag) { if (lane == 0) TR_FAIL(513); ok = false; break; }
         }
-        // P V of this half's tile before is in O
-        auto wait_before = [&]() {
-          const uint32_t before = it - STEP;
-          if (ok && !__all_sync(0xffffffffu, mbar_wait(&S.pv_full[h][before % STAGES], (before / STAGES) & 1, abort_flag))) {
-            if (lane == 0) TR_FAIL(508);
-            ok = false;
-          }
-        };
-        if (ok && warp_active) {
+        if (warp_active) {
           tc_fence_after();
           float sc[TR_KEYS];
           {
@@ -649,8 +643,11 @@ attention_tree_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
             packed[e >> 1] = u;
           }
           const bool move = __any_sync(0xffffffffu, grow);
-          if (!first && (move || bad)) wait_before();
-          if (ok && !first && move) {
+          if (!first && (move || bad)) {                 // P V of this half's tile before is in O
+            const uint32_t before = it - STEP;
+            TR_WAIT(&S.pv_full[h][before % STAGES], (before / STAGES) & 1, 508)
+          }
+          if (!first && move) {
             tc_fence_after();
 #pragma unroll 1
             for (int c = 0; c < HD; c += 32) {
@@ -663,7 +660,7 @@ attention_tree_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
             }
           }
           l = fmaf(l, corr, (sum[0] + sum[1]) + (sum[2] + sum[3]));
-          if (bad && ok) {                               // what values that are not finite give to the rows that see them
+          if (bad) {                                     // what values that are not finite give to the rows that see them
             tc_fence_after();
             tmem_st_wait();
             tree_add_bad<HD>(bad, vis, lane_addr + b * TR_KEYS, o_addr, to_log2, m_use,
@@ -676,16 +673,14 @@ attention_tree_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
         if (first && quarter == 0 && lane == 0) S.o_ready[h] = bad != 0;   // (`bad` is the same in all of them)
         tc_fence_before();
         __syncwarp();
-        if (ok && lane == 0) mbar_arrive(&S.p_full[h][b]);
+        if (lane == 0) mbar_arrive(&S.p_full[h][b]);
         i++;
       }
+      if (!ok) break;
       // ---- the run is over
       if (it_mine < it_end) {
         const uint32_t last = it - STEP;
-        if (ok && !__all_sync(0xffffffffu, mbar_wait(&S.pv_full[h][last % STAGES], (last / STAGES) & 1, abort_flag))) {
-          if (lane == 0) TR_FAIL(508);
-          ok = false;
-        }
+        TR_WAIT(&S.pv_full[h][last % STAGES], (last / STAGES) & 1, 508)
       }
       it = it_end;
       const bool whole = run.from_start && run.to_end;
@@ -693,7 +688,7 @@ attention_tree_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
       bf16* out_row = reinterpret_cast<bf16*>(P.out) + (size_t)token * P.ldo + (size_t)(run.kvh * gs + head) * HD;
       tc_fence_after();
       if (ROWS2) {
-        if (ok && !*abort_flag && warp_active) {
+        if (warp_active) {
           const float inv = 1.0f / l;
           float* po = P.part_o + ((size_t)slot * 256 + h * 128 + row) * HD;
 #pragma unroll 1
@@ -723,9 +718,9 @@ attention_tree_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
         // both halves hold the same rows: half of the dims for each of a row's two threads
         S.ml[h][row] = make_float2(m_ref, l);
         tc_fence_before();
-        tr_bar(3, 2 * TR_SOFTMAX_WARPS * 32);
+        if (!tr_meet(&S.run_meet, run_phase++, abort_flag)) { if (lane == 0) TR_FAIL(514); ok = false; break; }
         tc_fence_after();
-        if (ok && !*abort_flag && warp_active) {
+        if (warp_active) {
           const float2 a0 = S.ml[0][row], a1 = S.ml[1][row];
           const float M = fmaxf(a0.x, a1.x), Mu = M == -INFINITY ? 0.f : M;
           const float f0 = tr_exp2(a0.x - Mu), f1 = tr_exp2(a1.x - Mu);
@@ -774,8 +769,31 @@ attention_tree_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
           if (valid && !whole && h == 0) P.part_ml[(size_t)slot * 128 + row] = make_float2(M, L);
         }
         tc_fence_before();
-        tr_bar(3, 2 * TR_SOFTMAX_WARPS * 32);
+        if (!tr_meet(&S.run_meet, run_phase++, abort_flag)) { if (lane == 0) TR_FAIL(514); ok = false; break; }
       }
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&S.run_empty[r % TR_RUNS]);
+    }
+  } else {
+    // ---------------------------------------------------------------- the walk over the list
+    // A run is described here while the ones before it are worked on: what it takes from memory would otherwise stand
+    // between two runs of every other warp.
+    for (int r = 0;; r++) {
+      TreeRun& run = S.runs[r % TR_RUNS];
+      if (r >= TR_RUNS && !__all_sync(0xffffffffu, mbar_wait(&S.run_empty[r % TR_RUNS], ((r / TR_RUNS) - 1) & 1, abort_flag))) { if (lane == 0) TR_FAIL(512); break; }
+      if (lane == 0) cur.next(P, run);
+      __syncwarp();
+      const int n = run.n;
+      if (n > 0 && P.window > 0) {                       // the furthest window edge of the tile's rows, in both halves
+        const int per = half_tokens * (ROWS2 ? 2 : 1), t0 = run.s.row0 + run.rt * per, t1 = min(t0 + per, run.s.row0 + run.s.n_new);
+        int edge = 0;
+        for (int t = t0 + lane; t < t1; t += 32) edge = max(edge, __ldcg(P.token_pos + t) - P.window + 1);
+        edge = __reduce_max_sync(0xffffffffu, edge);
+        if (lane == 0) run.edge = edge;
+      }
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&S.run_full[r % TR_RUNS]);
+      if (n == 0) break;
     }
   }
   tc_fence_before();
@@ -807,7 +825,7 @@ attention_tree_simple_kernel(const TreeParams P) {
   extern __shared__ __align__(16) float tg_smem[];
   constexpr int ROWS = 16 * R, PK = TR_KEYS + 4;
   // what concerns the run and its rows lies in shared memory, as the registers are the products'
-  __shared__ TreeWalk walk;
+  __shared__ TreeRun run;
   __shared__ unsigned long long row_vis[ROWS];     // which keys of a masked page a row sees
   __shared__ int row_token[ROWS], row_lo[ROWS], edge;
   const int hd = P.head_dim, hp = (hd + 3) & ~3, pitch = hp + 4;
@@ -816,7 +834,7 @@ attention_tree_simple_kernel(const TreeParams P) {
   float* vs = ks + TR_KEYS * pitch;                // [64][hp]
   float* ps = vs + TR_KEYS * hp;                   // [ROWS][PK]
   pdl_wait();
-  const TreeStart start = tree_start(P, reinterpret_cast<long long*>(tg_smem));
+  TreeCursor cur = tree_start(P, reinterpret_cast<long long*>(tg_smem));
   const int tid = threadIdx.x, ty = tid >> 4, tx = tid & 15;
   const float scale_log2 = P.scale * 1.4426950408889634f;
   const bool direct = sizeof(T) == 4 && hd == hp && (((uintptr_t)P.k_cache | (uintptr_t)P.v_cache) & 15) == 0;
@@ -836,13 +854,11 @@ attention_tree_simple_kernel(const TreeParams P) {
     }
     cp_async_commit();
   };
-  if (tid == 0) walk.cur.begin(P, start.n_units, start.b, start.item, start.off);
-  const TreeRun& run = walk.run;
   for (;;) {
     __syncthreads();                               // (the run before, or the start, may still be reading)
-    if (tid == 0) { walk.more = walk.cur.next(P, walk.run); edge = 0; }
+    if (tid == 0) { cur.next(P, run); edge = 0; }
     __syncthreads();
-    if (!walk.more) break;
+    if (run.n == 0) break;
     const int r0 = run.rt * ROWS, n_rows = min(run.s.n_new * P.gs - r0, ROWS);
     const int* bt = P.block_table + (size_t)run.b * P.bt_stride + run.page0;
     int pg = __ldcg(bt);
@@ -879,7 +895,7 @@ attention_tree_simple_kernel(const TreeParams P) {
       __syncthreads();
       const bool masked = key0 + TR_KEYS > run.s.base || key0 < edge || !page_ok;
       if (masked && tid < ROWS)
-        row_vis[tid] = row_token[tid] >= 0 ? tree_visible(P, run.s, row_token[tid], row_lo[tid], key0, page_ok) : 0;
+        row_vis[tid] = row_token[tid] >= 0 ? tree_visible(P, run.s, row_token[tid], row_lo[tid], key0, page_ok, __ldcg(P.mask + (size_t)row_token[tid] * P.words)) : 0;
       float s[R][4];
 #pragma unroll
       for (int e = 0; e < R; e++)
@@ -1019,26 +1035,18 @@ attention_tree_simple_kernel(const TreeParams P) {
 // up where the stretches begin and fetch the pieces' maxima and sums.
 #define TM_ROWS 4
 template <typename T, int NJ>
-__global__ void __launch_bounds__(256)
+__global__ void __launch_bounds__(256, 2)
 attention_tree_merge_kernel(const TreeParams P, int G, int slot_half, int half_rows) {
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   pdl_wait();
   const int c = blockIdx.x + 1;
-  // (all of this was written by the kernel before, and is read past L1)
-  const int4 cut_lo = __ldcg(reinterpret_cast<const int4*>(P.cut + c)), cut_hi = __ldcg(reinterpret_cast<const int4*>(P.cut + c) + 1);
-  TreeCut cut;
-  reinterpret_cast<int4*>(&cut)[0] = cut_lo; reinterpret_cast<int4*>(&cut)[1] = cut_hi;
-  const long long u0 = cut.u0, ib = cut.item_begin, ie = ib + cut.n_pages;
-  if (cut.n_pages == 0 || u0 == ib) return;
-  // the last CTA before c that has anything (a short list leaves some idle)
-  int first = -1;
-  long long ub = 0;
-  for (int i0 = c - 1; first < 0 && i0 >= 0; i0 -= 32) {
-    const long long u = i0 - lane >= 0 ? __ldcg(&P.cut[i0 - lane].u0) : u0;
-    const unsigned have = __ballot_sync(0xffffffffu, u < u0);
-    if (have) { const int l = __ffs(have) - 1; first = i0 - l; ub = __shfl_sync(0xffffffffu, u, l); }
-  }
-  if (first < 0 || ub > ib) return;
+  TreeCut cut;                                     // (written by the kernel before, and read past L1)
+#pragma unroll
+  for (int x = 0; x < 3; x++) reinterpret_cast<int4*>(&cut)[x] = __ldcg(reinterpret_cast<const int4*>(P.cut + c) + x);
+  const long long T_ = cut.total, ib = cut.item_begin, ie = ib + cut.n_pages;
+  const int ctas = tree_ctas(T_, G), first = c - 1;
+  const long long ub = tree_begin(first, ctas, T_);
+  if (cut.n_pages == 0 || cut.u0 == ib || ub > ib) return;         // no cut, or not the item's first
   const int r0 = (blockIdx.y * 8 + warp) * TM_ROWS;
   if (r0 >= cut.n_rows) return;
   const int hd = P.head_dim, hp = (hd + 3) & ~3;
@@ -1057,22 +1065,17 @@ attention_tree_merge_kernel(const TreeParams P, int G, int slot_half, int half_r
 #pragma unroll
     for (int j = 0; j < NJ; j++) acc[x][j] = make_float4(0.f, 0.f, 0.f, 0.f);
   }
-  // 32 stretches at a time, from `first` on; an item of few pages is over within the first of them
-  for (int i0 = first; i0 < G; i0 += 32) {
+  // 32 pieces at a time, the stretches from `first` on that begin in front of the item's end
+  for (int i0 = first; ; i0 += 32) {
     const int i = i0 + lane;
-    const long long u = i < G ? __ldcg(&P.cut[i].u0) : ie;
-    const bool any = i < G && (i == first || (u < ie && __ldcg(&P.cut[i].n_pages) > 0));
+    const bool any = i == first || (i < ctas && tree_begin(i, ctas, T_) < ie);
     const unsigned have = __ballot_sync(0xffffffffu, any);
-    const bool over = __any_sync(0xffffffffu, u >= ie);
-    if (!have) {                                   // (a short list leaves stretches of idle CTAs between its pieces)
-      if (over) break;
-      continue;
-    }
-    const size_t slot = (size_t)(2 * i + ((i == first && ub != ib) ? 1 : 0)) * slot_rows;
+    const int count = __popc(have);
+    auto piece = [&](int at) { return (size_t)(2 * at + ((at == first && ub != ib) ? 1 : 0)) * slot_rows; };
     float w[TM_ROWS];
 #pragma unroll
     for (int x = 0; x < TM_ROWS; x++) {
-      const float2 ml = any ? __ldcg(&P.part_ml[slot + srow[x]]) : make_float2(-INFINITY, 0.f);
+      const float2 ml = any ? __ldcg(&P.part_ml[piece(i) + srow[x]]) : make_float2(-INFINITY, 0.f);
       const float m = fmaxf(M[x], warp_max(ml.x)), mu = m == -INFINITY ? 0.f : m;
       const float corr = exp2f(M[x] - mu);
       w[x] = exp2f(ml.x - mu);
@@ -1081,24 +1084,33 @@ attention_tree_merge_kernel(const TreeParams P, int G, int slot_half, int half_r
 #pragma unroll
       for (int j = 0; j < NJ; j++) { acc[x][j].x *= corr; acc[x][j].y *= corr; acc[x][j].z *= corr; acc[x][j].w *= corr; }
     }
-    for (unsigned left = have; left; left &= left - 1) {
-      const int l = __ffs(left) - 1;
-      const size_t piece = (size_t)(2 * (i0 + l) + ((i0 + l == first && ub != ib) ? 1 : 0)) * slot_rows;
+    constexpr int PB = 4;                          // pieces whose values are on their way together
+    for (int l0 = 0; l0 < count; l0 += PB) {
 #pragma unroll
-      for (int x = 0; x < TM_ROWS; x++) {
-        const float wk = __shfl_sync(0xffffffffu, w[x], l);
+      for (int j = 0; j < NJ; j++) {
+        const int d = 4 * (lane + 32 * j);
+        float4 v[PB][TM_ROWS];
 #pragma unroll
-        for (int j = 0; j < NJ; j++) {
-          const int d = 4 * (lane + 32 * j);
-          if (wk != 0.f && d < hp) {               // (no key seen: the piece may hold anything)
-            const float4 v = __ldcg(reinterpret_cast<const float4*>(P.part_o + (piece + srow[x]) * hp + d));
-            acc[x][j].x = fmaf(wk, v.x, acc[x][j].x); acc[x][j].y = fmaf(wk, v.y, acc[x][j].y);
-            acc[x][j].z = fmaf(wk, v.z, acc[x][j].z); acc[x][j].w = fmaf(wk, v.w, acc[x][j].w);
+        for (int y = 0; y < PB; y++)
+#pragma unroll
+          for (int x = 0; x < TM_ROWS; x++) {
+            v[y][x] = make_float4(0.f, 0.f, 0.f, 0.f);
+            if (l0 + y < count && d < hp)
+              v[y][x] = __ldcg(reinterpret_cast<const float4*>(P.part_o + (piece(i0 + l0 + y) + srow[x]) * hp + d));
           }
-        }
+#pragma unroll
+        for (int y = 0; y < PB; y++)
+#pragma unroll
+          for (int x = 0; x < TM_ROWS; x++) {
+            const float wk = __shfl_sync(0xffffffffu, w[x], (l0 + y) & 31);
+            if (l0 + y < count && wk != 0.f) {     // (no key seen: the piece may hold anything)
+              acc[x][j].x = fmaf(wk, v[y][x].x, acc[x][j].x); acc[x][j].y = fmaf(wk, v[y][x].y, acc[x][j].y);
+              acc[x][j].z = fmaf(wk, v[y][x].z, acc[x][j].z); acc[x][j].w = fmaf(wk, v[y][x].w, acc[x][j].w);
+            }
+          }
       }
     }
-    if (over) break;
+    if (count < 32) break;
   }
 #pragma unroll
   for (int x = 0; x < TM_ROWS; x++) {
@@ -1191,7 +1203,7 @@ STRATUM_EXPORT int stratum_attention_tree_ctas(int tensor, int many, int head_di
   return sm_count() * (room < 1 ? 1 : room < most ? room : most);
 }
 
-// Scratch: part_o float32 [G][2][slot rows][head_dim rounded up to 4], part_ml float32 [G][2][slot rows][2], cut 32 bytes
+// Scratch: part_o float32 [G][2][slot rows][head_dim rounded up to 4], part_ml float32 [G][2][slot rows][2], cut 48 bytes
 // a CTA.
 STRATUM_EXPORT int stratum_attention_tree(const void* q, int ldq, const void* k_cache, const void* v_cache, long long n_pages,
                                           int dtype, const int* token_pos, const void* mask, int words,

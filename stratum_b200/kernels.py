@@ -495,7 +495,7 @@ def check_status() -> None:
         _status_word.zero_()
         where = {101: "the TMA producer waiting for a free stage", 102: "the MMA warp waiting for a free accumulator",
                  103: "the MMA warp waiting for a loaded stage", 104: "the epilogue waiting for an accumulator",
-                 **{c: "the attention of drafted tokens" for c in (501, 502, 503, 504, 505, 506, 507, 508, 509, 510)},
+                 **{c: "the attention of drafted tokens" for c in range(501, 515)},
                  431: "the resident decode step's ring (a free stage)", 432: "the resident decode step's ring (a filled stage)",
                  **{c: "a block of the resident decode step waiting for the others" for c in (401, 402, 403, 405, 411, 421)}}
         raise KernelError(f"a device-side wait ran out in {where.get(code, f'code {code}')}; results are invalid")
@@ -1742,7 +1742,7 @@ def attention_tree(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor
                                    int(lib.stratum_attention_tree_slot_rows(int(tensor), int(many))))
     ctas, slots = plan[0], 2 * plan[0] * plan[1]
     # (scratch of this call's own: calls on several streams, and captured ones, do not meet in it)
-    scratch = torch.empty(slots * ((head_dim + 3) // 4 * 4 + 2) + 8 * ctas, dtype=torch.float32, device=q.device)
+    scratch = torch.empty(slots * ((head_dim + 3) // 4 * 4 + 2) + 12 * ctas, dtype=torch.float32, device=q.device)
     at = scratch.data_ptr()
     part_ml = at + 4 * slots * ((head_dim + 3) // 4 * 4)
     f = _fn("attention_tree", "stratum_attention_tree",
