@@ -1205,34 +1205,42 @@ STRATUM_EXPORT int stratum_attention_tree_ctas(int tensor, int many, int head_di
 
 // Scratch: part_o float32 [G][2][slot rows][head_dim rounded up to 4], part_ml float32 [G][2][slot rows][2], cut 48 bytes
 // a CTA.
-STRATUM_EXPORT int stratum_attention_tree(const void* q, int ldq, const void* k_cache, const void* v_cache, long long n_pages,
-                                          int dtype, const int* token_pos, const void* mask, int words,
-                                          const int* seq_start, const int* seq_len, const int* block_table, int bt_stride,
-                                          int bt_width, void* out, int ldo, int n_tokens, int n_seqs, int n_q, int n_kv,
-                                          int head_dim, int page_tokens, int window, float scale, int tensor, int many,
-                                          float* part_o, void* part_ml, void* cut, int* status, cudaStream_t stream) {
+// One call's numbers, as the launcher packs them (pointers first, then 8 bytes, then 4).
+struct TreeCall {
+  const void *q, *k_cache, *v_cache, *token_pos, *mask, *seq_start, *seq_len, *block_table;
+  void *out, *part_o, *part_ml, *cut, *status;
+  long long n_pages;
+  int dtype, ldq, ldo, words, bt_stride, bt_width, n_tokens, n_seqs, n_q, n_kv, head_dim, page_tokens, window, tensor, many;
+  float scale;
+};
+
+STRATUM_EXPORT int stratum_attention_tree(const TreeCall* call, cudaStream_t stream) {
+  const TreeCall& a = *call;
+  const int n_tokens = a.n_tokens, n_seqs = a.n_seqs, n_q = a.n_q, n_kv = a.n_kv, head_dim = a.head_dim, dtype = a.dtype;
+  const int ldq = a.ldq, ldo = a.ldo, tensor = a.tensor, many = a.many;
+  const long long n_pages = a.n_pages;
   if (n_tokens <= 0 || n_seqs <= 0) return 0;
   if (dtype != STRATUM_DT_F32 && dtype != STRATUM_DT_BF16) return STRATUM_ERR_DTYPE;
-  if (n_kv < 1 || n_q < 1 || n_q % n_kv != 0 || page_tokens != TR_KEYS || head_dim < 1 || head_dim > 256) return STRATUM_ERR_SHAPE;
-  if (words < 1 || bt_width < 1 || window < 0 || n_pages < 1) return STRATUM_ERR_SHAPE;
+  if (n_kv < 1 || n_q < 1 || n_q % n_kv != 0 || a.page_tokens != TR_KEYS || head_dim < 1 || head_dim > 256) return STRATUM_ERR_SHAPE;
+  if (a.words < 1 || a.bt_width < 1 || a.window < 0 || n_pages < 1) return STRATUM_ERR_SHAPE;
   if (n_seqs > TR_MAX_SEQS || n_pages * n_kv * TR_KEYS > 0x7fffffffLL) return STRATUM_ERR_LIMIT;
   const int gs = n_q / n_kv;
   if ((long long)n_tokens * gs > 0x7fffffffLL) return STRATUM_ERR_LIMIT;
-  if (!part_o || !part_ml || !cut || !status) return STRATUM_ERR_ALIGN;
+  if (!a.part_o || !a.part_ml || !a.cut || !a.status) return STRATUM_ERR_ALIGN;
   TreeParams P;
-  P.token_pos = token_pos; P.mask = (const unsigned long long*)mask; P.words = words;
-  P.seq_start = seq_start; P.seq_len = seq_len;
-  P.block_table = block_table; P.bt_stride = bt_stride; P.bt_width = bt_width;
-  P.q = q; P.ldq = ldq; P.k_cache = k_cache; P.v_cache = v_cache; P.out = out; P.ldo = ldo;
-  P.part_o = part_o; P.part_ml = (float2*)part_ml; P.cut = (TreeCut*)cut; P.status = status;
+  P.token_pos = (const int*)a.token_pos; P.mask = (const unsigned long long*)a.mask; P.words = a.words;
+  P.seq_start = (const int*)a.seq_start; P.seq_len = (const int*)a.seq_len;
+  P.block_table = (const int*)a.block_table; P.bt_stride = a.bt_stride; P.bt_width = a.bt_width;
+  P.q = a.q; P.ldq = ldq; P.k_cache = a.k_cache; P.v_cache = a.v_cache; P.out = a.out; P.ldo = ldo;
+  P.part_o = (float*)a.part_o; P.part_ml = (float2*)a.part_ml; P.cut = (TreeCut*)a.cut; P.status = (int*)a.status;
   P.n_tokens = n_tokens; P.n_seqs = n_seqs; P.n_q = n_q; P.n_kv = n_kv; P.gs = gs; P.head_dim = head_dim;
-  P.window = window; P.n_pages = (int)n_pages; P.scale = scale;
+  P.window = a.window; P.n_pages = (int)n_pages; P.scale = a.scale;
   const int G = stratum_attention_tree_ctas(tensor, many, head_dim);
   int st, slot_half, half_rows;
   if (tensor) {
-    if (dtype != STRATUM_DT_BF16 || (head_dim != 64 && head_dim != 128) || gs > 128 || !(scale > 0.f)) return STRATUM_ERR_SHAPE;
+    if (dtype != STRATUM_DT_BF16 || (head_dim != 64 && head_dim != 128) || gs > 128 || !(a.scale > 0.f)) return STRATUM_ERR_SHAPE;
     if (ldq % 8 != 0 || ldo % 8 != 0) return STRATUM_ERR_ALIGN;
-    if (((uintptr_t)q | (uintptr_t)k_cache | (uintptr_t)v_cache | (uintptr_t)out) & 15) return STRATUM_ERR_ALIGN;
+    if (((uintptr_t)a.q | (uintptr_t)a.k_cache | (uintptr_t)a.v_cache | (uintptr_t)a.out) & 15) return STRATUM_ERR_ALIGN;
     const int half_tokens = 128 / gs;
     slot_half = 128; half_rows = half_tokens * gs;
     P.rows_per_tile = half_rows * (many ? 2 : 1);
@@ -1241,14 +1249,14 @@ STRATUM_EXPORT int stratum_attention_tree(const void* q, int ldq, const void* k_
       cuuint64_t dims[3] = {(cuuint64_t)head_dim, (cuuint64_t)n_q, (cuuint64_t)n_tokens};
       cuuint64_t strides[2] = {(cuuint64_t)head_dim * sizeof(bf16), (cuuint64_t)ldq * sizeof(bf16)};
       cuuint32_t box[3] = {64, (cuuint32_t)gs, (cuuint32_t)half_tokens};
-      if ((st = tree_map(&mq, q, 3, dims, strides, box)) != 0) return st;
+      if ((st = tree_map(&mq, a.q, 3, dims, strides, box)) != 0) return st;
     }
     {  // the cache as [pages * n_kv * 64 rows][head_dim]; a box is 64 dims x 64 keys
       cuuint64_t dims[2] = {(cuuint64_t)head_dim, (cuuint64_t)n_pages * n_kv * TR_KEYS};
       cuuint64_t strides[1] = {(cuuint64_t)head_dim * sizeof(bf16)};
       cuuint32_t box[2] = {64, TR_KEYS};
-      if ((st = tree_map(&mk, k_cache, 2, dims, strides, box)) != 0) return st;
-      if ((st = tree_map(&mv, v_cache, 2, dims, strides, box)) != 0) return st;
+      if ((st = tree_map(&mk, a.k_cache, 2, dims, strides, box)) != 0) return st;
+      if ((st = tree_map(&mv, a.v_cache, 2, dims, strides, box)) != 0) return st;
     }
     if (head_dim == 64) st = many ? launch_tree_tc<64, true>(mq, mk, mv, P, G, stream) : launch_tree_tc<64, false>(mq, mk, mv, P, G, stream);
     else st = many ? launch_tree_tc<128, true>(mq, mk, mv, P, G, stream) : launch_tree_tc<128, false>(mq, mk, mv, P, G, stream);

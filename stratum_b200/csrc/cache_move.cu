@@ -88,39 +88,51 @@ STRATUM_EXPORT int stratum_copy_pages(void* a, void* b, long long pages, long lo
 #define CR_THREADS 256
 #define CR_ROWS 8
 
+// One call's numbers, as the launcher packs them.  k: [layers][pages][heads_k][page_tokens][bytes_k], v likewise (null:
+// heads_v 0).
+struct KeepRows {
+  uint8_t *k, *v;
+  const int *block_table, *seq_start, *seq_len, *path, *kept;
+  long long pages;
+  int heads_k, heads_v, bytes_k, bytes_v, layers, page_tokens, bt_stride, bt_width, n_tokens, n_seqs;
+};
+
 template <typename V>
-__global__ void __launch_bounds__(CR_THREADS)
-keep_rows_kernel(uint8_t* k, uint8_t* v, long long pages, int heads_k, int heads_v, int bytes_k, int bytes_v, int layers,
-                 int page_tokens, const int* block_table, int bt_stride, int bt_width, const int* seq_start, const int* seq_len,
-                 const int* path, const int* kept, int n_tokens, int per_seq) {
+__global__ void __launch_bounds__(CR_THREADS, 4)
+keep_rows_kernel(const KeepRows P, int per_seq) {
+  __shared__ V* from_s[CR_THREADS / 32][32];
+  __shared__ V* to_s[CR_THREADS / 32][32];
   pdl_wait();
-  const int lane = threadIdx.x & 31;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int s = blockIdx.x / per_seq;
-  int w = (blockIdx.x % per_seq) * (CR_THREADS / 32) + (threadIdx.x >> 5);          // layer, then keys' heads and values' heads
-  if (w >= layers * (heads_k + heads_v)) return;
-  const int layer = w / (heads_k + heads_v);
-  w %= heads_k + heads_v;
-  const bool second = w >= heads_k;
-  const int head = second ? w - heads_k : w, heads = second ? heads_v : heads_k;
-  const int units = (second ? bytes_v : bytes_k) / (int)sizeof(V);                  // of a row
-  const int a = min(max(__ldcg(seq_start + s), 0), n_tokens), n = min(max(__ldcg(seq_start + s + 1), a), n_tokens) - a;
-  const int base = __ldcg(seq_len + s) - n;
-  const int last = min(__ldcg(kept + s), n - 1);
+  int w = (blockIdx.x % per_seq) * (CR_THREADS / 32) + warp;       // layer, then keys' heads and values' heads
+  if (w >= P.layers * (P.heads_k + P.heads_v)) return;
+  // (fetched together: what the path says, where it lies and how much of it holds)
+  const int a0 = __ldcg(P.seq_start + s), a1 = __ldcg(P.seq_start + s + 1), len = __ldcg(P.seq_len + s), kept = __ldcg(P.kept + s);
+  const int layer = w / (P.heads_k + P.heads_v);
+  w %= P.heads_k + P.heads_v;
+  const bool second = w >= P.heads_k;
+  const int head = second ? w - P.heads_k : w, heads = second ? P.heads_v : P.heads_k;
+  const int units = (second ? P.bytes_v : P.bytes_k) / (int)sizeof(V);              // of a row
+  const int a = min(max(a0, 0), P.n_tokens), n = min(max(a1, a), P.n_tokens) - a;
+  const int base = len - n, last = min(kept, n - 1);
   if (last < 1 || base < 0) return;
-  V* all = reinterpret_cast<V*>(second ? v : k) + (long long)layer * pages * heads * page_tokens * units;
-  const int* bt = block_table + (long long)s * bt_stride;
+  V* all = reinterpret_cast<V*>(second ? P.v : P.k) + (long long)layer * P.pages * heads * P.page_tokens * units;
+  const int* bt = P.block_table + (long long)s * P.bt_stride;
   // where position p of this head lies, or null
   auto at = [&](int p) -> V* {
-    const int i = p / page_tokens;
-    if (i >= bt_width) return nullptr;
+    const int i = p / P.page_tokens;
+    if (i >= P.bt_width) return nullptr;
     const int pg = __ldcg(bt + i);
-    if (pg < 0 || pg >= pages) return nullptr;
-    return all + (((long long)pg * heads + head) * page_tokens + p % page_tokens) * units;
+    if (pg < 0 || pg >= P.pages) return nullptr;
+    return all + (((long long)pg * heads + head) * P.page_tokens + p % P.page_tokens) * units;
   };
+  // a row takes `g` lanes (the next power of two of its units, a warp at most); 32 / g rows go side by side
+  const int g = units >= 32 ? 32 : units <= 1 ? 1 : 1 << (32 - __clz(units - 1)), side = 32 / g, sub = lane / g, unit = lane % g;
   int before = 0;                                  // the path's entry in front; one that does not rise ends it
   for (int j0 = 1; j0 <= last; j0 += 32) {
     const int j = j0 + lane;
-    int node = j <= last ? __ldcg(path + a + j) : -1;
+    const int node = j <= last ? __ldcg(P.path + a + j) : -1;
     int prev = __shfl_up_sync(0xffffffffu, node, 1);
     if (lane == 0) prev = before;
     const unsigned wrong = __ballot_sync(0xffffffffu, j > last || node <= prev || node >= n);
@@ -129,28 +141,25 @@ keep_rows_kernel(uint8_t* k, uint8_t* v, long long pages, int heads_k, int heads
     V* from = nullptr;
     V* to = nullptr;
     if (lane < count && node != j) { from = at(base + node); to = at(base + j); }
-    if (!from || !to) from = to = nullptr;
-    const unsigned moves = __ballot_sync(0xffffffffu, from != nullptr);
-    for (unsigned left = moves; left;) {
-      // up to CR_ROWS rows of the path, in its order: read, then written
-      int l[CR_ROWS], m = 0;
-#pragma unroll
-      for (int x = 0; x < CR_ROWS; x++) {
-        l[x] = left ? __ffs(left) - 1 : 0;
-        if (left) { m = x + 1; left &= left - 1; }
-      }
-      for (int i0 = 0; i0 < units; i0 += 32) {
+    const bool moves = from && to;
+    const unsigned which = __ballot_sync(0xffffffffu, moves);
+    const int m = __popc(which), mine = __popc(which & ((1u << lane) - 1));
+    __syncwarp();
+    if (moves) { from_s[warp][mine] = from; to_s[warp][mine] = to; }
+    __syncwarp();
+    for (int r0 = 0; r0 < m; r0 += CR_ROWS * side) {              // rows in the path's order: read, then written
+      for (int i0 = 0; i0 < units; i0 += g) {
         V x[CR_ROWS];
 #pragma unroll
         for (int r = 0; r < CR_ROWS; r++) {
-          const V* f = reinterpret_cast<const V*>(__shfl_sync(0xffffffffu, (unsigned long long)from, l[r]));
-          if (r < m && i0 + lane < units) x[r] = __ldcg(f + i0 + lane);
+          const int at_ = r0 + r * side + sub;
+          if (at_ < m && i0 + unit < units) x[r] = __ldcg(from_s[warp][at_] + i0 + unit);
         }
         __syncwarp();
 #pragma unroll
         for (int r = 0; r < CR_ROWS; r++) {
-          V* t = reinterpret_cast<V*>(__shfl_sync(0xffffffffu, (unsigned long long)to, l[r]));
-          if (r < m && i0 + lane < units) t[i0 + lane] = x[r];
+          const int at_ = r0 + r * side + sub;
+          if (at_ < m && i0 + unit < units) to_s[warp][at_][i0 + unit] = x[r];
         }
         __syncwarp();
       }
@@ -159,25 +168,17 @@ keep_rows_kernel(uint8_t* k, uint8_t* v, long long pages, int heads_k, int heads
   }
 }
 
-// k: [layers][pages][heads_k][page_tokens][bytes_k], v likewise (null: heads_v 0).
-STRATUM_EXPORT int stratum_keep_rows(void* k, void* v, long long pages, int heads_k, int heads_v, int bytes_k, int bytes_v,
-                                     int layers, int page_tokens, const int* block_table, int bt_stride, int bt_width,
-                                     const int* seq_start, const int* seq_len, const int* path, const int* kept, int n_tokens,
-                                     int n_seqs, cudaStream_t stream) {
-  if (n_seqs <= 0 || layers <= 0 || n_tokens <= 0) return 0;
-  if (!k || heads_k < 1 || bytes_k < 1 || heads_v < 0 || (heads_v > 0 && (!v || bytes_v < 1)) || page_tokens < 1 || bt_width < 1)
+STRATUM_EXPORT int stratum_keep_rows(const KeepRows* call, cudaStream_t stream) {
+  const KeepRows P = *call;
+  if (P.n_seqs <= 0 || P.layers <= 0 || P.n_tokens <= 0) return 0;
+  if (!P.k || P.heads_k < 1 || P.bytes_k < 1 || P.heads_v < 0 || (P.heads_v > 0 && (!P.v || P.bytes_v < 1)) || P.page_tokens < 1 ||
+      P.bt_width < 1)
     return STRATUM_ERR_SHAPE;
-  const long long warps = (long long)layers * (heads_k + heads_v), per_seq = (warps + CR_THREADS / 32 - 1) / (CR_THREADS / 32);
-  if (warps > 0x7fffffffLL || per_seq * n_seqs > 0x7fffffffLL) return STRATUM_ERR_LIMIT;
-  const unsigned long long all = (unsigned long long)(uintptr_t)k | (uintptr_t)v | (unsigned)bytes_k | (unsigned)bytes_v;
-  const dim3 grid((unsigned)(per_seq * n_seqs)), block(CR_THREADS);
-  uint8_t* pk = (uint8_t*)k;
-  uint8_t* pv = (uint8_t*)v;
-#define KEEP(V)                                                                                                              \
-  launch_pdl(keep_rows_kernel<V>, grid, block, 0, stream, pk, pv, pages, heads_k, heads_v, bytes_k, bytes_v, layers, page_tokens, \
-             block_table, bt_stride, bt_width, seq_start, seq_len, path, kept, n_tokens, (int)per_seq)
-  if ((all & 15) == 0) return KEEP(uint4);
-  if ((all & 3) == 0) return KEEP(uint32_t);
-  return KEEP(uint8_t);
-#undef KEEP
+  const long long warps = (long long)P.layers * (P.heads_k + P.heads_v), per_seq = (warps + CR_THREADS / 32 - 1) / (CR_THREADS / 32);
+  if (warps > 0x7fffffffLL || per_seq * P.n_seqs > 0x7fffffffLL) return STRATUM_ERR_LIMIT;
+  const unsigned long long all = (unsigned long long)(uintptr_t)P.k | (uintptr_t)P.v | (unsigned)P.bytes_k | (unsigned)P.bytes_v;
+  const dim3 grid((unsigned)(per_seq * P.n_seqs)), block(CR_THREADS);
+  if ((all & 15) == 0) return launch_pdl(keep_rows_kernel<uint4>, grid, block, 0, stream, P, (int)per_seq);
+  if ((all & 3) == 0) return launch_pdl(keep_rows_kernel<uint32_t>, grid, block, 0, stream, P, (int)per_seq);
+  return launch_pdl(keep_rows_kernel<uint8_t>, grid, block, 0, stream, P, (int)per_seq);
 }

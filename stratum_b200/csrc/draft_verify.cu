@@ -196,11 +196,12 @@ STRATUM_EXPORT int stratum_token_probs(const float* logits, long long ld, const 
 #define VD_NODES 1024            // nodes of a sequence that are looked at
 
 struct VerifyParams {
-  const float* target; long long ldt;
-  const float* draft; long long ldd;       // null: looked up
+  const float* target;
+  const float* draft;                      // null: looked up
   const int* tokens; const int* parents; const int* seq_start; const float* uniform;
   int* path; int* kept; int* picked;
-  int n_tokens, n_seqs, vocab;
+  long long ldt, ldd;
+  int n_tokens, n_seqs, vocab, reserved;
 };
 
 __device__ __forceinline__ float vd_prob(float p) { return fminf(fmaxf(p, 0.f), 1.f); }     // (fmaxf drops what is no number)
@@ -416,19 +417,14 @@ verify_drafts_kernel(const VerifyParams P) {
   cluster.sync();                                  // nobody leaves while its sums may still be read
 }
 
-STRATUM_EXPORT int stratum_verify_drafts(const float* target, long long ldt, const float* draft, long long ldd, const int* tokens,
-                                         const int* parents, const int* seq_start, const float* uniform, int* path, int* kept,
-                                         int* picked, int n_tokens, int n_seqs, int vocab, cudaStream_t stream) {
-  if (n_seqs <= 0) return 0;
-  if (vocab < 1 || n_tokens < 0) return STRATUM_ERR_SHAPE;
-  if (n_seqs > (1 << 26) || vocab > (1 << 30)) return STRATUM_ERR_LIMIT;
-  VerifyParams P;
-  P.target = target; P.ldt = ldt; P.draft = draft; P.ldd = ldd;
-  P.tokens = tokens; P.parents = parents; P.seq_start = seq_start; P.uniform = uniform;
-  P.path = path; P.kept = kept; P.picked = picked;
-  P.n_tokens = n_tokens; P.n_seqs = n_seqs; P.vocab = vocab;
+// call: the parameters as the launcher packs them.
+STRATUM_EXPORT int stratum_verify_drafts(const VerifyParams* call, cudaStream_t stream) {
+  const VerifyParams P = *call;
+  if (P.n_seqs <= 0) return 0;
+  if (P.vocab < 1 || P.n_tokens < 0) return STRATUM_ERR_SHAPE;
+  if (P.n_seqs > (1 << 26) || P.vocab > (1 << 30)) return STRATUM_ERR_LIMIT;
   // as many blocks a row as leave every warp a few lines of it and all of them resident (two to an SM)
   int C = 1;
-  while (C < 16 && C * 2048 < vocab && (long long)n_seqs * C * 2 <= 2 * sms()) C *= 2;
-  return launch_clusters<verify_drafts_kernel>(n_seqs, C, VD_THREADS, stream, P);
+  while (C < 16 && C * 2048 < P.vocab && (long long)P.n_seqs * C * 2 <= 2 * sms()) C *= 2;
+  return launch_clusters<verify_drafts_kernel>(P.n_seqs, C, VD_THREADS, stream, P);
 }

@@ -8,9 +8,10 @@ there is no CPU or library-op fallback.
 from __future__ import annotations
 
 import ctypes
+import struct
 import threading
 from collections import OrderedDict
-from ctypes import c_float, c_int, c_size_t, c_uint32, c_uint64, c_void_p
+from ctypes import c_char_p, c_float, c_int, c_size_t, c_uint32, c_uint64, c_void_p
 from typing import Optional, Tuple
 
 import torch
@@ -1664,14 +1665,12 @@ def attention_stream(qkv: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Te
 # ------------------------------------------------------------------ drafted tokens
 def _one_device(what: str, *tensors: Optional[torch.Tensor]) -> None:
     """All on the current device, which is also the one this process's launches go to (see _stream, status_word)."""
-    here = torch.cuda.current_device() if torch.cuda.is_available() else None
-    for t in tensors:
-        if t is None:
-            continue
-        if not t.is_cuda:
-            raise KernelError(f"{what}: tensors must live on a CUDA device (no CPU path exists)")
-        if t.device.index != here:
-            raise KernelError(f"{what}: a tensor lives on {t.device}, the current device is cuda:{here}")
+    devices = {t.get_device() for t in tensors if t is not None}
+    if -1 in devices:
+        raise KernelError(f"{what}: tensors must live on a CUDA device (no CPU path exists)")
+    here = torch.cuda.current_device()
+    if devices != {here}:
+        raise KernelError(f"{what}: tensors on devices {sorted(devices)}, the current one is cuda:{here}")
     if _device_index is not None and _device_index != here:
         raise KernelError(f"{what}: this process launches on cuda:{_device_index}, the current device is cuda:{here}")
 
@@ -1685,6 +1684,9 @@ def _shaped(t: torch.Tensor, name: str, dtype, shape=None) -> None:
         raise KernelError(f"{name} must have the shape {shape}, has {tuple(t.shape)}")
 
 
+# Mirrors of struct TreeCall in csrc/attention_tree.cu, VerifyParams in csrc/draft_verify.cu and KeepRows in csrc/cache_move.cu.
+# (One packed argument: converting thirty of them one by one took a fifth of a short call.)
+_TREE_CALL, _VERIFY_CALL, _KEEP_CALL = struct.Struct("<14q15if"), struct.Struct("<11q4i"), struct.Struct("<8q10i")
 _tree_plans: dict = {}         # (tensor cores, many rows, head size) -> CTAs, scratch rows of a CTA's slot
 
 
@@ -1713,9 +1715,10 @@ def attention_tree(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor
     if k_cache.dim() != 4 or tuple(k_cache.shape[1:]) != (n_kv, page_tokens, head_dim) or n_q < 1 or n_q % max(n_kv, 1):
         raise KernelError("attention_tree: the caches are [pages, n_kv, page_tokens, head_dim], n_q a multiple of n_kv")
     T, B = q.shape[0], seq_len.numel()
+    width = n_q * head_dim
     for t, name in ((q, "q"), (out, "out")):
-        if t.dim() != 2 or t.dtype != dt or t.shape[0] != T or t.shape[1] < n_q * head_dim or t.stride(1) != 1 \
-                or (T > 1 and t.stride(0) < n_q * head_dim):
+        shape, stride = t.shape, t.stride()
+        if len(shape) != 2 or t.dtype != dt or shape[0] != T or shape[1] < width or stride[1] != 1 or (T > 1 and stride[0] < width):
             raise KernelError(f"attention_tree: {name} must be [tokens, >= n_q * head_dim] of the cache's dtype, rows contiguous")
     _shaped(token_pos, "token_pos", torch.int32, (T,)); _shaped(seq_len, "seq_len", torch.int32, (B,))
     _shaped(seq_start, "seq_start", torch.int32, (B + 1,)); _shaped(tree_mask, "tree_mask", torch.int64)
@@ -1729,8 +1732,10 @@ def attention_tree(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor
     if T == 0 or B == 0:
         return
     group = n_q // n_kv
-    tensor = (dt == torch.bfloat16 and head_dim in (64, 128) and group <= 128 and scale > 0 and q.stride(0) % 8 == 0
-              and out.stride(0) % 8 == 0 and not (q.data_ptr() | out.data_ptr() | k_cache.data_ptr() | v_cache.data_ptr()) & 15)
+    at_q, at_k, at_v, at_out, ldq, ldo = (q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), out.data_ptr(), q.stride()[0],
+                                          out.stride()[0])
+    tensor = (code == DT_BF16 and head_dim in (64, 128) and group <= 128 and scale > 0 and ldq % 8 == 0 and ldo % 8 == 0
+              and not (at_q | at_k | at_v | at_out) & 15)
     # more rows than a half of a CTA holds: both halves share every page (else they take pages in turn); on the CUDA cores:
     # tiles of 64 rows
     many = max_new * group > (128 if tensor else 32)
@@ -1745,15 +1750,11 @@ def attention_tree(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor
     scratch = torch.empty(slots * ((head_dim + 3) // 4 * 4 + 2) + 12 * ctas, dtype=torch.float32, device=q.device)
     at = scratch.data_ptr()
     part_ml = at + 4 * slots * ((head_dim + 3) // 4 * 4)
-    f = _fn("attention_tree", "stratum_attention_tree",
-            [c_void_p, c_int, c_void_p, c_void_p, ctypes.c_longlong, c_int, c_void_p, c_void_p, c_int, c_void_p, c_void_p,
-             c_void_p, c_int, c_int, c_void_p, c_int, c_int, c_int, c_int, c_int, c_int, c_int, c_int, c_float, c_int, c_int,
-             c_void_p, c_void_p, c_void_p, c_void_p, c_void_p])
-    _check(f(q.data_ptr(), q.stride(0), k_cache.data_ptr(), v_cache.data_ptr(), k_cache.shape[0], code,
-             token_pos.data_ptr(), tree_mask.data_ptr(), tree_mask.shape[1], seq_start.data_ptr(), seq_len.data_ptr(),
-             block_table.data_ptr(), block_table.stride(0), block_table.shape[1], out.data_ptr(), out.stride(0), T, B, n_q,
-             n_kv, head_dim, page_tokens, window, scale, int(tensor), int(many), at, part_ml, part_ml + 8 * slots,
-             status_word().data_ptr(), _stream()), "attention_tree")
+    f = _fn("attention_tree", "stratum_attention_tree", [c_char_p, c_void_p])
+    _check(f(_TREE_CALL.pack(at_q, at_k, at_v, token_pos.data_ptr(), tree_mask.data_ptr(), seq_start.data_ptr(), seq_len.data_ptr(),
+                             block_table.data_ptr(), at_out, at, part_ml, part_ml + 8 * slots, status_word().data_ptr(),
+                             k_cache.shape[0], code, ldq, ldo, tree_mask.shape[1], block_table.stride()[0], block_table.shape[1],
+                             T, B, n_q, n_kv, head_dim, page_tokens, window, tensor, many, scale), _stream()), "attention_tree")
     count_launches(1)          # the merge kernel
 
 
@@ -1829,12 +1830,11 @@ def verify_drafts(target: torch.Tensor, draft: Optional[torch.Tensor], tokens: t
         raise KernelError(f"verify_drafts: {T} rows are more than {VERIFY_MAX_NODES} for each of {B} sequences")
     if B == 0:
         return
-    f = _fn("draft_verify", "stratum_verify_drafts",
-            [c_void_p, ctypes.c_longlong, c_void_p, ctypes.c_longlong, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p,
-             c_void_p, c_void_p, c_int, c_int, c_int, c_void_p])
-    _check(f(target.data_ptr(), target.stride(0), None if draft is None else draft.data_ptr(),
-             0 if draft is None else draft.stride(0), tokens.data_ptr(), parents.data_ptr(), seq_start.data_ptr(),
-             uniform.data_ptr(), path.data_ptr(), n_kept.data_ptr(), next_ids.data_ptr(), T, B, V, _stream()), "verify_drafts")
+    f = _fn("draft_verify", "stratum_verify_drafts", [c_char_p, c_void_p])
+    _check(f(_VERIFY_CALL.pack(target.data_ptr(), 0 if draft is None else draft.data_ptr(), tokens.data_ptr(), parents.data_ptr(),
+                               seq_start.data_ptr(), uniform.data_ptr(), path.data_ptr(), n_kept.data_ptr(), next_ids.data_ptr(),
+                               target.stride()[0], 0 if draft is None else draft.stride()[0], T, B, V, 0), _stream()),
+           "verify_drafts")
 
 
 def _storage(k: torch.Tensor, v: Optional[torch.Tensor], what: str) -> None:
@@ -1866,13 +1866,11 @@ def keep_rows(k: torch.Tensor, v: Optional[torch.Tensor], block_table: torch.Ten
     if B == 0 or T == 0:
         return
     L, pages, heads, page_tokens, size = k.shape
-    f = _fn("cache_move", "stratum_keep_rows",
-            [c_void_p, c_void_p, ctypes.c_longlong, c_int, c_int, c_int, c_int, c_int, c_int, c_void_p, c_int, c_int, c_void_p,
-             c_void_p, c_void_p, c_void_p, c_int, c_int, c_void_p])
-    _check(f(k.data_ptr(), None if v is None else v.data_ptr(), pages, heads, 0 if v is None else v.shape[2],
-             size * k.element_size(), 0 if v is None else v.shape[4] * v.element_size(), L, page_tokens,
-             block_table.data_ptr(), block_table.stride(0), block_table.shape[1], seq_start.data_ptr(), seq_len.data_ptr(),
-             path.data_ptr(), n_kept.data_ptr(), T, B, _stream()), "keep_rows")
+    f = _fn("cache_move", "stratum_keep_rows", [c_char_p, c_void_p])
+    _check(f(_KEEP_CALL.pack(k.data_ptr(), 0 if v is None else v.data_ptr(), block_table.data_ptr(), seq_start.data_ptr(),
+                             seq_len.data_ptr(), path.data_ptr(), n_kept.data_ptr(), pages, heads, 0 if v is None else v.shape[2],
+                             size * k.element_size(), 0 if v is None else v.shape[4] * v.element_size(), L, page_tokens,
+                             block_table.stride()[0], block_table.shape[1], T, B), _stream()), "keep_rows")
 
 
 COPY_PAGES_MAX = 480               # pairs of a launch
