@@ -35,7 +35,7 @@ EXTRA_DEPS = {"attention_general": ("attention_general.h",),
               "gla": ("gla.h",), "gla_chunked": ("gla.h", "mma_common.cuh"),
               "attention_static": ("attention_mma.cu", "attention_static.h", "mma_common.cuh"),   # files a source includes
               "attention_mma": ("mma_common.cuh",), "decode_layers": ("mma_common.cuh", "tc_common.cuh"), "attention_stream": ("mma_common.cuh", "tc_common.cuh"),
-              "gemm_tc": ("tc_common.cuh",), "attention_tc": ("tc_common.cuh",), "attention_tree": ("tc_common.cuh",)}
+              "gemm_tc": ("tc_common.cuh",), "attention_tc": ("tc_common.cuh",), "attention_tree": ("tc_common.cuh",), "draft_verify": ("tc_common.cuh",)}
 
 _lock = threading.Lock()
 _loaded: Dict[str, ctypes.CDLL] = {}

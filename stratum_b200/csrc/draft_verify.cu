@@ -22,18 +22,24 @@
 #include <cooperative_groups.h>
 #include <math.h>
 
-#include "common.cuh"
+#include "tc_common.cuh"
 
 namespace cg = cooperative_groups;
 
-static int sms() {
-  static int n = 0;
-  if (!n) {
-    int dev = 0;
-    cudaGetDevice(&dev);
-    cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev);
-    if (n <= 0) n = 148;
-  }
+// Clusters of C blocks of a kernel that are resident at a time (at most 16 blocks; 0: none).
+static int resident_clusters(const void* kernel, int C, int threads) {
+  if (C > 8 && cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1) != cudaSuccess) { cudaGetLastError(); return 0; }
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(C);
+  cfg.blockDim = dim3(threads);
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = C;
+  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  int n = 0;
+  if (cudaOccupancyMaxActiveClusters(&n, kernel, &cfg) != cudaSuccess) { cudaGetLastError(); return 0; }
   return n;
 }
 
@@ -64,31 +70,31 @@ static int launch_clusters(unsigned rows, unsigned cluster, unsigned threads, cu
 }
 
 // ================================================================ probabilities
-// A row is read once and written once: its values stay in registers, 32 to a thread, 16,384 to a block, the rest of the row
-// in the other blocks of the cluster.  Every thread takes its exponentials against the largest of its own values, so the
-// blocks meet once: each tells the others its maximum (and where it is) and its sum against it, and a thread's values then
-// need one factor.  (A row longer than sixteen blocks hold is read a second time.)
-#define PR_THREADS 512
+// A row is read once and written once: its values stay in registers, 32 to a thread of a block, the rest of the row in the
+// other blocks of the cluster.  A block takes its exponentials against its own largest value, so the blocks meet
+// once: each tells the others that value (and where it is) and its sum, and its weights then need one factor.  (A row longer
+// than sixteen blocks hold is read a second and a third time.)
+//
+// With ordinary numbers a weight is a difference, a product and an exponential; infinities, and temperatures that are so large
+// or small that the product is none, are told apart once for a block: decided for every value they were fifty instructions
+// a value, and the time was theirs.
 #define PR_HELD 32
 
-struct Best { float v; int i; float sum; };        // the largest value, where it is first, sum of exp2((x - v) to_log2)
-// Both together.  (A part without any value above -inf has the sum zero, and infinite values count one each.)
-__device__ __forceinline__ Best both(Best a, Best b, float to_log2) {
-  const bool second = b.v > a.v || (b.v == a.v && b.i < a.i);
-  Best r = second ? b : a;
-  const Best o = second ? a : b;
-  r.sum += o.v == r.v ? o.sum : o.v == -INFINITY ? 0.f : o.sum * exp2f((o.v - r.v) * to_log2);
-  return r;
+struct Part { float v, sum; int i; };              // the largest value, the sum of weights against it, where it is first
+
+// A weight against `m`, no less than v, in all cases: 1 at the maximum (infinite ones too), 0 at -inf.
+__device__ __forceinline__ float any_weight(float v, float m, float to_log2) {
+  return v == m ? 1.f : v == -INFINITY ? 0.f : exp2f((v - m) * to_log2);
 }
-__device__ __forceinline__ Best shfl_xor(Best b, int o) {
-  return Best{__shfl_xor_sync(0xffffffffu, b.v, o), __shfl_xor_sync(0xffffffffu, b.i, o), __shfl_xor_sync(0xffffffffu, b.sum, o)};
-}
+__device__ __forceinline__ float clean(float v) { return fmaxf(v, -INFINITY); }        // (fmaxf drops what is no number)
 
 // W: values of a load and a store (4 where every row begins on 16 bytes)
-template <bool HELD, int W>
-__global__ void __launch_bounds__(PR_THREADS, 2)
+template <bool HELD, int W, int PR_THREADS>
+__global__ void __launch_bounds__(PR_THREADS, 1024 / PR_THREADS)
 token_probs_kernel(const float* logits, long long ld, const float* temperature, float* out, long long ldo, int vocab, int slice) {
-  __shared__ Best parts[PR_THREADS / 32], blocks[16];
+  __shared__ float warp_v[PR_THREADS / 32], warp_sum_[PR_THREADS / 32];
+  __shared__ int first;
+  __shared__ Part told[16];
   cg::cluster_group cluster = cg::this_cluster();
   const int C = cluster.num_blocks(), c = cluster.block_rank();
   const int row = blockIdx.x / C, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
@@ -97,78 +103,94 @@ token_probs_kernel(const float* logits, long long ld, const float* temperature, 
   const float* in = logits + row * ld + i0;
   float* to = out + row * ldo + i0;
   const float t = ld_fresh(temperature + row);
-  const bool greedy = !(t > 0.f);
-  const float to_log2 = greedy ? 0.f : 1.4426950408889634f / t;
-  auto clean = [](float v) { return v == v ? v : -INFINITY; };
-  // against `m`, no less than v: 1 at the maximum (infinite ones too), 0 at -inf
-  auto weight = [&](float v, float m) { return v == m ? 1.f : v == -INFINITY ? 0.f : exp2f((v - m) * to_log2); };
-  float x[HELD ? PR_HELD : 1];
-  Best b{-INFINITY, 0x7fffffff, 0.f};
+  float x[PR_HELD], v = -INFINITY;
   auto place = [&](int k) { return ((k / W) * PR_THREADS + tid) * W + k % W; };      // of a thread's k-th value in the slice
   if (HELD) {
 #pragma unroll
     for (int k = 0; k < PR_HELD; k += W) {
       const int i = place(k);
       if (W == 4 && i + 3 < n) {
-        const float4 v = ld_fresh(reinterpret_cast<const float4*>(in + i));
-        x[k] = v.x; x[k + W / 4] = v.y; x[k + W / 2] = v.z; x[k + W - 1] = v.w;
+        const float4 y = ld_fresh(reinterpret_cast<const float4*>(in + i));
+        x[k] = y.x; x[k + W / 4] = y.y; x[k + W / 2] = y.z; x[k + W - 1] = y.w;
       } else {
 #pragma unroll
         for (int e = 0; e < W; e++) x[k + e] = i + e < n ? ld_fresh(in + i + e) : -INFINITY;
       }
     }
+    if (tid == 0) first = 0x7fffffff;
+    float most[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-    for (int k = 0; k < PR_HELD; k++) { x[k] = clean(x[k]); if (x[k] > b.v) { b.v = x[k]; b.i = i0 + place(k); } }
-    if (b.v != -INFINITY) {
-#pragma unroll
-      for (int k = 0; k < PR_HELD; k++) { x[k] = weight(x[k], b.v); b.sum += x[k]; }
-    }
+    for (int k = 0; k < PR_HELD; k++) { x[k] = clean(x[k]); most[k & 3] = fmaxf(most[k & 3], x[k]); }
+    v = fmaxf(fmaxf(most[0], most[1]), fmaxf(most[2], most[3]));
   } else {
-    for (int i = tid; i < n; i += PR_THREADS) {
-      const float v = clean(ld_fresh(in + i));
-      if (v > b.v) {
-        b.sum = b.v == -INFINITY ? 0.f : b.sum * exp2f((b.v - v) * to_log2);
-        b.v = v; b.i = i0 + i;
-      }
-      if (v != -INFINITY) b.sum += weight(v, b.v);
+    if (tid == 0) first = 0x7fffffff;
+    for (int i = tid; i < n; i += PR_THREADS) v = fmaxf(v, ld_fresh(in + i));
+  }
+  v = warp_max(v);
+  if (lane == 0) warp_v[warp] = v;
+  __syncthreads();
+  const float m = warp_max(warp_v[lane % (PR_THREADS / 32)]);                        // the block's largest value
+  const bool greedy = !(t > 0.f);
+  const float to_log2 = greedy ? 0.f : 1.4426950408889634f / t;
+  const bool ordinary = fabsf(m) < INFINITY && to_log2 > 0.f && to_log2 < INFINITY;
+  float sum = 0.f;
+  if (greedy) {
+    if (HELD) {
+#pragma unroll
+      for (int k = 0; k < PR_HELD; k++) if (x[k] == m && place(k) < n) atomicMin(&first, i0 + place(k));
+    } else {
+      for (int i = tid; i < n; i += PR_THREADS) if (clean(ld_fresh(in + i)) == m) atomicMin(&first, i0 + i);
+    }
+  } else if (HELD && ordinary) {
+    float part[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int k = 0; k < PR_HELD; k++) {
+      asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(x[k]) : "f"((x[k] - m) * to_log2));
+      part[k & 3] += x[k];
+    }
+    sum = (part[0] + part[1]) + (part[2] + part[3]);
+  } else if (m != -INFINITY) {
+    if (HELD) {
+#pragma unroll
+      for (int k = 0; k < PR_HELD; k++) { x[k] = any_weight(x[k], m, to_log2); sum += x[k]; }
+    } else {
+      for (int i = tid; i < n; i += PR_THREADS) sum += any_weight(clean(ld_fresh(in + i)), m, to_log2);
     }
   }
-  const float mine = b.v;
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) b = both(b, shfl_xor(b, o), to_log2);
-  if (lane == 0) parts[warp] = b;
+  sum = warp_sum(sum);
+  if (lane == 0) warp_sum_[warp] = sum;
   __syncthreads();
   if (warp == 0) {
-    b = parts[lane % (PR_THREADS / 32)];
-#pragma unroll
-    for (int o = PR_THREADS / 64; o > 0; o >>= 1) b = both(b, shfl_xor(b, o), to_log2);
-    if (lane < C) *cluster.map_shared_rank(&blocks[c], lane) = b;
+    sum = warp_sum(lane < PR_THREADS / 32 ? warp_sum_[lane] : 0.f);
+    if (lane < C) *cluster.map_shared_rank(&told[c], lane) = Part{m, sum, first};
   }
   cluster.sync();                                  // (nothing of another block is touched behind it)
-  b = blocks[0];
-  for (int i = 1; i < C; i++) b = both(b, blocks[i], to_log2);
-  if (greedy || b.v == -INFINITY) {                // (the same in the whole cluster)
-    const int best = b.v == -INFINITY ? -1 : b.i - i0;
-    for (int i = tid; i < n; i += PR_THREADS) to[i] = i == best ? 1.f : 0.f;
+  const Part p = lane < C ? told[lane] : Part{-INFINITY, 0.f, 0x7fffffff};
+  const float M = warp_max(p.v);                   // of the row
+  if (greedy || M == -INFINITY) {                  // (the same in the whole cluster)
+    const int best = __reduce_min_sync(0xffffffffu, p.v == M ? p.i : 0x7fffffff);    // (-inf: nowhere)
+    for (int i = tid; i < n; i += PR_THREADS) to[i] = M != -INFINITY && i0 + i == best ? 1.f : 0.f;
     return;
   }
-  const float inv = 1.0f / b.sum;
+  const float inv = 1.0f / warp_sum(p.v == -INFINITY ? 0.f : p.sum * any_weight(p.v, M, to_log2));
+  const float f = m == -INFINITY ? 0.f : any_weight(m, M, to_log2) * inv;
   if (HELD) {
-    const float f = mine == -INFINITY ? 0.f : weight(mine, b.v) * inv;
+    if (m == -INFINITY) {
 #pragma unroll
-    for (int k = 0; k < PR_HELD; k++) x[k] = mine == -INFINITY ? 0.f : x[k] * f;
+      for (int k = 0; k < PR_HELD; k++) x[k] = 0.f;
+    }
 #pragma unroll
     for (int k = 0; k < PR_HELD; k += W) {
       const int i = place(k);
       if (W == 4 && i + 3 < n) {
-        *reinterpret_cast<float4*>(to + i) = make_float4(x[k], x[k + W / 4], x[k + W / 2], x[k + W - 1]);
+        *reinterpret_cast<float4*>(to + i) = make_float4(x[k] * f, x[k + W / 4] * f, x[k + W / 2] * f, x[k + W - 1] * f);
       } else {
 #pragma unroll
-        for (int e = 0; e < W; e++) if (i + e < n) to[i + e] = x[k + e];
+        for (int e = 0; e < W; e++) if (i + e < n) to[i + e] = x[k + e] * f;
       }
     }
   } else {
-    for (int i = tid; i < n; i += PR_THREADS) to[i] = weight(clean(ld_fresh(in + i)), b.v) * inv;
+    for (int i = tid; i < n; i += PR_THREADS) to[i] = any_weight(clean(ld_fresh(in + i)), M, to_log2) * inv;
   }
 }
 
@@ -178,16 +200,18 @@ STRATUM_EXPORT int stratum_token_probs(const float* logits, long long ld, const 
                                        int rows, int vocab, cudaStream_t stream) {
   if (rows <= 0 || vocab <= 0) return 0;
   if (rows > (1 << 26) || vocab > (1 << 30)) return STRATUM_ERR_LIMIT;
+  const bool four = (((uintptr_t)logits | (uintptr_t)out) & 15) == 0 && (rows == 1 || (ld % 4 == 0 && ldo % 4 == 0));
+  const int threads = vocab <= 16 * 256 * PR_HELD ? 256 : 512;
   // enough blocks to hold a row; beyond that, where a few rows leave the GPU empty, blocks of shorter slices
   int C = 1;
-  while (C < 16 && ((long long)C * PR_THREADS * PR_HELD < vocab || (C * 4096 < vocab && (long long)rows * C * 2 <= sms()))) C *= 2;
+  while (C < 16 && ((long long)C * threads * PR_HELD < vocab || (C * 4096 < vocab && (long long)rows * C * 2 <= sm_count()))) C *= 2;
   const int slice = (((vocab + C - 1) / C) + 3) & ~3;
-  const bool four = (((uintptr_t)logits | (uintptr_t)out) & 15) == 0 && (rows == 1 || (ld % 4 == 0 && ldo % 4 == 0));
-  if (slice <= PR_THREADS * PR_HELD) {
-    if (four) return launch_clusters<token_probs_kernel<true, 4>>(rows, C, PR_THREADS, stream, logits, ld, temperature, out, ldo, vocab, slice);
-    return launch_clusters<token_probs_kernel<true, 1>>(rows, C, PR_THREADS, stream, logits, ld, temperature, out, ldo, vocab, slice);
-  }
-  return launch_clusters<token_probs_kernel<false, 1>>(rows, C, PR_THREADS, stream, logits, ld, temperature, out, ldo, vocab, slice);
+#define PROBS(HELD, W, THREADS) \
+  launch_clusters<token_probs_kernel<HELD, W, THREADS>>(rows, C, THREADS, stream, logits, ld, temperature, out, ldo, vocab, slice)
+  if (slice > threads * PR_HELD) return PROBS(false, 1, 512);
+  if (threads == 256) return four ? PROBS(true, 4, 256) : PROBS(true, 1, 256);
+  return four ? PROBS(true, 4, 512) : PROBS(true, 1, 512);
+#undef PROBS
 }
 
 // ================================================================ verification
@@ -206,6 +230,15 @@ struct VerifyParams {
 
 __device__ __forceinline__ float vd_prob(float p) { return fminf(fmaxf(p, 0.f), 1.f); }     // (fmaxf drops what is no number)
 
+// A clamped probability in 64 bits.  Conversions from 32 to 64 bits run at a quarter of the rate of the additions they feed,
+// so a normal number's bits are moved by hand; zero stays zero, and what is smaller than a normal number is converted.
+__device__ __forceinline__ double vd_wide(float p) {
+  const unsigned b = __float_as_uint(p);
+  if (b - 1u < 0x007fffffu) return (double)p;
+  return __hiloint2double(b ? (int)((b >> 3) + (896u << 20)) : 0, (int)(b << 29));
+}
+__device__ __forceinline__ double vd_positive(double w) { return __double2hiint(w) < 0 ? 0.0 : w; }
+
 struct VdSmem {
   int parent[VD_NODES], token[VD_NODES];
   float u[VD_NODES], p[VD_NODES], q[VD_NODES];   // a node's number, and its parent's probabilities of it
@@ -217,8 +250,11 @@ struct VdSmem {
   double all[16 * VD_WARPS];               // the whole cluster's sums, running
 };
 
+// W: ids of a load (4 where every row begins on 16 bytes); a warp has LINES loads of a row on their way together.
+template <int W>
 __global__ void __launch_bounds__(VD_THREADS, 2)
 verify_drafts_kernel(const VerifyParams P) {
+  constexpr int LINES = W == 4 ? 4 : 8, LINE = 32 * W;
   __shared__ VdSmem S;
   cg::cluster_group cluster = cg::this_cluster();
   const int C = cluster.num_blocks(), c = cluster.block_rank();
@@ -246,39 +282,51 @@ verify_drafts_kernel(const VerifyParams P) {
   if (c == 0) for (int i = tid; i < n; i += VD_THREADS) P.path[a + i] = i == 0 ? 0 : -1;
   __syncthreads();
 
-  // A warp's stretch of the row, in whole lines of 32.
-  const int n_seg = C * VD_WARPS, lines = (P.vocab + 31) / 32, per = (lines + n_seg - 1) / n_seg;
-  const int seg = c * VD_WARPS + warp, s0 = min(seg * per * 32, P.vocab), s1 = min(s0 + per * 32, P.vocab);
-  // d at eight places 32 apart, from i on: the target's row, lowered at k masses, without the ids it has lost (those of the
-  // list that lie in this warp's stretch, if any do)
-  auto weights = [&](const float* trow, const float* drow, int i, int end, int k, bool lost, double (&w)[8]) {
-    float p[8], q[8];
+  // A warp's stretch of the row, in whole lines of LINE ids.
+  const int n_seg = C * VD_WARPS, lines = (P.vocab + LINE - 1) / LINE, per = (lines + n_seg - 1) / n_seg * LINE;
+  const int seg = c * VD_WARPS + warp, s0 = (int)min((long long)seg * per, (long long)P.vocab), s1 = min(s0 + per, P.vocab);
+  // this lane's ids i .. i + W - 1 of LINES lines from i on, of the target's row and, where it is to be lowered, the draft's
+  auto fetch = [&](const float* trow, const float* drow, int i, int end, bool low, float (&p)[LINES][W], float (&q)[LINES][W]) {
 #pragma unroll
-    for (int x = 0; x < 8; x++) {
-      p[x] = i + 32 * x < end ? __ldcg(trow + i + 32 * x) : 0.f;
-      q[x] = i + 32 * x < end && k > 0 ? __ldcg(drow + i + 32 * x) : 0.f;
+    for (int x = 0; x < LINES; x++) {
+      const int at = i + x * LINE;
+#pragma unroll
+      for (int e = 0; e < W; e++) p[x][e] = q[x][e] = 0.f;
+      if (W == 4 && at + 3 < end) {
+        const float4 y = __ldcg(reinterpret_cast<const float4*>(trow + at));
+        p[x][0] = y.x; p[x][W / 4] = y.y; p[x][W / 2] = y.z; p[x][W - 1] = y.w;
+        if (low) {
+          const float4 z = __ldcg(reinterpret_cast<const float4*>(drow + at));
+          q[x][0] = z.x; q[x][W / 4] = z.y; q[x][W / 2] = z.z; q[x][W - 1] = z.w;
+        }
+      } else {
+#pragma unroll
+        for (int e = 0; e < W; e++)
+          if (at + e < end) { p[x][e] = __ldcg(trow + at + e); if (low) q[x][e] = __ldcg(drow + at + e); }
+      }
     }
+  };
+  // d of W ids from i on: the target's row, lowered at k masses, without the ids it has lost (those of the list that lie in
+  // this warp's stretch, if any do)
+  auto weights = [&](const float (&p)[W], const float (&q)[W], int i, int k, bool lost, double (&w)[W]) {
 #pragma unroll
-    for (int x = 0; x < 8; x++) w[x] = (double)vd_prob(p[x]);
+    for (int e = 0; e < W; e++) w[e] = vd_wide(vd_prob(p[e]));
     if (k > 0) {
-      double qd[8];
+      double qd[W];
 #pragma unroll
-      for (int x = 0; x < 8; x++) qd[x] = (double)vd_prob(q[x]);
+      for (int e = 0; e < W; e++) { qd[e] = vd_wide(vd_prob(q[e])); w[e] = vd_positive(w[e] - qd[e]); }    // (a row's first mass is one)
 #pragma unroll 1
-      for (int j = 0; j < k; j++) {
+      for (int j = 1; j < k; j++) {
         const double m = S.masses[j];
 #pragma unroll
-        for (int x = 0; x < 8; x++) {
-          const double y = __dsub_rn(w[x], __dmul_rn(m, qd[x]));
-          w[x] = y > 0.0 ? y : 0.0;
-        }
+        for (int e = 0; e < W; e++) w[e] = vd_positive(__dsub_rn(w[e], __dmul_rn(m, qd[e])));
       }
     }
     if (lost) {
 #pragma unroll 1
       for (int j = 0; j < S.n_zeroed; j++)
 #pragma unroll
-        for (int x = 0; x < 8; x++) if (S.zeroed[j] == i + 32 * x) w[x] = 0.0;
+        for (int e = 0; e < W; e++) if (S.zeroed[j] == i + e) w[e] = 0.0;
     }
   };
   auto loses_between = [&](int from, int end) {
@@ -337,10 +385,18 @@ verify_drafts_kernel(const VerifyParams P) {
       const bool lost = S.n_zeroed > 0 && loses_between(s0, s1);
       double sum = 0.0;
 #pragma unroll 1
-      for (int i0 = s0; i0 < s1; i0 += 32 * 8) {
-        double w[8];
-        weights(trow, drow, i0 + lane, s1, k, lost, w);
-        sum += ((w[0] + w[1]) + (w[2] + w[3])) + ((w[4] + w[5]) + (w[6] + w[7]));
+      for (int i0 = s0; i0 < s1; i0 += LINES * LINE) {
+        float p[LINES][W], q[LINES][W];
+        fetch(trow, drow, i0 + lane * W, s1, k > 0, p, q);
+#pragma unroll
+        for (int x = 0; x < LINES; x++) {
+          double w[W];
+          weights(p[x], q[x], i0 + x * LINE + lane * W, k, lost, w);
+          double part = 0.0;
+#pragma unroll
+          for (int e = 0; e < W; e++) part += w[e];
+          sum += part;
+        }
       }
 #pragma unroll
       for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
@@ -386,25 +442,37 @@ verify_drafts_kernel(const VerifyParams P) {
     if (found / VD_WARPS == c && total > 0.0) {
       const float* trow = P.target + (long long)(a + S.node) * P.ldt;
       const float* drow = P.draft ? P.draft + (long long)(a + S.node) * P.ldd : nullptr;
-      const int f0 = min(found * per * 32, P.vocab), f1 = min(f0 + per * 32, P.vocab);
+      const int f0 = (int)min((long long)found * per, (long long)P.vocab), f1 = min(f0 + per, P.vocab), k = S.n_masses;
       const bool lost = S.n_zeroed > 0 && loses_between(f0, f1);
       double base = found > 0 ? S.all[found - 1] : 0.0;
-      for (int i0 = f0; i0 < f1 && pick < 0; i0 += 32 * 8) {
-        double w[8];
-        weights(trow, drow, i0 + lane, f1, S.n_masses, lost, w);
+      for (int i0 = f0; i0 < f1 && pick < 0; i0 += LINES * LINE) {
+        float p[LINES][W], q[LINES][W];
+        fetch(trow, drow, i0 + lane * W, f1, k > 0, p, q);
 #pragma unroll
-        for (int x = 0; x < 8; x++) {
-          double v = w[x];
+        for (int x = 0; x < LINES; x++) {
+          const int i = i0 + x * LINE + lane * W;
+          double w[W];
+          weights(p[x], q[x], i, k, lost, w);
+          double v = 0.0;
+#pragma unroll
+          for (int e = 0; e < W; e++) v += w[e];
+          double up = v;                           // running sums over the lanes
 #pragma unroll
           for (int d = 1; d < 32; d <<= 1) {
-            const double o = __shfl_up_sync(0xffffffffu, v, d);
-            if (lane >= d) v += o;
+            const double o = __shfl_up_sync(0xffffffffu, up, d);
+            if (lane >= d) up += o;
           }
-          const unsigned over = __ballot_sync(0xffffffffu, w[x] > 0.0 && base + v > aim);
-          const unsigned any = __ballot_sync(0xffffffffu, w[x] > 0.0);
-          if (any) positive = i0 + 32 * x + 31 - __clz(any);
-          if (crossed && over && pick < 0) pick = i0 + 32 * x + __ffs(over) - 1;
-          base += __shfl_sync(0xffffffffu, v, 31);
+          double run = base + (up - v);
+          int over = -1, any = -1;                 // this lane's first id over the aim, and last one with any weight
+#pragma unroll
+          for (int e = 0; e < W; e++) {
+            run += w[e];
+            if (w[e] > 0.0) { any = i + e; if (over < 0 && run > aim) over = i + e; }
+          }
+          const unsigned overs = __ballot_sync(0xffffffffu, over >= 0), anys = __ballot_sync(0xffffffffu, any >= 0);
+          if (anys) positive = __shfl_sync(0xffffffffu, any, 31 - __clz(anys));
+          if (overs && crossed && pick < 0) pick = __shfl_sync(0xffffffffu, over, __ffs(overs) - 1);
+          base += __shfl_sync(0xffffffffu, up, 31);
         }
       }
       if (lane == 0) P.picked[b] = pick >= 0 ? pick : positive;
@@ -417,14 +485,23 @@ verify_drafts_kernel(const VerifyParams P) {
   cluster.sync();                                  // nobody leaves while its sums may still be read
 }
 
+static int vd_resident(int C) {
+  static int known[17];                            // n + 1
+  if (!known[C]) known[C] = 1 + resident_clusters((const void*)verify_drafts_kernel<4>, C, VD_THREADS);
+  return known[C] - 1;
+}
+
 // call: the parameters as the launcher packs them.
 STRATUM_EXPORT int stratum_verify_drafts(const VerifyParams* call, cudaStream_t stream) {
   const VerifyParams P = *call;
   if (P.n_seqs <= 0) return 0;
   if (P.vocab < 1 || P.n_tokens < 0) return STRATUM_ERR_SHAPE;
   if (P.n_seqs > (1 << 26) || P.vocab > (1 << 30)) return STRATUM_ERR_LIMIT;
-  // as many blocks a row as leave every warp a few lines of it and all of them resident (two to an SM)
+  const bool four = (((uintptr_t)P.target | (uintptr_t)P.draft) & 15) == 0 && P.ldt % 4 == 0 && P.ldd % 4 == 0;
+  // As many blocks a row as leave every warp some lines of it, while all sequences' clusters find room at once (a cluster
+  // lies within one part of the GPU: 37 clusters of eight do not, and took 17 us where 37 of four took 12)
   int C = 1;
-  while (C < 16 && C * 2048 < P.vocab && (long long)P.n_seqs * C * 2 <= 2 * sms()) C *= 2;
-  return launch_clusters<verify_drafts_kernel>(P.n_seqs, C, VD_THREADS, stream, P);
+  while (C < 16 && C * 2048 < P.vocab && P.n_seqs <= vd_resident(2 * C)) C *= 2;
+  if (four) return launch_clusters<verify_drafts_kernel<4>>(P.n_seqs, C, VD_THREADS, stream, P);
+  return launch_clusters<verify_drafts_kernel<1>>(P.n_seqs, C, VD_THREADS, stream, P);
 }

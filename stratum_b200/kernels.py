@@ -1788,8 +1788,8 @@ def token_probs(logits: torch.Tensor, temperature: torch.Tensor, out: torch.Tens
             raise KernelError("token_probs: out is logits itself or memory of its own")
     f = _fn("draft_verify", "stratum_token_probs",
             [c_void_p, ctypes.c_longlong, c_void_p, c_void_p, ctypes.c_longlong, c_int, c_int, c_void_p])
-    _check(f(logits.data_ptr(), logits.stride(0), temperature.data_ptr(), out.data_ptr(), out.stride(0), R, V, _stream()),
-           "token_probs")
+    _check(f(logits.data_ptr(), logits.stride()[0], temperature.data_ptr(), out.data_ptr(), out.stride()[0], R, V,
+             _stream()), "token_probs")
 
 
 VERIFY_MAX_NODES = 1024            # of a sequence

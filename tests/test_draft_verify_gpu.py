@@ -79,6 +79,26 @@ def test_probabilities_of_odd_rows():
         assert torch.equal(wide[:, :1003], out[:, :1003])
 
 
+@pytest.mark.parametrize("rows,vocab", [(600, 8192), (601, 4100), (330, 30000), (150, 65540), (100, 128256), (75, 200000)])
+def test_probabilities_of_many_rows(rows, vocab):
+    """Rows enough for the blocks that stay; rows apart, in place, and odd ones among them."""
+    from stratum_b200 import kernels as K
+    rng = np.random.default_rng(rows)
+    base = (rng.standard_normal((rows, vocab)) * 3).astype(np.float32)
+    base[3], base[5, 7:9], base[7, 11], base[9, ::2] = -np.inf, np.inf, np.nan, -np.inf
+    base[11, 100], base[11, vocab - 2] = 30.0, 30.0
+    t = rng.uniform(0.3, 1.5, rows).astype(np.float32)
+    t[11], t[rows - 1] = 0.0, 0.0
+    x = torch.zeros(rows, vocab + 4, device="cuda")
+    x[:, :vocab] = dev(base, torch.float32)
+    out = torch.full((rows, vocab + 8), 9.0, device="cuda")
+    K.token_probs(x[:, :vocab], dev(t, torch.float32), out[:, :vocab])
+    K.token_probs(x[:, :vocab], dev(t, torch.float32), x[:, :vocab])
+    K.check_status()
+    check_probs(base, t, out[:, :vocab])
+    assert (out[:, vocab:] == 9.0).all() and (x[:, vocab:] == 0.0).all() and torch.equal(x[:, :vocab], out[:, :vocab])
+
+
 def test_probabilities_do_not_depend_on_the_batch():
     """(as long as the rows are cut alike: a row's bits follow from its values and the blocks it is given)"""
     from stratum_b200 import kernels as K
