@@ -8,7 +8,8 @@
 // the others are drafts, each behind its parent.  The walk begins at the first node with d = the target's probabilities
 // behind it and mass = 1, and tries the node's children in order, child x with its own number u:
 //   drawn from a draft distribution q (that of the parent's row):  taken if u mass q(x) < d(x);  else  d = max(d - mass q, 0)
-//     and mass = sum d, unless nothing would be left;
+//     and mass = sum d, unless nothing would be left (after several rejections d = max(p - cover q, 0) with the sum of the
+//     masses so far for `cover`, since max(max(a, 0) - b, 0) = max(a - b, 0));
 //   looked up, without a distribution:  taken if u mass < d(x);  else  mass = max(mass - d(x), 0) and d(x) = 0.
 // A child that is taken is the next node.  Where none is, the next token is drawn from d: the first index whose running sum
 // is over u_0 sum(d), u_0 being the first node's number (the last index with any weight if rounding leaves none).  Whoever
@@ -69,6 +70,11 @@ static int launch_clusters(unsigned rows, unsigned cluster, unsigned threads, cu
   return (int)cudaLaunchKernelEx(&cfg, kernel, args...);
 }
 
+// A block may write to another one's shared memory once that one has begun: everybody says so at the start and looks, when it
+// comes to that, whether the others have.
+__device__ __forceinline__ void cluster_begun() { asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory"); }
+__device__ __forceinline__ void cluster_all_begun() { asm volatile("barrier.cluster.wait.aligned;" ::: "memory"); }
+
 // ================================================================ probabilities
 // A row is read once and written once: its values stay in registers, 32 to a thread of a block, the rest of the row in the
 // other blocks of the cluster.  A block takes its exponentials against its own largest value, so the blocks meet
@@ -98,6 +104,7 @@ token_probs_kernel(const float* logits, long long ld, const float* temperature, 
   cg::cluster_group cluster = cg::this_cluster();
   const int C = cluster.num_blocks(), c = cluster.block_rank();
   const int row = blockIdx.x / C, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  cluster_begun();
   pdl_wait();
   const int i0 = min(c * slice, vocab), n = min(vocab - i0, slice);
   const float* in = logits + row * ld + i0;
@@ -160,6 +167,7 @@ token_probs_kernel(const float* logits, long long ld, const float* temperature, 
   sum = warp_sum(sum);
   if (lane == 0) warp_sum_[warp] = sum;
   __syncthreads();
+  cluster_all_begun();
   if (warp == 0) {
     sum = warp_sum(lane < PR_THREADS / 32 ? warp_sum_[lane] : 0.f);
     if (lane < C) *cluster.map_shared_rank(&told[c], lane) = Part{m, sum, first};
@@ -230,24 +238,28 @@ struct VerifyParams {
 
 __device__ __forceinline__ float vd_prob(float p) { return fminf(fmaxf(p, 0.f), 1.f); }     // (fmaxf drops what is no number)
 
-// A clamped probability in 64 bits.  Conversions from 32 to 64 bits run at a quarter of the rate of the additions they feed,
-// so a normal number's bits are moved by hand; zero stays zero, and what is smaller than a normal number is converted.
+// A clamped probability in 64 bits, times 2^-896: a float's bits moved into a double's, whose exponent has another offset.
+// Exact, for zero and what is below the smallest normal number too; sums, differences and comparisons of such numbers need no
+// scale.  (Conversions from 32 to 64 bits run at a quarter of the rate of the additions they feed.)
+#define VD_SCALE 0x1p-896
 __device__ __forceinline__ double vd_wide(float p) {
   const unsigned b = __float_as_uint(p);
-  if (b - 1u < 0x007fffffu) return (double)p;
-  return __hiloint2double(b ? (int)((b >> 3) + (896u << 20)) : 0, (int)(b << 29));
+  return __hiloint2double((int)(b >> 3), (int)(b << 29));
 }
-__device__ __forceinline__ double vd_positive(double w) { return __double2hiint(w) < 0 ? 0.0 : w; }
+__device__ __forceinline__ double vd_lower(double p, double cover, double q) {
+  const double w = fma(-cover, q, p);
+  return __double2hiint(w) < 0 ? 0.0 : w;
+}
 
 struct VdSmem {
   int parent[VD_NODES], token[VD_NODES];
   float u[VD_NODES], p[VD_NODES], q[VD_NODES];   // a node's number, and its parent's probabilities of it
-  double seg[2][VD_WARPS];                 // sums of the warps' stretches of the row; every other sum has the other array
-  double masses[VD_NODES];                 // the masses the row has been lowered at
+  double seg[VD_WARPS];                    // sums of the warps' stretches of the row, then running
+  double told[2][16];                      // the blocks' sums, from everyone; every other sum has the other places
   int zeroed[VD_NODES];                    // ids the row has lost (looked up)
-  double mass;
-  int node, depth, n_masses, n_zeroed, want;
-  double all[16 * VD_WARPS];               // the whole cluster's sums, running
+  double mass, cover;                      // (cover: 0 until the row has been lowered)
+  int node, depth, n_zeroed, want;
+  double all[16];                          // the blocks' sums, running
 };
 
 // W: ids of a load (4 where every row begins on 16 bytes); a warp has LINES loads of a row on their way together.
@@ -259,9 +271,11 @@ verify_drafts_kernel(const VerifyParams P) {
   cg::cluster_group cluster = cg::this_cluster();
   const int C = cluster.num_blocks(), c = cluster.block_rank();
   const int b = blockIdx.x / C, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  cluster_begun();
   pdl_wait();
   const int a = min(max(__ldcg(P.seq_start + b), 0), P.n_tokens), n = min(max(__ldcg(P.seq_start + b + 1), a), P.n_tokens) - a;
   if (n == 0) {                                    // (the same in the whole cluster)
+    cluster_all_begun();
     if (c == 0 && tid == 0) { P.kept[b] = 0; P.picked[b] = -1; }
     return;
   }
@@ -278,9 +292,10 @@ verify_drafts_kernel(const VerifyParams P) {
     }
     S.parent[i] = parent; S.token[i] = token; S.u[i] = __ldcg(P.uniform + a + i); S.p[i] = p; S.q[i] = q;
   }
-  if (tid == 0) { S.mass = 1.0; S.node = 0; S.depth = 0; S.n_masses = 0; S.n_zeroed = 0; }
+  if (tid == 0) { S.mass = 1.0; S.cover = 0.0; S.node = 0; S.depth = 0; S.n_zeroed = 0; }
   if (c == 0) for (int i = tid; i < n; i += VD_THREADS) P.path[a + i] = i == 0 ? 0 : -1;
   __syncthreads();
+  cluster_all_begun();
 
   // A warp's stretch of the row, in whole lines of LINE ids.
   const int n_seg = C * VD_WARPS, lines = (P.vocab + LINE - 1) / LINE, per = (lines + n_seg - 1) / n_seg * LINE;
@@ -306,21 +321,21 @@ verify_drafts_kernel(const VerifyParams P) {
       }
     }
   };
-  // d of W ids from i on: the target's row, lowered at k masses, without the ids it has lost (those of the list that lie in
-  // this warp's stretch, if any do)
-  auto weights = [&](const float (&p)[W], const float (&q)[W], int i, int k, bool lost, double (&w)[W]) {
+  // d of W ids from i on, times VD_SCALE: the target's row, lowered by the draft's, without the ids it has lost (those of the
+  // list that lie in this warp's stretch, if any do)
+  auto weights = [&](float (&p)[W], float (&q)[W], int i, double cover, bool lost, double (&w)[W]) {
+    unsigned most = 0;                             // (a number in [0, 1] has no larger bits than 1 has)
 #pragma unroll
-    for (int e = 0; e < W; e++) w[e] = vd_wide(vd_prob(p[e]));
-    if (k > 0) {
-      double qd[W];
+    for (int e = 0; e < W; e++) most = max(most, max(__float_as_uint(p[e]), __float_as_uint(q[e])));
+    if (most > 0x3f800000u) {
 #pragma unroll
-      for (int e = 0; e < W; e++) { qd[e] = vd_wide(vd_prob(q[e])); w[e] = vd_positive(w[e] - qd[e]); }    // (a row's first mass is one)
-#pragma unroll 1
-      for (int j = 1; j < k; j++) {
-        const double m = S.masses[j];
+      for (int e = 0; e < W; e++) { p[e] = vd_prob(p[e]); q[e] = vd_prob(q[e]); }
+    }
 #pragma unroll
-        for (int e = 0; e < W; e++) w[e] = vd_positive(__dsub_rn(w[e], __dmul_rn(m, qd[e])));
-      }
+    for (int e = 0; e < W; e++) w[e] = vd_wide(p[e]);
+    if (cover > 0.0) {
+#pragma unroll
+      for (int e = 0; e < W; e++) w[e] = vd_lower(w[e], cover, vd_wide(q[e]));
     }
     if (lost) {
 #pragma unroll 1
@@ -352,22 +367,22 @@ verify_drafts_kernel(const VerifyParams P) {
         last = child;
         const int token = S.token[child];
         if (token < 0) continue;
-        const double mass = S.mass, q = (double)S.q[child];              // (looked up: q = 1)
-        double w = (double)S.p[child];
-        for (int j = 0; j < S.n_masses; j++) { w = __dsub_rn(w, __dmul_rn(S.masses[j], q)); w = w > 0.0 ? w : 0.0; }
+        const double mass = S.mass, q = P.draft ? vd_wide(S.q[child]) : VD_SCALE;
+        double w = vd_wide(S.p[child]);
+        if (S.cover > 0.0) w = vd_lower(w, S.cover, q);
         for (int j = 0; j < S.n_zeroed; j++) if (S.zeroed[j] == token) w = 0.0;
         __syncwarp();
         if (__dmul_rn(__dmul_rn((double)S.u[child], mass), q) < w) {
           node = child; depth++;                   // (its children come behind it)
           if (lane == 0) {
             if (c == 0) P.path[a + depth] = child;
-            S.mass = 1.0; S.n_masses = 0; S.n_zeroed = 0;
+            S.mass = 1.0; S.cover = 0.0; S.n_zeroed = 0;
           }
           summed = false;
         } else if (P.draft) {
-          if (lane == 0) S.masses[S.n_masses] = mass;
           want = 1;
         } else {
+          w *= 1.0 / VD_SCALE;
           if (lane == 0) { S.mass = mass - w > 0.0 ? mass - w : 0.0; S.zeroed[S.n_zeroed++] = token; }
           summed = false;
         }
@@ -381,17 +396,17 @@ verify_drafts_kernel(const VerifyParams P) {
     {
       const float* trow = P.target + (long long)(a + S.node) * P.ldt;
       const float* drow = P.draft ? P.draft + (long long)(a + S.node) * P.ldd : nullptr;
-      const int k = S.n_masses + (want == 1 ? 1 : 0);
+      const double cover = S.cover + (want == 1 ? S.mass : 0.0);
       const bool lost = S.n_zeroed > 0 && loses_between(s0, s1);
       double sum = 0.0;
 #pragma unroll 1
       for (int i0 = s0; i0 < s1; i0 += LINES * LINE) {
         float p[LINES][W], q[LINES][W];
-        fetch(trow, drow, i0 + lane * W, s1, k > 0, p, q);
+        fetch(trow, drow, i0 + lane * W, s1, cover > 0.0, p, q);
 #pragma unroll
         for (int x = 0; x < LINES; x++) {
           double w[W];
-          weights(p[x], q[x], i0 + x * LINE + lane * W, k, lost, w);
+          weights(p[x], q[x], i0 + x * LINE + lane * W, cover, lost, w);
           double part = 0.0;
 #pragma unroll
           for (int e = 0; e < W; e++) part += w[e];
@@ -400,24 +415,28 @@ verify_drafts_kernel(const VerifyParams P) {
       }
 #pragma unroll
       for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-      if (lane == 0) S.seg[parity][warp] = sum;
+      if (lane == 0) S.seg[warp] = sum;
     }
-    cluster.sync();
-    if (warp == 0) {                               // running sums over all stretches of the cluster, in order
-      double carry = 0.0;
-      for (int i0 = 0; i0 < n_seg; i0 += 32) {
-        const int i = i0 + lane;
-        double v = i < n_seg ? cluster.map_shared_rank(&S, i / VD_WARPS)->seg[parity][i % VD_WARPS] : 0.0;
+    __syncthreads();
+    auto scan = [&](double v, int n) {             // running sums over the first n lanes
 #pragma unroll
-        for (int d = 1; d < 32; d <<= 1) {
-          const double o = __shfl_up_sync(0xffffffffu, v, d);
-          if (lane >= d) v += o;
-        }
-        if (i < n_seg) S.all[i] = carry + v;
-        carry += __shfl_sync(0xffffffffu, v, 31);
+      for (int d = 1; d < 16; d <<= 1) {
+        const double o = __shfl_up_sync(0xffffffffu, v, d);
+        if (lane >= d && lane < n) v += o;
       }
+      return v;
+    };
+    if (warp == 0) {
+      const double v = scan(lane < VD_WARPS ? S.seg[lane] : 0.0, VD_WARPS), total = __shfl_sync(0xffffffffu, v, VD_WARPS - 1);
+      if (lane < VD_WARPS) S.seg[lane] = v;
+      if (lane < C) cluster.map_shared_rank(&S, lane)->told[parity][c] = total;
+    }
+    cluster.sync();                                // (behind the last of these nothing of another block is touched)
+    if (warp == 0) {
+      const double v = scan(lane < C ? S.told[parity][lane] : 0.0, C), carry = __shfl_sync(0xffffffffu, v, C - 1);
+      if (lane < C) S.all[lane] = v;
       summed = want == 2 || carry > 0.0;
-      if (want == 1 && carry > 0.0 && lane == 0) { S.mass = carry; S.n_masses++; }      // (else the row stays as it was)
+      if (want == 1 && carry > 0.0 && lane == 0) { S.cover += S.mass; S.mass = carry * (1.0 / VD_SCALE); }      // (else the row stays as it was)
       __syncwarp();
     }
     parity ^= 1;
@@ -425,34 +444,37 @@ verify_drafts_kernel(const VerifyParams P) {
   }
   // ---- the draw
   if (warp == 0) {
-    const double total = S.all[n_seg - 1], aim = __dmul_rn((double)S.u[0], total);
-    // the first stretch whose running sum is over the aim; none (rounding): the last one that has any weight
-    int found = -1, last_any = 0;
-    for (int i0 = 0; i0 < n_seg; i0 += 32) {
-      const int i = i0 + lane;
-      const double v = i < n_seg ? S.all[i] : 0.0, before = i > 0 && i < n_seg ? S.all[i - 1] : 0.0;
-      const unsigned over = __ballot_sync(0xffffffffu, i < n_seg && v > aim);
-      const unsigned any = __ballot_sync(0xffffffffu, i < n_seg && v > before);
-      if (over && found < 0) found = i0 + __ffs(over) - 1;
-      if (any) last_any = i0 + 31 - __clz(any);
-    }
-    const bool crossed = found >= 0;
-    if (!crossed) found = last_any;
+    const double total = S.all[C - 1], aim = __dmul_rn((double)S.u[0], total);
+    // the first block, and in it the first warp, whose running sum is over the aim; none (rounding): the last one that has
+    // any weight
+    auto find = [&](double v, double before, int n, bool& over) {
+      const unsigned overs = __ballot_sync(0xffffffffu, lane < n && v > aim), anys = __ballot_sync(0xffffffffu, lane < n && v > before);
+      over = overs != 0;
+      return overs ? __ffs(overs) - 1 : anys ? 31 - __clz(anys) : 0;
+    };
+    bool crossed;
+    const int block = find(lane < C ? S.all[lane] : 0.0, lane > 0 && lane < C ? S.all[lane - 1] : 0.0, C, crossed);
     int pick = -1, positive = 0;
-    if (found / VD_WARPS == c && total > 0.0) {
+    if (block == c && total > 0.0) {
+      const double front = c > 0 ? S.all[c - 1] : 0.0;
+      const double mine = lane < VD_WARPS ? S.seg[lane] : 0.0, less = lane > 0 && lane < VD_WARPS ? S.seg[lane - 1] : 0.0;
+      bool here;
+      const int w_ = find(front + mine, front + less, VD_WARPS, here), found = c * VD_WARPS + w_;
+      crossed = crossed && here;
       const float* trow = P.target + (long long)(a + S.node) * P.ldt;
       const float* drow = P.draft ? P.draft + (long long)(a + S.node) * P.ldd : nullptr;
-      const int f0 = (int)min((long long)found * per, (long long)P.vocab), f1 = min(f0 + per, P.vocab), k = S.n_masses;
+      const int f0 = (int)min((long long)found * per, (long long)P.vocab), f1 = min(f0 + per, P.vocab);
+      const double cover = S.cover;
       const bool lost = S.n_zeroed > 0 && loses_between(f0, f1);
-      double base = found > 0 ? S.all[found - 1] : 0.0;
+      double base = front + (w_ > 0 ? S.seg[w_ - 1] : 0.0);
       for (int i0 = f0; i0 < f1 && pick < 0; i0 += LINES * LINE) {
         float p[LINES][W], q[LINES][W];
-        fetch(trow, drow, i0 + lane * W, f1, k > 0, p, q);
+        fetch(trow, drow, i0 + lane * W, f1, cover > 0.0, p, q);
 #pragma unroll
         for (int x = 0; x < LINES; x++) {
           const int i = i0 + x * LINE + lane * W;
           double w[W];
-          weights(p[x], q[x], i, k, lost, w);
+          weights(p[x], q[x], i, cover, lost, w);
           double v = 0.0;
 #pragma unroll
           for (int e = 0; e < W; e++) v += w[e];
@@ -482,7 +504,6 @@ verify_drafts_kernel(const VerifyParams P) {
       if (!(total > 0.0)) P.picked[b] = 0;         // nothing to draw from
     }
   }
-  cluster.sync();                                  // nobody leaves while its sums may still be read
 }
 
 static int vd_resident(int C) {
