@@ -28,14 +28,15 @@ def pages_for(n_tokens: int) -> int:
 
 
 class PagePool:
-    """Free list of page numbers 0..n_pages-1.  Lowest numbers are handed out first."""
+    """Free list of page numbers 0..n_pages-1.  Lowest numbers are handed out first.  A page may have several holders (a
+    sequence and its forks share the pages that are full); it is free again when the last one gives it back."""
 
     def __init__(self, n_pages: int):
         if n_pages < 1:
             raise ValueError("a page pool needs at least one page")
         self.n_pages = n_pages
         self._free: List[int] = list(range(n_pages - 1, -1, -1))   # pop() yields the lowest
-        self._held = [False] * n_pages
+        self._held = [0] * n_pages                                  # holders of each page
 
     @property
     def free_pages(self) -> int:
@@ -47,8 +48,19 @@ class PagePool:
                             f"(of {self.n_pages})")
         out = [self._free.pop() for _ in range(n)]
         for p in out:
-            self._held[p] = True
+            self._held[p] = 1
         return out
+
+    def share(self, pages: List[int]) -> None:
+        """One more holder for each of these pages."""
+        for p in pages:
+            if not (0 <= p < self.n_pages) or not self._held[p]:
+                raise CacheMisuse(f"page {p} shared but not held")
+        for p in pages:
+            self._held[p] += 1
+
+    def holders(self, page: int) -> int:
+        return self._held[page]
 
     def give(self, pages: List[int]) -> None:
         seen = set()
@@ -57,9 +69,9 @@ class PagePool:
                 raise CacheMisuse(f"page {p} given back but not held")
             seen.add(p)
         for p in pages:
-            self._held[p] = False
+            self._held[p] -= 1
         # keep the free list sorted descending so that take() stays lowest-first and deterministic
-        self._free.extend(pages)
+        self._free.extend(p for p in pages if not self._held[p])
         self._free.sort(reverse=True)
 
     def check(self) -> None:
@@ -68,7 +80,7 @@ class PagePool:
         if len(free) != len(self._free):
             raise CacheMisuse("a page is on the free list twice")
         for p in range(self.n_pages):
-            if self._held[p] == (p in free):
+            if (self._held[p] > 0) == (p in free):
                 raise CacheMisuse(f"page {p} is {'both held and free' if self._held[p] else 'lost'}")
 
 
@@ -160,6 +172,26 @@ class SequencePages:
                     self.table[i] = -1
                 return True
         return False
+
+    def trim(self) -> bool:
+        """Pages beyond the sequence's length (taken for drafted tokens that were not kept) go back; True if there were any."""
+        beyond = self.table[pages_for(self.length):]
+        del self.table[pages_for(self.length):]
+        self.pool.give([p for p in beyond if p >= 0])
+        return bool(beyond)
+
+    def fork(self) -> "tuple[SequencePages, Optional[tuple[int, int]]]":
+        """A second holder of the sequence as it is: its full pages are shared (nobody writes to a full page), the last,
+        partly filled one is to be copied.  (the new sequence's pages, (from, to) of the copy or None)."""
+        new = SequencePages(self.pool, self.window, self.keep_first, self.chunk)
+        full = self.length // PAGE_TOKENS
+        part = self.table[full] if self.length % PAGE_TOKENS else -1
+        copy = (part, self.pool.take(1)[0]) if part >= 0 else None
+        shared = self.table[:full]
+        self.pool.share([p for p in shared if p >= 0])
+        new.table = shared + ([copy[1]] if copy else [-1] if self.length % PAGE_TOKENS else [])
+        new.length = self.length
+        return new, copy
 
     def release(self) -> None:
         self.pool.give([p for p in self.table if p >= 0])

@@ -19,6 +19,7 @@ from typing import Dict, List, Optional, Sequence, Tuple, Union
 
 import torch
 
+from .. import kernels as K
 from .pages import (PAGE_TOKENS, CacheFull, CacheMisuse, PagePool, SequencePages, SlotTable,
                     pages_for)
 
@@ -208,6 +209,56 @@ class SequenceCache:
         self.slots.release(slot)
         self.epoch += 1
 
+    def trim(self, slots: Sequence[int]) -> None:
+        """Pages that sequences hold beyond their lengths (for drafted tokens that were not kept) go back."""
+        for s in slots:
+            self._need(s)
+            for sp in self._seq[s]:
+                if sp is not None and sp.trim():
+                    self.epoch += 1
+
+    def fork(self, slot: int, n: int = 1) -> List[int]:
+        """n new sequences that begin as copies of one: the pages that are full are shared between them, the last one and
+        the fixed-size state are copied, one launch per group of layers.  For all of them or for none."""
+        self._need(slot)
+        if n < 0:
+            raise CacheMisuse("a sequence is forked a number of times")
+        if n > self.slots.free_slots:
+            raise CacheFull(f"{n} forks need {n} sequence slots, {self.slots.free_slots} of {self.max_seqs} are free")
+        partial = self._len[slot] % PAGE_TOKENS != 0
+        for gi, g in enumerate(self.groups):
+            if g.pool is not None and partial and n > g.pool.free_pages:
+                raise CacheFull(f"{n} forks need {n} more pages of {PAGE_TOKENS} tokens; {g.pool.free_pages} of {self.n_pages} are free")
+        new = [self.slots.acquire() for _ in range(n)]
+        copies: List[List[Tuple[int, int]]] = [[] for _ in self.groups]
+        for s in new:
+            pages: List[Optional[SequencePages]] = []
+            for gi, sp in enumerate(self._seq[slot]):
+                if sp is None:
+                    copies[gi].append((slot, s))
+                    pages.append(None)
+                    continue
+                forked, copy = sp.fork()
+                pages.append(forked)
+                if copy is not None:
+                    copies[gi].append(copy)
+            self._seq[s] = pages
+            self._len[s] = self._len[slot]
+        self.epoch += bool(new)
+        for g, pairs in zip(self.groups, copies):
+            src, dst = [a for a, _ in pairs], [b for _, b in pairs]
+            if pairs and g.k is not None:
+                K.copy_pages(g.k, g.v, src, dst)
+            elif pairs and g.state is not None:
+                K.copy_pages(g.state, None, src, dst)
+        return new
+
+    def keep_rows(self, group: int, block_table: torch.Tensor, seq_start: torch.Tensor, seq_len: torch.Tensor, path: torch.Tensor,
+                  n_kept: torch.Tensor) -> None:
+        """Move the kept drafted tokens' rows of one key/value group together (see kernels.keep_rows)."""
+        g = self.groups[group]
+        K.keep_rows(g.k, g.v, block_table, seq_start, seq_len, path, n_kept)
+
     def release_all(self) -> None:
         for s in self.slots.live():
             self.release(s)
@@ -224,14 +275,14 @@ class SequenceCache:
             if g.pool is None:
                 continue
             g.pool.check()
-            seen = set()
+            seen: Dict[int, int] = {}
             for s, per_group in self._seq.items():
                 for p in per_group[gi].table:
-                    if p < 0:
-                        continue
-                    if p in seen:
-                        raise CacheMisuse(f"page {p} is held by two sequences")
-                    seen.add(p)
+                    if p >= 0:
+                        seen[p] = seen.get(p, 0) + 1
+            for p, n in seen.items():
+                if n != g.pool.holders(p):
+                    raise CacheMisuse(f"page {p} is held by {n} sequences and counted for {g.pool.holders(p)}")
             if len(seen) != self.n_pages - g.pool.free_pages:
                 raise CacheMisuse("pages held by sequences and pages missing from the pool differ")
         if set(self._seq) != set(self.slots.live()):

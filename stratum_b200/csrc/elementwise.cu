@@ -606,7 +606,8 @@ __global__ void rope_store_kernel(T* __restrict__ qkv, const int* __restrict__ t
                                   const int* __restrict__ token_seq, const int* __restrict__ block_table,
                                   int bt_stride, const float* __restrict__ inv_freq, int n_pairs,
                                   int interleaved, float mscale, T* __restrict__ k_cache, T* __restrict__ v_cache,
-                                  int n_q, int n_kv, int head_dim, int page_tokens, int write_cache) {
+                                  int n_q, int n_kv, int head_dim, int page_tokens, int write_cache,
+                                  const int* __restrict__ token_row) {
   // a block covers one token and blockDim.y heads (q heads, then k heads, then v heads); one thread per pair
   // of dimensions.  Decode steps use one head per block (many small blocks, shortest latency), prompts several.
   pdl_trigger();
@@ -636,10 +637,11 @@ __global__ void rope_store_kernel(T* __restrict__ qkv, const int* __restrict__ t
   }
   T* dst = nullptr;
   if (!is_q) {
-    const int page = block_table[(size_t)seq * bt_stride + pos / page_tokens];
+    const int at = token_row ? token_row[t] : pos;          // (drafted tokens: siblings share a position)
+    const int page = block_table[(size_t)seq * bt_stride + at / page_tokens];
     const int kvh = is_k ? h - n_q : h - n_q - n_kv;
     dst = (is_k ? k_cache : v_cache) +
-          (((size_t)page * n_kv + kvh) * page_tokens + (pos % page_tokens)) * (size_t)head_dim;
+          (((size_t)page * n_kv + kvh) * page_tokens + (at % page_tokens)) * (size_t)head_dim;
   }
   T* hp = qkv + (size_t)t * ((size_t)(n_q + 2 * n_kv) * head_dim) + (size_t)h * head_dim;
   pdl_wait();
@@ -664,7 +666,7 @@ rope_store_prompt_kernel(bf16* __restrict__ qkv, const int* __restrict__ token_p
                          const int* __restrict__ token_seq, const int* __restrict__ block_table, int bt_stride,
                          const float* __restrict__ inv_freq, int n_pairs, float mscale, bf16* __restrict__ k_cache,
                          bf16* __restrict__ v_cache, int n_q, int n_kv, int head_dim, int page_tokens,
-                         int write_cache) {
+                         int write_cache, const int* __restrict__ token_row) {
   extern __shared__ float2 cs[];                 // [n_pairs] (cos, sin) * mscale
   pdl_trigger();
   const int t = blockIdx.x;
@@ -679,8 +681,9 @@ rope_store_prompt_kernel(bf16* __restrict__ qkv, const int* __restrict__ token_p
     sincosf((float)pos * inv_freq[k], &sn, &c);
     cs[k] = make_float2(c * mscale, sn * mscale);
   }
-  const int page = write_cache ? block_table[(size_t)seq * bt_stride + pos / page_tokens] : 0;
-  const size_t cache_row = ((size_t)page * n_kv * page_tokens + (pos % page_tokens)) * (size_t)head_dim;
+  const int at = token_row ? token_row[t] : pos;
+  const int page = write_cache ? block_table[(size_t)seq * bt_stride + at / page_tokens] : 0;
+  const size_t cache_row = ((size_t)page * n_kv * page_tokens + (at % page_tokens)) * (size_t)head_dim;
   const size_t kv_stride = (size_t)page_tokens * head_dim;
   bf16* row = qkv + (size_t)t * ((size_t)(n_q + 2 * n_kv) * head_dim);
   __syncthreads();
@@ -733,11 +736,12 @@ rope_store_prompt_kernel(bf16* __restrict__ qkv, const int* __restrict__ token_p
   }
 }
 
+// token_row (or null): the place in its sequence's cache where a token's key and value go, where that is not its position.
 STRATUM_EXPORT int stratum_rope_store(void* qkv, int dtype, const int* token_pos, const int* token_seq,
                                       const int* block_table, int bt_stride, const float* inv_freq, int n_pairs,
                                       int interleaved, float mscale, void* k_cache, void* v_cache, int n_tokens,
                                       int n_q, int n_kv, int head_dim, int page_tokens, int write_cache,
-                                      cudaStream_t stream) {
+                                      const int* token_row, cudaStream_t stream) {
   if (n_tokens <= 0) return 0;
   if (head_dim % 2 != 0 || 2 * n_pairs > head_dim || n_pairs < 0 || head_dim > 2048) return STRATUM_ERR_SHAPE;
   if (n_q + 2 * n_kv > 65535) return STRATUM_ERR_LIMIT;
@@ -747,10 +751,10 @@ STRATUM_EXPORT int stratum_rope_store(void* qkv, int dtype, const int* token_pos
     if (interleaved)
       return launch_pdl(rope_store_prompt_kernel<true>, n_tokens, 256, smem, stream, (bf16*)qkv, token_pos, token_seq,
                         block_table, bt_stride, inv_freq, n_pairs, mscale, (bf16*)k_cache, (bf16*)v_cache, n_q, n_kv,
-                        head_dim, page_tokens, write_cache);
+                        head_dim, page_tokens, write_cache, token_row);
     return launch_pdl(rope_store_prompt_kernel<false>, n_tokens, 256, smem, stream, (bf16*)qkv, token_pos, token_seq,
                       block_table, bt_stride, inv_freq, n_pairs, mscale, (bf16*)k_cache, (bf16*)v_cache, n_q, n_kv,
-                      head_dim, page_tokens, write_cache);
+                      head_dim, page_tokens, write_cache, token_row);
   }
   const int slots = ((head_dim / 2 + 31) / 32) * 32;
   const int heads = n_q + 2 * n_kv;
@@ -762,11 +766,11 @@ STRATUM_EXPORT int stratum_rope_store(void* qkv, int dtype, const int* token_pos
   if (dtype == STRATUM_DT_F32)
     return launch_pdl(rope_store_kernel<float>, grid, threads, 0, stream, (float*)qkv, token_pos, token_seq,
                       block_table, bt_stride, inv_freq, n_pairs, interleaved, mscale, (float*)k_cache,
-                      (float*)v_cache, n_q, n_kv, head_dim, page_tokens, write_cache);
+                      (float*)v_cache, n_q, n_kv, head_dim, page_tokens, write_cache, token_row);
   if (dtype == STRATUM_DT_BF16)
     return launch_pdl(rope_store_kernel<bf16>, grid, threads, 0, stream, (bf16*)qkv, token_pos, token_seq,
                       block_table, bt_stride, inv_freq, n_pairs, interleaved, mscale, (bf16*)k_cache,
-                      (bf16*)v_cache, n_q, n_kv, head_dim, page_tokens, write_cache);
+                      (bf16*)v_cache, n_q, n_kv, head_dim, page_tokens, write_cache, token_row);
   return STRATUM_ERR_DTYPE;
 }
 

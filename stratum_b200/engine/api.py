@@ -12,14 +12,16 @@ from __future__ import annotations
 import os
 from typing import Callable, List, Optional, Sequence, Tuple
 
+import numpy as np
 import torch
 
+from .. import kernels as K
 from ..config.base import ModelConfig
 from ..sampling import Pcg32, Sampler, SamplingParams
 from .generate import Backend, GenerationResult, generate
 from .graphs import DecodeGraphs, PromptGraphs
 from .model import load_model, random_model_on_device
-from .step import Engine, StepEntry
+from .step import DraftEntry, Engine, StepEntry
 
 _DTYPES = {"float32": torch.float32, "fp32": torch.float32, "bfloat16": torch.bfloat16, "bf16": torch.bfloat16}
 
@@ -149,6 +151,56 @@ class Stratum:
     def collect(self, handle):
         ids, vals, _ = self.graphs.collect(handle)
         return ids, vals
+
+    def fork(self, slot: int, n: int = 1) -> List[int]:
+        """n new sequences that begin as copies of the one in `slot`: pages that are full are shared, the last one is copied.
+        They go on, end and are released each by itself."""
+        return self.engine.fork(slot, n)
+
+    def draft_step(self, entries: Sequence[DraftEntry], sampling: SamplingParams = SamplingParams(),
+                   streams: Optional[Sequence[Pcg32]] = None, draft: Optional[torch.Tensor] = None) -> List[List[int]]:
+        """One step over trees of drafted tokens: for every entry the tokens it adds behind tokens[0], the kept drafts and
+        the one the model picks behind them (one at least).  That last one is tokens[0] of the sequence's next step.
+
+        The tokens are those of the model's own picks: with temperature 0 the greedy ones, else draws from
+        softmax(logits / temperature), distributed as decode_step's are (top_k and top_p have to be off).  Every entry draws a
+        number for each of its tokens from its stream.  draft (float32 [tokens of all entries, vocab] on the device): for
+        every token the distribution its children were drawn from, each for itself; None: they were looked up or guessed.
+        On error no sequence is longer than before."""
+        entries = list(entries)
+        if sampling.top_k > 0 or sampling.top_p < 1.0:
+            raise ValueError("draft_step draws from all ids: top_k and top_p have to be off")
+        if not sampling.greedy and (streams is None or len(streams) != len(entries)):
+            raise ValueError("draft_step: one random stream per entry")
+        eng, device = self.engine, self.model.runtime.device
+        eng.validate_drafts(entries)
+        T, B = sum(len(e.tokens) for e in entries), len(entries)
+        if draft is not None and tuple(draft.shape) != (T, self.model.vocab):
+            raise ValueError(f"draft_step: draft must be [{T}, {self.model.vocab}]")
+        slots = [e.slot for e in entries]
+        try:
+            logits, batch = eng.run_drafts(entries)
+            numbers = np.zeros((2, T), dtype=np.float32)
+            numbers[0] = sampling.temperature
+            if not sampling.greedy:
+                numbers[1] = [st.uniform() for e, st in zip(entries, streams) for _ in e.tokens]
+            dev = torch.from_numpy(numbers).to(device)
+            K.token_probs(logits, dev[0], logits)
+            out = torch.empty(T + 2 * B, dtype=torch.int32, device=device)
+            path, kept, picked = out[:T], out[T:T + B], out[T + B:]
+            K.verify_drafts(logits, draft, batch.token_ids, batch.drafts.parent, batch.seq_start, dev[1], path, kept, picked)
+            eng.move_kept(batch, path, kept)
+            host = out.tolist()
+            eng.check_kernels()
+        except Exception:
+            eng.cache.trim([s for s in slots if eng.cache.slots.is_live(s)])
+            raise
+        n_kept, result, r = host[T:T + B], [], 0
+        for e, n, last in zip(entries, n_kept, host[T + B:]):
+            result.append([int(e.tokens[i]) for i in host[r + 1:r + 1 + n]] + [last])
+            r += len(e.tokens)
+        eng.keep_drafts(batch, n_kept)
+        return result
 
     # -- generation ---------------------------------------------------------------
     def generate(self, prompts: Sequence[Sequence[int]], max_new_tokens=16, stop_ids: Optional[Sequence[int]] = None,

@@ -13,11 +13,11 @@ from typing import Dict, List, Mapping, Optional, Tuple
 import torch
 
 from .. import architectures  # noqa: F401  (registers the built-in architectures)
-from ..cache.store import CacheSpec
+from ..cache.store import CacheSpec, KVSpec
 from ..config.base import ModelConfig, read_config_json
 from ..config.registry import find_architecture
 from ..parts import find_part
-from ..parts.base import Runtime
+from ..parts.base import Mixer, Runtime
 from ..parts.spec import LayerSpec, ModelSpec, TensorSpec
 from .resident import ResidentSteps
 from ..weights.loader import check_tensors, load_weights, place, tensor_shapes
@@ -128,6 +128,12 @@ class Model:
         for layer in self.layers:
             parts += list(layer.parts()) + [layer.arrangement]
         return all(getattr(p, "replays_prompts", False) for p in parts)
+
+    def takes_drafts(self) -> bool:
+        """Whether a step may carry drafted tokens: every mixer serves them, and nothing is kept per sequence but keys and
+        values (a state that a thrown away draft has changed could not be given back)."""
+        mixers = [p for layer in self.layers for p in layer.parts() if isinstance(p, Mixer)]
+        return (all(m.takes_drafts for m in mixers) and all(s is None or isinstance(s, KVSpec) for s in self.cache_specs()))
 
     def resident_steps(self) -> Optional[ResidentSteps]:
         """How decode steps of a few rows run as one kernel; None where the model's parts are not the ones it knows."""

@@ -36,6 +36,30 @@ class StepEntry:
 
 
 @dataclass
+class DraftEntry:
+    """A sequence's part of a step of drafted tokens.  tokens[0] is the token the sequence goes on with (picked, not yet run),
+    the others are drafts; parents[i] is the place among `tokens` of the one that tokens[i] was drafted behind (-1 for the
+    first, smaller than i for the others; None: each behind the one before)."""
+    slot: int
+    tokens: Sequence[int]
+    parents: Optional[Sequence[int]] = None
+
+    def tree(self) -> List[int]:
+        return list(range(-1, len(self.tokens) - 1)) if self.parents is None else [int(p) for p in self.parents]
+
+
+@dataclass
+class DraftRows:
+    """What a step of drafted tokens has beside a StepBatch's fields (there token_pos is the depth in the tree, counted on
+    from the sequence's length, and seq_len counts the drafts)."""
+    row: torch.Tensor                 # int32 [T] place in its sequence where a token's key and value go
+    parent: torch.Tensor              # int32 [T] as DraftEntry.parents
+    masks: Dict[int, torch.Tensor]    # window -> int64 [T, words]: which drafted rows of its sequence a token sees
+    lengths: List[int]                # of the sequences before the step, in the order of the entries
+    entries: List[DraftEntry]
+
+
+@dataclass
 class StepBatch:
     """Device-side description of one step, shared by every part."""
     n_tokens: int
@@ -55,6 +79,7 @@ class StepBatch:
     fixed_qblocks: Optional[Dict[int, tuple]] = None   # a captured prompt step: its query blocks, padded lists
     sizes_seen: Optional[set] = None  # when set: the block sizes `query_blocks` was asked for are noted here
     kept: Dict[str, torch.Tensor] = field(default_factory=dict)   # rows a layer leaves for later layers of the same step
+    drafts: Optional[DraftRows] = None        # set in a step of drafted tokens
     embedded: Optional[torch.Tensor] = None   # float32 [T, hidden]: the embedded tokens, for models that re-read them
     _qblocks: Dict[int, tuple] = field(default_factory=dict)
     _rotation: Dict[object, torch.Tensor] = field(default_factory=dict)
@@ -277,6 +302,21 @@ class StepDescription:
                          fixed_qblocks=fixed)
 
 
+def tree_depths_and_masks(tree: Sequence[int], window: int, words: int):
+    """Of a tree of drafted tokens: every node's depth, and which nodes it sees, itself and its ancestors (with a window
+    those less than `window` deep above it), as `words` numbers of 64 bits."""
+    depth: List[int] = []
+    above: List[List[int]] = []                   # a node and its ancestors, the nearest first
+    for i, p in enumerate(tree):
+        depth.append(0 if p < 0 else depth[p] + 1)
+        above.append([i] + (above[p] if p >= 0 else []))
+    masks = np.zeros((len(tree), words), dtype=np.uint64)
+    for i, nodes in enumerate(above):
+        for j in nodes[:window] if window > 0 else nodes:
+            masks[i, j >> 6] |= np.uint64(1) << np.uint64(j & 63)
+    return depth, masks.view(np.int64)
+
+
 class Engine:
     """A model, its cache and the step function over them."""
 
@@ -293,6 +333,10 @@ class Engine:
     # ------------------------------------------------------------------ sequences
     def acquire(self) -> int:
         return self.cache.acquire()
+
+    def fork(self, slot: int, n: int = 1) -> List[int]:
+        """n new sequences that begin as copies of one (see SequenceCache.fork)."""
+        return self.cache.fork(slot, n)
 
     def release(self, slot: int) -> None:
         self.cache.release(slot)
@@ -335,6 +379,67 @@ class Engine:
         d.write_tokens([e.tokens for e in entries], before)
         d.upload()
         return d.batch(max_len)
+
+    # ------------------------------------------------------------------ steps of drafted tokens
+    def validate_drafts(self, entries: Sequence[DraftEntry]) -> None:
+        """Refuse a step of drafted tokens before anything runs."""
+        if not self.model.takes_drafts():
+            raise StepError("this model's layers do not take drafted tokens (attention over keys and values alone does)")
+        self.validate([e.slot for e in entries], [e.tokens for e in entries])
+        for e in entries:
+            tree = e.tree()
+            if len(e.tokens) > K.VERIFY_MAX_NODES:
+                raise StepError(f"slot {e.slot}: {len(e.tokens)} drafted tokens, at most {K.VERIFY_MAX_NODES}")
+            if len(tree) != len(e.tokens) or tree[0] != -1 or any(not 0 <= p < i for i, p in enumerate(tree) if i > 0):
+                raise StepError(f"slot {e.slot}: a draft's parent is a token in front of it, the first token's is -1")
+
+    def run_drafts(self, entries: Sequence[DraftEntry]):
+        """Run trees of drafted tokens, each behind its sequence: (float32 logits of every token [tokens, vocab], the
+        StepBatch).  The sequences' lengths stay as they are: `keep_drafts` says which tokens were kept."""
+        entries = list(entries)
+        self.validate_drafts(entries)
+        slots, n_new = [e.slot for e in entries], [len(e.tokens) for e in entries]
+        self.cache.reserve(slots, n_new)          # raises CacheFull before anything is launched
+        lengths = [self.cache.length(s) for s in slots]
+        T = sum(n_new)
+        max_len = max(b + n for b, n in zip(lengths, n_new))
+        d = StepDescription(self, T, len(entries), T, max(1, pages_for(max_len)), extras=(("row", T), ("parent", T)))
+        d.write_membership(slots, n_new, [range(n) for n in n_new])
+        d.write_tokens([e.tokens for e in entries], lengths)
+        d.views["row"][:] = d.views["pos"]        # one behind the other, whatever their depths
+        windows = sorted({self.cache.groups[gi].spec.window for gi in self.kv_groups})
+        words, r = (max(n_new) + 63) // 64, 0
+        masks = np.zeros((len(windows), T, words), dtype=np.int64)
+        for e, base, n in zip(entries, lengths, n_new):
+            tree = e.tree()
+            for i, window in enumerate(windows):
+                depth, masks[i, r:r + n] = tree_depths_and_masks(tree, window, words)
+            d.views["pos"][r:r + n] = base + np.asarray(depth, dtype=np.int32)
+            d.views["parent"][r:r + n] = tree
+            r += n
+        d.upload()
+        batch = d.batch(max_len)
+        batch.all_single = False                  # (single tokens take the forms of trees too)
+        on_device = torch.from_numpy(masks).to(self.runtime.device)
+        batch.drafts = DraftRows(row=d.field("row"), parent=d.field("parent"), lengths=lengths, entries=entries,
+                                 masks={w: on_device[i] for i, w in enumerate(windows)})
+        return self.model.forward(batch, self.cache), batch
+
+    def move_kept(self, batch: StepBatch, path: torch.Tensor, n_kept: torch.Tensor) -> None:
+        """The kept drafts' keys and values move together behind the tokens in front of them (device tensors as
+        kernels.verify_drafts writes them)."""
+        for gi in self.kv_groups:
+            self.cache.keep_rows(gi, batch.block_tables[gi], batch.seq_start, batch.seq_len, path, n_kept)
+
+    def keep_drafts(self, batch: StepBatch, n_kept: Sequence[int]) -> None:
+        """Book what a step of drafted tokens left: every sequence grows by its first token and the kept drafts; pages taken
+        for the others go back."""
+        slots = [e.slot for e in batch.drafts.entries]
+        for s, before in zip(slots, batch.drafts.lengths):
+            if self.cache.length(s) != before:
+                raise StepError(f"slot {s} has gone on since its drafts were run")
+        self.cache.advance(slots, [1 + int(n) for n in n_kept])
+        self.cache.trim(slots)
 
     def check_kernels(self) -> None:
         """Raise if a kernel gave up a bounded wait since the last check (synchronises)."""

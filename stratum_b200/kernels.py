@@ -311,8 +311,14 @@ def swiglu(gu: torch.Tensor, out: torch.Tensor, act: int = 0, limit=0.0) -> None
 def rope_store(qkv: torch.Tensor, token_pos: torch.Tensor, token_seq: torch.Tensor,
                block_table: Optional[torch.Tensor], inv_freq: Optional[torch.Tensor], interleaved: bool,
                mscale: float, k_cache: Optional[torch.Tensor], v_cache: Optional[torch.Tensor],
-               n_q: int, n_kv: int, head_dim: int, page_tokens: int, write_cache: bool) -> None:
-    """Rotate q (in place) and k, and store k and v into the paged cache."""
+               n_q: int, n_kv: int, head_dim: int, page_tokens: int, write_cache: bool,
+               token_row: Optional[torch.Tensor] = None) -> None:
+    """Rotate q (in place) and k, and store k and v into the paged cache: at the token's position or, where token_row
+    (int32 [tokens]) is given, at that place of its sequence (drafted tokens: siblings share a position)."""
+    if token_row is not None:
+        _need(token_row, "token_row", torch.int32)
+        if token_row.numel() != qkv.shape[0]:
+            raise KernelError("rope_store: token_row and qkv disagree")
     _need(qkv, "qkv"); _need(token_pos, "token_pos", torch.int32); _need(token_seq, "token_seq", torch.int32)
     n_pairs = 0 if inv_freq is None else inv_freq.numel()
     if inv_freq is not None:
@@ -324,11 +330,11 @@ def rope_store(qkv: torch.Tensor, token_pos: torch.Tensor, token_seq: torch.Tens
         raise KernelError("rope_store: qkv width is not (n_q + 2 n_kv) * head_dim")
     f = _fn("elementwise", "stratum_rope_store",
             [c_void_p, c_int, c_void_p, c_void_p, c_void_p, c_int, c_void_p, c_int, c_int, c_float, c_void_p,
-             c_void_p, c_int, c_int, c_int, c_int, c_int, c_int, c_void_p])
+             c_void_p, c_int, c_int, c_int, c_int, c_int, c_int, c_void_p, c_void_p])
     _check(f(_ptr(qkv), dtype_code(qkv.dtype), _ptr(token_pos), _ptr(token_seq), _ptr(block_table),
              0 if block_table is None else block_table.stride(0), _ptr(inv_freq), n_pairs, int(interleaved),
              c_float(mscale), _ptr(k_cache), _ptr(v_cache), qkv.shape[0], n_q, n_kv, head_dim, page_tokens,
-             int(write_cache), _stream()), "rope_store")
+             int(write_cache), _ptr(token_row), _stream()), "rope_store")
 
 
 def rope_table(token_pos: torch.Tensor, inv_freq: torch.Tensor, mscale: float, out: torch.Tensor) -> None:

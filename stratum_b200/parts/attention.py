@@ -40,6 +40,7 @@ class GQAAttention(Mixer):
     norm of size head_dim applied to every query / key head between projection and rotation, or None), prefix."""
     takes_normed_rows = True
     hands_on = True
+    takes_drafts = True
 
     @property
     def replays_prompts(self) -> bool:
@@ -143,7 +144,7 @@ class GQAAttention(Mixer):
         STRATUM_FUSE_ROPE=0 turns it off, =2 turns it on for prompts too (measurements)."""
         from . import gemm_dispatch
         mode = os.environ.get("STRATUM_FUSE_ROPE", "1")
-        if mode == "0" or (mode != "2" and not step.all_single):
+        if mode == "0" or (mode != "2" and not step.all_single) or step.drafts is not None:
             return False
         x = xn.x if isinstance(xn, NormedRows) else xn
         return (self.head_dim % 32 == 0 and self.q_norm is None and self.k_norm is None
@@ -165,7 +166,8 @@ class GQAAttention(Mixer):
             K.rope_store(qkv, step.token_pos, step.token_seq, cache.block_table,
                          None if rot is None else rot.inv_freq, rot is not None,       # pairs are neighbours: see bind
                          1.0 if rot is None else rot.magnitude, cache.k, cache.v,
-                         self.n_heads, self.n_kv_heads, self.head_dim, PAGE_TOKENS, cache.writes)
+                         self.n_heads, self.n_kv_heads, self.head_dim, PAGE_TOKENS, cache.writes,
+                         None if step.drafts is None else step.drafts.row)
         out = self.runtime.empty(qkv.shape[0], self.n_heads * self.head_dim)
         from . import attention_dispatch
         attention_dispatch.run(self, qkv, cache, step, out)

@@ -4,6 +4,7 @@ float32, and head sizes the tensor-core kernel refuses (above 128, or no multipl
 kernel with the fixed key order.  bfloat16 decode steps: the TMA-fed kernel that spreads all pages evenly over
 the SMs (head size 64 or 128, up to 8 heads per kv head), else the kernel whose keys are cut into splits per
 sequence, which needs scratch for the partial results.  bfloat16 prompts: the tcgen05 kernel, else the tile kernel.
+Steps of drafted tokens: the tree kernel, which chooses between its two forms by itself.
 """
 from __future__ import annotations
 
@@ -39,6 +40,11 @@ def _stream_form() -> str:
 
 def run(att, qkv: torch.Tensor, cache, step, out: torch.Tensor) -> None:
     hd = att.head_dim
+    drafts = getattr(step, "drafts", None)
+    if drafts is not None:                       # trees of drafted tokens
+        K.attention_tree(qkv, cache.k, cache.v, step.token_pos, drafts.masks[att.window], step.seq_start, step.seq_len, cache.block_table, out,
+                         att.n_heads, att.n_kv_heads, hd, PAGE_TOKENS, att.window, att.scale, step.max_new)
+        return
     if qkv.dtype != torch.bfloat16 or hd % 16 != 0 or hd > 128 or qkv.stride(0) % 8 != 0:
         K.attention_simple(qkv, cache.k, cache.v, step.token_pos, step.token_seq, cache.block_table, out,
                            att.n_heads, att.n_kv_heads, hd, PAGE_TOKENS, att.window, att.scale, step.all_single)

@@ -171,6 +171,9 @@ class Mixer(Part):
     # forward takes `proj`, its float32 result [T, rows of the matrix]: a mixer made of mixers that read the same input
     # runs their products as one (and binds them with own_projection=False)
     splits_projection = False
+    # forward also serves a step of drafted tokens (step.drafts): keys and values go to drafts.row of their sequence, a
+    # token sees what drafts.mask says beside the tokens in front of its tree
+    takes_drafts = False
 
     def cache_spec(self) -> Optional[CacheSpec]:
         """What this mixer keeps per sequence between steps (keys and values, fixed-size state, nothing)."""
