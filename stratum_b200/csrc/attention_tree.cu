@@ -54,7 +54,7 @@ struct TreeParams {
   float2* part_ml;                         // [G][2][rows per tile]: their (maximum, sum)
   struct TreeCut* cut;                     // [G]: what each CTA's stretch begins in
   int* status;
-  int n_tokens, n_seqs, n_q, n_kv, gs, head_dim, window, n_pages, rows_per_tile;
+  int n_tokens, n_seqs, n_q, n_kv, gs, head_dim, window, n_pages, rows_per_tile, even_tiles;
   float scale;
 };
 
@@ -67,7 +67,7 @@ struct alignas(16) TreeCut {
 };
 
 struct TreeSeq {                           // a sequence's share of the list
-  int row0, n_new, base, len, first, n_pages, n_tiles;
+  int row0, n_new, base, len, first, n_pages, n_tiles, tile_rows;
 };
 __device__ __forceinline__ TreeSeq tree_seq(const TreeParams& P, int b) {
   TreeSeq s;
@@ -79,7 +79,10 @@ __device__ __forceinline__ TreeSeq tree_seq(const TreeParams& P, int b) {
   const int lo = (P.window > 0 && s.base - P.window + 1 > 0) ? s.base - P.window + 1 : 0;
   s.first = min(lo / TR_KEYS, pages - 1);
   s.n_pages = pages - s.first;
-  s.n_tiles = (int)(((long long)s.n_new * P.gs + P.rows_per_tile - 1) / P.rows_per_tile);
+  const int rows = s.n_new * P.gs;
+  s.n_tiles = (rows + P.rows_per_tile - 1) / P.rows_per_tile;
+  // (where time goes by rows, a tree's rows are shared out evenly: 68 as 40 and 28, not as 64 and 4)
+  s.tile_rows = P.even_tiles && s.n_tiles > 1 ? ((rows + s.n_tiles - 1) / s.n_tiles + 7) & ~7 : P.rows_per_tile;
   return s;
 }
 // The list of units: every item (sequence, kv head, tile of rows) has one for each of its pages and TREE_ITEM_UNITS more
@@ -179,8 +182,8 @@ __device__ __forceinline__ TreeCursor tree_start(const TreeParams& P, long long*
       const int rt = t.item % t.s.n_tiles;
       cut.item_begin = u0 - t.off;
       cut.n_pages = t.s.n_pages; cut.kvh = t.item / t.s.n_tiles;
-      cut.flat0 = t.s.row0 * P.gs + rt * P.rows_per_tile;
-      cut.n_rows = min(t.s.n_new * P.gs - rt * P.rows_per_tile, P.rows_per_tile);
+      cut.flat0 = t.s.row0 * P.gs + rt * t.s.tile_rows;
+      cut.n_rows = min(t.s.n_new * P.gs - rt * t.s.tile_rows, t.s.tile_rows);
     }
   }
   if (threadIdx.x == 0) P.cut[c] = cut;
@@ -805,12 +808,13 @@ attention_tree_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
 }
 
 // ================================================================ any head size, CUDA cores
-// 256 threads take 16 R rows of a (sequence, kv head) through pages of 64 keys held in shared memory as float32.  Thread
-// (ty, tx) owns rows R ty .. R ty + R - 1: the scores of keys tx, tx + 16, .., and the output dims 4 (tx + 16 j) .. + 3; the
-// running maximum and sum of a row are kept by its sixteen threads alike.  Everything is float32, exponentials included.
-// R = 4 (a tree of more than 32 rows) reads shared memory three times for every sixteen multiplications that two rows'
-// threads would read it for five times, and shared memory is what bounds this kernel.  float32 pages come by cp.async: the
-// next keys while this page's values are summed, the next values while the next scores are computed.
+// 256 threads take up to 16 R rows of a (sequence, kv head) through pages of 64 keys held in shared memory as float32.  Thread
+// (ty, tx) owns rows ty, ty + 16, .. and of them the scores of keys tx, tx + 16, .. and the output dims 4 (tx + 16 j) .. + 3;
+// the running maximum and sum of a row are kept by its sixteen threads alike.  Everything is float32; the exponentials are
+// the hardware's, off by 2^-22 of themselves.  What bounds it is multiplications: with rows dealt out one by one every warp has
+// the same number of them, and the loops are made for 1 to R rows a thread, so that a tree of 28 rows pays for 32 and not for
+// 64.  float32 pages come by cp.async: the next keys while this page's values are summed, the next values while the next
+// scores are computed.
 #define TG_THREADS 256
 
 __device__ __forceinline__ void cp_async16(void* dst, const void* src) {
@@ -818,6 +822,14 @@ __device__ __forceinline__ void cp_async16(void* dst, const void* src) {
 }
 __device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int N> __device__ __forceinline__ void cp_async_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
+
+// f(rows) with the number as a constant, 1 .. R
+template <int N> struct RowsTag { static constexpr int value = N; };
+template <int R, typename F>
+__device__ __forceinline__ void tg_rows(int used, F f) {
+  if (used >= R) f(RowsTag<R>());
+  else if constexpr (R > 1) tg_rows<R - 1>(used, f);
+}
 
 template <typename T, int NC, int R>
 __global__ void __launch_bounds__(TG_THREADS, NC == 1 ? (R == 2 ? 3 : 2) : NC == 2 ? (R == 2 ? 2 : 1) : 1)
@@ -838,6 +850,7 @@ attention_tree_simple_kernel(const TreeParams P) {
   const int tid = threadIdx.x, ty = tid >> 4, tx = tid & 15;
   const float scale_log2 = P.scale * 1.4426950408889634f;
   const bool direct = sizeof(T) == 4 && hd == hp && (((uintptr_t)P.k_cache | (uintptr_t)P.v_cache) & 15) == 0;
+  const bool q_direct = sizeof(T) == 4 && hd == hp && ((uintptr_t)P.q & 15) == 0 && P.ldq % 4 == 0;
   // a page's keys (or values) into rows of `to` that lie `step` apart; nothing of a page outside the pool
   auto fetch = [&](const void* cache, int pg, int kvh, float* to, int step) {
     if ((unsigned)pg < (unsigned)P.n_pages) {
@@ -859,26 +872,28 @@ attention_tree_simple_kernel(const TreeParams P) {
     if (tid == 0) { cur.next(P, run); edge = 0; }
     __syncthreads();
     if (run.n == 0) break;
-    const int r0 = run.rt * ROWS, n_rows = min(run.s.n_new * P.gs - r0, ROWS);
+    const int r0 = run.rt * run.s.tile_rows, n_rows = min(run.s.n_new * P.gs - r0, run.s.tile_rows);
     const int* bt = P.block_table + (size_t)run.b * P.bt_stride + run.page0;
     int pg = __ldcg(bt);
     fetch(P.k_cache, pg, run.kvh, ks, pitch);
-    fetch(P.v_cache, pg, run.kvh, vs, hp);
-    for (int e = tid; e < ROWS * hp; e += TG_THREADS) {
-      const int r = e / hp, d = e % hp;
-      float x = 0.f;
-      if (r < n_rows && d < hd)
-        x = ld_fresh(reinterpret_cast<const T*>(P.q) + (size_t)(run.s.row0 + (r0 + r) / P.gs) * P.ldq +
-                     (size_t)(run.kvh * P.gs + (r0 + r) % P.gs) * hd + d);
-      qs[r * pitch + d] = x;
+    const int used = (n_rows + 15) >> 4;           // rows of a thread
+    for (int r = ty; r < n_rows; r += 16) {        // (a row behind the last one: whatever lies there, and nobody looks at it)
+      const T* from = reinterpret_cast<const T*>(P.q) + (size_t)(run.s.row0 + (r0 + r) / P.gs) * P.ldq +
+                      (size_t)(run.kvh * P.gs + (r0 + r) % P.gs) * hd;
+      if (q_direct) {
+        for (int d = 4 * tx; d < hp; d += 64) cp_async16(qs + r * pitch + d, from + d);
+      } else {
+        for (int d = tx; d < hp; d += 16) qs[r * pitch + d] = d < hd ? ld_fresh(from + d) : 0.f;
+      }
     }
+    cp_async_commit();
+    fetch(P.v_cache, pg, run.kvh, vs, hp);
     if (tid < ROWS) {
       const int token = tid < n_rows ? run.s.row0 + (r0 + tid) / P.gs : -1;
       const int lo = (P.window > 0 && token >= 0) ? max(__ldcg(P.token_pos + token) - P.window + 1, 0) : 0;
       row_token[tid] = token; row_lo[tid] = lo;
       if (lo > 0) atomicMax(&edge, lo);
     }
-    const bool busy = 2 * R * (tid >> 5) < n_rows;   // (warps without rows load and wait with the others)
     float m[R], l[R];
     float4 acc[R][NC];
 #pragma unroll
@@ -901,32 +916,33 @@ attention_tree_simple_kernel(const TreeParams P) {
       for (int e = 0; e < R; e++)
 #pragma unroll
         for (int j = 0; j < 4; j++) s[e][j] = 0.f;
-      if (page_ok && busy) {
-        const float* q0 = qs + R * ty * pitch;
+      if (page_ok) tg_rows<R>(used, [&](auto rows) {
+        constexpr int RR = decltype(rows)::value;
+        const float* q0 = qs + ty * pitch;
         const float* k0 = ks + tx * pitch;
 #pragma unroll 2
         for (int d = 0; d < hp; d += 4) {
-          float4 a[R];
+          float4 a[RR];
 #pragma unroll
-          for (int e = 0; e < R; e++) a[e] = *reinterpret_cast<const float4*>(q0 + e * pitch + d);
+          for (int e = 0; e < RR; e++) a[e] = *reinterpret_cast<const float4*>(q0 + 16 * e * pitch + d);
 #pragma unroll
           for (int j = 0; j < 4; j++) {
             const float4 x = *reinterpret_cast<const float4*>(k0 + 16 * j * pitch + d);
 #pragma unroll
-            for (int e = 0; e < R; e++) {
+            for (int e = 0; e < RR; e++) {
               s[e][j] = fmaf(a[e].x, x.x, s[e][j]); s[e][j] = fmaf(a[e].y, x.y, s[e][j]);
               s[e][j] = fmaf(a[e].z, x.z, s[e][j]); s[e][j] = fmaf(a[e].w, x.w, s[e][j]);
             }
           }
         }
-      }
+      });
       __syncthreads();                             // the keys are read
       if (i + 1 < run.n) fetch(P.k_cache, pg_next, run.kvh, ks, pitch); else cp_async_commit();
 #pragma unroll
       for (int e = 0; e < R; e++) {
-        if (!busy) continue;
+        if (e >= used) break;
         float mx = -INFINITY;
-        const unsigned long long vis = masked ? row_vis[R * ty + e] >> tx : ~0ull;
+        const unsigned long long vis = masked ? row_vis[ty + 16 * e] >> tx : ~0ull;
 #pragma unroll
         for (int j = 0; j < 4; j++) {
           s[e][j] = (vis >> (16 * j)) & 1 ? s[e][j] * scale_log2 : -INFINITY;
@@ -935,14 +951,14 @@ attention_tree_simple_kernel(const TreeParams P) {
 #pragma unroll
         for (int d = 1; d < 16; d <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, d));
         const float m_new = fmaxf(m[e], mx), m_use = m_new == -INFINITY ? 0.f : m_new;
-        const float corr = exp2f(m[e] - m_use);
+        const float corr = tr_exp2(m[e] - m_use);
         m[e] = m_new;
         float sum = 0.f;
 #pragma unroll
         for (int j = 0; j < 4; j++) {
-          const float p = exp2f(s[e][j] - m_use);
+          const float p = tr_exp2(s[e][j] - m_use);
           sum += p;
-          ps[(R * ty + e) * PK + tx + 16 * j] = p;
+          ps[(ty + 16 * e) * PK + tx + 16 * j] = p;
         }
 #pragma unroll
         for (int d = 1; d < 16; d <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
@@ -958,8 +974,8 @@ attention_tree_simple_kernel(const TreeParams P) {
           for (int e = tid; e < TR_KEYS * hp; e += TG_THREADS) odd = odd || !isfinite(vs[e]);
         odd = __syncthreads_or(odd);
       }
-      const float* p0 = ps + R * ty * PK;          // (a row's probabilities come from its own warp)
-      if (!page_ok || !busy) {
+      const float* p0 = ps + ty * PK;              // (a row's probabilities come from its own warp)
+      if (!page_ok) {
       } else if (odd) {                            // then masked keys are left out, one by one
         for (int k = 0; k < TR_KEYS; k++) {
 #pragma unroll
@@ -969,19 +985,20 @@ attention_tree_simple_kernel(const TreeParams P) {
             const float4 x = *reinterpret_cast<const float4*>(vs + k * hp + d);
 #pragma unroll
             for (int e = 0; e < R; e++) {
-              if (!((row_vis[R * ty + e] >> k) & 1)) continue;
-              const float p = p0[e * PK + k];
+              if (e >= used || !((row_vis[ty + 16 * e] >> k) & 1)) continue;
+              const float p = p0[16 * e * PK + k];
               acc[e][j].x = fmaf(p, x.x, acc[e][j].x); acc[e][j].y = fmaf(p, x.y, acc[e][j].y);
               acc[e][j].z = fmaf(p, x.z, acc[e][j].z); acc[e][j].w = fmaf(p, x.w, acc[e][j].w);
             }
           }
         }
-      } else {
+      } else tg_rows<R>(used, [&](auto rows) {
+        constexpr int RR = decltype(rows)::value;
 #pragma unroll 1
         for (int k = 0; k < TR_KEYS; k += 4) {
-          float4 p[R];
+          float4 p[RR];
 #pragma unroll
-          for (int e = 0; e < R; e++) p[e] = *reinterpret_cast<const float4*>(p0 + e * PK + k);
+          for (int e = 0; e < RR; e++) p[e] = *reinterpret_cast<const float4*>(p0 + 16 * e * PK + k);
 #pragma unroll
           for (int kk = 0; kk < 4; kk++)
 #pragma unroll
@@ -990,14 +1007,14 @@ attention_tree_simple_kernel(const TreeParams P) {
               if (NC * 64 != hp && d >= hp) continue;
               const float4 x = *reinterpret_cast<const float4*>(vs + (k + kk) * hp + d);
 #pragma unroll
-              for (int e = 0; e < R; e++) {
+              for (int e = 0; e < RR; e++) {
                 const float w = kk == 0 ? p[e].x : kk == 1 ? p[e].y : kk == 2 ? p[e].z : p[e].w;
                 acc[e][j].x = fmaf(w, x.x, acc[e][j].x); acc[e][j].y = fmaf(w, x.y, acc[e][j].y);
                 acc[e][j].z = fmaf(w, x.z, acc[e][j].z); acc[e][j].w = fmaf(w, x.w, acc[e][j].w);
               }
             }
         }
-      }
+      });
       __syncthreads();                             // the values are read
       pg = pg_next;
       if (i + 1 < run.n) fetch(P.v_cache, pg, run.kvh, vs, hp); else cp_async_commit();
@@ -1006,8 +1023,8 @@ attention_tree_simple_kernel(const TreeParams P) {
     const int slot = 2 * blockIdx.x + (run.holds_u0 ? 0 : 1);
 #pragma unroll
     for (int e = 0; e < R; e++) {
-      const int r = R * ty + e;
-      if (r >= n_rows) continue;
+      const int r = ty + 16 * e;
+      if (r >= n_rows) break;
       const float inv = 1.0f / l[e];
       T* op = reinterpret_cast<T*>(P.out) + (size_t)row_token[r] * P.ldo + (size_t)(run.kvh * P.gs + (r0 + r) % P.gs) * hd;
       float* po = P.part_o + ((size_t)slot * ROWS + r) * hp;
@@ -1234,6 +1251,7 @@ STRATUM_EXPORT int stratum_attention_tree(const TreeCall* call, cudaStream_t str
   P.q = a.q; P.ldq = ldq; P.k_cache = a.k_cache; P.v_cache = a.v_cache; P.out = a.out; P.ldo = ldo;
   P.part_o = (float*)a.part_o; P.part_ml = (float2*)a.part_ml; P.cut = (TreeCut*)a.cut; P.status = (int*)a.status;
   P.n_tokens = n_tokens; P.n_seqs = n_seqs; P.n_q = n_q; P.n_kv = n_kv; P.gs = gs; P.head_dim = head_dim;
+  P.even_tiles = !tensor;
   P.window = a.window; P.n_pages = (int)n_pages; P.scale = a.scale;
   const int G = stratum_attention_tree_ctas(tensor, many, head_dim);
   int st, slot_half, half_rows;
