@@ -22,7 +22,7 @@
 //   ROWS2 = true: the halves hold 128 rows each and share every page, which then is fetched once for 256 rows.
 // P goes back into tensor memory, over the scores it came from, and is the first operand of P V there: with P in shared
 // memory its writing and its reading by the MMAs took a third of what shared memory moves per tile, and every tile had to
-// wait for the one before to be read (91 us against XX for one sequence of 32,700 tokens and 61 drafted ones).
+// wait for the one before to be read (91 us against 83 for one sequence of 32,700 tokens and 61 drafted ones).
 // One thread of warp 0 feeds rings of K and V pages by TMA, and the queries of the run that comes next.
 //
 // The products with masked keys: P is zero there, but zero times an infinity or a NaN is not, and a page that is masked for
@@ -30,8 +30,16 @@
 // tile is looked through; rows of V that are not finite are zeroed in shared memory, and what they give to the rows that do
 // see them is added by hand.
 //
-// Every mbarrier wait is bounded: on expiry a code goes to the status word; the softmax warps then walk through the rest of
-// their barriers without work, so that all leave together.
+// Every mbarrier wait is bounded: on expiry a code goes to the status word and a flag is set that ends every other wait of
+// the block, so that all leave together.
+//
+// What bounds the tcgen05 kernel.  64 keys of 256 rows take 2,000 to 2,300 cycles, of which the tensor cores are busy for
+// 1,270 (a product of 128 x 64 x 16 takes them 48 cycles with both halves at it, as the rows of Q are read from shared memory
+// each time, one of 128 x 128 x 16 takes 64) and the exponentials' units for 1,024; the rest is one waiting for the other
+// at the ends of tiles.  Measured: one sequence of 32,700 tokens and 61 drafted ones, 8 kv heads of 8 queries: 63 us (128 MB
+// of keys and values, 2.1 TB/s); 64 sequences of 4,000: 275 us, 325 where the card is held back by its power limit.
+// Tried without a gain: every other exponential as a polynomial, a lock that keeps the halves' products apart, halves that
+// start half a tile apart, one thread that issues for both, a guess at the maximum before the scores are there.
 #include <math.h>
 
 #include "tc_common.cuh"
@@ -248,6 +256,23 @@ struct TreeSmem {
 __device__ __forceinline__ float tr_max3(float a, float b, float c) {
   float r;
   asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
+}
+// two floats in a register pair: an instruction does both (what the softmax threads have too many of is instructions)
+__device__ __forceinline__ uint64_t tr_pair(float a, float b) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ void tr_split(uint64_t v, float& a, float& b) { asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(v)); }
+__device__ __forceinline__ uint64_t tr_fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+__device__ __forceinline__ uint64_t tr_add2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
   return r;
 }
 __device__ __forceinline__ float tr_exp2(float x) {
@@ -633,18 +658,20 @@ attention_tree_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
           if (grow) m_ref = tile_max;
           const float m_use = (m_ref == -INFINITY) ? 0.f : m_ref;
           uint32_t packed[TR_KEYS / 2];
-          float sum[4] = {0.f, 0.f, 0.f, 0.f};
+          const uint64_t mul2 = tr_pair(to_log2, to_log2), neg2 = tr_pair(-m_use, -m_use);
+          uint64_t sum2[2] = {0, 0};
 #pragma unroll
           for (int e = 0; e < TR_KEYS; e += 2) {
-            const float p0 = tr_exp2(fmaf(sc[e], to_log2, -m_use));
-            const float p1 = tr_exp2(fmaf(sc[e + 1], to_log2, -m_use));
-            // to bfloat16 by dropping the low mantissa bits; the sums run over the same shortened values, so the common
-            // part of the shortening divides out and what stays is as wide as round-to-nearest's error
-            const uint32_t u = __byte_perm(__float_as_uint(p0), __float_as_uint(p1), 0x7632);
-            sum[e & 2] += __uint_as_float(u << 16);
-            sum[(e & 2) + 1] += __uint_as_float(u & 0xffff0000u);
+            float x0, x1;
+            tr_split(tr_fma2(tr_pair(sc[e], sc[e + 1]), mul2, neg2), x0, x1);
+            const float p0 = tr_exp2(x0), p1 = tr_exp2(x1);
+            uint32_t u;                                  // P V takes them as bfloat16, off by at most 2^-9; the sum as they are
+            asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(u) : "f"(p1), "f"(p0));
+            sum2[(e >> 1) & 1] = tr_add2(sum2[(e >> 1) & 1], tr_pair(p0, p1));
             packed[e >> 1] = u;
           }
+          float sum[4];
+          tr_split(sum2[0], sum[0], sum[1]); tr_split(sum2[1], sum[2], sum[3]);
           const bool move = __any_sync(0xffffffffu, grow);
           if (!first && (move || bad)) {                 // P V of this half's tile before is in O
             const uint32_t before = it - STEP;
