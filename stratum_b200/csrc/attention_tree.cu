@@ -381,7 +381,10 @@ attention_tree_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
   Smem& S = *reinterpret_cast<Smem*>(smem_raw);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   if (smem_u32(smem_raw) & 1023) {                      // (the swizzled tiles need it)
-    if (threadIdx.x == 0) atomicCAS(P.status, 0, 510);
+    if (threadIdx.x == 0) {
+      atomicCAS(P.status, 0, 510);
+      P.cut[blockIdx.x] = TreeCut{};                   // (nothing to add up)
+    }
     return;
   }
   volatile int* abort_flag = &S.abort_flag;
