@@ -1690,6 +1690,15 @@ def _shaped(t: torch.Tensor, name: str, dtype, shape=None) -> None:
         raise KernelError(f"{name} must have the shape {shape}, has {tuple(t.shape)}")
 
 
+def _meet(a: int, step_a: int, width_a: int, b: int, step_b: int, width_b: int, rows: int) -> bool:
+    """Whether two matrices of `rows` rows have memory in common (addresses, distances of rows and widths in bytes); columns of
+    one wider matrix have none."""
+    if a >= b + (rows - 1) * step_b + width_b or b >= a + (rows - 1) * step_a + width_a:
+        return False
+    apart = (b - a) % step_a if step_a > 0 else 0
+    return step_a != step_b or apart < width_a or step_a - apart < width_b
+
+
 # Mirrors of struct TreeCall in csrc/attention_tree.cu, VerifyParams in csrc/draft_verify.cu and KeepRows in csrc/cache_move.cu.
 # (One packed argument: converting thirty of them one by one took a fifth of a short call.)
 _TREE_CALL, _VERIFY_CALL, _KEEP_CALL = struct.Struct("<14q15if"), struct.Struct("<11q4i"), struct.Struct("<8q10i")
@@ -1709,7 +1718,8 @@ def attention_tree(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor
     its sequence (itself among them, if it is to).  In front of the drafted rows a token sees every cached key or, with a
     window, those at positions above token_pos - window; token_pos is not below the position of the sequence's first
     drafted row, and the window does not touch what the mask says.  A token that sees nothing gets zeros; rows behind the
-    last sequence are left as they were; a page number outside the pool holds keys that nobody sees.
+    last sequence are left as they were; a page number outside the pool holds keys that nobody sees.  q and out may be columns
+    of one matrix, but have no element in common.
     max_new: drafted tokens of the sequence that has most (how the work is cut, not what comes out).
 
     bfloat16 heads of 64 or 128 on tcgen05, with probabilities rounded to bfloat16 as the value product's operand has to
@@ -1738,8 +1748,11 @@ def attention_tree(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor
     if T == 0 or B == 0:
         return
     group = n_q // n_kv
-    at_q, at_k, at_v, at_out, ldq, ldo = (q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), out.data_ptr(), q.stride()[0],
-                                          out.stride()[0])
+    at_q, at_k, at_v, at_out = q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), out.data_ptr()
+    ldq, ldo = (q.stride()[0], out.stride()[0]) if T > 1 else (width, width)          # (of a single row it means nothing)
+    size = q.element_size()
+    if _meet(at_q, ldq * size, width * size, at_out, ldo * size, width * size, T):
+        raise KernelError("attention_tree: out is memory of its own, not q's")
     tensor = (code == DT_BF16 and head_dim in (64, 128) and group <= 128 and scale > 0 and ldq % 8 == 0 and ldo % 8 == 0
               and not (at_q | at_k | at_v | at_out) & 15)
     # more rows than a half of a CTA holds: both halves share every page (else they take pages in turn); on the CUDA cores:
@@ -1789,8 +1802,7 @@ def token_probs(logits: torch.Tensor, temperature: torch.Tensor, out: torch.Tens
         return
     same = out.data_ptr() == logits.data_ptr() and (R == 1 or out.stride(0) == logits.stride(0))
     if not same:
-        a, b = logits.data_ptr(), out.data_ptr()
-        if a < b + 4 * ((R - 1) * out.stride(0) + V) and b < a + 4 * ((R - 1) * logits.stride(0) + V):
+        if _meet(logits.data_ptr(), 4 * (logits.stride(0) if R > 1 else V), 4 * V, out.data_ptr(), 4 * (out.stride(0) if R > 1 else V), 4 * V, R):
             raise KernelError("token_probs: out is logits itself or memory of its own")
     f = _fn("draft_verify", "stratum_token_probs",
             [c_void_p, ctypes.c_longlong, c_void_p, c_void_p, ctypes.c_longlong, c_int, c_int, c_void_p])
@@ -1852,6 +1864,13 @@ def _storage(k: torch.Tensor, v: Optional[torch.Tensor], what: str) -> None:
             raise KernelError(f"{what}: {name} must be contiguous [layers, pages, heads, page_tokens, size]")
     if v is not None and (v.shape[:2] != k.shape[:2] or v.shape[3] != k.shape[3]):
         raise KernelError(f"{what}: k and v have layers, pages and page_tokens in common")
+    _apart(what, k, v)
+
+
+def _apart(what: str, k: torch.Tensor, v: Optional[torch.Tensor]) -> None:
+    """Two contiguous tensors without a byte in common."""
+    if v is not None and k.data_ptr() < v.data_ptr() + v.nbytes and v.data_ptr() < k.data_ptr() + k.nbytes:
+        raise KernelError(f"{what}: k and v are memory of their own each")
 
 
 def keep_rows(k: torch.Tensor, v: Optional[torch.Tensor], block_table: torch.Tensor, seq_start: torch.Tensor,
@@ -1893,6 +1912,7 @@ def copy_pages(k: torch.Tensor, v: Optional[torch.Tensor], src, dst) -> None:
             raise KernelError(f"copy_pages: {name} must be contiguous [layers, pages, ...]")
     if v is not None and v.shape[:2] != k.shape[:2]:
         raise KernelError("copy_pages: k and v have layers and pages in common")
+    _apart("copy_pages", k, v)
     L, pages = k.shape[:2]
     if len(src) != len(dst):
         raise KernelError("copy_pages: one destination for every source")

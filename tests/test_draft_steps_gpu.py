@@ -8,7 +8,7 @@ import pytest
 import torch
 
 from draft_helpers import random_tree
-from helpers import TINY, assert_close, load_plain, make_model_dir, plain_logits, rand_tokens
+from helpers import TINY, TOL, assert_close, load_plain, make_model_dir, plain_logits, rand_tokens
 from plain import llama_plain as P
 
 pytestmark = pytest.mark.gpu
@@ -259,3 +259,48 @@ def test_forks_of_models_with_states(tmp_path, family):
     for slot in (s, f, g):
         llm.release(slot)
     llm.engine.cache.check()
+
+
+def test_drafts_between_ordinary_steps(setup):
+    """Ordinary steps (captured ones), steps of drafted tokens, forks and steps of several tokens in turn: a sequence goes on as if it
+    had been decoded one token at a time, whoever joined or left meanwhile."""
+    from stratum_b200 import DraftEntry, StepEntry
+    name, dtype, cfg, w, llm = setup
+    rng = np.random.default_rng(21)
+    V = cfg["vocab_size"]
+    prompts = [rand_tokens(rng, n, V) for n in (61, 5, 90)]
+    want = [r.tokens for r in llm.generate(prompts, max_new_tokens=30, stop_ids=())]
+    slots = [llm.acquire() for _ in prompts]
+    have = [[t] for t in llm.step([StepEntry(s, p, [len(p) - 1]) for s, p in zip(slots, prompts)]).argmax(1).tolist()]
+    drafted = 0
+    for turn in range(30):
+        live = [i for i in range(3) if len(have[i]) < 26]
+        if not live:
+            break
+        if turn % 3 == 1:                                 # drafts: some right, some wrong
+            entries = []
+            for i in live:
+                n = len(have[i])
+                good = want[i][n:n + 2] if have[i] == want[i][:n] else [1, 2]
+                entries.append(DraftEntry(slots[i], [have[i][-1], good[0], (good[-1] + 1) % V, good[-1]], [-1, 0, 1, 1]))
+            for i, t in zip(live, llm.draft_step(entries)):
+                have[i] += t
+                drafted += len(t) - 1
+        elif turn % 3 == 2:                               # another sequence comes and goes
+            f = llm.fork(slots[live[0]])
+            llm.draft_step([DraftEntry(f[0], rand_tokens(rng, 9, V))])
+            llm.decode_step(f, [1])
+            llm.release(f[0])
+        else:
+            for i, t in zip(live, llm.decode_step([slots[i] for i in live], [have[i][-1] for i in live])[0]):
+                have[i].append(t)
+    llm.engine.cache.check()
+    for i, s in enumerate(slots):
+        assert llm.engine.length(s) == len(prompts[i]) + len(have[i]) - 1
+        # every token is the model's own pick behind the ones in front of it, as far as near-equal logits allow
+        ref = plain_logits(cfg, w, prompts[i] + have[i][:-1])[len(prompts[i]) - 1:]
+        span = np.abs(ref).max()
+        for r, t in zip(ref, have[i]):
+            assert r.max() - r[t] <= 2 * TOL[dtype] * span    # (the errors of two logits)
+        llm.release(s)
+    assert drafted > 0 and llm.engine.cache.tokens_held() == 0
