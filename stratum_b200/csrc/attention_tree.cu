@@ -58,21 +58,25 @@ struct TreeParams {
   const void* q; int ldq;
   const void* k_cache; const void* v_cache;
   void* out; int ldo;
-  float* part_o;                           // [G][2][rows per tile][head_dim]: pieces, unnormalised
+  float4* part_o;                          // [G][2][head_dim / 4][rows of a slot]: pieces, unnormalised (a warp has rows)
   float2* part_ml;                         // [G][2][rows per tile]: their (maximum, sum)
   struct TreeCut* cut;                     // [G]: what each CTA's stretch begins in
   int* status;
   int n_tokens, n_seqs, n_q, n_kv, gs, head_dim, window, n_pages, rows_per_tile, even_tiles;
+  int item_units;                          // (see the list of units)
+  int out_by_16;                           // a head's row of the output begins on 16 bytes and is a multiple of them
   float scale;
 };
 
-// What CTA c's stretch begins in, for the merge.
+// The cut in front of CTA c's stretch, for the merge.
 struct alignas(16) TreeCut {
-  long long u0, item_begin, total;         // the stretch's first unit, the first unit of the item that holds it, units in all
-  int n_pages, kvh;                        // pages of the item (0: the stretch begins in none of its pages); its kv head,
+  int first, cuts;                         // the CTA that has the item's first page, how many cuts go through the item (0: this one
+                                           // goes through none)
+  int late, kvh;                           // whether that CTA's stretch begins in front of the item; the item's kv head,
   int flat0, n_rows;                       // its first row (token of the batch * gs + head), its rows
   int pad[2];
 };
+static_assert(sizeof(TreeCut) == 32, "as the launcher lays them out");
 
 struct TreeSeq {                           // a sequence's share of the list
   int row0, n_new, base, len, first, n_pages, n_tiles, tile_rows;
@@ -93,11 +97,12 @@ __device__ __forceinline__ TreeSeq tree_seq(const TreeParams& P, int b) {
   s.tile_rows = P.even_tiles && s.n_tiles > 1 ? ((rows + s.n_tiles - 1) / s.n_tiles + 7) & ~7 : P.rows_per_tile;
   return s;
 }
-// The list of units: every item (sequence, kv head, tile of rows) has one for each of its pages and TREE_ITEM_UNITS more
-// behind them, for what an item costs besides its pages.  (Without them a CTA whose stretch was made of short sequences took
-// 80 us where the others took 46.)  A short list is cut among fewer CTAs, TREE_LEAST_UNITS to each: what a piece of one page
-// saves in its own time, adding up its pieces costs again.
-#define TREE_ITEM_UNITS 3
+// The list of units: every item (sequence, kv head, tile of rows) has one for each of its pages and a few more behind them, for
+// what an item costs besides its pages (on the tensor cores: its masked pages, which take twice as long, its outputs, and the
+// next item's first scores).  Without them a CTA whose stretch was made of short sequences took 80 us where the others took
+// 46; with 3 instead of 7 on the tensor cores 24 sequences took 58 us instead of 53, with 7 instead of 3 on the CUDA cores five
+// took 76 instead of 66.  A short list is cut among fewer CTAs, TREE_LEAST_UNITS to each: what a piece of one page saves in its
+// own time, adding up its pieces costs again.
 #define TREE_LEAST_UNITS 4
 __device__ __forceinline__ int tree_ctas(long long T, int G) {
   const long long n = (T + TREE_LEAST_UNITS - 1) / TREE_LEAST_UNITS;
@@ -121,14 +126,14 @@ struct TreeCursor {
   __device__ __forceinline__ void step(const TreeParams& P, int n) {
     moved = true;
     off += n; left -= n;
-    if (off < s.n_pages + TREE_ITEM_UNITS) return;
+    if (off < s.n_pages + P.item_units) return;
     off = 0;
     if (++item < s.n_tiles * P.n_kv) return;
     item = 0;
     do { b++; if (b < P.n_seqs) s = tree_seq(P, b); } while (b < P.n_seqs && s.n_tiles == 0);
   }
   __device__ __forceinline__ void next(const TreeParams& P, TreeRun& r) {
-    if (left > 0 && off >= s.n_pages) step(P, min(s.n_pages + TREE_ITEM_UNITS - off, left));
+    if (left > 0 && off >= s.n_pages) step(P, min(s.n_pages + P.item_units - off, left));
     if (left <= 0) { r.n = 0; return; }
     const int n = min(s.n_pages - off, left);
     r.s = s; r.b = b;
@@ -144,11 +149,11 @@ struct TreeCursor {
 };
 
 // Where CTA c begins; every thread of the block calls it.  `sums` holds a running sum per sequence for the while.
-__device__ __forceinline__ TreeCursor tree_start(const TreeParams& P, long long* sums) {
+__device__ __forceinline__ TreeCursor tree_start(const TreeParams& P, long long* sums, long long& u0_, long long& total_) {
   const int n_threads = blockDim.x, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   for (int b = threadIdx.x; b < P.n_seqs; b += n_threads) {
     const TreeSeq s = tree_seq(P, b);
-    sums[b + 1] = (long long)(s.n_pages + TREE_ITEM_UNITS) * s.n_tiles * P.n_kv;
+    sums[b + 1] = (long long)(s.n_pages + P.item_units) * s.n_tiles * P.n_kv;
   }
   if (threadIdx.x == 0) sums[0] = 0;
   __syncthreads();
@@ -174,8 +179,7 @@ __device__ __forceinline__ TreeCursor tree_start(const TreeParams& P, long long*
   t.left = (int)(tree_begin(c + 1, ctas, T) - u0);
   t.b = t.item = t.off = 0;
   t.moved = false;
-  TreeCut cut;
-  cut.u0 = u0; cut.item_begin = 0; cut.total = T; cut.n_pages = cut.kvh = cut.flat0 = cut.n_rows = 0;
+  u0_ = u0; total_ = T;
   if (t.left > 0) {
     int lo = 0, hi = P.n_seqs - 1;                // the last sequence that begins at or before u0 and is not empty
     while (lo < hi) {
@@ -184,18 +188,32 @@ __device__ __forceinline__ TreeCursor tree_start(const TreeParams& P, long long*
     }
     t.s = tree_seq(P, lo);
     const long long r = u0 - sums[lo];
-    const int per = t.s.n_pages + TREE_ITEM_UNITS;
+    const int per = t.s.n_pages + P.item_units;
     t.b = lo; t.item = (int)(r / per); t.off = (int)(r % per);
-    if (t.off < t.s.n_pages) {
-      const int rt = t.item % t.s.n_tiles;
-      cut.item_begin = u0 - t.off;
-      cut.n_pages = t.s.n_pages; cut.kvh = t.item / t.s.n_tiles;
-      cut.flat0 = t.s.row0 * P.gs + rt * t.s.tile_rows;
-      cut.n_rows = min(t.s.n_new * P.gs - rt * t.s.tile_rows, t.s.tile_rows);
-    }
   }
-  if (threadIdx.x == 0) P.cut[c] = cut;
   return t;
+}
+// The last CTA whose stretch begins at or before unit u (0 <= u < T).
+__device__ __forceinline__ int tree_cta_of(long long u, int ctas, long long T) {
+  int c = min((int)(u * ctas / T), ctas - 1);      // floor(c T / ctas) <= u, and at most one short
+  while (c + 1 < ctas && tree_begin(c + 1, ctas, T) <= u) c++;
+  return c;
+}
+// One thread, with the cursor as tree_start left it: what the merge is to know about the cut in front of this stretch.
+__device__ __forceinline__ void tree_cut(const TreeParams& P, const TreeCursor& t, long long u0, long long T) {
+  TreeCut cut;
+  cut.first = cut.cuts = cut.late = cut.kvh = cut.flat0 = cut.n_rows = 0;
+  if (t.left > 0 && t.off > 0 && t.off < t.s.n_pages) {
+    const long long begin = u0 - t.off;
+    const int ctas = tree_ctas(T, gridDim.x), rt = t.item % t.s.n_tiles;
+    cut.first = tree_cta_of(begin, ctas, T);
+    cut.cuts = tree_cta_of(begin + t.s.n_pages - 1, ctas, T) - cut.first;
+    cut.late = tree_begin(cut.first, ctas, T) != begin;
+    cut.kvh = t.item / t.s.n_tiles;
+    cut.flat0 = t.s.row0 * P.gs + rt * t.s.tile_rows;
+    cut.n_rows = min(t.s.n_new * P.gs - rt * t.s.tile_rows, t.s.tile_rows);
+  }
+  P.cut[blockIdx.x] = cut;
 }
 
 // Which of the 64 keys from position `key0` on a drafted token sees; word0: the first word of its mask.
@@ -383,7 +401,7 @@ attention_tree_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
   if (smem_u32(smem_raw) & 1023) {                      // (the swizzled tiles need it)
     if (threadIdx.x == 0) {
       atomicCAS(P.status, 0, 510);
-      P.cut[blockIdx.x] = TreeCut{};                   // (nothing to add up)
+      P.cut[blockIdx.x] = TreeCut{};
     }
     return;
   }
@@ -409,7 +427,8 @@ attention_tree_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
     tmem_relinquish();
   }
   pdl_wait();                                           // everything below may read what the kernel before this one wrote
-  TreeCursor cur = tree_start(P, reinterpret_cast<long long*>(S.k));
+  long long u0, total;
+  TreeCursor cur = tree_start(P, reinterpret_cast<long long*>(S.k), u0, total);
   fence_async_shared();                                 // the sums lie where TMA will write
   tc_fence_before();
   __syncthreads();
@@ -723,7 +742,7 @@ attention_tree_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
       if (ROWS2) {
         if (warp_active) {
           const float inv = 1.0f / l;
-          float* po = P.part_o + ((size_t)slot * 256 + h * 128 + row) * HD;
+          float4* po = P.part_o + (size_t)slot * (HD / 4) * 256 + h * 128 + row;
 #pragma unroll 1
           for (int c = 0; c < HD; c += 32) {
             float o[32];
@@ -741,7 +760,7 @@ attention_tree_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
             } else if (valid) {
 #pragma unroll
               for (int e = 0; e < 32; e += 4)
-                *reinterpret_cast<float4*>(po + c + e) = make_float4(o[e], o[e + 1], o[e + 2], o[e + 3]);
+                po[((c + e) >> 2) * 256] = make_float4(o[e], o[e + 1], o[e + 2], o[e + 3]);
             }
           }
           if (valid && !whole) P.part_ml[(size_t)slot * 256 + h * 128 + row] = make_float2(m_ref, l);
@@ -761,7 +780,7 @@ attention_tree_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
           // a half that had no page in this run left its accumulator alone; one that saw no key of the row has nothing to
           // give, whatever lies in it
           const bool has0 = run.n > 1 || (it_first & 1) == 0, has1 = run.n > 1 || (it_first & 1) == 1;
-          float* po = P.part_o + ((size_t)slot * 128 + row) * HD;
+          float4* po = P.part_o + (size_t)slot * (HD / 4) * 128 + row;
 #pragma unroll 1
           for (int c = h * (HD / 2); c < (h + 1) * (HD / 2); c += 32) {
             float o[32];
@@ -796,7 +815,7 @@ attention_tree_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
             } else if (valid) {
 #pragma unroll
               for (int e = 0; e < 32; e += 4)
-                *reinterpret_cast<float4*>(po + c + e) = make_float4(o[e], o[e + 1], o[e + 2], o[e + 3]);
+                po[((c + e) >> 2) * 128] = make_float4(o[e], o[e + 1], o[e + 2], o[e + 3]);
             }
           }
           if (valid && !whole && h == 0) P.part_ml[(size_t)slot * 128 + row] = make_float2(M, L);
@@ -811,6 +830,7 @@ attention_tree_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
     // ---------------------------------------------------------------- the walk over the list
     // A run is described here while the ones before it are worked on: what it takes from memory would otherwise stand
     // between two runs of every other warp.
+    const TreeCursor begin = cur;
     for (int r = 0;; r++) {
       TreeRun& run = S.runs[r % TR_RUNS];
       if (r >= TR_RUNS && !__all_sync(0xffffffffu, mbar_wait(&S.run_empty[r % TR_RUNS], ((r / TR_RUNS) - 1) & 1, abort_flag))) { if (lane == 0) TR_FAIL(512); break; }
@@ -828,6 +848,7 @@ attention_tree_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
       if (lane == 0) mbar_arrive(&S.run_full[r % TR_RUNS]);
       if (n == 0) break;
     }
+    if (lane == 0) tree_cut(P, begin, u0, total);
   }
   tc_fence_before();
   __syncthreads();
@@ -876,7 +897,9 @@ attention_tree_simple_kernel(const TreeParams P) {
   float* vs = ks + TR_KEYS * pitch;                // [64][hp]
   float* ps = vs + TR_KEYS * hp;                   // [ROWS][PK]
   pdl_wait();
-  TreeCursor cur = tree_start(P, reinterpret_cast<long long*>(tg_smem));
+  long long u0, total;
+  TreeCursor cur = tree_start(P, reinterpret_cast<long long*>(tg_smem), u0, total);
+  if (threadIdx.x == TG_THREADS - 1) tree_cut(P, cur, u0, total);
   const int tid = threadIdx.x, ty = tid >> 4, tx = tid & 15;
   const float scale_log2 = P.scale * 1.4426950408889634f;
   const bool direct = sizeof(T) == 4 && hd == hp && (((uintptr_t)P.k_cache | (uintptr_t)P.v_cache) & 15) == 0;
@@ -1057,7 +1080,6 @@ attention_tree_simple_kernel(const TreeParams P) {
       if (r >= n_rows) break;
       const float inv = 1.0f / l[e];
       T* op = reinterpret_cast<T*>(P.out) + (size_t)row_token[r] * P.ldo + (size_t)(run.kvh * P.gs + (r0 + r) % P.gs) * hd;
-      float* po = P.part_o + ((size_t)slot * ROWS + r) * hp;
 #pragma unroll
       for (int j = 0; j < NC; j++) {
         const int d = 4 * (tx + 16 * j);
@@ -1067,113 +1089,109 @@ attention_tree_simple_kernel(const TreeParams P) {
           for (int x = 0; x < 4; x++)
             if (d + x < hd) op[d + x] = from_float<T>(l[e] == 0.f ? 0.f : y[x] * inv);
         } else if (d < hp) {
-          *reinterpret_cast<float4*>(po + d) = acc[e][j];
+          *reinterpret_cast<float4*>(ks + r * pitch + d) = acc[e][j];              // (the keys are read, and no more asked for)
         }
       }
       if (!whole && tx == 0) P.part_ml[(size_t)slot * ROWS + r] = make_float2(m[e], l[e]);
+    }
+    if (!whole) {                                  // a piece, turned in shared memory: a warp writes rows side by side
+      __syncthreads();
+      float4* po = P.part_o + (size_t)slot * (hp >> 2) * ROWS;
+      for (int x = tid; x < (hp >> 2) * ROWS; x += TG_THREADS) {
+        const int r = x % ROWS, chunk = x / ROWS;
+        if (r < n_rows) po[x] = *reinterpret_cast<const float4*>(ks + r * pitch + 4 * chunk);
+      }
     }
   }
   cp_async_wait<0>();
 }
 
 // ================================================================ the pieces of what several CTAs saw
-// Block (c, y): rows 32 y .. 32 y + 31 of the item that the cut between CTAs c and c + 1 goes through, where it is the first
-// one to do so; a warp takes four rows at a time, so that the pieces of all four are on their way together.  The lanes look
-// up where the stretches begin and fetch the pieces' maxima and sums.
-#define TM_ROWS 4
-template <typename T, int NJ>
-__global__ void __launch_bounds__(256, 2)
-attention_tree_merge_kernel(const TreeParams P, int G, int slot_half, int half_rows) {
+// Blocks (c, y) look at the cut between the stretches of CTAs c and c + 1.  The cuts that go through one item share out its
+// rows and dims; a lane has a row, so that what a warp reads of a piece lies in one stretch, as the softmax threads, a row each,
+// have written it.  A thread has PIECES pieces of 4 CHUNKS dims on their way together, with their maxima and sums: sixteen loads
+// whether an item lies in two CTAs or in twenty.
+#define TM_WARPS 4
+template <typename T, int CHUNKS, int PIECES>
+__device__ __forceinline__ void tree_add_up(const TreeParams& P, const TreeCut& cut, int slot_half, int half_rows) {
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  pdl_wait();
-  const int c = blockIdx.x + 1;
-  TreeCut cut;                                     // (written by the kernel before, and read past L1)
+  const int hd = P.head_dim, chunks = (hd + 3) >> 2;               // of four dims
+  const int slot_rows = (P.rows_per_tile / half_rows) * slot_half;
+  const int wide = (chunks + CHUNKS * TM_WARPS - 1) / (CHUNKS * TM_WARPS), shares = ((cut.n_rows + 31) >> 5) * wide;
+  for (int at = blockIdx.y * cut.cuts + (int)blockIdx.x - cut.first; at < shares; at += gridDim.y * cut.cuts) {
+    const int r = (at / wide) * 32 + lane, k0 = ((at % wide) * TM_WARPS + warp) * CHUNKS;
+    if (r >= cut.n_rows || k0 >= chunks) continue;
+    const int srow = (r / half_rows) * slot_half + r % half_rows;
+    float M = -INFINITY, L = 0.f;
+    float4 acc[CHUNKS];
 #pragma unroll
-  for (int x = 0; x < 3; x++) reinterpret_cast<int4*>(&cut)[x] = __ldcg(reinterpret_cast<const int4*>(P.cut + c) + x);
-  const long long T_ = cut.total, ib = cut.item_begin, ie = ib + cut.n_pages;
-  const int ctas = tree_ctas(T_, G), first = c - 1;
-  const long long ub = tree_begin(first, ctas, T_);
-  if (cut.n_pages == 0 || cut.u0 == ib || ub > ib) return;         // no cut, or not the item's first
-  const int r0 = (blockIdx.y * 8 + warp) * TM_ROWS;
-  if (r0 >= cut.n_rows) return;
-  const int hd = P.head_dim, hp = (hd + 3) & ~3;
-  const int slot_rows = (P.rows_per_tile / half_rows) * slot_half, n = min(TM_ROWS, cut.n_rows - r0);
-  int srow[TM_ROWS];
+    for (int j = 0; j < CHUNKS; j++) acc[j] = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 1
+    for (int i0 = 0; i0 <= cut.cuts; i0 += PIECES) {
+      float2 ml[PIECES];
+      float4 v[PIECES][CHUNKS];
 #pragma unroll
-  for (int x = 0; x < TM_ROWS; x++) {
-    const int r = min(r0 + x, cut.n_rows - 1);
-    srow[x] = (r / half_rows) * slot_half + r % half_rows;
-  }
-  float M[TM_ROWS], L[TM_ROWS];
-  float4 acc[TM_ROWS][NJ];
+      for (int y = 0; y < PIECES; y++) {
+        const bool have = i0 + y <= cut.cuts;
+        const size_t slot = 2 * (cut.first + i0 + y) + (i0 + y == 0 ? cut.late : 0);
+        ml[y] = have ? __ldcg(P.part_ml + slot * slot_rows + srow) : make_float2(-INFINITY, 0.f);
 #pragma unroll
-  for (int x = 0; x < TM_ROWS; x++) {
-    M[x] = -INFINITY; L[x] = 0.f;
+        for (int j = 0; j < CHUNKS; j++)
+          v[y][j] = have && k0 + j < chunks ? __ldcg(P.part_o + (slot * chunks + k0 + j) * slot_rows + srow) : make_float4(0.f, 0.f, 0.f, 0.f);
+      }
+      float m = M;
 #pragma unroll
-    for (int j = 0; j < NJ; j++) acc[x][j] = make_float4(0.f, 0.f, 0.f, 0.f);
-  }
-  // 32 pieces at a time, the stretches from `first` on that begin in front of the item's end
-  for (int i0 = first; ; i0 += 32) {
-    const int i = i0 + lane;
-    const bool any = i == first || (i < ctas && tree_begin(i, ctas, T_) < ie);
-    const unsigned have = __ballot_sync(0xffffffffu, any);
-    const int count = __popc(have);
-    auto piece = [&](int at) { return (size_t)(2 * at + ((at == first && ub != ib) ? 1 : 0)) * slot_rows; };
-    float w[TM_ROWS];
+      for (int y = 0; y < PIECES; y++) m = fmaxf(m, ml[y].x);
+      const float mu = m == -INFINITY ? 0.f : m, corr = exp2f(M - mu);
+      M = m;
+      L *= corr;
 #pragma unroll
-    for (int x = 0; x < TM_ROWS; x++) {
-      const float2 ml = any ? __ldcg(&P.part_ml[piece(i) + srow[x]]) : make_float2(-INFINITY, 0.f);
-      const float m = fmaxf(M[x], warp_max(ml.x)), mu = m == -INFINITY ? 0.f : m;
-      const float corr = exp2f(M[x] - mu);
-      w[x] = exp2f(ml.x - mu);
-      L[x] = fmaf(L[x], corr, warp_sum(w[x] * ml.y));
-      M[x] = m;
+      for (int j = 0; j < CHUNKS; j++) { acc[j].x *= corr; acc[j].y *= corr; acc[j].z *= corr; acc[j].w *= corr; }
 #pragma unroll
-      for (int j = 0; j < NJ; j++) { acc[x][j].x *= corr; acc[x][j].y *= corr; acc[x][j].z *= corr; acc[x][j].w *= corr; }
-    }
-    constexpr int PB = 4;                          // pieces whose values are on their way together
-    for (int l0 = 0; l0 < count; l0 += PB) {
+      for (int y = 0; y < PIECES; y++) {
+        const float w = exp2f(ml[y].x - mu);
+        L = fmaf(w, ml[y].y, L);
+        if (w != 0.f) {                            // (no key seen: the piece may hold anything)
 #pragma unroll
-      for (int j = 0; j < NJ; j++) {
-        const int d = 4 * (lane + 32 * j);
-        float4 v[PB][TM_ROWS];
-#pragma unroll
-        for (int y = 0; y < PB; y++)
-#pragma unroll
-          for (int x = 0; x < TM_ROWS; x++) {
-            v[y][x] = make_float4(0.f, 0.f, 0.f, 0.f);
-            if (l0 + y < count && d < hp)
-              v[y][x] = __ldcg(reinterpret_cast<const float4*>(P.part_o + (piece(i0 + l0 + y) + srow[x]) * hp + d));
+          for (int j = 0; j < CHUNKS; j++) {
+            acc[j].x = fmaf(w, v[y][j].x, acc[j].x); acc[j].y = fmaf(w, v[y][j].y, acc[j].y);
+            acc[j].z = fmaf(w, v[y][j].z, acc[j].z); acc[j].w = fmaf(w, v[y][j].w, acc[j].w);
           }
-#pragma unroll
-        for (int y = 0; y < PB; y++)
-#pragma unroll
-          for (int x = 0; x < TM_ROWS; x++) {
-            const float wk = __shfl_sync(0xffffffffu, w[x], (l0 + y) & 31);
-            if (l0 + y < count && wk != 0.f) {     // (no key seen: the piece may hold anything)
-              acc[x][j].x = fmaf(wk, v[y][x].x, acc[x][j].x); acc[x][j].y = fmaf(wk, v[y][x].y, acc[x][j].y);
-              acc[x][j].z = fmaf(wk, v[y][x].z, acc[x][j].z); acc[x][j].w = fmaf(wk, v[y][x].w, acc[x][j].w);
-            }
-          }
+        }
       }
     }
-    if (count < 32) break;
-  }
+    const int flat = cut.flat0 + r;
+    const float inv = 1.0f / L;
+    T* op = reinterpret_cast<T*>(P.out) + (size_t)(flat / P.gs) * P.ldo + (size_t)(cut.kvh * P.gs + flat % P.gs) * hd + 4 * k0;
+    if (sizeof(T) == 2 && P.out_by_16 && CHUNKS % 2 == 0) {
 #pragma unroll
-  for (int x = 0; x < TM_ROWS; x++) {
-    if (x >= n) break;
-    const int flat = cut.flat0 + r0 + x;
-    const float inv = 1.0f / L[x];
-    T* op = reinterpret_cast<T*>(P.out) + (size_t)(flat / P.gs) * P.ldo + (size_t)(cut.kvh * P.gs + flat % P.gs) * hd;
+      for (int j = 0; j + 1 < CHUNKS; j += 2)
+        if (k0 + j < chunks)
+          *reinterpret_cast<uint4*>(op + 4 * j) = make_uint4(tr_pack(L, acc[j].x * inv, acc[j].y * inv), tr_pack(L, acc[j].z * inv, acc[j].w * inv),
+                                                             tr_pack(L, acc[j + 1].x * inv, acc[j + 1].y * inv), tr_pack(L, acc[j + 1].z * inv, acc[j + 1].w * inv));
+    } else {
 #pragma unroll
-    for (int j = 0; j < NJ; j++) {
-      const int d = 4 * (lane + 32 * j);
-      const float y[4] = {acc[x][j].x, acc[x][j].y, acc[x][j].z, acc[x][j].w};
+      for (int j = 0; j < CHUNKS; j++) {
+        const float y[4] = {acc[j].x, acc[j].y, acc[j].z, acc[j].w};
 #pragma unroll
-      for (int e = 0; e < 4; e++)
-        if (d + e < hd) op[d + e] = from_float<T>(L[x] == 0.f ? 0.f : y[e] * inv);
+        for (int d = 0; d < 4; d++)
+          if (4 * (k0 + j) + d < hd) op[4 * j + d] = from_float<T>(L == 0.f ? 0.f : y[d] * inv);
+      }
     }
   }
+}
+
+template <typename T>
+__global__ void __launch_bounds__(32 * TM_WARPS, 4)
+attention_tree_merge_kernel(const TreeParams P, int slot_half, int half_rows) {
+  pdl_wait();
+  TreeCut cut;                                     // (written by the kernel before, and read past L1)
+#pragma unroll
+  for (int x = 0; x < 2; x++) reinterpret_cast<int4*>(&cut)[x] = __ldcg(reinterpret_cast<const int4*>(P.cut + blockIdx.x + 1) + x);
+  if (cut.cuts == 0) return;
+  if (cut.cuts == 1) tree_add_up<T, 8, 2>(P, cut, slot_half, half_rows);
+  else if (cut.cuts < 4) tree_add_up<T, 4, 4>(P, cut, slot_half, half_rows);
+  else tree_add_up<T, 1, 16>(P, cut, slot_half, half_rows);
 }
 
 // ---------------------------------------------------------------- host side
@@ -1250,7 +1268,7 @@ STRATUM_EXPORT int stratum_attention_tree_ctas(int tensor, int many, int head_di
   return sm_count() * (room < 1 ? 1 : room < most ? room : most);
 }
 
-// Scratch: part_o float32 [G][2][slot rows][head_dim rounded up to 4], part_ml float32 [G][2][slot rows][2], cut 48 bytes
+// Scratch: part_o float32 [G][2][head_dim rounded up to 4, / 4][slot rows][4], part_ml float32 [G][2][slot rows][2], cut 32 bytes
 // a CTA.
 // One call's numbers, as the launcher packs them (pointers first, then 8 bytes, then 4).
 struct TreeCall {
@@ -1279,9 +1297,11 @@ STRATUM_EXPORT int stratum_attention_tree(const TreeCall* call, cudaStream_t str
   P.seq_start = (const int*)a.seq_start; P.seq_len = (const int*)a.seq_len;
   P.block_table = (const int*)a.block_table; P.bt_stride = a.bt_stride; P.bt_width = a.bt_width;
   P.q = a.q; P.ldq = ldq; P.k_cache = a.k_cache; P.v_cache = a.v_cache; P.out = a.out; P.ldo = ldo;
-  P.part_o = (float*)a.part_o; P.part_ml = (float2*)a.part_ml; P.cut = (TreeCut*)a.cut; P.status = (int*)a.status;
+  P.part_o = (float4*)a.part_o; P.part_ml = (float2*)a.part_ml; P.cut = (TreeCut*)a.cut; P.status = (int*)a.status;
   P.n_tokens = n_tokens; P.n_seqs = n_seqs; P.n_q = n_q; P.n_kv = n_kv; P.gs = gs; P.head_dim = head_dim;
   P.even_tiles = !tensor;
+  P.item_units = tensor ? 7 : 3;
+  P.out_by_16 = head_dim % 8 == 0 && ldo % 8 == 0 && ((uintptr_t)a.out & 15) == 0;
   P.window = a.window; P.n_pages = (int)n_pages; P.scale = a.scale;
   const int G = stratum_attention_tree_ctas(tensor, many, head_dim);
   int st, slot_half, half_rows;
@@ -1313,10 +1333,7 @@ STRATUM_EXPORT int stratum_attention_tree(const TreeCall* call, cudaStream_t str
     st = dtype == STRATUM_DT_F32 ? launch_tree_simple_of<float>(P, G, stream) : launch_tree_simple_of<bf16>(P, G, stream);
   }
   if (st != 0 || G < 2) return st;
-  const dim3 grid(G - 1, (P.rows_per_tile + 8 * TM_ROWS - 1) / (8 * TM_ROWS)), block(256);
-  if (dtype == STRATUM_DT_F32)
-    return head_dim <= 128 ? launch_pdl(attention_tree_merge_kernel<float, 1>, grid, block, 0, stream, P, G, slot_half, half_rows)
-                           : launch_pdl(attention_tree_merge_kernel<float, 2>, grid, block, 0, stream, P, G, slot_half, half_rows);
-  return head_dim <= 128 ? launch_pdl(attention_tree_merge_kernel<bf16, 1>, grid, block, 0, stream, P, G, slot_half, half_rows)
-                         : launch_pdl(attention_tree_merge_kernel<bf16, 2>, grid, block, 0, stream, P, G, slot_half, half_rows);
+  const dim3 grid(G - 1, 4), block(32 * TM_WARPS);               // (one wave: four blocks to an SM)
+  if (dtype == STRATUM_DT_F32) return launch_pdl(attention_tree_merge_kernel<float>, grid, block, 0, stream, P, slot_half, half_rows);
+  return launch_pdl(attention_tree_merge_kernel<bf16>, grid, block, 0, stream, P, slot_half, half_rows);
 }

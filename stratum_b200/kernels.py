@@ -1766,7 +1766,7 @@ def attention_tree(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor
                                    int(lib.stratum_attention_tree_slot_rows(int(tensor), int(many))))
     ctas, slots = plan[0], 2 * plan[0] * plan[1]
     # (scratch of this call's own: calls on several streams, and captured ones, do not meet in it)
-    scratch = torch.empty(slots * ((head_dim + 3) // 4 * 4 + 2) + 12 * ctas, dtype=torch.float32, device=q.device)
+    scratch = torch.empty(slots * ((head_dim + 3) // 4 * 4 + 2) + 8 * ctas, dtype=torch.float32, device=q.device)
     at = scratch.data_ptr()
     part_ml = at + 4 * slots * ((head_dim + 3) // 4 * 4)
     f = _fn("attention_tree", "stratum_attention_tree", [c_char_p, c_void_p])
