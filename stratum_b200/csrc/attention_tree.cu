@@ -23,12 +23,13 @@
 // P goes back into tensor memory, over the scores it came from, and is the first operand of P V there: with P in shared
 // memory its writing and its reading by the MMAs took a third of what shared memory moves per tile, and every tile had to
 // wait for the one before to be read (91 us against 83 for one sequence of 32,700 tokens and 61 drafted ones).
-// One thread of warp 0 feeds rings of K and V pages by TMA, and the queries of the run that comes next.
+// One thread of warp 0 feeds rings of K and V pages by TMA, and the queries of the run that comes next; the last warp walks the
+// list ahead of the others.
 //
 // The products with masked keys: P is zero there, but zero times an infinity or a NaN is not, and a page that is masked for
 // some row may hold either (rows behind the sequence's end, a drafted branch that overflowed).  So the V page of a masked
-// tile is looked through; rows of V that are not finite are zeroed in shared memory, and what they give to the rows that do
-// see them is added by hand.
+// tile is looked through, by the last warp as soon as it is there; rows of V that are not finite are zeroed in shared memory, and
+// what they give to the rows that do see them is added by hand.
 //
 // Every mbarrier wait is bounded: on expiry a code goes to the status word and a flag is set that ends every other wait of
 // the block, so that all leave together.
@@ -49,6 +50,7 @@
 #define TR_SOFTMAX_WARPS 4                  // per half, a thread a row
 #define TR_THREADS (32 + 2 * 32 + 2 * TR_SOFTMAX_WARPS * 32 + 32)
 #define TR_RUNS 4
+#define TR_LOOKS 16
 
 struct TreeParams {
   const int* token_pos;                    // [tokens]
@@ -114,8 +116,9 @@ __device__ __forceinline__ long long tree_begin(int c, int ctas, long long T) { 
 struct TreeRun {
   TreeSeq s;
   int b, kvh, rt, page0, n;                // n = 0: there are no more
-  int edge;                                // the furthest window edge of the tile's rows
+  int clean0, clean1;                      // of its pages, those that every row sees whole; the others are masked
   bool from_start, to_end, holds_u0;
+  bool pages_ok;                           // no page lies outside the pool
 };
 
 struct TreeCursor {
@@ -140,7 +143,6 @@ struct TreeCursor {
     r.kvh = item / s.n_tiles; r.rt = item % s.n_tiles;
     r.page0 = s.first + off;
     r.n = n;
-    r.edge = 0;
     r.from_start = off == 0;
     r.to_end = off + n == s.n_pages;
     r.holds_u0 = !moved;
@@ -261,10 +263,12 @@ struct TreeSmem {
   float2 ml[2][ROWS2 ? 1 : 128];                                    // a row's maximum and sum in either half, at the end of a run
   uint64_t q_full[QB], q_empty[QB], k_full[STAGES], v_full[STAGES];
   uint64_t s_full[2][STAGES], pv_full[2][STAGES], p_full[2][2];
-  unsigned long long bad[2][2];
+  unsigned long long bad[2][TR_LOOKS];                  // per half (ROWS2: for both), of its masked tiles in turn: keys with values not finite
+  uint64_t look_full[2][TR_LOOKS];
+  uint32_t v_asked;                                     // tiles whose values have been asked for
   TreeRun runs[TR_RUNS];                                // the runs ahead, from the warp that walks the list
-  uint64_t run_full[TR_RUNS], run_empty[TR_RUNS];
-  uint64_t tile_meet[2], run_meet;                      // softmax warps wait for one another (bounded, as every wait)
+  uint64_t run_full[TR_RUNS], run_seen[TR_RUNS], run_empty[TR_RUNS];     // (seen: what only the softmax warps ask for is there too)
+  uint64_t run_meet;                                    // softmax warps wait for one another (bounded, as every wait)
   int row_of[32];                                       // cache row of a tile's page, from the K to the V request
   uint32_t tmem_base;
   int o_ready[2];
@@ -327,37 +331,35 @@ __device__ __forceinline__ void umma_bf16_ts(uint32_t tmem_d, uint32_t tmem_a, u
 
 #define TR_FAIL(code) { atomicCAS(P.status, 0, code); S.abort_flag = 1; }
 
-// The two parts that only masked tiles need are functions of their own, so that the loop over the other tiles keeps its
-// registers.
+// What only masked tiles need is functions of their own, so that the loop over the other tiles keeps its registers.
 
-// The keys of a page of values (in shared memory) that hold anything not finite; their rows are zeroed.  The `n` threads that
-// meet at `bar` come here together, numbered by `tid`; `words` are two, used in turn (the other one is cleared for the next
-// time, by when everybody has seen it).  They meet once, and once more where there are such keys.  Whoever waits in vain
-// sets the flag.
+// The keys of a page of values (in shared memory) that hold anything not finite; their rows are zeroed.  One warp, two keys a
+// lane.
 template <int HD>
-__device__ __noinline__ unsigned long long tree_look_through(uint4* v, unsigned long long* words, int n, int tid, uint64_t* bar,
-                                                             uint32_t phase, uint32_t turn, volatile int* abort_flag) {
-  const int key = tid & 63, part = tid >> 6, n_parts = n >> 6;
-  uint4* row = v + key * 8;                              // 8 chunks of 16 bytes a key and block of 64 dims, visited from another
-  auto chunk = [&](int c) { return (c >> 3) * (TR_KEYS * 8) + ((c + key) & 7); };        // one on by each key: all banks
-  bool mine = false;
-  for (int c = part; c < HD / 8; c += n_parts) {
-    const uint4 x = row[chunk(c)];
+__device__ __noinline__ unsigned long long tree_look_through(uint4* v) {
+  const int lane = threadIdx.x & 31;
+  uint32_t most[2] = {0, 0};                             // largest magnitude, as two numbers of 15 bits
+  // 8 chunks of 16 bytes a key and block of 64 dims, visited from another one on by each key: all banks
+  auto chunk = [&](int c, int key) { return v + key * 8 + (c >> 3) * (TR_KEYS * 8) + ((c + key) & 7); };
+#pragma unroll 4
+  for (int c = 0; c < HD / 8; c++)
 #pragma unroll
-    for (int e = 0; e < 4; e++) {
-      const uint32_t w = e == 0 ? x.x : e == 1 ? x.y : e == 2 ? x.z : x.w;
-      mine = mine || (w & 0x7f80u) == 0x7f80u || (w & 0x7f800000u) == 0x7f800000u;
+    for (int e = 0; e < 2; e++) {
+      const uint4 x = *chunk(c, lane + 32 * e);
+      most[e] = __vmaxu2(__vmaxu2(most[e], x.x & 0x7fff7fffu), __vmaxu2(__vmaxu2(x.y & 0x7fff7fffu, x.z & 0x7fff7fffu), x.w & 0x7fff7fffu));
     }
+  bool odd[2];
+#pragma unroll
+  for (int e = 0; e < 2; e++) odd[e] = (most[e] & 0xffffu) >= 0x7f80u || (most[e] >> 16) >= 0x7f80u;
+  const unsigned long long bad = __ballot_sync(0xffffffffu, odd[0]) | (unsigned long long)__ballot_sync(0xffffffffu, odd[1]) << 32;
+  if (bad) {
+#pragma unroll
+    for (int e = 0; e < 2; e++)
+      if (odd[e])
+        for (int c = 0; c < HD / 8; c++) *chunk(c, lane + 32 * e) = make_uint4(0, 0, 0, 0);
+    fence_async_shared();
+    __syncwarp();
   }
-  if (mine) atomicOr(&words[turn & 1], 1ull << key);
-  if (tid == 0) *(volatile unsigned long long*)&words[(turn & 1) ^ 1] = 0;
-  if (!tr_meet(bar, phase, abort_flag)) { *abort_flag = 1; return 0; }
-  const unsigned long long bad = *(volatile unsigned long long*)&words[turn & 1];
-  if (!bad) return 0;
-  if ((bad >> key) & 1)
-    for (int c = part; c < HD / 8; c += n_parts) row[chunk(c)] = make_uint4(0, 0, 0, 0);
-  fence_async_shared();
-  if (!tr_meet(bar, phase + 1, abort_flag)) *abort_flag = 1;
   return bad;
 }
 
@@ -396,6 +398,7 @@ attention_tree_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
   constexpr int STAGES = Smem::STAGES, QB = Smem::QB, DB = HD / 64;
   constexpr uint32_t COL_PV = 128;
   static_assert(sizeof(Smem) <= 227 * 1024, "shared memory of an SM");
+  static_assert(STAGES < TR_LOOKS, "a masked tile's entry is read before the tile that has it next is there");
   Smem& S = *reinterpret_cast<Smem*>(smem_raw);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   if (smem_u32(smem_raw) & 1023) {                      // (the swizzled tiles need it)
@@ -414,10 +417,11 @@ attention_tree_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
     }
     for (int h = 0; h < 2; h++) {
       mbar_init(&S.p_full[h][0], TR_SOFTMAX_WARPS); mbar_init(&S.p_full[h][1], TR_SOFTMAX_WARPS);
-      S.bad[h][0] = S.bad[h][1] = 0; S.o_ready[h] = 0;
-      mbar_init(&S.tile_meet[h], ROWS2 ? 2 * TR_SOFTMAX_WARPS : TR_SOFTMAX_WARPS);
+      S.o_ready[h] = 0;
+      for (int i = 0; i < TR_LOOKS; i++) mbar_init(&S.look_full[h][i], 1);
     }
-    for (int i = 0; i < TR_RUNS; i++) { mbar_init(&S.run_full[i], 1); mbar_init(&S.run_empty[i], 3 + 2 * TR_SOFTMAX_WARPS); }
+    for (int i = 0; i < TR_RUNS; i++) { mbar_init(&S.run_full[i], 1); mbar_init(&S.run_seen[i], 1); mbar_init(&S.run_empty[i], 4 + 2 * TR_SOFTMAX_WARPS); }
+    S.v_asked = 0;
     mbar_init(&S.run_meet, 2 * TR_SOFTMAX_WARPS);
     S.abort_flag = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -508,6 +512,7 @@ attention_tree_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
           mbar_expect_tx(&S.v_full[s], TR_KEYS * HD * sizeof(bf16));
           for (int db = 0; db < DB; db++) tma_load_2d(&map_v, S.v[s] + db * TR_KEYS * 64, &S.v_full[s], db * 64, row);
           jv++;
+          *(volatile uint32_t*)&S.v_asked = jv;
           moved = true;
         }
         if (moved) { idle = 0; continue; }
@@ -608,10 +613,8 @@ attention_tree_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
     const uint32_t o_addr = lane_addr + COL_PV;
     const float to_log2 = P.scale * 1.4426950408889634f;
     constexpr int STEP = ROWS2 ? 1 : 2;                  // from a tile of this half to the next
-    const int tile_threads = ROWS2 ? 2 * TR_SOFTMAX_WARPS * 32 : TR_SOFTMAX_WARPS * 32;
-    const int tile_tid = ROWS2 ? threadIdx.x - 96 : threadIdx.x - 96 - h * TR_SOFTMAX_WARPS * 32;
     bool ok = true;
-    uint32_t it = 0, i = 0, tile_phase = 0, run_phase = 0, turn = 0;
+    uint32_t it = 0, i = 0, run_phase = 0, looks = 0;    // tiles of the stretch, of this half, meetings, masked tiles of this half
 #define TR_WAIT(bar, parity, code) \
   if (!__all_sync(0xffffffffu, mbar_wait(bar, parity, abort_flag))) { if (lane == 0) TR_FAIL(code); ok = false; break; }
     for (int r = 0; ok; r++) {
@@ -629,26 +632,23 @@ attention_tree_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
       if (!ROWS2 && (int)(it & 1) != h) it++;
       const uint32_t it_mine = it;                       // this half's first tile of the run (it_end or beyond: none)
       const int* bt = P.block_table + (size_t)run.b * P.bt_stride + run.page0 - (int)it_first;   // [it]: the tile's page
-      int pg_next = it < it_end ? __ldcg(bt + (int)it) : 0;
+      TR_WAIT(&S.run_seen[r % TR_RUNS], (r / TR_RUNS) & 1, 511)
+      const uint32_t clean_from = it_first + run.clean0, clean_to = it_first + run.clean1;
       float m_ref = -INFINITY, l = 0.f;
       for (; it < it_end; it += STEP) {
         const int s = it % STAGES, b = i & 1;
-        const int key0 = (run.page0 + (int)(it - it_first)) * TR_KEYS;
-        const int pg = pg_next;
-        if (it + STEP < it_end) pg_next = __ldcg(bt + (int)it + STEP);
-        const bool page_ok = (unsigned)pg < (unsigned)P.n_pages;
-        const bool needs_mask = key0 + TR_KEYS > sq.base || key0 < run.edge || !page_ok;
-        const bool first = it == it_mine;
+        const bool needs_mask = it < clean_from || it >= clean_to, first = it == it_mine;
         TR_WAIT(&S.s_full[h][s], (it / STAGES) & 1, 509)
         unsigned long long vis = 0, bad = 0;
         if (needs_mask) {
-          if (valid) vis = tree_visible(P, sq, token, lo, key0, page_ok, word0);
-          TR_WAIT(&S.v_full[s], (it / STAGES) & 1, 507)
-          bad = tree_look_through<HD>(reinterpret_cast<uint4*>(S.v[s]), S.bad[ROWS2 ? 0 : h], tile_threads, tile_tid,
-                                      &S.tile_meet[ROWS2 ? 0 : h], tile_phase, turn, abort_flag);
-          turn++;
-          tile_phase += bad ? 2 : 1;
-          if (*abort_flag) { if (lane == 0) TR_FAIL(513); ok = false; break; }
+          if (valid) {
+            const bool page_ok = run.pages_ok || (unsigned)__ldcg(bt + (int)it) < (unsigned)P.n_pages;
+            vis = tree_visible(P, sq, token, lo, (run.page0 + (int)(it - it_first)) * TR_KEYS, page_ok, word0);
+          }
+          const int e = looks % TR_LOOKS;
+          TR_WAIT(&S.look_full[ROWS2 ? 0 : h][e], (looks / TR_LOOKS) & 1, 507)
+          bad = *(volatile unsigned long long*)&S.bad[ROWS2 ? 0 : h][e];
+          looks++;
         }
         if (warp_active) {
           tc_fence_after();
@@ -717,7 +717,7 @@ attention_tree_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
             tmem_st_wait();
             tree_add_bad<HD>(bad, vis, lane_addr + b * TR_KEYS, o_addr, to_log2, m_use,
                              reinterpret_cast<const bf16*>(P.v_cache) +
-                                 ((size_t)(page_ok ? pg : 0) * P.n_kv + run.kvh) * TR_KEYS * HD, first);
+                                 ((size_t)((unsigned)__ldcg(bt + (int)it) < (unsigned)P.n_pages ? __ldcg(bt + (int)it) : 0) * P.n_kv + run.kvh) * TR_KEYS * HD, first);
           }
           tmem_st32(lane_addr + b * TR_KEYS, packed);    // over the scores
           tmem_st_wait();
@@ -829,24 +829,76 @@ attention_tree_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
   } else {
     // ---------------------------------------------------------------- the walk over the list
     // A run is described here while the ones before it are worked on: what it takes from memory would otherwise stand
-    // between two runs of every other warp.
+    // between two runs of every other warp.  And the values of masked tiles are looked through as they come, ahead of the
+    // softmax warps (with these doing it themselves a masked tile took 3 us where the others took 1.2).
     const TreeCursor begin = cur;
-    for (int r = 0;; r++) {
-      TreeRun& run = S.runs[r % TR_RUNS];
-      if (r >= TR_RUNS && !__all_sync(0xffffffffu, mbar_wait(&S.run_empty[r % TR_RUNS], ((r / TR_RUNS) - 1) & 1, abort_flag))) { if (lane == 0) TR_FAIL(512); break; }
-      if (lane == 0) cur.next(P, run);
-      __syncwarp();
-      const int n = run.n;
-      if (n > 0 && P.window > 0) {                       // the furthest window edge of the tile's rows, in both halves
-        const int per = half_tokens * (ROWS2 ? 2 : 1), t0 = run.s.row0 + run.rt * per, t1 = min(t0 + per, run.s.row0 + run.s.n_new);
-        int edge = 0;
-        for (int t = t0 + lane; t < t1; t += 32) edge = max(edge, __ldcg(P.token_pos + t) - P.window + 1);
-        edge = __reduce_max_sync(0xffffffffu, edge);
-        if (lane == 0) run.edge = edge;
+    int described = 0, r = 0, t = 0;                       // runs described, the run and the tile of it that is next to be looked at
+    uint32_t it0 = 0, looks[2] = {0, 0}, idle = 0;         // tiles in front of that run, masked tiles of the halves
+    bool more = true;
+    while (more || r < described) {
+      bool moved = false;
+      if (more && (described < TR_RUNS || __all_sync(0xffffffffu, mbar_test_wait(&S.run_empty[described % TR_RUNS], ((described / TR_RUNS) - 1) & 1)))) {
+        TreeRun& run = S.runs[described % TR_RUNS];
+        if (lane == 0) cur.next(P, run);
+        __syncwarp();
+        const int n = run.n;
+        if (lane == 0) mbar_arrive(&S.run_full[described % TR_RUNS]);
+        if (n == 0) more = false;
+        else {
+          // what only the softmax warps ask for, while the first keys are fetched: the furthest window edge of the tile's
+          // rows (of both halves), whether all pages lie in the pool
+          int edge = 0;
+          if (P.window > 0) {
+            const int per = half_tokens * (ROWS2 ? 2 : 1), t0 = run.s.row0 + run.rt * per, t1 = min(t0 + per, run.s.row0 + run.s.n_new);
+            for (int x = t0 + lane; x < t1; x += 32) edge = max(edge, __ldcg(P.token_pos + x) - P.window + 1);
+            edge = __reduce_max_sync(0xffffffffu, edge);
+          }
+          const int* bt = P.block_table + (size_t)run.b * P.bt_stride + run.page0;
+          bool ok = true;
+#pragma unroll 8
+          for (int x = lane; x < n; x += 32) ok &= (unsigned)__ldcg(bt + x) < (unsigned)P.n_pages;
+          ok = __all_sync(0xffffffffu, ok);
+          if (lane == 0) {
+            run.clean0 = min(max((int)(((unsigned)edge + TR_KEYS - 1) / TR_KEYS) - run.page0, 0), n);
+            run.clean1 = ok ? min(max(run.s.base / TR_KEYS - run.page0, 0), n) : 0;
+            run.pages_ok = ok;
+            mbar_arrive(&S.run_seen[described % TR_RUNS]);
+          }
+          described++;
+        }
+        __syncwarp();
+        moved = true;
       }
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&S.run_full[r % TR_RUNS]);
-      if (n == 0) break;
+      if (r < described) {
+        const TreeRun& run = S.runs[r % TR_RUNS];
+        if (t >= run.clean0 && t < run.clean1) t = run.clean1;
+        if (t >= run.n) {
+          it0 += run.n;
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&S.run_empty[r % TR_RUNS]);
+          r++; t = 0;
+          moved = true;
+        } else {
+          // (a barrier tells a phase from the one before it only: it is asked once the tile's values are on their way)
+          const uint32_t it = it0 + t;
+          const int s = it % STAGES;
+          if (__all_sync(0xffffffffu, *(volatile uint32_t*)&S.v_asked > it && mbar_test_wait(&S.v_full[s], (it / STAGES) & 1))) {
+            const int h = ROWS2 ? 0 : it & 1, e = (h ? looks[1]++ : looks[0]++) % TR_LOOKS;
+            const unsigned long long bad = tree_look_through<HD>(reinterpret_cast<uint4*>(S.v[s]));
+            if (lane == 0) {
+              *(volatile unsigned long long*)&S.bad[h][e] = bad;
+              mbar_arrive(&S.look_full[h][e]);
+            }
+            __syncwarp();
+            t++;
+            moved = true;
+          }
+        }
+      }
+      if (moved) { idle = 0; continue; }
+      __nanosleep(50);
+      idle++;
+      if (__any_sync(0xffffffffu, idle >= 4u * TC_SPIN_LIMIT || ((idle & 1023u) == 0 && *abort_flag))) { if (lane == 0) TR_FAIL(512); break; }
     }
     if (lane == 0) tree_cut(P, begin, u0, total);
   }
