@@ -313,6 +313,21 @@ __device__ __forceinline__ uint32_t tr_pack(float L, float a, float b) {
   const __nv_bfloat162 v = __floats2bfloat162_rn(L == 0.f ? 0.f : a, L == 0.f ? 0.f : b);
   return *reinterpret_cast<const uint32_t*>(&v);
 }
+// Four lanes hold 64 bytes of a row each: behind this each has 16 bytes of all four rows, w[k] of the k-th, so that what a store
+// writes lies together (a row a lane, every store touched 32 lines, and a run's outputs took 4 us).
+__device__ __forceinline__ void tr_turn(uint4 (&w)[4]) {
+  const int lane = threadIdx.x & 31;
+#pragma unroll
+  for (int x = 1; x < 4; x *= 2)
+#pragma unroll
+    for (int k = 0; k < 4; k++) {
+      if (k & x) continue;
+      uint4 give = lane & x ? w[k] : w[k + x];
+      give.x = __shfl_xor_sync(0xffffffffu, give.x, x); give.y = __shfl_xor_sync(0xffffffffu, give.y, x);
+      give.z = __shfl_xor_sync(0xffffffffu, give.z, x); give.w = __shfl_xor_sync(0xffffffffu, give.w, x);
+      if (lane & x) w[k] = give; else w[k + x] = give;
+    }
+}
 __device__ __forceinline__ float tmem_ld1f(uint32_t taddr) {
   uint32_t r;
   asm volatile("tcgen05.ld.sync.aligned.32x32b.x1.b32 {%0}, [%1];" : "=r"(r) : "r"(taddr));
@@ -556,11 +571,20 @@ attention_tree_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
       }
       __syncwarp();
     };
+    // ROWS2, whose next queries come once this run's scores are through: until they are here, the product that the softmax warps
+    // need to end this run (with the halves in turn on one tile the queries are there already)
+    auto or_values = [&](uint64_t* bar, uint32_t parity) {
+      if (ROWS2 && pend && !__all_sync(0xffffffffu, mbar_test_wait(bar, parity))) { values(); pend = false; }
+    };
     for (int r = 0; ok; r++) {
+      or_values(&S.run_full[r % TR_RUNS], (r / TR_RUNS) & 1);
+      if (!ok) break;
       if (!__all_sync(0xffffffffu, mbar_wait(&S.run_full[r % TR_RUNS], (r / TR_RUNS) & 1, abort_flag))) { if (lane == 0) TR_FAIL(511); ok = false; break; }
       const TreeRun& run = S.runs[r % TR_RUNS];
       if (run.n == 0) break;
       const bool active = !ROWS2 || half_ntok(run, h) > 0;
+      or_values(&S.q_full[r % QB], (r / QB) & 1);
+      if (!ok) break;
       if (!__all_sync(0xffffffffu, mbar_wait(&S.q_full[r % QB], (r / QB) & 1, abort_flag))) { if (lane == 0) TR_FAIL(502); ok = false; break; }
       const uint64_t qd = smem_desc_sw128(smem_u32(S.q[ROWS2 ? h : r % QB]));
       bool first = true;
@@ -738,6 +762,10 @@ attention_tree_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
       const bool whole = run.from_start && run.to_end;
       const int slot = 2 * blockIdx.x + (run.holds_u0 ? 0 : 1);
       bf16* out_row = reinterpret_cast<bf16*>(P.out) + (size_t)token * P.ldo + (size_t)(run.kvh * gs + head) * HD;
+      bf16* to[4];                                       // the rows of this lane's group of four
+#pragma unroll
+      for (int k = 0; k < 4; k++)
+        to[k] = reinterpret_cast<bf16*>(__shfl_sync(0xffffffffu, valid ? (unsigned long long)out_row : 0ull, (lane & ~3) + k));
       tc_fence_after();
       if (ROWS2) {
         if (warp_active) {
@@ -748,15 +776,16 @@ attention_tree_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
             float o[32];
             tmem_ld32f(o_addr + c, o);                   // (all lanes take part; only valid rows store)
             tmem_ld_wait();
-            if (valid && whole) {
+            if (whole) {
+              uint4 w[4];
 #pragma unroll
-              for (int e = 0; e < 32; e += 8) {
-                uint4 w;
-                uint32_t* wp = reinterpret_cast<uint32_t*>(&w);
+              for (int e = 0; e < 4; e++)
+                w[e] = make_uint4(tr_pack(l, o[8 * e] * inv, o[8 * e + 1] * inv), tr_pack(l, o[8 * e + 2] * inv, o[8 * e + 3] * inv),
+                                  tr_pack(l, o[8 * e + 4] * inv, o[8 * e + 5] * inv), tr_pack(l, o[8 * e + 6] * inv, o[8 * e + 7] * inv));
+              tr_turn(w);
 #pragma unroll
-                for (int x = 0; x < 4; x++) wp[x] = tr_pack(l, o[e + 2 * x] * inv, o[e + 2 * x + 1] * inv);
-                *reinterpret_cast<uint4*>(out_row + c + e) = w;
-              }
+              for (int k = 0; k < 4; k++)
+                if (to[k]) *reinterpret_cast<uint4*>(to[k] + c + 8 * (lane & 3)) = w[k];
             } else if (valid) {
 #pragma unroll
               for (int e = 0; e < 32; e += 4)
@@ -803,15 +832,16 @@ attention_tree_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
                 for (int e = 0; e < 32; e++) o[e] = fmaf(f1, __uint_as_float(r[e]), o[e]);
               }
             }
-            if (valid && whole) {
+            if (whole) {
+              uint4 w[4];
 #pragma unroll
-              for (int e = 0; e < 32; e += 8) {
-                uint4 w;
-                uint32_t* wp = reinterpret_cast<uint32_t*>(&w);
+              for (int e = 0; e < 4; e++)
+                w[e] = make_uint4(tr_pack(L, o[8 * e] * inv, o[8 * e + 1] * inv), tr_pack(L, o[8 * e + 2] * inv, o[8 * e + 3] * inv),
+                                  tr_pack(L, o[8 * e + 4] * inv, o[8 * e + 5] * inv), tr_pack(L, o[8 * e + 6] * inv, o[8 * e + 7] * inv));
+              tr_turn(w);
 #pragma unroll
-                for (int x = 0; x < 4; x++) wp[x] = tr_pack(L, o[e + 2 * x] * inv, o[e + 2 * x + 1] * inv);
-                *reinterpret_cast<uint4*>(out_row + c + e) = w;
-              }
+              for (int k = 0; k < 4; k++)
+                if (to[k]) *reinterpret_cast<uint4*>(to[k] + c + 8 * (lane & 3)) = w[k];
             } else if (valid) {
 #pragma unroll
               for (int e = 0; e < 32; e += 4)
