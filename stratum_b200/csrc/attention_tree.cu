@@ -34,13 +34,15 @@
 // Every mbarrier wait is bounded: on expiry a code goes to the status word and a flag is set that ends every other wait of
 // the block, so that all leave together.
 //
-// What bounds the tcgen05 kernel.  64 keys of 256 rows take 2,000 to 2,300 cycles, of which the tensor cores are busy for
+// What bounds the tcgen05 kernel.  64 keys of 256 rows take 2,000 to 2,200 cycles, of which the tensor cores are busy for
 // 1,270 (a product of 128 x 64 x 16 takes them 48 cycles with both halves at it, as the rows of Q are read from shared memory
 // each time, one of 128 x 128 x 16 takes 64) and the exponentials' units for 1,024; the rest is one waiting for the other
-// at the ends of tiles.  Measured: one sequence of 32,700 tokens and 61 drafted ones, 8 kv heads of 8 queries: 63 us (128 MB
-// of keys and values, 2.1 TB/s); 64 sequences of 4,000: 275 us, 325 where the card is held back by its power limit.
-// Tried without a gain: every other exponential as a polynomial, a lock that keeps the halves' products apart, halves that
-// start half a tile apart, one thread that issues for both, a guess at the maximum before the scores are there.
+// at the ends of tiles.  Around the tiles: 3 us to read the list, 3 more to the first scores, 3 at the end of a run (the last
+// product, the outputs), 6 to add pieces up.  Measured, 8 kv heads of 4 queries, head size 128: one sequence of 32,700 tokens and
+// 61 drafted ones 53 us (134 MB of keys and values, 2.5 TB/s, 615 TFLOP/s); 64 sequences of 4,000 and 33 to 64 drafted ones 264 us
+// (3.7 TB/s, 670 TFLOP/s), 315 where the card is held back by its power limit.
+// Tried without a gain: more of the exponentials as polynomials, a lock that keeps the halves' products apart, halves that start
+// half a tile apart, one thread that issues for both, a guess at the maximum before the scores are there.
 #include <math.h>
 
 #include "tc_common.cuh"
@@ -292,6 +294,11 @@ __device__ __forceinline__ uint64_t tr_fma2(uint64_t a, uint64_t b, uint64_t c) 
   asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
   return r;
 }
+__device__ __forceinline__ uint64_t tr_mul2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
 __device__ __forceinline__ uint64_t tr_add2(uint64_t a, uint64_t b) {
   uint64_t r;
   asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
@@ -301,6 +308,24 @@ __device__ __forceinline__ float tr_exp2(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
+}
+// 2^a and 2^b with additions and products alone (no larger than 2^9): the whole part n goes into a float's exponent, 2^f of the
+// rest, |f| <= 1/2, is a cubic, fitted to the smallest largest relative error there, 7.5e-5 (2^-13.7: what is rounded to bfloat16 does
+// not notice).  0 below 2^-126; no number stays none.
+__device__ __forceinline__ void tr_exp2_pair(float& a, float& b) {
+  float x0, x1, t0, t1;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(x0) : "f"(a), "f"(-127.f));
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(x1) : "f"(b), "f"(-127.f));
+  const uint64_t x = tr_pair(x0, x1);
+  const float shift = 12582912.f + 127.f;                // 1.5 * 2^23: behind it the last bits hold n + 127
+  const uint64_t t = tr_add2(x, tr_pair(shift, shift));
+  const uint64_t f = tr_fma2(tr_add2(t, tr_pair(-shift, -shift)), tr_pair(-1.f, -1.f), x);
+  uint64_t p = tr_fma2(f, tr_pair(0.05517167f, 0.05517167f), tr_pair(0.24261113f, 0.24261113f));
+  p = tr_fma2(p, f, tr_pair(0.69326097f, 0.69326097f));
+  p = tr_fma2(p, f, tr_pair(0.99992806f, 0.99992806f));
+  tr_split(t, t0, t1);
+  const uint64_t power = tr_pair(__uint_as_float(__float_as_uint(t0) << 23), __uint_as_float(__float_as_uint(t1) << 23));
+  tr_split(tr_mul2(p, power), a, b);
 }
 // The warps that `bar` counts wait for one another: false if one of them has given up.
 __device__ __forceinline__ bool tr_meet(uint64_t* bar, uint32_t phase, volatile int* abort_flag) {
@@ -710,10 +735,16 @@ attention_tree_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
           for (int e = 0; e < TR_KEYS; e += 2) {
             float x0, x1;
             tr_split(tr_fma2(tr_pair(sc[e], sc[e + 1]), mul2, neg2), x0, x1);
-            const float p0 = tr_exp2(x0), p1 = tr_exp2(x1);
-            uint32_t u;                                  // P V takes them as bfloat16, off by at most 2^-9; the sum as they are
+            // ROWS2: a quarter of them without the exponentials' unit, which eight full warps wait for (64 sequences of 4,000
+            // tokens: 4 % less; where rows are few it costs 4 %)
+            float p0 = x0, p1 = x1;
+            if (ROWS2 && (e & 6) == 6) tr_exp2_pair(p0, p1);
+            else { p0 = tr_exp2(x0); p1 = tr_exp2(x1); }
+            // P V takes them as bfloat16, off by at most 2^-8 of themselves; the sum runs over the same rounded values, so that
+            // a row's weights add up to one and what the values have in common is not touched
+            uint32_t u;
             asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(u) : "f"(p1), "f"(p0));
-            sum2[(e >> 1) & 1] = tr_add2(sum2[(e >> 1) & 1], tr_pair(p0, p1));
+            sum2[(e >> 1) & 1] = tr_add2(sum2[(e >> 1) & 1], tr_pair(__uint_as_float(u << 16), __uint_as_float(u & 0xffff0000u)));
             packed[e >> 1] = u;
           }
           float sum[4];
