@@ -215,3 +215,31 @@ def test_pages_beyond_32_bits_of_bytes():
     K.attention_tree(dev(b.q, torch.bfloat16), k, v, dev(np.array(b.pos, np.int32)), dev(b.mask()), dev(b.start), dev(b.length),
                      dev(table), out, 8, 8, hd, PAGE, 0, b.scale, 9)
     check(b, torch.bfloat16, out)
+
+
+@pytest.mark.parametrize("dtype,hd", [("bfloat16", 64), ("bfloat16", 128), ("bfloat16", 200), ("float32", 80), ("float32", 6)])
+@pytest.mark.parametrize("new", [3, 70])
+def test_pieces_of_many_stretches(dtype, hd, new):
+    """One sequence that dozens of CTAs see pieces of, beside one that two see."""
+    b = TreeBatch(hd, [12000, 400], [new, 2], 2, 1, hd).round_to(DT[dtype])
+    check(b, DT[dtype], run_tree(b, DT[dtype]))
+
+
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("new", [4, 40])
+def test_stretches_of_masked_pages(hd, new):
+    """A page outside the pool in every sequence, so that whole stretches of pages take the masked way, more of them than are looked
+    through at a time; the pool's other pages, and rows behind the ends, hold what is not finite."""
+    b = TreeBatch(hd + new, [3000 - 7 * i for i in range(24)], [new] * 24, 8, 2, hd).round_to(torch.bfloat16)
+    for s in range(24):
+        b.table[s, 5 + s] = -1 if s % 2 else b.n_pages + s
+    used = set(b.table[(b.table >= 0) & (b.table < b.n_pages)].tolist())
+    for p in range(b.n_pages):
+        if p not in used:
+            b.k[p], b.v[p] = np.nan, np.inf
+    for s in range(24):
+        last = int(b.length[s])
+        if last % PAGE:
+            page, row = b.place(s, last)
+            b.k[page, :, row:], b.v[page, :, row:] = np.inf, np.nan
+    check(b, torch.bfloat16, run_tree(b, torch.bfloat16))
