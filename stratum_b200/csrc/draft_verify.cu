@@ -268,7 +268,7 @@ struct VdSmem {
 
 // What a walk costs is passes over a row, one behind the other: every rejection of a drawn child sums the lowered row before the
 // next child can be tried, and the draw at the end sums it where that has not been done.  Measured: 64 trees of 9 to 16 nodes,
-// 128,256 ids, drawn: 40 us (one pass over the 64 first rows and the draft's would be 10); 37 looked-up trees of 32,000 ids and a
+// 128,256 ids, drawn: 36 us (one pass over the 64 first rows and the draft's would be 10); 37 looked-up trees of 32,000 ids and a
 // chain of six behind 128,256: 7.5 us, of which 3 are the dependent reads of the tree, its numbers and the row.
 //
 // W: ids of a load (4 where every row begins on 16 bytes); a warp has LINES loads of a row on their way together.
@@ -358,6 +358,35 @@ verify_drafts_kernel(const VerifyParams P) {
     for (int j = lane; j < S.n_zeroed; j += 32) mine = mine || (S.zeroed[j] >= from && S.zeroed[j] < end);
     return __any_sync(0xffffffffu, mine) != 0;
   };
+  auto sum_of = [&](const float* trow, const float* drow, double cover, int from, int end) {       // by one warp
+    const bool lost = S.n_zeroed > 0 && loses_between(from, end);
+    double sum = 0.0;
+#pragma unroll 1
+    for (int i0 = from; i0 < end; i0 += LINES * LINE) {
+      float p[LINES][W], q[LINES][W];
+      fetch(trow, drow, i0 + lane * W, end, cover > 0.0, p, q);
+#pragma unroll
+      for (int x = 0; x < LINES; x++) {
+        double w[W];
+        weights(p[x], q[x], i0 + x * LINE + lane * W, cover, lost, w);
+        double part = 0.0;
+#pragma unroll
+        for (int e = 0; e < W; e++) part += w[e];
+        sum += part;
+      }
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+    return sum;
+  };
+  auto scan = [&](double v, int n) {               // running sums over the first n lanes
+#pragma unroll
+    for (int d = 1; d < 16; d <<= 1) {
+      const double o = __shfl_up_sync(0xffffffffu, v, d);
+      if (lane >= d && lane < n) v += o;
+    }
+    return v;
+  };
   // The walk is warp 0's in every block, with the same numbers and so the same way everywhere; where it needs the sum of a
   // row, all blocks work that out together.
   bool summed = false;                             // S.all holds the running sums of the row as it is (warp 0's)
@@ -406,35 +435,10 @@ verify_drafts_kernel(const VerifyParams P) {
       const float* trow = P.target + (long long)(a + S.node) * P.ldt;
       const float* drow = P.draft ? P.draft + (long long)(a + S.node) * P.ldd : nullptr;
       const double cover = S.cover + (want == 1 ? S.mass : 0.0);
-      const bool lost = S.n_zeroed > 0 && loses_between(s0, s1);
-      double sum = 0.0;
-#pragma unroll 1
-      for (int i0 = s0; i0 < s1; i0 += LINES * LINE) {
-        float p[LINES][W], q[LINES][W];
-        fetch(trow, drow, i0 + lane * W, s1, cover > 0.0, p, q);
-#pragma unroll
-        for (int x = 0; x < LINES; x++) {
-          double w[W];
-          weights(p[x], q[x], i0 + x * LINE + lane * W, cover, lost, w);
-          double part = 0.0;
-#pragma unroll
-          for (int e = 0; e < W; e++) part += w[e];
-          sum += part;
-        }
-      }
-#pragma unroll
-      for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+      const double sum = sum_of(trow, drow, cover, s0, s1);
       if (lane == 0) S.seg[warp] = sum;
     }
     __syncthreads();
-    auto scan = [&](double v, int n) {             // running sums over the first n lanes
-#pragma unroll
-      for (int d = 1; d < 16; d <<= 1) {
-        const double o = __shfl_up_sync(0xffffffffu, v, d);
-        if (lane >= d && lane < n) v += o;
-      }
-      return v;
-    };
     if (warp == 0) {
       const double v = scan(lane < VD_WARPS ? S.seg[lane] : 0.0, VD_WARPS), total = __shfl_sync(0xffffffffu, v, VD_WARPS - 1);
       if (lane < VD_WARPS) S.seg[lane] = v;
@@ -451,68 +455,80 @@ verify_drafts_kernel(const VerifyParams P) {
     parity ^= 1;
     if (want == 2) break;
   }
-  // ---- the draw
-  if (warp == 0) {
-    const double total = S.all[C - 1], aim = __dmul_rn((double)S.u[0], total);
-    // the first block, and in it the first warp, whose running sum is over the aim; none (rounding): the last one that has
-    // any weight
-    auto find = [&](double v, double before, int n, bool& over) {
-      const unsigned overs = __ballot_sync(0xffffffffu, lane < n && v > aim), anys = __ballot_sync(0xffffffffu, lane < n && v > before);
-      over = overs != 0;
-      return overs ? __ffs(overs) - 1 : anys ? 31 - __clz(anys) : 0;
-    };
-    bool crossed;
-    const int block = find(lane < C ? S.all[lane] : 0.0, lane > 0 && lane < C ? S.all[lane - 1] : 0.0, C, crossed);
-    int pick = -1, positive = 0;
-    if (block == c && total > 0.0) {
-      const double front = c > 0 ? S.all[c - 1] : 0.0;
-      const double mine = lane < VD_WARPS ? S.seg[lane] : 0.0, less = lane > 0 && lane < VD_WARPS ? S.seg[lane - 1] : 0.0;
-      bool here;
-      const int w_ = find(front + mine, front + less, VD_WARPS, here), found = c * VD_WARPS + w_;
-      crossed = crossed && here;
-      const float* trow = P.target + (long long)(a + S.node) * P.ldt;
-      const float* drow = P.draft ? P.draft + (long long)(a + S.node) * P.ldd : nullptr;
-      const int f0 = (int)min((long long)found * per, (long long)P.vocab), f1 = min(f0 + per, P.vocab);
-      const double cover = S.cover;
-      const bool lost = S.n_zeroed > 0 && loses_between(f0, f1);
-      double base = front + (w_ > 0 ? S.seg[w_ - 1] : 0.0);
-      for (int i0 = f0; i0 < f1 && pick < 0; i0 += LINES * LINE) {
-        float p[LINES][W], q[LINES][W];
-        fetch(trow, drow, i0 + lane * W, f1, cover > 0.0, p, q);
+  // ---- the draw: the first block whose running sum is over the aim, in it the first warp's stretch, then, its lines shared out
+  // among the warps, the first part of that, and the first id
+  __syncthreads();                                 // (the blocks' sums are there)
+  const double total = S.all[C - 1], aim = __dmul_rn((double)S.u[0], total);
+  // the first of n lanes whose running sum is over the aim; none (rounding): the last one that has any weight
+  auto find = [&](double v, double before, int n, bool& over) {
+    const unsigned overs = __ballot_sync(0xffffffffu, lane < n && v > aim), anys = __ballot_sync(0xffffffffu, lane < n && v > before);
+    over = overs != 0;
+    return overs ? __ffs(overs) - 1 : anys ? 31 - __clz(anys) : 0;
+  };
+  bool crossed;
+  const int block = find(lane < C ? S.all[lane] : 0.0, lane > 0 && lane < C ? S.all[lane - 1] : 0.0, C, crossed);
+  if (c == 0 && tid == 0) {
+    P.kept[b] = S.depth;
+    if (!(total > 0.0)) P.picked[b] = 0;           // nothing to draw from
+  }
+  if (block != c || !(total > 0.0)) return;        // (the same in the whole block; nothing of another block is touched any more)
+  const double front = c > 0 ? S.all[c - 1] : 0.0;
+  const double mine = lane < VD_WARPS ? S.seg[lane] : 0.0, less = lane > 0 && lane < VD_WARPS ? S.seg[lane - 1] : 0.0;
+  bool here;
+  const int w_ = find(front + mine, front + less, VD_WARPS, here), found = c * VD_WARPS + w_;
+  crossed = crossed && here;
+  double base = front + (w_ > 0 ? S.seg[w_ - 1] : 0.0);
+  const float* trow = P.target + (long long)(a + S.node) * P.ldt;
+  const float* drow = P.draft ? P.draft + (long long)(a + S.node) * P.ldd : nullptr;
+  const double cover = S.cover;
+  const int f0 = (int)min((long long)found * per, (long long)P.vocab), f1 = min(f0 + per, P.vocab);
+  const int part = (per / LINE + VD_WARPS - 1) / VD_WARPS * LINE;
+  auto part_from = [&](int w) { return min(f0 + w * part, f1); };
+  const double sum = sum_of(trow, drow, cover, part_from(warp), part_from(warp + 1));
+  __syncthreads();                                 // (the stretches' sums are read)
+  if (lane == 0) S.seg[warp] = sum;
+  __syncthreads();
+  if (warp != 0) return;
+  const double upto = scan(lane < VD_WARPS ? S.seg[lane] : 0.0, VD_WARPS);
+  double before = __shfl_up_sync(0xffffffffu, upto, 1);
+  if (lane == 0) before = 0.0;
+  const int w2 = find(base + upto, base + before, VD_WARPS, here), g0 = part_from(w2), g1 = part_from(w2 + 1);
+  crossed = crossed && here;
+  base += __shfl_sync(0xffffffffu, before, w2);
+  const bool lost = S.n_zeroed > 0 && loses_between(g0, g1);
+  int pick = -1, positive = 0;
+  for (int i0 = g0; i0 < g1 && pick < 0; i0 += LINES * LINE) {
+    float p[LINES][W], q[LINES][W];
+    fetch(trow, drow, i0 + lane * W, g1, cover > 0.0, p, q);
 #pragma unroll
-        for (int x = 0; x < LINES; x++) {
-          const int i = i0 + x * LINE + lane * W;
-          double w[W];
-          weights(p[x], q[x], i, cover, lost, w);
-          double v = 0.0;
+    for (int x = 0; x < LINES; x++) {
+      if (i0 + x * LINE >= g1) break;
+      const int i = i0 + x * LINE + lane * W;
+      double w[W];
+      weights(p[x], q[x], i, cover, lost, w);
+      double v = 0.0;
 #pragma unroll
-          for (int e = 0; e < W; e++) v += w[e];
-          double up = v;                           // running sums over the lanes
+      for (int e = 0; e < W; e++) v += w[e];
+      double up = v;                               // running sums over the lanes
 #pragma unroll
-          for (int d = 1; d < 32; d <<= 1) {
-            const double o = __shfl_up_sync(0xffffffffu, up, d);
-            if (lane >= d) up += o;
-          }
-          double run = base + (up - v);
-          int over = -1, any = -1;                 // this lane's first id over the aim, and last one with any weight
-#pragma unroll
-          for (int e = 0; e < W; e++) {
-            run += w[e];
-            if (w[e] > 0.0) { any = i + e; if (over < 0 && run > aim) over = i + e; }
-          }
-          const unsigned overs = __ballot_sync(0xffffffffu, over >= 0), anys = __ballot_sync(0xffffffffu, any >= 0);
-          if (anys) positive = __shfl_sync(0xffffffffu, any, 31 - __clz(anys));
-          if (overs && crossed && pick < 0) pick = __shfl_sync(0xffffffffu, over, __ffs(overs) - 1);
-          base += __shfl_sync(0xffffffffu, up, 31);
-        }
+      for (int d = 1; d < 32; d <<= 1) {
+        const double o = __shfl_up_sync(0xffffffffu, up, d);
+        if (lane >= d) up += o;
       }
-      if (lane == 0) P.picked[b] = pick >= 0 ? pick : positive;
-    }
-    if (c == 0 && lane == 0) {
-      P.kept[b] = S.depth;
-      if (!(total > 0.0)) P.picked[b] = 0;         // nothing to draw from
+      double run = base + (up - v);
+      int over = -1, any = -1;                     // this lane's first id over the aim, and last one with any weight
+#pragma unroll
+      for (int e = 0; e < W; e++) {
+        run += w[e];
+        if (w[e] > 0.0) { any = i + e; if (over < 0 && run > aim) over = i + e; }
+      }
+      const unsigned overs = __ballot_sync(0xffffffffu, over >= 0), anys = __ballot_sync(0xffffffffu, any >= 0);
+      if (anys) positive = __shfl_sync(0xffffffffu, any, 31 - __clz(anys));
+      if (overs && crossed && pick < 0) pick = __shfl_sync(0xffffffffu, over, __ffs(overs) - 1);
+      base += __shfl_sync(0xffffffffu, up, 31);
     }
   }
+  if (lane == 0) P.picked[b] = pick >= 0 ? pick : positive;
 }
 
 static int vd_resident(int C) {
