@@ -90,7 +90,18 @@ __device__ __forceinline__ void cluster_all_begun() { asm volatile("barrier.clus
 // stay and take row after row: 316 us.)  Nine rows: 5 us, launch and three trips to memory.
 #define PR_HELD 32
 
-struct Part { float v, sum; int i; };              // the largest value, the sum of weights against it, where it is first
+struct alignas(16) Part { float v, sum; int i, unused; };   // the largest value, the sum of weights against it, where it is first
+
+// 16 bytes to block `rank` of the cluster, whose barrier counts them: nobody waits for a fence, and a block goes on once it has
+// heard from all.
+__device__ __forceinline__ void tell(const Part* place, const uint64_t* bar, int rank, float v, float sum, int i) {
+  asm volatile(
+      "{\n\t.reg .b32 a, b;\n\t"
+      "mapa.shared::cluster.u32 a, %0, %2;\n\t"
+      "mapa.shared::cluster.u32 b, %1, %2;\n\t"
+      "st.async.weak.shared::cluster.mbarrier::complete_tx::bytes.v4.b32 [a], {%3, %4, %5, %6}, [b];\n\t}"
+      ::"r"(smem_u32(place)), "r"(smem_u32(bar)), "r"(rank), "r"(__float_as_uint(v)), "r"(__float_as_uint(sum)), "r"(i), "r"(0) : "memory");
+}
 
 // A weight against `m`, no less than v, in all cases: 1 at the maximum (infinite ones too), 0 at -inf.
 __device__ __forceinline__ float any_weight(float v, float m, float to_log2) {
@@ -101,13 +112,21 @@ __device__ __forceinline__ float clean(float v) { return fmaxf(v, -INFINITY); } 
 // W: values of a load and a store (4 where every row begins on 16 bytes)
 template <bool HELD, int W, int PR_THREADS>
 __global__ void __launch_bounds__(PR_THREADS, 1024 / PR_THREADS)
-token_probs_kernel(const float* logits, long long ld, const float* temperature, float* out, long long ldo, int vocab, int slice) {
+token_probs_kernel(const float* logits, long long ld, const float* temperature, float* out, long long ldo, int vocab, int slice, int* status) {
   __shared__ float warp_v[PR_THREADS / 32], warp_sum_[PR_THREADS / 32];
   __shared__ int first;
   __shared__ Part told[16];
+  __shared__ uint64_t all_told;
+  __shared__ int given_up;
   cg::cluster_group cluster = cg::this_cluster();
   const int C = cluster.num_blocks(), c = cluster.block_rank();
   const int row = blockIdx.x / C, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  if (tid == 0) {
+    given_up = 0;
+    mbar_init(&all_told, 1);
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    mbar_expect_tx(&all_told, C * sizeof(Part));
+  }
   cluster_begun();
   pdl_wait();
   const int i0 = min(c * slice, vocab), n = min(vocab - i0, slice);
@@ -174,10 +193,13 @@ token_probs_kernel(const float* logits, long long ld, const float* temperature, 
   cluster_all_begun();
   if (warp == 0) {
     sum = warp_sum(lane < PR_THREADS / 32 ? warp_sum_[lane] : 0.f);
-    if (lane < C) *cluster.map_shared_rank(&told[c], lane) = Part{m, sum, first};
+    if (lane < C) tell(&told[c], &all_told, lane, m, sum, first);
   }
-  cluster.sync();                                  // (nothing of another block is touched behind it)
-  const Part p = lane < C ? told[lane] : Part{-INFINITY, 0.f, 0x7fffffff};
+  if (!mbar_wait(&all_told, 0, &given_up)) {       // (the others have told this block: none writes here any more)
+    atomicCAS(status, 0, 521);
+    return;
+  }
+  const Part p = lane < C ? told[lane] : Part{-INFINITY, 0.f, 0x7fffffff, 0};
   const float M = warp_max(p.v);                   // of the row
   if (greedy || M == -INFINITY) {                  // (the same in the whole cluster)
     const int best = __reduce_min_sync(0xffffffffu, p.v == M ? p.i : 0x7fffffff);    // (-inf: nowhere)
@@ -209,7 +231,7 @@ token_probs_kernel(const float* logits, long long ld, const float* temperature, 
 // logits float32 [rows][ld], temperature float32 [rows], out float32 [rows][ldo]; out may be logits (the same rows at the same
 // distance).
 STRATUM_EXPORT int stratum_token_probs(const float* logits, long long ld, const float* temperature, float* out, long long ldo,
-                                       int rows, int vocab, cudaStream_t stream) {
+                                       int rows, int vocab, int* status, cudaStream_t stream) {
   if (rows <= 0 || vocab <= 0) return 0;
   if (rows > (1 << 26) || vocab > (1 << 30)) return STRATUM_ERR_LIMIT;
   const bool four = (((uintptr_t)logits | (uintptr_t)out) & 15) == 0 && (rows == 1 || (ld % 4 == 0 && ldo % 4 == 0));
@@ -219,7 +241,7 @@ STRATUM_EXPORT int stratum_token_probs(const float* logits, long long ld, const 
   while (C < 16 && ((long long)C * threads * PR_HELD < vocab || (C * 4096 < vocab && (long long)rows * C * 2 <= sm_count()))) C *= 2;
   const int slice = (((vocab + C - 1) / C) + 3) & ~3;
 #define PROBS(HELD, W, THREADS) \
-  launch_clusters<token_probs_kernel<HELD, W, THREADS>>(rows, C, THREADS, stream, logits, ld, temperature, out, ldo, vocab, slice)
+  launch_clusters<token_probs_kernel<HELD, W, THREADS>>(rows, C, THREADS, stream, logits, ld, temperature, out, ldo, vocab, slice, status)
   if (slice > threads * PR_HELD) return PROBS(false, 1, 512);
   if (threads == 256) return four ? PROBS(true, 4, 256) : PROBS(true, 1, 256);
   return four ? PROBS(true, 4, 512) : PROBS(true, 1, 512);

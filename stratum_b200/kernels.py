@@ -502,7 +502,7 @@ def check_status() -> None:
         _status_word.zero_()
         where = {101: "the TMA producer waiting for a free stage", 102: "the MMA warp waiting for a free accumulator",
                  103: "the MMA warp waiting for a loaded stage", 104: "the epilogue waiting for an accumulator",
-                 **{c: "the attention of drafted tokens" for c in range(501, 515)},
+                 **{c: "the attention of drafted tokens" for c in range(501, 515)}, 521: "a block of a row's probabilities waiting for the others",
                  431: "the resident decode step's ring (a free stage)", 432: "the resident decode step's ring (a filled stage)",
                  **{c: "a block of the resident decode step waiting for the others" for c in (401, 402, 403, 405, 411, 421)}}
         raise KernelError(f"a device-side wait ran out in {where.get(code, f'code {code}')}; results are invalid")
@@ -1805,9 +1805,9 @@ def token_probs(logits: torch.Tensor, temperature: torch.Tensor, out: torch.Tens
         if _meet(logits.data_ptr(), 4 * (logits.stride(0) if R > 1 else V), 4 * V, out.data_ptr(), 4 * (out.stride(0) if R > 1 else V), 4 * V, R):
             raise KernelError("token_probs: out is logits itself or memory of its own")
     f = _fn("draft_verify", "stratum_token_probs",
-            [c_void_p, ctypes.c_longlong, c_void_p, c_void_p, ctypes.c_longlong, c_int, c_int, c_void_p])
+            [c_void_p, ctypes.c_longlong, c_void_p, c_void_p, ctypes.c_longlong, c_int, c_int, c_void_p, c_void_p])
     _check(f(logits.data_ptr(), logits.stride()[0], temperature.data_ptr(), out.data_ptr(), out.stride()[0], R, V,
-             _stream()), "token_probs")
+             status_word().data_ptr(), _stream()), "token_probs")
 
 
 VERIFY_MAX_NODES = 1024            # of a sequence
