@@ -83,11 +83,13 @@ __device__ __forceinline__ void cluster_all_begun() { asm volatile("barrier.clus
 //
 // With ordinary numbers a weight is a difference, a product and an exponential; infinities, and temperatures that are so large
 // or small that the product is none, are told apart once for a block: decided for every value they were fifty instructions
-// a value, and the time was theirs (287 us against 224 for 1,024 rows of 128,256).
+// a value, and the time was theirs (287 us against 224 for 1,024 rows of 128,256, then).
 //
-// Measured: 1,024 rows of 128,256 in 225 us, 4.7 TB/s read and written, 0.71 of a plain copy; what is missing is a row's blocks
-// waiting for one another between reading and writing, while the other three or so on their SM read or write.  (Blocks that
-// stay and take row after row: 316 us.)  Nine rows: 5 us, launch and three trips to memory.
+// Measured: 1,024 rows of 128,256 in 200 us, 5.25 TB/s read and written, 0.80 of a plain copy; what is missing is a row's blocks
+// waiting for one another between reading and writing, while the other three or so on their SM read or write.  (With a
+// meeting of the cluster, whose fence waits for all that a block has under way: 225.  Blocks that stay and take row after row:
+// 316.  Three blocks to an SM, without spills: 226.  Blocks of 512 threads: 203.)  Nine rows: 5 us, launch and three trips to
+// memory.
 #define PR_HELD 32
 
 struct alignas(16) Part { float v, sum; int i, unused; };   // the largest value, the sum of weights against it, where it is first
