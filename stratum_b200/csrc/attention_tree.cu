@@ -39,8 +39,8 @@
 // each time, one of 128 x 128 x 16 takes 64) and the exponentials' units for 1,024; the rest is one waiting for the other
 // at the ends of tiles.  Around the tiles: 3 us to read the list, 3 more to the first scores, 3 at the end of a run (the last
 // product, the outputs), 6 to add pieces up.  Measured, 8 kv heads of 4 queries, head size 128: one sequence of 32,700 tokens and
-// 61 drafted ones 53 us (134 MB of keys and values, 2.5 TB/s, 615 TFLOP/s); 64 sequences of 4,000 and 33 to 64 drafted ones 264 us
-// (3.7 TB/s, 670 TFLOP/s), 315 where the card is held back by its power limit.
+// 61 drafted ones 53 us (134 MB of keys and values, 2.5 TB/s, 615 TFLOP/s); 64 sequences of 4,000 and 33 to 64 drafted ones 256 us
+// (3.8 TB/s, 695 TFLOP/s), 302 where the card is held back by its power limit.
 // Tried without a gain: more of the exponentials as polynomials, a lock that keeps the halves' products apart, halves that start
 // half a tile apart, one thread that issues for both, a guess at the maximum before the scores are there.
 #include <math.h>
