@@ -66,7 +66,7 @@ struct TreeParams {
   float2* part_ml;                         // [G][2][rows per tile]: their (maximum, sum)
   struct TreeCut* cut;                     // [G]: what each CTA's stretch begins in
   int* status;
-  int n_tokens, n_seqs, n_q, n_kv, gs, head_dim, window, n_pages, rows_per_tile, even_tiles;
+  int n_tokens, n_seqs, n_q, n_kv, gs, head_dim, window, n_pages, rows_per_tile;
   int item_units;                          // (see the list of units)
   int out_by_16;                           // a head's row of the output begins on 16 bytes and is a multiple of them
   float scale;
@@ -84,7 +84,11 @@ static_assert(sizeof(TreeCut) == 32, "as the launcher lays them out");
 
 struct TreeSeq {                           // a sequence's share of the list
   int row0, n_new, base, len, first, n_pages, n_tiles, tile_rows;
+  int w, units;                            // units of a page (on the CUDA cores: else one), of an item
 };
+// CORES: for the CUDA cores, where time goes by rows: a tree's rows are shared out evenly among its tiles (68 as 40 and 28, not
+// as 64 and 4), and a page weighs as many units as a thread has rows of it, and two.
+template <bool CORES>
 __device__ __forceinline__ TreeSeq tree_seq(const TreeParams& P, int b) {
   TreeSeq s;
   s.row0 = min(max(__ldcg(P.seq_start + b), 0), P.n_tokens);
@@ -97,19 +101,25 @@ __device__ __forceinline__ TreeSeq tree_seq(const TreeParams& P, int b) {
   s.n_pages = pages - s.first;
   const int rows = s.n_new * P.gs;
   s.n_tiles = (rows + P.rows_per_tile - 1) / P.rows_per_tile;
-  // (where time goes by rows, a tree's rows are shared out evenly: 68 as 40 and 28, not as 64 and 4)
-  s.tile_rows = P.even_tiles && s.n_tiles > 1 ? ((rows + s.n_tiles - 1) / s.n_tiles + 7) & ~7 : P.rows_per_tile;
+  s.tile_rows = CORES && s.n_tiles > 1 ? ((rows + s.n_tiles - 1) / s.n_tiles + 7) & ~7 : P.rows_per_tile;
+  s.w = CORES ? ((min(rows, s.tile_rows) + 15) >> 4) + 2 : 1;
+  s.units = s.w * s.n_pages + P.item_units;
   return s;
 }
-// The list of units: every item (sequence, kv head, tile of rows) has one for each of its pages and a few more behind them, for
-// what an item costs besides its pages (on the tensor cores: its masked pages, which take twice as long, its outputs, and the
-// next item's first scores).  Without them a CTA whose stretch was made of short sequences took 80 us where the others took
-// 46; with 3 instead of 7 on the tensor cores 24 sequences took 58 us instead of 53, with 7 instead of 3 on the CUDA cores five
-// took 76 instead of 66.  A short list is cut among fewer CTAs, TREE_LEAST_UNITS to each: what a piece of one page saves in its
-// own time, adding up its pieces costs again.
+// The list of units: every item (sequence, kv head, tile of rows) has those of its pages (one each on the tensor cores) and a few
+// more behind them, for what an item costs besides its pages (on the tensor cores: its masked pages, its outputs, and the next
+// item's first scores).  A page is the CTA's whose stretch its first unit lies in.  Without the few more a CTA whose stretch was made
+// of short sequences took 80 us where the others took 46; with 3 instead of 7 on the tensor cores 24 sequences took 58 us instead
+// of 53; with pages of one unit on the CUDA cores, whatever their rows, five sequences took 62 instead of 56.  A short list is cut
+// among fewer CTAs, TREE_LEAST_UNITS to each (three times as many on the CUDA cores): what a piece of one page saves in its own
+// time, adding up its pieces costs again.  No stretch is then shorter than a page's units (at most 6, and a list of more than 12
+// (n - 1) units is cut among n CTAs, n > 1: 6 each at least), so every stretch that begins in front of an item's last page has a
+// page of it.
 #define TREE_LEAST_UNITS 4
+template <bool CORES>
 __device__ __forceinline__ int tree_ctas(long long T, int G) {
-  const long long n = (T + TREE_LEAST_UNITS - 1) / TREE_LEAST_UNITS;
+  const int least = CORES ? 3 * TREE_LEAST_UNITS : TREE_LEAST_UNITS;
+  const long long n = (T + least - 1) / least;
   return n < 1 ? 1 : n < G ? (int)n : G;
 }
 __device__ __forceinline__ long long tree_begin(int c, int ctas, long long T) { return c >= ctas ? T : (long long)c * T / ctas; }
@@ -123,6 +133,7 @@ struct TreeRun {
   bool pages_ok;                           // no page lies outside the pool
 };
 
+template <bool CORES>
 struct TreeCursor {
   int left;                                // units of the stretch that are still ahead
   int b, item, off;
@@ -131,33 +142,40 @@ struct TreeCursor {
   __device__ __forceinline__ void step(const TreeParams& P, int n) {
     moved = true;
     off += n; left -= n;
-    if (off < s.n_pages + P.item_units) return;
+    if (off < s.units) return;
     off = 0;
     if (++item < s.n_tiles * P.n_kv) return;
     item = 0;
-    do { b++; if (b < P.n_seqs) s = tree_seq(P, b); } while (b < P.n_seqs && s.n_tiles == 0);
+    do { b++; if (b < P.n_seqs) s = tree_seq<CORES>(P, b); } while (b < P.n_seqs && s.n_tiles == 0);
   }
   __device__ __forceinline__ void next(const TreeParams& P, TreeRun& r) {
-    if (left > 0 && off >= s.n_pages) step(P, min(s.n_pages + P.item_units - off, left));
+    int p0 = 0, n = 0;
+    while (left > 0) {
+      const int w = CORES ? s.w : 1;
+      p0 = (off + w - 1) / w;                    // the first page that begins in the stretch, and how many do
+      n = min((off + left + w - 1) / w, s.n_pages) - p0;
+      if (n > 0) break;
+      step(P, min(s.units - off, left));
+    }
     if (left <= 0) { r.n = 0; return; }
-    const int n = min(s.n_pages - off, left);
     r.s = s; r.b = b;
     r.kvh = item / s.n_tiles; r.rt = item % s.n_tiles;
-    r.page0 = s.first + off;
+    r.page0 = s.first + p0;
     r.n = n;
-    r.from_start = off == 0;
-    r.to_end = off + n == s.n_pages;
+    r.from_start = p0 == 0;
+    r.to_end = p0 + n == s.n_pages;
     r.holds_u0 = !moved;
-    step(P, n);
+    step(P, min(s.units - off, left));
   }
 };
 
 // Where CTA c begins; every thread of the block calls it.  `sums` holds a running sum per sequence for the while.
-__device__ __forceinline__ TreeCursor tree_start(const TreeParams& P, long long* sums, long long& u0_, long long& total_) {
+template <bool CORES>
+__device__ __forceinline__ TreeCursor<CORES> tree_start(const TreeParams& P, long long* sums, long long& u0_, long long& total_) {
   const int n_threads = blockDim.x, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   for (int b = threadIdx.x; b < P.n_seqs; b += n_threads) {
-    const TreeSeq s = tree_seq(P, b);
-    sums[b + 1] = (long long)(s.n_pages + P.item_units) * s.n_tiles * P.n_kv;
+    const TreeSeq s = tree_seq<CORES>(P, b);
+    sums[b + 1] = (long long)s.units * s.n_tiles * P.n_kv;
   }
   if (threadIdx.x == 0) sums[0] = 0;
   __syncthreads();
@@ -176,9 +194,9 @@ __device__ __forceinline__ TreeCursor tree_start(const TreeParams& P, long long*
     }
   }
   __syncthreads();
-  TreeCursor t;
+  TreeCursor<CORES> t;
   const long long T = sums[P.n_seqs];
-  const int c = blockIdx.x, ctas = tree_ctas(T, gridDim.x);
+  const int c = blockIdx.x, ctas = tree_ctas<CORES>(T, gridDim.x);
   const long long u0 = tree_begin(c, ctas, T);
   t.left = (int)(tree_begin(c + 1, ctas, T) - u0);
   t.b = t.item = t.off = 0;
@@ -190,9 +208,9 @@ __device__ __forceinline__ TreeCursor tree_start(const TreeParams& P, long long*
       const int mid = (lo + hi + 1) >> 1;
       if (sums[mid] <= u0) lo = mid; else hi = mid - 1;
     }
-    t.s = tree_seq(P, lo);
+    t.s = tree_seq<CORES>(P, lo);
     const long long r = u0 - sums[lo];
-    const int per = t.s.n_pages + P.item_units;
+    const int per = t.s.units;
     t.b = lo; t.item = (int)(r / per); t.off = (int)(r % per);
   }
   return t;
@@ -204,14 +222,16 @@ __device__ __forceinline__ int tree_cta_of(long long u, int ctas, long long T) {
   return c;
 }
 // One thread, with the cursor as tree_start left it: what the merge is to know about the cut in front of this stretch.
-__device__ __forceinline__ void tree_cut(const TreeParams& P, const TreeCursor& t, long long u0, long long T) {
+template <bool CORES>
+__device__ __forceinline__ void tree_cut(const TreeParams& P, const TreeCursor<CORES>& t, long long u0, long long T) {
   TreeCut cut;
   cut.first = cut.cuts = cut.late = cut.kvh = cut.flat0 = cut.n_rows = 0;
-  if (t.left > 0 && t.off > 0 && t.off < t.s.n_pages) {
+  const int last = (CORES ? t.s.w : 1) * (t.s.n_pages - 1);      // where the item's last page begins
+  if (t.left > 0 && t.off > 0 && t.off <= last) {
     const long long begin = u0 - t.off;
-    const int ctas = tree_ctas(T, gridDim.x), rt = t.item % t.s.n_tiles;
+    const int ctas = tree_ctas<CORES>(T, gridDim.x), rt = t.item % t.s.n_tiles;
     cut.first = tree_cta_of(begin, ctas, T);
-    cut.cuts = tree_cta_of(begin + t.s.n_pages - 1, ctas, T) - cut.first;
+    cut.cuts = tree_cta_of(begin + last, ctas, T) - cut.first;
     cut.late = tree_begin(cut.first, ctas, T) != begin;
     cut.kvh = t.item / t.s.n_tiles;
     cut.flat0 = t.s.row0 * P.gs + rt * t.s.tile_rows;
@@ -472,7 +492,7 @@ attention_tree_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
   }
   pdl_wait();                                           // everything below may read what the kernel before this one wrote
   long long u0, total;
-  TreeCursor cur = tree_start(P, reinterpret_cast<long long*>(S.k), u0, total);
+  TreeCursor<false> cur = tree_start<false>(P, reinterpret_cast<long long*>(S.k), u0, total);
   fence_async_shared();                                 // the sums lie where TMA will write
   tc_fence_before();
   __syncthreads();
@@ -892,7 +912,7 @@ attention_tree_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
     // A run is described here while the ones before it are worked on: what it takes from memory would otherwise stand
     // between two runs of every other warp.  And the values of masked tiles are looked through as they come, ahead of the
     // softmax warps (with these doing it themselves a masked tile took 3 us where the others took 1.2).
-    const TreeCursor begin = cur;
+    const TreeCursor<false> begin = cur;
     int described = 0, r = 0, t = 0;                       // runs described, the run and the tile of it that is next to be looked at
     uint32_t it0 = 0, looks[2] = {0, 0}, idle = 0;         // tiles in front of that run, masked tiles of the halves
     bool more = true;
@@ -980,7 +1000,7 @@ attention_tree_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
 // the same number of them, and the loops are made for 1 to R rows a thread, so that a tree of 28 rows pays for 32 and not for
 // 64.  float32 pages come by cp.async: the next keys while this page's values are summed, the next values while the next
 // scores are computed.  Measured: 5 sequences of 300 to 2,500 tokens and 3 to 17 drafted ones, 8 kv heads of 4 queries, head size
-// 64: 62 us, of which 5 to the first keys, 7 to 8 a page where two blocks share an SM (the multiplications alone would be 4), four
+// 64: 56 us, of which 5 to the first keys, 7 to 8 a page where two blocks share an SM (the multiplications alone would be 4), four
 // or five pages a block.
 #define TG_THREADS 256
 
@@ -1014,7 +1034,7 @@ attention_tree_simple_kernel(const TreeParams P) {
   float* ps = vs + TR_KEYS * hp;                   // [ROWS][PK]
   pdl_wait();
   long long u0, total;
-  TreeCursor cur = tree_start(P, reinterpret_cast<long long*>(tg_smem), u0, total);
+  TreeCursor<true> cur = tree_start<true>(P, reinterpret_cast<long long*>(tg_smem), u0, total);
   if (threadIdx.x == TG_THREADS - 1) tree_cut(P, cur, u0, total);
   const int tid = threadIdx.x, ty = tid >> 4, tx = tid & 15;
   const float scale_log2 = P.scale * 1.4426950408889634f;
@@ -1415,8 +1435,7 @@ STRATUM_EXPORT int stratum_attention_tree(const TreeCall* call, cudaStream_t str
   P.q = a.q; P.ldq = ldq; P.k_cache = a.k_cache; P.v_cache = a.v_cache; P.out = a.out; P.ldo = ldo;
   P.part_o = (float4*)a.part_o; P.part_ml = (float2*)a.part_ml; P.cut = (TreeCut*)a.cut; P.status = (int*)a.status;
   P.n_tokens = n_tokens; P.n_seqs = n_seqs; P.n_q = n_q; P.n_kv = n_kv; P.gs = gs; P.head_dim = head_dim;
-  P.even_tiles = !tensor;
-  P.item_units = tensor ? 7 : 3;
+  P.item_units = tensor ? 7 : 8;                 // (see the list of units)
   P.out_by_16 = head_dim % 8 == 0 && ldo % 8 == 0 && ((uintptr_t)a.out & 15) == 0;
   P.window = a.window; P.n_pages = (int)n_pages; P.scale = a.scale;
   const int G = stratum_attention_tree_ctas(tensor, many, head_dim);
