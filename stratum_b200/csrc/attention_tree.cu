@@ -1400,7 +1400,7 @@ STRATUM_EXPORT int stratum_attention_tree_slot_rows(int tensor, int many) { retu
 STRATUM_EXPORT int stratum_attention_tree_ctas(int tensor, int many, int head_dim) {
   if (tensor) return sm_count();
   const int most = head_dim <= 64 ? (many ? 2 : 3) : head_dim <= 128 ? (many ? 1 : 2) : 1;     // (by registers: see the kernel)
-  const int room = (int)((size_t)(227 * 1024) / (simple_smem(head_dim, many ? 64 : 32, 0) + 3072));
+  const int room = (int)((size_t)(227 * 1024) / (simple_smem(head_dim, many ? 64 : 32, 0) + 3 * 1024));
   return sm_count() * (room < 1 ? 1 : room < most ? room : most);
 }
 

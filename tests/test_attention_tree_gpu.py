@@ -243,3 +243,25 @@ def test_stretches_of_masked_pages(hd, new):
             page, row = b.place(s, last)
             b.k[page, :, row:], b.v[page, :, row:] = np.inf, np.nan
     check(b, torch.bfloat16, run_tree(b, torch.bfloat16))
+
+
+@pytest.mark.parametrize("dtype", ["bfloat16", "float32"])
+def test_sequences_without_drafted_tokens(dtype):
+    """A padded batch: sequences without rows in front, between and behind change nothing, and a batch of nothing else writes nothing."""
+    from stratum_b200 import kernels as K
+    dev = lambda a, dt=None: torch.from_numpy(np.ascontiguousarray(a)).to(device="cuda", dtype=dt)      # noqa: E731
+    b = TreeBatch(12, [700, 90], [9, 20], 8, 2, 64).round_to(DT[dtype])
+    held = (dev(b.q, DT[dtype]), dev(b.k, DT[dtype]), dev(b.v, DT[dtype]), dev(np.array(b.pos, np.int32)), dev(b.mask()))
+
+    def call(start, length, table):
+        out = torch.full((29, 512), 7.0, dtype=DT[dtype], device="cuda")
+        K.attention_tree(*held, dev(np.array(start, np.int32)), dev(np.array(length, np.int32)), dev(np.array(table, np.int32)), out, 8, 2, 64,
+                         PAGE, 0, b.scale, 20)
+        return out
+
+    t, no = b.table.tolist(), [-1] * b.table.shape[1]
+    out = call([0, 0, 0, 9, 9, 29, 29, 29], [0, 500, b.length[0], 0, b.length[1], 64, 0], [no, t[0], t[0], no, t[1], no, no])
+    check(b, DT[dtype], out)
+    assert (call([0, 0, 0, 0], [0, 700, 5], [no, t[0], t[1]]) == 7.0).all()
+    assert (call([29, 29], [64], [t[0]]) == 7.0).all()
+    K.check_status()
