@@ -1828,8 +1828,8 @@ def verify_drafts(target: torch.Tensor, draft: Optional[torch.Tensor], tokens: t
 
     path (int32 [rows]): in place j behind seq_start[s] the number of the node kept j-th, 0 (the first node) in front, -1
     behind the last.  n_kept (int32 [seqs]): drafts kept; next_ids (int32 [seqs]): the next token (0 where the target's row
-    has no weight, -1 for a sequence without nodes).  Rows behind the last sequence are left as they were.  At most
-    VERIFY_MAX_NODES nodes of a sequence are looked at."""
+    has no weight, -1 for a sequence without nodes); all three are memory of their own.  Rows behind the last sequence are
+    left as they were.  At most VERIFY_MAX_NODES nodes of a sequence are looked at."""
     _one_device("verify_drafts", target, draft, tokens, parents, seq_start, uniform, path, n_kept, next_ids)
     _rows_of(target, "target")
     T, V = target.shape
@@ -1848,11 +1848,13 @@ def verify_drafts(target: torch.Tensor, draft: Optional[torch.Tensor], tokens: t
         raise KernelError(f"verify_drafts: {T} rows are more than {VERIFY_MAX_NODES} for each of {B} sequences")
     if B == 0:
         return
+    read = (tokens.data_ptr(), parents.data_ptr(), seq_start.data_ptr(), uniform.data_ptr())
+    written = (path.data_ptr(), n_kept.data_ptr(), next_ids.data_ptr())
+    if T > 0 and (written[0] in read or written[1] in read or written[2] in read or len(set(written)) < 3):
+        raise KernelError("verify_drafts: path, n_kept and next_ids are memory of their own")
     f = _fn("draft_verify", "stratum_verify_drafts", [c_char_p, c_void_p])
-    _check(f(_VERIFY_CALL.pack(target.data_ptr(), 0 if draft is None else draft.data_ptr(), tokens.data_ptr(), parents.data_ptr(),
-                               seq_start.data_ptr(), uniform.data_ptr(), path.data_ptr(), n_kept.data_ptr(), next_ids.data_ptr(),
-                               target.stride()[0], 0 if draft is None else draft.stride()[0], T, B, V, 0), _stream()),
-           "verify_drafts")
+    _check(f(_VERIFY_CALL.pack(target.data_ptr(), 0 if draft is None else draft.data_ptr(), *read, *written, target.stride()[0],
+                               0 if draft is None else draft.stride()[0], T, B, V, 0), _stream()), "verify_drafts")
 
 
 def _storage(k: torch.Tensor, v: Optional[torch.Tensor], what: str) -> None:

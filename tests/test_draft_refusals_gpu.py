@@ -125,6 +125,9 @@ def test_verify_drafts():
                ("uniform", args["uniform"][:4]), ("seq_start", i32(0, 5)), ("seq_start", args["seq_start"].long()), ("path", z(4)),
                ("path", z(5).long()), ("n_kept", z(3)), ("n_kept", z(2).long()), ("next_ids", z(3)), ("next_ids", z(2).float())]
     refused(K.verify_drafts, args, changes, list(args), ["path", "n_kept", "next_ids"])
+    for name, other in (("path", "tokens"), ("path", "parents"), ("next_ids", "n_kept")):        # what is written is also read, or written twice
+        with pytest.raises(K.KernelError):
+            K.verify_drafts(**{**args, name: args[other]})
     n = K.VERIFY_MAX_NODES + 1
     with pytest.raises(K.KernelError):
         K.verify_drafts(torch.zeros(n, 4, device="cuda"), None, z(n), z(n), i32(0, n), torch.zeros(n, device="cuda"), z(n), z(1), z(1))
