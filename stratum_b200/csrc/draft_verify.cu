@@ -231,9 +231,21 @@ token_probs_kernel(const float* logits, long long ld, const float* temperature, 
 }
 
 // logits float32 [rows][ld], temperature float32 [rows], out float32 [rows][ldo]; out may be logits (the same rows at the same
-// distance).
-STRATUM_EXPORT int stratum_token_probs(const float* logits, long long ld, const float* temperature, float* out, long long ldo,
-                                       int rows, int vocab, int* status, cudaStream_t stream) {
+// distance).  As the launcher packs them.
+struct ProbsCall {
+  const float *logits, *temperature;
+  float* out;
+  int* status;
+  long long ld, ldo;
+  int rows, vocab;
+};
+
+STRATUM_EXPORT int stratum_token_probs(const ProbsCall* call, cudaStream_t stream) {
+  const float *logits = call->logits, *temperature = call->temperature;
+  float* out = call->out;
+  int* status = call->status;
+  const long long ld = call->ld, ldo = call->ldo;
+  const int rows = call->rows, vocab = call->vocab;
   if (rows <= 0 || vocab <= 0) return 0;
   if (rows > (1 << 26) || vocab > (1 << 30)) return STRATUM_ERR_LIMIT;
   const bool four = (((uintptr_t)logits | (uintptr_t)out) & 15) == 0 && (rows == 1 || (ld % 4 == 0 && ldo % 4 == 0));

@@ -1669,14 +1669,25 @@ def attention_stream(qkv: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Te
 
 
 # ------------------------------------------------------------------ drafted tokens
+# (a tensor on the device says that torch has been there: its own current_device() asks that first)
+_current_device = getattr(torch._C, "_cuda_getDevice", None) or torch.cuda.current_device
+
+
 def _one_device(what: str, *tensors: Optional[torch.Tensor]) -> None:
     """All on the current device, which is also the one this process's launches go to (see _stream, status_word)."""
-    devices = {t.get_device() for t in tensors if t is not None}
-    if -1 in devices:
-        raise KernelError(f"{what}: tensors must live on a CUDA device (no CPU path exists)")
-    here = torch.cuda.current_device()
-    if devices != {here}:
-        raise KernelError(f"{what}: tensors on devices {sorted(devices)}, the current one is cuda:{here}")
+    there = tensors[0].get_device()
+    same = True
+    for t in tensors:
+        if t is not None and t.get_device() != there:
+            same = False
+    if not same or there < 0:
+        devices = {t.get_device() for t in tensors if t is not None}
+        if -1 in devices:
+            raise KernelError(f"{what}: tensors must live on a CUDA device (no CPU path exists)")
+        raise KernelError(f"{what}: tensors on devices {sorted(devices)}")
+    here = _current_device()
+    if there != here:
+        raise KernelError(f"{what}: tensors on cuda:{there}, the current device is cuda:{here}")
     if _device_index is not None and _device_index != here:
         raise KernelError(f"{what}: this process launches on cuda:{_device_index}, the current device is cuda:{here}")
 
@@ -1699,8 +1710,9 @@ def _meet(a: int, step_a: int, width_a: int, b: int, step_b: int, width_b: int, 
     return step_a != step_b or apart < width_a or step_a - apart < width_b
 
 
-# Mirrors of struct TreeCall in csrc/attention_tree.cu, VerifyParams in csrc/draft_verify.cu and KeepRows in csrc/cache_move.cu.
-# (One packed argument: converting thirty of them one by one took a fifth of a short call.)
+# Mirrors of struct TreeCall in csrc/attention_tree.cu, ProbsCall and VerifyParams in csrc/draft_verify.cu and KeepRows in
+# csrc/cache_move.cu.  (One packed argument: converting thirty of them one by one took a fifth of a short call.)
+_PROBS_CALL = struct.Struct("<6q2i")
 _TREE_CALL, _VERIFY_CALL, _KEEP_CALL = struct.Struct("<14q15if"), struct.Struct("<11q4i"), struct.Struct("<8q10i")
 _tree_plans: dict = {}         # (tensor cores, many rows, head size) -> CTAs, scratch rows of a CTA's slot
 
@@ -1777,14 +1789,18 @@ def attention_tree(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor
     count_launches(1)          # the merge kernel
 
 
-def _rows_of(t: torch.Tensor, name: str, rows: Optional[int] = None) -> None:
-    """A float32 matrix with contiguous rows (any distance between them)."""
-    if t.dtype != torch.float32 or t.dim() != 2:
-        raise KernelError(f"{name} must be a float32 matrix, is {t.dtype} with {t.dim()} dimensions")
-    if (t.shape[1] > 1 and t.stride(1) != 1) or (t.shape[0] > 1 and t.stride(0) < t.shape[1]):
+def _rows_of(t: torch.Tensor, name: str, rows: Optional[int] = None):
+    """A float32 matrix with contiguous rows (any distance between them): rows, their length, their distance."""
+    shape = t.shape
+    if t.dtype != torch.float32 or len(shape) != 2:
+        raise KernelError(f"{name} must be a float32 matrix, is {t.dtype} with {len(shape)} dimensions")
+    R, V = shape
+    step, one = t.stride()
+    if (V > 1 and one != 1) or (R > 1 and step < V):
         raise KernelError(f"{name}: rows must be contiguous and not overlap")
-    if rows is not None and t.shape[0] != rows:
-        raise KernelError(f"{name} must have {rows} rows, has {t.shape[0]}")
+    if rows is not None and R != rows:
+        raise KernelError(f"{name} must have {rows} rows, has {R}")
+    return R, V, step
 
 
 def token_probs(logits: torch.Tensor, temperature: torch.Tensor, out: torch.Tensor) -> None:
@@ -1793,21 +1809,20 @@ def token_probs(logits: torch.Tensor, temperature: torch.Tensor, out: torch.Tens
     float32 [rows].  A logit that is no number counts as -inf, infinite ones share the row, a row of nothing but -inf
     gives zeros."""
     _one_device("token_probs", logits, temperature, out)
-    _rows_of(logits, "logits"); _rows_of(out, "out", logits.shape[0])
-    R, V = logits.shape
-    if out.shape[1] != V:
+    R, V, ld = _rows_of(logits, "logits")
+    _, width, ldo = _rows_of(out, "out", R)
+    if width != V:
         raise KernelError("token_probs: out and logits disagree")
     _shaped(temperature, "temperature", torch.float32, (R,))
     if R == 0 or V == 0:
         return
-    same = out.data_ptr() == logits.data_ptr() and (R == 1 or out.stride(0) == logits.stride(0))
-    if not same:
-        if _meet(logits.data_ptr(), 4 * (logits.stride(0) if R > 1 else V), 4 * V, out.data_ptr(), 4 * (out.stride(0) if R > 1 else V), 4 * V, R):
-            raise KernelError("token_probs: out is logits itself or memory of its own")
-    f = _fn("draft_verify", "stratum_token_probs",
-            [c_void_p, ctypes.c_longlong, c_void_p, c_void_p, ctypes.c_longlong, c_int, c_int, c_void_p, c_void_p])
-    _check(f(logits.data_ptr(), logits.stride()[0], temperature.data_ptr(), out.data_ptr(), out.stride()[0], R, V,
-             status_word().data_ptr(), _stream()), "token_probs")
+    if R == 1:
+        ld = ldo = V                                         # (of a single row it means nothing)
+    at, to = logits.data_ptr(), out.data_ptr()
+    if (at != to or ld != ldo) and _meet(at, 4 * ld, 4 * V, to, 4 * ldo, 4 * V, R):
+        raise KernelError("token_probs: out is logits itself or memory of its own")
+    f = _fn("draft_verify", "stratum_token_probs", [c_char_p, c_void_p])
+    _check(f(_PROBS_CALL.pack(at, temperature.data_ptr(), to, status_word().data_ptr(), ld, ldo, R, V), _stream()), "token_probs")
 
 
 VERIFY_MAX_NODES = 1024            # of a sequence
@@ -1831,15 +1846,14 @@ def verify_drafts(target: torch.Tensor, draft: Optional[torch.Tensor], tokens: t
     has no weight, -1 for a sequence without nodes); all three are memory of their own.  Rows behind the last sequence are
     left as they were.  At most VERIFY_MAX_NODES nodes of a sequence are looked at."""
     _one_device("verify_drafts", target, draft, tokens, parents, seq_start, uniform, path, n_kept, next_ids)
-    _rows_of(target, "target")
-    T, V = target.shape
+    T, V, ldt = _rows_of(target, "target")
+    ldd = 0
     if draft is not None:
-        _rows_of(draft, "draft", T)
-        if draft.shape[1] != V:
+        _, width, ldd = _rows_of(draft, "draft", T)
+        if width != V:
             raise KernelError("verify_drafts: draft and target disagree")
     B = n_kept.numel()
-    for t, name in ((tokens, "tokens"), (parents, "parents"), (path, "path")):
-        _shaped(t, name, torch.int32, (T,))
+    _shaped(tokens, "tokens", torch.int32, (T,)); _shaped(parents, "parents", torch.int32, (T,)); _shaped(path, "path", torch.int32, (T,))
     _shaped(uniform, "uniform", torch.float32, (T,)); _shaped(seq_start, "seq_start", torch.int32, (B + 1,))
     _shaped(n_kept, "n_kept", torch.int32, (B,)); _shaped(next_ids, "next_ids", torch.int32, (B,))
     if V < 1:
@@ -1853,8 +1867,8 @@ def verify_drafts(target: torch.Tensor, draft: Optional[torch.Tensor], tokens: t
     if T > 0 and (written[0] in read or written[1] in read or written[2] in read or len(set(written)) < 3):
         raise KernelError("verify_drafts: path, n_kept and next_ids are memory of their own")
     f = _fn("draft_verify", "stratum_verify_drafts", [c_char_p, c_void_p])
-    _check(f(_VERIFY_CALL.pack(target.data_ptr(), 0 if draft is None else draft.data_ptr(), *read, *written, target.stride()[0],
-                               0 if draft is None else draft.stride()[0], T, B, V, 0), _stream()), "verify_drafts")
+    _check(f(_VERIFY_CALL.pack(target.data_ptr(), 0 if draft is None else draft.data_ptr(), *read, *written, ldt, ldd, T,
+                               B, V, 0), _stream()), "verify_drafts")
 
 
 def _storage(k: torch.Tensor, v: Optional[torch.Tensor], what: str) -> None:
