@@ -1739,21 +1739,25 @@ def attention_tree(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor
     dt = q.dtype
     code = dtype_code(dt)
     _one_device("attention_tree", q, k_cache, v_cache, token_pos, tree_mask, seq_start, seq_len, block_table, out)
-    _shaped(k_cache, "k_cache", dt); _shaped(v_cache, "v_cache", dt, k_cache.shape)
-    if k_cache.dim() != 4 or tuple(k_cache.shape[1:]) != (n_kv, page_tokens, head_dim) or n_q < 1 or n_q % max(n_kv, 1):
+    cache_shape = k_cache.shape
+    _shaped(k_cache, "k_cache", dt); _shaped(v_cache, "v_cache", dt, cache_shape)
+    if len(cache_shape) != 4 or cache_shape[1:] != (n_kv, page_tokens, head_dim) or n_q < 1 or n_q % max(n_kv, 1):
         raise KernelError("attention_tree: the caches are [pages, n_kv, page_tokens, head_dim], n_q a multiple of n_kv")
     T, B = q.shape[0], seq_len.numel()
     width = n_q * head_dim
+    steps = []
     for t, name in ((q, "q"), (out, "out")):
         shape, stride = t.shape, t.stride()
         if len(shape) != 2 or t.dtype != dt or shape[0] != T or shape[1] < width or stride[1] != 1 or (T > 1 and stride[0] < width):
             raise KernelError(f"attention_tree: {name} must be [tokens, >= n_q * head_dim] of the cache's dtype, rows contiguous")
+        steps.append(stride[0] if T > 1 else width)          # (of a single row it means nothing)
     _shaped(token_pos, "token_pos", torch.int32, (T,)); _shaped(seq_len, "seq_len", torch.int32, (B,))
     _shaped(seq_start, "seq_start", torch.int32, (B + 1,)); _shaped(tree_mask, "tree_mask", torch.int64)
     _shaped(block_table, "block_table", torch.int32)
-    if tree_mask.dim() != 2 or tree_mask.shape[0] != T or (T > 0 and tree_mask.shape[1] < 1):
+    mask_shape, table_shape = tree_mask.shape, block_table.shape
+    if len(mask_shape) != 2 or mask_shape[0] != T or (T > 0 and mask_shape[1] < 1):
         raise KernelError("attention_tree: tree_mask is [tokens, words]")
-    if block_table.dim() != 2 or block_table.shape[0] != B or (B > 0 and block_table.shape[1] < 1):
+    if len(table_shape) != 2 or table_shape[0] != B or (B > 0 and table_shape[1] < 1):
         raise KernelError("attention_tree: block_table is [sequences, pages]")
     if window < 0 or max_new < 0:
         raise KernelError("attention_tree: window and max_new are not negative")
@@ -1761,7 +1765,7 @@ def attention_tree(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor
         return
     group = n_q // n_kv
     at_q, at_k, at_v, at_out = q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), out.data_ptr()
-    ldq, ldo = (q.stride()[0], out.stride()[0]) if T > 1 else (width, width)          # (of a single row it means nothing)
+    ldq, ldo = steps
     size = q.element_size()
     if _meet(at_q, ldq * size, width * size, at_out, ldo * size, width * size, T):
         raise KernelError("attention_tree: out is memory of its own, not q's")
@@ -1778,14 +1782,15 @@ def attention_tree(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor
                                    int(lib.stratum_attention_tree_slot_rows(int(tensor), int(many))))
     ctas, slots = plan[0], 2 * plan[0] * plan[1]
     # (scratch of this call's own: calls on several streams, and captured ones, do not meet in it)
-    scratch = torch.empty(slots * ((head_dim + 3) // 4 * 4 + 2) + 8 * ctas, dtype=torch.float32, device=q.device)
+    padded = (head_dim + 3) // 4 * 4
+    scratch = q.new_empty((slots * (padded + 2) + 8 * ctas) * (4 // size))
     at = scratch.data_ptr()
-    part_ml = at + 4 * slots * ((head_dim + 3) // 4 * 4)
+    part_ml = at + 4 * slots * padded
     f = _fn("attention_tree", "stratum_attention_tree", [c_char_p, c_void_p])
     _check(f(_TREE_CALL.pack(at_q, at_k, at_v, token_pos.data_ptr(), tree_mask.data_ptr(), seq_start.data_ptr(), seq_len.data_ptr(),
                              block_table.data_ptr(), at_out, at, part_ml, part_ml + 8 * slots, status_word().data_ptr(),
-                             k_cache.shape[0], code, ldq, ldo, tree_mask.shape[1], block_table.stride()[0], block_table.shape[1],
-                             T, B, n_q, n_kv, head_dim, page_tokens, window, tensor, many, scale), _stream()), "attention_tree")
+                             cache_shape[0], code, ldq, ldo, mask_shape[1], table_shape[1], table_shape[1], T, B, n_q, n_kv,
+                             head_dim, page_tokens, window, tensor, many, scale), _stream()), "attention_tree")
     count_launches(1)          # the merge kernel
 
 
