@@ -10,7 +10,9 @@
 //   drawn from a draft distribution q (that of the parent's row):  taken if u mass q(x) < d(x);  else  d = max(d - mass q, 0)
 //     and mass = sum d, unless nothing would be left (after several rejections d = max(p - cover q, 0) with the sum of the
 //     masses so far for `cover`, since max(max(a, 0) - b, 0) = max(a - b, 0));
-//   looked up, without a distribution:  taken if u mass < d(x);  else  mass = max(mass - d(x), 0) and d(x) = 0.
+//   looked up, without a distribution:  taken if u mass < d(x);  else  mass = max(mass - d(x), 0) and d(x) = 0, unless nothing
+//     would be left: a row of rounded probabilities adds up to a little less than one, so that children that hold all of it
+//     may all be refused.  The last one with any weight is then what there is to draw.
 // A child that is taken is the next node.  Where none is, the next token is drawn from d: the first index whose running sum
 // is over u_0 sum(d), u_0 being the first node's number (the last index with any weight if rounding leaves none).  Whoever
 // drafts, the kept tokens and the one behind them are distributed as the target's own draws
@@ -299,6 +301,7 @@ struct VdSmem {
   int zeroed[VD_NODES];                    // ids the row has lost (looked up)
   double mass, cover;                      // (cover: 0 until the row has been lowered)
   int node, depth, n_zeroed, want;
+  int last_lost;                           // the last id with any weight that the row has lost (looked up; 0: none)
   double all[16];                          // the blocks' sums, running
 };
 
@@ -337,7 +340,7 @@ verify_drafts_kernel(const VerifyParams P) {
     }
     S.parent[i] = parent; S.token[i] = token; S.u[i] = __ldcg(P.uniform + a + i); S.p[i] = p; S.q[i] = q;
   }
-  if (tid == 0) { S.mass = 1.0; S.cover = 0.0; S.node = 0; S.depth = 0; S.n_zeroed = 0; }
+  if (tid == 0) { S.mass = 1.0; S.cover = 0.0; S.node = 0; S.depth = 0; S.n_zeroed = 0; S.last_lost = 0; }
   if (c == 0) for (int i = tid; i < n; i += VD_THREADS) P.path[a + i] = i == 0 ? 0 : -1;
   __syncthreads();
   cluster_all_begun();
@@ -450,14 +453,18 @@ verify_drafts_kernel(const VerifyParams P) {
           node = child; depth++;                   // (its children come behind it)
           if (lane == 0) {
             if (c == 0) P.path[a + depth] = child;
-            S.mass = 1.0; S.cover = 0.0; S.n_zeroed = 0;
+            S.mass = 1.0; S.cover = 0.0; S.n_zeroed = 0; S.last_lost = 0;
           }
           summed = false;
         } else if (P.draft) {
           want = 1;
         } else {
           w *= 1.0 / VD_SCALE;
-          if (lane == 0) { S.mass = mass - w > 0.0 ? mass - w : 0.0; S.zeroed[S.n_zeroed++] = token; }
+          if (lane == 0) {
+            S.mass = mass - w > 0.0 ? mass - w : 0.0;
+            S.zeroed[S.n_zeroed++] = token;
+            if (w > 0.0) S.last_lost = token;
+          }
           summed = false;
         }
         __syncwarp();
@@ -505,7 +512,7 @@ verify_drafts_kernel(const VerifyParams P) {
   const int block = find(lane < C ? S.all[lane] : 0.0, lane > 0 && lane < C ? S.all[lane - 1] : 0.0, C, crossed);
   if (c == 0 && tid == 0) {
     P.kept[b] = S.depth;
-    if (!(total > 0.0)) P.picked[b] = 0;           // nothing to draw from
+    if (!(total > 0.0)) P.picked[b] = S.last_lost; // nothing left to draw from: what was lost last, or 0
   }
   if (block != c || !(total > 0.0)) return;        // (the same in the whole block; nothing of another block is touched any more)
   const double front = c > 0 ? S.all[c - 1] : 0.0;

@@ -1847,9 +1847,9 @@ def verify_drafts(target: torch.Tensor, draft: Optional[torch.Tensor], tokens: t
     distributed as the target's own.
 
     path (int32 [rows]): in place j behind seq_start[s] the number of the node kept j-th, 0 (the first node) in front, -1
-    behind the last.  n_kept (int32 [seqs]): drafts kept; next_ids (int32 [seqs]): the next token (0 where the target's row
-    has no weight, -1 for a sequence without nodes); all three are memory of their own.  Rows behind the last sequence are
-    left as they were.  At most VERIFY_MAX_NODES nodes of a sequence are looked at."""
+    behind the last.  n_kept (int32 [seqs]): drafts kept; next_ids (int32 [seqs]): the next token (always one with weight in
+    the target's row; 0 where that has none, -1 for a sequence without nodes); all three are memory of their own.  Rows behind
+    the last sequence are left as they were.  At most VERIFY_MAX_NODES nodes of a sequence are looked at."""
     _one_device("verify_drafts", target, draft, tokens, parents, seq_start, uniform, path, n_kept, next_ids)
     T, V, ldt = _rows_of(target, "target")
     ldd = 0
