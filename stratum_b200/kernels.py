@@ -1710,6 +1710,17 @@ def _meet(a: int, step_a: int, width_a: int, b: int, step_b: int, width_b: int, 
     return step_a != step_b or apart < width_a or step_a - apart < width_b
 
 
+def _in_rows(lo: int, hi: int, at: int, step: int, width: int, rows: int) -> bool:
+    """Whether the bytes lo .. hi have any in common with the rows of a matrix (its address, its rows' distance and width in
+    bytes); what lies between two rows has none."""
+    if rows < 1 or hi <= lo or hi <= at or lo >= at + (rows - 1) * step + width:
+        return False
+    if rows == 1 or lo < at:
+        return True
+    off = (lo - at) % step
+    return off < width or off + hi - lo > step
+
+
 # Mirrors of struct TreeCall in csrc/attention_tree.cu, ProbsCall and VerifyParams in csrc/draft_verify.cu and KeepRows in
 # csrc/cache_move.cu.  (One packed argument: converting thirty of them one by one took a fifth of a short call.)
 _PROBS_CALL = struct.Struct("<6q2i")
@@ -1867,13 +1878,20 @@ def verify_drafts(target: torch.Tensor, draft: Optional[torch.Tensor], tokens: t
         raise KernelError(f"verify_drafts: {T} rows are more than {VERIFY_MAX_NODES} for each of {B} sequences")
     if B == 0:
         return
+    at_target, at_draft = target.data_ptr(), 0 if draft is None else draft.data_ptr()
     read = (tokens.data_ptr(), parents.data_ptr(), seq_start.data_ptr(), uniform.data_ptr())
     written = (path.data_ptr(), n_kept.data_ptr(), next_ids.data_ptr())
-    if T > 0 and (written[0] in read or written[1] in read or written[2] in read or len(set(written)) < 3):
-        raise KernelError("verify_drafts: path, n_kept and next_ids are memory of their own")
+    ends = (written[0] + 4 * T, written[1] + 4 * B, written[2] + 4 * B)
+    taken = [(read[0], read[0] + 4 * T), (read[1], read[1] + 4 * T), (read[2], read[2] + 4 * B + 4), (read[3], read[3] + 4 * T)]
+    for lo, hi in zip(written, ends):                        # (empty ones begin nowhere and meet nothing)
+        for a, b in taken:
+            if lo < b and a < hi and lo < hi and a < b:
+                raise KernelError("verify_drafts: path, n_kept and next_ids are memory of their own")
+        if _in_rows(lo, hi, at_target, 4 * ldt, 4 * V, T) or (at_draft and _in_rows(lo, hi, at_draft, 4 * ldd, 4 * V, T)):
+            raise KernelError("verify_drafts: path, n_kept and next_ids are memory of their own")
+        taken.append((lo, hi))
     f = _fn("draft_verify", "stratum_verify_drafts", [c_char_p, c_void_p])
-    _check(f(_VERIFY_CALL.pack(target.data_ptr(), 0 if draft is None else draft.data_ptr(), *read, *written, ldt, ldd, T,
-                               B, V, 0), _stream()), "verify_drafts")
+    _check(f(_VERIFY_CALL.pack(at_target, at_draft, *read, *written, ldt, ldd, T, B, V, 0), _stream()), "verify_drafts")
 
 
 def _storage(k: torch.Tensor, v: Optional[torch.Tensor], what: str) -> None:

@@ -1,0 +1,94 @@
+"""Memory that a call of drafted decoding would write while it is read: refused before anything runs.  (No GPU: the device check and
+the launch are replaced.)"""
+import pytest
+import torch
+
+from stratum_b200 import kernels as K
+
+
+@pytest.fixture
+def launches(monkeypatch):
+    """The calls that would have been launched."""
+    seen = []
+    monkeypatch.setattr(K, "_one_device", lambda *a: None)
+    monkeypatch.setattr(K, "_stream", lambda: 0)
+    monkeypatch.setattr(K, "status_word", lambda: torch.zeros(1, dtype=torch.int32))
+    monkeypatch.setattr(K, "_fn", lambda lib, name, types: lambda *a: seen.append(name) or 0)
+    return seen
+
+
+def i32(n):
+    return torch.zeros(n, dtype=torch.int32)
+
+
+def verify_args(T=6, B=2, V=40):
+    return dict(target=torch.zeros(T, V), draft=torch.zeros(T, V), tokens=i32(T), parents=i32(T), seq_start=i32(B + 1), uniform=torch.zeros(T),
+                path=i32(T), n_kept=i32(B), next_ids=i32(B))
+
+
+@pytest.mark.parametrize("shift", [-5, -1, 0, 1, 5])
+@pytest.mark.parametrize("read", ["tokens", "parents", "uniform", "seq_start"])
+@pytest.mark.parametrize("written", ["path", "n_kept", "next_ids"])
+def test_verify_outputs_that_meet_an_input(launches, written, read, shift):
+    args = verify_args()
+    n, m = args[read].numel(), args[written].numel()
+    buf = torch.zeros(40, dtype=args[read].dtype)
+    args[read] = buf[10:10 + n]
+    args[written] = buf.view(torch.int32)[10 + shift:10 + shift + m]
+    meets = shift < n and shift + m > 0
+    if meets:
+        with pytest.raises(K.KernelError, match="memory of their own"):
+            K.verify_drafts(**args)
+    else:
+        K.verify_drafts(**args)
+    assert launches == ([] if meets else ["stratum_verify_drafts"])
+
+
+@pytest.mark.parametrize("T", [6, 0])
+@pytest.mark.parametrize("a,b", [("path", "n_kept"), ("n_kept", "next_ids"), ("next_ids", "path")])
+def test_verify_outputs_that_meet_one_another(launches, a, b, T):
+    args = verify_args(T)
+    na, nb = args[a].numel(), args[b].numel()
+    buf = i32(40)
+    for shift in range(-8, 9):
+        args[a], args[b] = buf[10:10 + na], buf[10 + shift:10 + shift + nb]
+        launches.clear()
+        if na and nb and shift < na and shift + nb > 0:
+            with pytest.raises(K.KernelError, match="memory of their own"):
+                K.verify_drafts(**args)
+            assert not launches
+        else:
+            K.verify_drafts(**args)
+            assert launches
+
+
+@pytest.mark.parametrize("name", ["target", "draft"])
+def test_verify_outputs_inside_a_row(launches, name):
+    """Rows of 40 in a matrix of 60 columns: the columns between the rows are nobody's."""
+    for at, meets in ((0, True), (34, True), (39, True), (40, False), (54, False), (55, True), (5 * 60 + 39, True), (5 * 60 + 40, False),
+                      (61, True), (104, False)):
+        args = verify_args()
+        buf = torch.zeros(6 * 60 + 60)
+        args[name] = buf[:360].view(6, 60)[:, :40]
+        args["path"] = buf.view(torch.int32)[at:at + 6]
+        launches.clear()
+        if meets:
+            with pytest.raises(K.KernelError, match="memory of their own"):
+                K.verify_drafts(**args)
+            assert not launches
+        else:
+            K.verify_drafts(**args)
+            assert launches
+
+
+def test_verify_takes_views_side_by_side(launches):
+    """One buffer cut into the three outputs, inputs that are one another's views, a row without a distance."""
+    args = verify_args()
+    out = i32(10)
+    args.update(path=out[:6], n_kept=out[6:8], next_ids=out[8:], parents=args["tokens"], draft=args["target"])
+    K.verify_drafts(**args)
+    one = verify_args(T=1, B=1)
+    one["target"] = torch.as_strided(torch.zeros(200), (1, 40), (3, 1))
+    K.verify_drafts(**one)
+    K.verify_drafts(**{**verify_args(), "draft": None})
+    assert len(launches) == 3
