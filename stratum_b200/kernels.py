@@ -1822,7 +1822,7 @@ def _rows_of(t: torch.Tensor, name: str, rows: Optional[int] = None):
 def token_probs(logits: torch.Tensor, temperature: torch.Tensor, out: torch.Tensor) -> None:
     """out[r] = softmax(logits[r] / temperature[r]); temperature <= 0 (or no number): one at the largest logit, the lowest
     index among equals.  logits and out float32 [rows, vocab] (rows contiguous; out may be logits itself), temperature
-    float32 [rows].  A logit that is no number counts as -inf, infinite ones share the row, a row of nothing but -inf
+    float32 [rows] (no part of out).  A logit that is no number counts as -inf, infinite ones share the row, a row of nothing but -inf
     gives zeros."""
     _one_device("token_probs", logits, temperature, out)
     R, V, ld = _rows_of(logits, "logits")
@@ -1837,6 +1837,8 @@ def token_probs(logits: torch.Tensor, temperature: torch.Tensor, out: torch.Tens
     at, to = logits.data_ptr(), out.data_ptr()
     if (at != to or ld != ldo) and _meet(at, 4 * ld, 4 * V, to, 4 * ldo, 4 * V, R):
         raise KernelError("token_probs: out is logits itself or memory of its own")
+    if _in_rows(temperature.data_ptr(), temperature.data_ptr() + 4 * R, to, 4 * ldo, 4 * V, R):
+        raise KernelError("token_probs: the temperatures are no part of out")
     f = _fn("draft_verify", "stratum_token_probs", [c_char_p, c_void_p])
     _check(f(_PROBS_CALL.pack(at, temperature.data_ptr(), to, status_word().data_ptr(), ld, ldo, R, V), _stream()), "token_probs")
 

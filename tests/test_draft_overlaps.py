@@ -92,3 +92,20 @@ def test_verify_takes_views_side_by_side(launches):
     K.verify_drafts(**one)
     K.verify_drafts(**{**verify_args(), "draft": None})
     assert len(launches) == 3
+
+
+@pytest.mark.parametrize("in_place", [False, True])
+def test_temperatures_inside_the_probabilities(launches, in_place):
+    """out: 3 rows of 40 in a matrix of 50 columns."""
+    for at, meets in ((0, True), (38, True), (40, False), (47, False), (48, True), (100, True), (138, True), (140, False)):
+        buf = torch.zeros(200)
+        out = buf[:150].view(3, 50)[:, :40]
+        args = (out if in_place else torch.zeros(3, 40), buf[at:at + 3], out)
+        launches.clear()
+        if meets:
+            with pytest.raises(K.KernelError, match="no part of out"):
+                K.token_probs(*args)
+            assert not launches
+        else:
+            K.token_probs(*args)
+            assert launches
