@@ -1742,7 +1742,7 @@ def attention_tree(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor
     window, those at positions above token_pos - window; token_pos is not below the position of the sequence's first
     drafted row, and the window does not touch what the mask says.  A token that sees nothing gets zeros; rows behind the
     last sequence are left as they were; a page number outside the pool holds keys that nobody sees.  q and out may be columns
-    of one matrix, but have no element in common.
+    of one matrix, but out has no element in common with q or anything else that is read.
     max_new: drafted tokens of the sequence that has most (how the work is cut, not what comes out).
 
     bfloat16 heads of 64 or 128 on tcgen05, with probabilities rounded to bfloat16 as the value product's operand has to
@@ -1780,6 +1780,13 @@ def attention_tree(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor
     size = q.element_size()
     if _meet(at_q, ldq * size, width * size, at_out, ldo * size, width * size, T):
         raise KernelError("attention_tree: out is memory of its own, not q's")
+    at_pos, at_mask, at_start, at_len, at_table = (token_pos.data_ptr(), tree_mask.data_ptr(), seq_start.data_ptr(), seq_len.data_ptr(),
+                                                   block_table.data_ptr())
+    end, cached = at_out + ((T - 1) * ldo + width) * size, cache_shape[0] * n_kv * page_tokens * head_dim * size
+    for a, n in ((at_k, cached), (at_v, cached), (at_pos, 4 * T), (at_mask, 8 * T * mask_shape[1]), (at_start, 4 * B + 4), (at_len, 4 * B),
+                 (at_table, 4 * B * table_shape[1])):
+        if a < end and at_out < a + n and _in_rows(a, a + n, at_out, ldo * size, width * size, T):
+            raise KernelError("attention_tree: out is memory of its own, not part of what is read")
     tensor = (code == DT_BF16 and head_dim in (64, 128) and group <= 128 and scale > 0 and ldq % 8 == 0 and ldo % 8 == 0
               and not (at_q | at_k | at_v | at_out) & 15)
     # more rows than a half of a CTA holds: both halves share every page (else they take pages in turn); on the CUDA cores:
@@ -1798,8 +1805,8 @@ def attention_tree(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor
     at = scratch.data_ptr()
     part_ml = at + 4 * slots * padded
     f = _fn("attention_tree", "stratum_attention_tree", [c_char_p, c_void_p])
-    _check(f(_TREE_CALL.pack(at_q, at_k, at_v, token_pos.data_ptr(), tree_mask.data_ptr(), seq_start.data_ptr(), seq_len.data_ptr(),
-                             block_table.data_ptr(), at_out, at, part_ml, part_ml + 8 * slots, status_word().data_ptr(),
+    _check(f(_TREE_CALL.pack(at_q, at_k, at_v, at_pos, at_mask, at_start, at_len, at_table, at_out, at, part_ml, part_ml + 8 * slots,
+                             status_word().data_ptr(),
                              cache_shape[0], code, ldq, ldo, mask_shape[1], table_shape[1], table_shape[1], T, B, n_q, n_kv,
                              head_dim, page_tokens, window, tensor, many, scale), _stream()), "attention_tree")
     count_launches(1)          # the merge kernel

@@ -13,6 +13,7 @@ def launches(monkeypatch):
     monkeypatch.setattr(K, "_one_device", lambda *a: None)
     monkeypatch.setattr(K, "_stream", lambda: 0)
     monkeypatch.setattr(K, "status_word", lambda: torch.zeros(1, dtype=torch.int32))
+    monkeypatch.setattr(K, "_tree_plans", {(False, False, 64): (148, 32)})
     monkeypatch.setattr(K, "_fn", lambda lib, name, types: lambda *a: seen.append(name) or 0)
     return seen
 
@@ -109,3 +110,33 @@ def test_temperatures_inside_the_probabilities(launches, in_place):
         else:
             K.token_probs(*args)
             assert launches
+
+
+@pytest.mark.parametrize("name,dtype", [("k_cache", torch.float32), ("v_cache", torch.float32), ("token_pos", torch.int32),
+                                        ("tree_mask", torch.int64), ("seq_start", torch.int32), ("seq_len", torch.int32),
+                                        ("block_table", torch.int32)])
+def test_attention_outputs_inside_what_is_read(launches, name, dtype):
+    """out: 3 rows of 128 in a matrix of 160 columns."""
+    shapes = dict(k_cache=(2, 2, 64, 64), v_cache=(2, 2, 64, 64), token_pos=(3,), tree_mask=(3, 1), seq_start=(3,), seq_len=(2,),
+                  block_table=(2, 2))
+    n = 1
+    for x in shapes[name]:
+        n *= x
+    words = n * (2 if dtype == torch.int64 else 1)         # of 32 bits
+    front = 2 * 16384
+    for at in (0, 60, 126, 128, 130, 158, 160, 320 + 126, 320 + 128, -words, -2):
+        meets = any(at < r * 160 + 128 and at + words > r * 160 for r in range(3))
+        buf = torch.zeros(front + 480 + 16384)
+        args = dict(q=torch.zeros(3, 128), out=buf[front:front + 480].view(3, 160)[:, :128], n_q=2, n_kv=2, head_dim=64, page_tokens=64,
+                    window=0, scale=0.125, max_new=2)
+        for other, shape in shapes.items():
+            args[other] = torch.zeros(shape, dtype={"tree_mask": torch.int64}.get(other, torch.float32 if "cache" in other else torch.int32))
+        args[name] = buf[front + at:front + at + words].view(dtype).view(shapes[name])
+        launches.clear()
+        if meets:
+            with pytest.raises(K.KernelError, match="memory of its own"):
+                K.attention_tree(**args)
+            assert not launches
+        else:
+            K.attention_tree(**args)
+            assert launches == ["stratum_attention_tree"]
