@@ -245,12 +245,17 @@ class SequenceCache:
             self._seq[s] = pages
             self._len[s] = self._len[slot]
         self.epoch += bool(new)
-        for g, pairs in zip(self.groups, copies):
-            src, dst = [a for a, _ in pairs], [b for _, b in pairs]
-            if pairs and g.k is not None:
-                K.copy_pages(g.k, g.v, src, dst)
-            elif pairs and g.state is not None:
-                K.copy_pages(g.state, None, src, dst)
+        try:
+            for g, pairs in zip(self.groups, copies):
+                src, dst = [a for a, _ in pairs], [b for _, b in pairs]
+                if pairs and g.k is not None:
+                    K.copy_pages(g.k, g.v, src, dst)
+                elif pairs and g.state is not None:
+                    K.copy_pages(g.state, None, src, dst)
+        except Exception:
+            for s in new:
+                self.release(s)
+            raise
         return new
 
     def keep_rows(self, group: int, block_table: torch.Tensor, seq_start: torch.Tensor, seq_len: torch.Tensor, path: torch.Tensor,
