@@ -166,7 +166,7 @@ class Stratum:
         softmax(logits / temperature), distributed as decode_step's are (top_k and top_p have to be off).  Every entry draws a
         number for each of its tokens from its stream.  draft (float32 [tokens of all entries, vocab] on the device): for
         every token the distribution its children were drawn from, each for itself; None: they were looked up or guessed.
-        On error no sequence is longer than before."""
+        On error no sequence is longer than before and no stream has moved: the same call again draws the same numbers."""
         entries = list(entries)
         if sampling.top_k > 0 or sampling.top_p < 1.0:
             raise ValueError("draft_step draws from all ids: top_k and top_p have to be off")
@@ -178,6 +178,7 @@ class Stratum:
         if draft is not None and tuple(draft.shape) != (T, self.model.vocab):
             raise ValueError(f"draft_step: draft must be [{T}, {self.model.vocab}]")
         slots = [e.slot for e in entries]
+        before = [] if sampling.greedy else [st.state for st in streams]
         try:
             logits, batch = eng.run_drafts(entries)
             numbers = np.zeros((2, T), dtype=np.float32)
@@ -193,6 +194,8 @@ class Stratum:
             host = out.tolist()
             eng.check_kernels()
         except Exception:
+            for st, state in zip(streams or (), before):
+                st.state = state
             eng.cache.trim([s for s in slots if eng.cache.slots.is_live(s)])
             raise
         n_kept, result, r = host[T:T + B], [], 0
