@@ -1342,26 +1342,14 @@ static int tree_map(CUtensorMap* map, const void* base, int rank, const cuuint64
   return r == CUDA_SUCCESS ? 0 : STRATUM_ERR_SHAPE;
 }
 
-// Whether this device's function attributes are set (they are a device's own).
-static bool first_on_device(unsigned long long* done) {
-  int dev = 0;
-  cudaGetDevice(&dev);
-  const unsigned long long bit = 1ull << (dev & 63);
-  const bool first = !(*done & bit);
-  *done |= bit;
-  return first;
-}
-
+// (The opt-in to more shared memory is the current device's, and a cheap call: it is made at every launch.)
 template <int HD, bool ROWS2>
 static int launch_tree_tc(const CUtensorMap& mq, const CUtensorMap& mk, const CUtensorMap& mv, const TreeParams& P, int G,
                           cudaStream_t stream) {
   const size_t smem = sizeof(TreeSmem<HD, ROWS2>);
   auto kern = attention_tree_tc_kernel<HD, ROWS2>;
-  static unsigned long long done = 0;
-  if (first_on_device(&done)) {
-    cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
-    if (e != cudaSuccess) { done = 0; return (int)e; }
-  }
+  const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+  if (e != cudaSuccess) return (int)e;
   return launch_pdl(kern, dim3(G), dim3(TR_THREADS), smem, stream, mq, mk, mv, P);
 }
 
@@ -1376,11 +1364,8 @@ template <typename T, int NC, int R>
 static int launch_tree_simple(const TreeParams& P, int G, cudaStream_t stream) {
   const size_t smem = simple_smem(P.head_dim, 16 * R, P.n_seqs);
   auto kern = attention_tree_simple_kernel<T, NC, R>;
-  static unsigned long long done = 0;
-  if (first_on_device(&done)) {
-    cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, 220 * 1024);
-    if (e != cudaSuccess) { done = 0; return (int)e; }
-  }
+  const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, 220 * 1024);
+  if (e != cudaSuccess) return (int)e;
   return launch_pdl(kern, dim3(G), dim3(TG_THREADS), smem, stream, P);
 }
 template <typename T>

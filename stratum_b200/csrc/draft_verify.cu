@@ -49,13 +49,9 @@ static int resident_clusters(const void* kernel, int C, int threads) {
 // rows clusters of `cluster` blocks each
 template <auto kernel, typename... Args>
 static int launch_clusters(unsigned rows, unsigned cluster, unsigned threads, cudaStream_t stream, Args... args) {
-  static unsigned long long done = 0;              // devices on which this kernel may have clusters of sixteen
-  int dev = 0;
-  cudaGetDevice(&dev);
-  if (cluster > 8 && !(done & (1ull << (dev & 63)))) {
-    cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+  if (cluster > 8) {                               // clusters of sixteen: the current device's opt-in
+    const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
     if (e != cudaSuccess) return (int)e;
-    done |= 1ull << (dev & 63);
   }
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(rows * cluster);
