@@ -1891,14 +1891,19 @@ def verify_drafts(target: torch.Tensor, draft: Optional[torch.Tensor], tokens: t
     read = (tokens.data_ptr(), parents.data_ptr(), seq_start.data_ptr(), uniform.data_ptr())
     written = (path.data_ptr(), n_kept.data_ptr(), next_ids.data_ptr())
     ends = (written[0] + 4 * T, written[1] + 4 * B, written[2] + 4 * B)
-    taken = [(read[0], read[0] + 4 * T), (read[1], read[1] + 4 * T), (read[2], read[2] + 4 * B + 4), (read[3], read[3] + 4 * T)]
-    for lo, hi in zip(written, ends):                        # (empty ones begin nowhere and meet nothing)
-        for a, b in taken:
-            if lo < b and a < hi and lo < hi and a < b:
+    (p0, k0, n0), (p1, k1, n1) = written, ends
+    taken = ((read[0], read[0] + 4 * T), (read[1], read[1] + 4 * T), (read[2], read[2] + 4 * B + 4), (read[3], read[3] + 4 * T))
+    rows = ((at_target, at_target + 4 * ((T - 1) * ldt + V)), (at_draft, at_draft + 4 * ((T - 1) * ldd + V)))
+    near = (p0 < k1 and k0 < p1) or (k0 < n1 and n0 < k1) or (n0 < p1 and p0 < n1)
+    for a, b in taken + rows:
+        if (p0 < b and a < p1) or (k0 < b and a < k1) or (n0 < b and a < n1):
+            near = True
+    if near:                                                 # (empty ones meet nothing, nor does what lies between two rows)
+        for lo, hi in zip(written, ends):
+            if (any(lo < b and a < hi and lo < hi and a < b for a, b in taken) or _in_rows(lo, hi, at_target, 4 * ldt, 4 * V, T)
+                    or (at_draft and _in_rows(lo, hi, at_draft, 4 * ldd, 4 * V, T))):
                 raise KernelError("verify_drafts: path, n_kept and next_ids are memory of their own")
-        if _in_rows(lo, hi, at_target, 4 * ldt, 4 * V, T) or (at_draft and _in_rows(lo, hi, at_draft, 4 * ldd, 4 * V, T)):
-            raise KernelError("verify_drafts: path, n_kept and next_ids are memory of their own")
-        taken.append((lo, hi))
+            taken += ((lo, hi),)
     f = _fn("draft_verify", "stratum_verify_drafts", [c_char_p, c_void_p])
     _check(f(_VERIFY_CALL.pack(at_target, at_draft, *read, *written, ldt, ldd, T, B, V, 0), _stream()), "verify_drafts")
 
