@@ -5,13 +5,11 @@
 // A page of a layer is one stretch of n_kv * 64 * head_dim elements, a token's row of a (page, head) one of head_dim.
 #include "common.cuh"
 
-static int sms() {
-  static int n = 0;
-  if (!n) {
-    int dev = 0;
-    cudaGetDevice(&dev);
-    cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev);
-    if (n <= 0) n = 148;
+static int sms() {                                  // of the current device
+  int n = 0, dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess || n <= 0) {
+    cudaGetLastError();
+    return 148;
   }
   return n;
 }

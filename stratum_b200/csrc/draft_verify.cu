@@ -25,6 +25,8 @@
 #include <cooperative_groups.h>
 #include <math.h>
 
+#include <atomic>
+
 #include "tc_common.cuh"
 
 namespace cg = cooperative_groups;
@@ -570,10 +572,18 @@ verify_drafts_kernel(const VerifyParams P) {
   if (lane == 0) P.picked[b] = pick >= 0 ? pick : positive;
 }
 
+// (a property of the device and the kernel, and dear to ask for: kept for each device; an answer of none is not)
 static int vd_resident(int C) {
-  static int known[17];                            // n + 1
-  if (!known[C]) known[C] = 1 + resident_clusters((const void*)verify_drafts_kernel<4>, C, VD_THREADS);
-  return known[C] - 1;
+  static std::atomic<int> known[64][5];            // clusters of 1, 2, 4, 8, 16
+  int dev = 0, at = 0;
+  while ((1 << at) < C) at++;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return resident_clusters((const void*)verify_drafts_kernel<4>, C, VD_THREADS);
+  int n = known[dev][at].load(std::memory_order_relaxed);
+  if (n == 0) {
+    n = resident_clusters((const void*)verify_drafts_kernel<4>, C, VD_THREADS);
+    known[dev][at].store(n, std::memory_order_relaxed);
+  }
+  return n;
 }
 
 // call: the parameters as the launcher packs them.

@@ -32,3 +32,12 @@ def test_opt_ins_are_made_at_every_launch(name, functions):
         for guard in re.findall(r"if \(([^{};]*?)\)\s*\{?[^{}]*?cudaFuncSetAttribute", body):
             assert re.match(r"(cluster|C) > 8\b", guard), (function, guard)      # (sizes of this launch alone)
     assert found == functions
+
+
+def test_what_is_kept_of_a_device_is_kept_for_that_device():
+    """Of the answers of one device (SMs, resident clusters) the next one has no use, and a failure is no answer."""
+    for name in ("draft_verify", "cache_move"):
+        with open(os.path.join(CSRC, name + ".cu")) as f:
+            source = re.sub(r"//[^\n]*", "", f.read())
+        for kept in re.findall(r"^[ \t]+static (?!constexpr|const\b)([^;]*);", source, re.M):
+            assert re.match(r"std::atomic<int> \w+\[64\]", kept), (name, kept)
