@@ -105,9 +105,11 @@ __device__ __forceinline__ void tell(const Part* place, const uint64_t* bar, int
       ::"r"(smem_u32(place)), "r"(smem_u32(bar)), "r"(rank), "r"(__float_as_uint(v)), "r"(__float_as_uint(sum)), "r"(i), "r"(0) : "memory");
 }
 
-// A weight against `m`, no less than v, in all cases: 1 at the maximum (infinite ones too), 0 at -inf.
+// A weight against `m`, no less than v and above -inf, in all cases: 1 at the maximum (infinite ones too), 0 at -inf and beside an
+// infinite one (there the product may be none: fmaxf drops it).  Halves, as the difference of two numbers may be none of its
+// own: with T that large as well the weight is not 0.
 __device__ __forceinline__ float any_weight(float v, float m, float to_log2) {
-  return v == m ? 1.f : v == -INFINITY ? 0.f : exp2f((v - m) * to_log2);
+  return v == m ? 1.f : exp2f(2.f * fmaxf((0.5f * v - 0.5f * m) * to_log2, -1000.f));
 }
 __device__ __forceinline__ float clean(float v) { return fmaxf(v, -INFINITY); }        // (fmaxf drops what is no number)
 
@@ -164,7 +166,8 @@ token_probs_kernel(const float* logits, long long ld, const float* temperature, 
   const float m = warp_max(warp_v[lane % (PR_THREADS / 32)]);                        // the block's largest value
   const bool greedy = !(t > 0.f);
   const float to_log2 = greedy ? 0.f : 1.4426950408889634f / t;
-  const bool ordinary = fabsf(m) < INFINITY && to_log2 > 0.f && to_log2 < INFINITY;
+  // (below 1e-30 a difference that has overflowed may still have a weight)
+  const bool ordinary = fabsf(m) < INFINITY && to_log2 > 1e-30f && to_log2 < INFINITY;
   float sum = 0.f;
   if (greedy) {
     if (HELD) {
