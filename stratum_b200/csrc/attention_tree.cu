@@ -380,6 +380,13 @@ __device__ __forceinline__ float tmem_ld1f(uint32_t taddr) {
   return __uint_as_float(r);
 }
 
+__device__ __forceinline__ void tr_store16(uint32_t taddr, const uint32_t (&r)[16]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};"
+      ::"r"(taddr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
+      "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]) : "memory");
+}
+
 // D += A B with A (128 rows x 16 bfloat16) in tensor memory: two values of k to a column
 __device__ __forceinline__ void umma_bf16_ts(uint32_t tmem_d, uint32_t tmem_a, uint64_t desc_b, uint32_t idesc, uint32_t accumulate) {
   asm volatile(
@@ -423,6 +430,37 @@ __device__ __noinline__ unsigned long long tree_look_through(uint4* v) {
   return bad;
 }
 
+// A weight is 2^(score to_log2 - m_ref) with one rounding.  m_ref is a rounded product itself, so that all weights of a row have a
+// factor in common, which their sum takes out again: 2^64 at most for references below TR_LARGE, without end above.  There the
+// score's product is rounded too, as m_ref was, and the largest weight is one.
+#define TR_LARGE 0x1p30f
+__device__ __forceinline__ float tree_weight(float score, float to_log2, float m_use) {
+  return tr_exp2(fabsf(m_use) >= TR_LARGE ? __fmul_rn(score, to_log2) - m_use : fmaf(score, to_log2, -m_use));
+}
+
+// P of a tile of a warp that has rows of such scores, over the scores (the first half's end where the second half's begin); the sum
+// of this thread's row.
+__device__ __noinline__ float tree_large_scores(unsigned long long vis, uint32_t s_addr, float to_log2, float m_use) {
+  float sum = 0.f;
+#pragma unroll 1
+  for (int c = 0; c < TR_KEYS; c += 32) {
+    uint32_t r[32], packed[16];
+    tmem_ld32(s_addr + c, r);
+    tmem_ld_wait();
+#pragma unroll
+    for (int e = 0; e < 32; e += 2) {
+      const float p0 = (vis >> (c + e)) & 1 ? tree_weight(__uint_as_float(r[e]), to_log2, m_use) : 0.f;
+      const float p1 = (vis >> (c + e + 1)) & 1 ? tree_weight(__uint_as_float(r[e + 1]), to_log2, m_use) : 0.f;
+      uint32_t u;
+      asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(u) : "f"(p1), "f"(p0));
+      sum += __uint_as_float(u << 16) + __uint_as_float(u & 0xffff0000u);
+      packed[e >> 1] = u;
+    }
+    tr_store16(s_addr + c / 2, packed);
+  }
+  return sum;
+}
+
 // Adds what the keys in `bad` give to this thread's row of the output in tensor memory (or to zeros where it holds nothing
 // yet).  v: the page's values in the cache.
 template <int HD>
@@ -438,7 +476,7 @@ __device__ __noinline__ void tree_add_bad(unsigned long long bad, unsigned long 
     }
     for (int k = 0; k < 64; k++) {
       if (!((bad >> k) & 1)) continue;
-      const float p = tr_exp2(fmaf(tmem_ld1f(s_addr + k), to_log2, -m_use));
+      const float p = tree_weight(tmem_ld1f(s_addr + k), to_log2, m_use);
       const bool sees = (vis >> k) & 1;
 #pragma unroll
       for (int e = 0; e < 32; e++)
@@ -704,6 +742,7 @@ attention_tree_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
       TR_WAIT(&S.run_seen[r % TR_RUNS], (r / TR_RUNS) & 1, 511)
       const uint32_t clean_from = it_first + run.clean0, clean_to = it_first + run.clean1;
       float m_ref = -INFINITY, l = 0.f;
+      bool any_large = false;                            // some row of the warp has a reference beyond TR_LARGE
       for (; it < it_end; it += STEP) {
         const int s = it % STAGES, b = i & 1;
         const bool needs_mask = it < clean_from || it >= clean_to, first = it == it_mine;
@@ -767,7 +806,7 @@ attention_tree_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
             sum2[(e >> 1) & 1] = tr_add2(sum2[(e >> 1) & 1], tr_pair(__uint_as_float(u << 16), __uint_as_float(u & 0xffff0000u)));
             packed[e >> 1] = u;
           }
-          float sum[4];
+          float sum[4], total;
           tr_split(sum2[0], sum[0], sum[1]); tr_split(sum2[1], sum[2], sum[3]);
           const bool move = __any_sync(0xffffffffu, grow);
           if (!first && (move || bad)) {                 // P V of this half's tile before is in O
@@ -786,7 +825,7 @@ attention_tree_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
               tmem_st32(o_addr + c, r);
             }
           }
-          l = fmaf(l, corr, (sum[0] + sum[1]) + (sum[2] + sum[3]));
+          total = (sum[0] + sum[1]) + (sum[2] + sum[3]);
           if (bad) {                                     // what values that are not finite give to the rows that see them
             tc_fence_after();
             tmem_st_wait();
@@ -794,8 +833,11 @@ attention_tree_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
                              reinterpret_cast<const bf16*>(P.v_cache) +
                                  ((size_t)((unsigned)__ldcg(bt + (int)it) < (unsigned)P.n_pages ? __ldcg(bt + (int)it) : 0) * P.n_kv + run.kvh) * TR_KEYS * HD, first);
           }
-          tmem_st32(lane_addr + b * TR_KEYS, packed);    // over the scores
+          if (move) any_large = __any_sync(0xffffffffu, fabsf(m_use) >= TR_LARGE);
+          if (any_large) total = tree_large_scores(needs_mask ? vis : ~0ull, lane_addr + b * TR_KEYS, to_log2, m_use);
+          else tmem_st32(lane_addr + b * TR_KEYS, packed);           // over the scores
           tmem_st_wait();
+          l = fmaf(l, corr, total);
         }
         if (first && quarter == 0 && lane == 0) S.o_ready[h] = bad != 0;   // (`bad` is the same in all of them)
         tc_fence_before();
