@@ -1943,6 +1943,12 @@ def keep_rows(k: torch.Tensor, v: Optional[torch.Tensor], block_table: torch.Ten
         raise KernelError("keep_rows: block_table is [sequences, pages]")
     if B == 0 or T == 0:
         return
+    for held in (k, v):
+        if held is not None:
+            lo, hi = held.data_ptr(), held.data_ptr() + held.nbytes
+            for t in (block_table, seq_start, seq_len, path, n_kept):
+                if t.data_ptr() < hi and lo < t.data_ptr() + t.nbytes:
+                    raise KernelError("keep_rows: tables, lengths and paths are no part of the cache")
     L, pages, heads, page_tokens, size = k.shape
     f = _fn("cache_move", "stratum_keep_rows", [c_char_p, c_void_p])
     _check(f(_KEEP_CALL.pack(k.data_ptr(), 0 if v is None else v.data_ptr(), block_table.data_ptr(), seq_start.data_ptr(),

@@ -140,3 +140,25 @@ def test_attention_outputs_inside_what_is_read(launches, name, dtype):
         else:
             K.attention_tree(**args)
             assert launches == ["stratum_attention_tree"]
+
+
+@pytest.mark.parametrize("name", ["block_table", "seq_start", "seq_len", "path", "n_kept"])
+@pytest.mark.parametrize("where", ["k", "v"])
+def test_kept_rows_described_inside_the_cache(launches, where, name):
+    shapes = dict(block_table=(2, 2), seq_start=(3,), seq_len=(2,), path=(6,), n_kept=(2,))
+    n = shapes[name][0] * (shapes[name][1] if len(shapes[name]) > 1 else 1)
+    size = 2 * 3 * 2 * 64 * 4                               # of keys and of values
+    for at, meets in ((0, True), (size - 1, True), (size, False), (-n, False), (-n + 1, True), (size // 2, True)):
+        buf = i32(size + 40)
+        args = {k: i32(s) for k, s in shapes.items()}
+        args[name] = buf[20 + at:20 + at + n].view(shapes[name])
+        for kv in "kv":
+            args[kv] = (buf[20:20 + size] if kv == where else i32(size)).view(2, 3, 2, 64, 4)
+        launches.clear()
+        if meets:
+            with pytest.raises(K.KernelError, match="no part of the cache"):
+                K.keep_rows(**args)
+            assert not launches
+        else:
+            K.keep_rows(**args)
+            assert launches == ["stratum_keep_rows"]
