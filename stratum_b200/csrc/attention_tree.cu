@@ -38,9 +38,10 @@
 // 1,270 (a product of 128 x 64 x 16 takes them 48 cycles with both halves at it, as the rows of Q are read from shared memory
 // each time, one of 128 x 128 x 16 takes 64) and the exponentials' units for 1,024; the rest is one waiting for the other
 // at the ends of tiles.  Around the tiles: 3 us to read the list, 3 more to the first scores, 3 at the end of a run (the last
-// product, the outputs), 6 to add pieces up.  Measured, 8 kv heads of 4 queries, head size 128: one sequence of 32,700 tokens and
-// 61 drafted ones 53 us (134 MB of keys and values, 2.5 TB/s, 615 TFLOP/s); 64 sequences of 4,000 and 33 to 64 drafted ones 256 us
-// (3.8 TB/s, 695 TFLOP/s), 302 where the card is held back by its power limit.
+// product, the outputs), 6 to add pieces up.  Measured, 8 kv heads of 4 queries, head size 128, calls one behind the other:
+// one sequence of 32,700 tokens and 61 drafted ones 58 us (134 MB of keys and values, 2.3 TB/s, 560 TFLOP/s; 54 in a replayed graph of
+// ten calls); 64 sequences of 4,000 and 33 to 64 drafted ones 315 (3.1 TB/s, 565 TFLOP/s: the card is at its power limit; 267 in
+// the graph, before it gets there).
 // Tried without a gain: more of the exponentials as polynomials, a lock that keeps the halves' products apart, halves that start
 // half a tile apart, one thread that issues for both, a guess at the maximum before the scores are there.
 #include <math.h>

@@ -83,7 +83,7 @@ STRATUM_EXPORT int stratum_copy_pages(void* a, void* b, long long pages, long lo
 // only and, taken in ascending stretches of which each is read before it is written, none is written that is still to be read.
 //
 // A warp owns a (sequence, layer, head, keys or values) and moves its rows CR_ROWS at a time; what it moves is its own, so
-// nothing waits for other warps.  Measured: 32 sequences that keep up to 30 of 31 drafted rows, 32 layers of 8 heads of 128 (77 MB)
+// nothing waits for other warps.  Measured: 32 sequences that keep up to 15 of 31 drafted rows, 32 layers of 8 heads of 128 (77 MB)
 // in 20 us, 3.8 TB/s: a warp's few rows are one chain (what the path says, where it lies, the rows), which 16,384 warps hide
 // only in part.
 #define CR_THREADS 256

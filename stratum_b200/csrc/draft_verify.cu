@@ -85,11 +85,11 @@ __device__ __forceinline__ void cluster_all_begun() { asm volatile("barrier.clus
 // or small that the product is none, are told apart once for a block: decided for every value they were fifty instructions
 // a value, and the time was theirs (287 us against 224 for 1,024 rows of 128,256, then).
 //
-// Measured: 1,024 rows of 128,256 in 200 us, 5.25 TB/s read and written, 0.80 of a plain copy; what is missing is a row's blocks
-// waiting for one another between reading and writing, while the other three or so on their SM read or write.  (With a
-// meeting of the cluster, whose fence waits for all that a block has under way: 225.  Blocks that stay and take row after row:
-// 316.  Three blocks to an SM, without spills: 226.  Blocks of 512 threads: 203.)  Nine rows: 5 us, launch and three trips to
-// memory.
+// Measured: 1,024 rows of 128,256 in 203 to 210 us from card to card, 5.0 to 5.2 TB/s read and written, 0.77 to 0.79 of a plain copy;
+// what is missing is a row's blocks waiting for one another between reading and writing, while the other three or so on their SM
+// read or write.  (Where this form took 200: with a meeting of the cluster, whose fence waits for all that a block has under way,
+// 225; blocks that stay and take row after row 316; three blocks to an SM, without spills, 226; blocks of 512 threads 203.)
+// Nine rows: 5 us, launch and three trips to memory.
 #define PR_HELD 32
 
 struct alignas(16) Part { float v, sum; int i, unused; };   // the largest value, the sum of weights against it, where it is first
@@ -308,8 +308,8 @@ struct VdSmem {
 
 // What a walk costs is passes over a row, one behind the other: every rejection of a drawn child sums the lowered row before the
 // next child can be tried, and the draw at the end sums it where that has not been done.  Measured: 64 trees of 9 to 16 nodes,
-// 128,256 ids, drawn: 36 us (one pass over the 64 first rows and the draft's would be 10); 37 looked-up trees of 32,000 ids and a
-// chain of six behind 128,256: 7.5 us, of which 3 are the dependent reads of the tree, its numbers and the row.
+// 128,256 ids, drawn: 34 to 39 us (one pass over the 64 first rows and the draft's would be 10); a chain of six behind 128,256, in a
+// replayed graph: 7.4 us, of which 3 are the dependent reads of the tree, its numbers and the row.
 //
 // W: ids of a load (4 where every row begins on 16 bytes); a warp has LINES loads of a row on their way together.
 template <int W>

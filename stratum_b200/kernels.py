@@ -1743,10 +1743,12 @@ def attention_tree(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor
     drafted row, and the window does not touch what the mask says.  A token that sees nothing gets zeros; rows behind the
     last sequence are left as they were; a page number outside the pool holds keys that nobody sees.  q and out may be columns
     of one matrix, but out has no element in common with q or anything else that is read.
-    max_new: drafted tokens of the sequence that has most (how the work is cut, not what comes out).
+    max_new: drafted tokens of the sequence that has most.  It decides how the work is cut: a wrong one costs time, and the
+    results' last bits.
 
     bfloat16 heads of 64 or 128 on tcgen05, with probabilities rounded to bfloat16 as the value product's operand has to
-    be; float32 and every other head size up to 256 on the CUDA cores in float32."""
+    be (2^-8 of each); where max_new * n_q / n_kv is over 128, a quarter of the exponentials are polynomials, off by 2^-13.7
+    before that.  float32 and every other head size up to 256 on the CUDA cores in float32."""
     dt = q.dtype
     code = dtype_code(dt)
     _one_device("attention_tree", q, k_cache, v_cache, token_pos, tree_mask, seq_start, seq_len, block_table, out)
@@ -1932,7 +1934,8 @@ def keep_rows(k: torch.Tensor, v: Optional[torch.Tensor], block_table: torch.Ten
     rows lie at positions seq_len[s] - rows ..., rows = seq_start[s + 1] - seq_start[s], and the row of node
     path[seq_start[s] + j], j = 1 .. n_kept[s], goes to place j of them (path and n_kept as verify_drafts writes them: a
     path that does not rise ends there).  k, v [layers, pages, heads, page_tokens, size] of any element type (v None: keys
-    alone), block_table int32 [seqs, pages]; a page number outside the pool is passed over."""
+    alone), block_table int32 [seqs, pages]; a page number outside the pool is passed over, and no page that rows move in
+    belongs to two of the sequences."""
     _one_device("keep_rows", k, v, block_table, seq_start, seq_len, path, n_kept)
     _storage(k, v, "keep_rows")
     B, T = n_kept.numel(), path.numel()

@@ -172,7 +172,7 @@ class Mixer(Part):
     # runs their products as one (and binds them with own_projection=False)
     splits_projection = False
     # forward also serves a step of drafted tokens (step.drafts): keys and values go to drafts.row of their sequence, a
-    # token sees what drafts.mask says beside the tokens in front of its tree
+    # token sees what drafts.masks[its window] says beside the tokens in front of its tree
     takes_drafts = False
 
     def cache_spec(self) -> Optional[CacheSpec]:
