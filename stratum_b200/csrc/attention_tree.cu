@@ -330,7 +330,7 @@ __device__ __forceinline__ float tr_exp2(float x) {
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
-// 2^a and 2^b with additions and products alone (no larger than 2^9): the whole part n goes into a float's exponent, 2^f of the
+// 2^a and 2^b with additions and products alone (a and b below 2^7): the whole part n goes into a float's exponent, 2^f of the
 // rest, |f| <= 1/2, is a cubic, fitted to the smallest largest relative error there, 7.5e-5 (2^-13.7: what is rounded to bfloat16 does
 // not notice).  0 below 2^-126; no number stays none.
 __device__ __forceinline__ void tr_exp2_pair(float& a, float& b) {
