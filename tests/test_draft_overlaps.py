@@ -147,13 +147,13 @@ def test_attention_outputs_inside_what_is_read(launches, name, dtype):
 def test_kept_rows_described_inside_the_cache(launches, where, name):
     shapes = dict(block_table=(2, 2), seq_start=(3,), seq_len=(2,), path=(6,), n_kept=(2,))
     n = shapes[name][0] * (shapes[name][1] if len(shapes[name]) > 1 else 1)
-    size = 2 * 3 * 2 * 64 * 4                               # of keys and of values
+    size = 2 * 3 * 2 * 64 * 5                               # of keys and of values
     for at, meets in ((0, True), (size - 1, True), (size, False), (-n, False), (-n + 1, True), (size // 2, True)):
         buf = i32(size + 40)
         args = {k: i32(s) for k, s in shapes.items()}
         args[name] = buf[20 + at:20 + at + n].view(shapes[name])
         for kv in "kv":
-            args[kv] = (buf[20:20 + size] if kv == where else i32(size)).view(2, 3, 2, 64, 4)
+            args[kv] = (buf[20:20 + size] if kv == where else i32(size)).view(2, 3, 2, 64, 5)
         launches.clear()
         if meets:
             with pytest.raises(K.KernelError, match="no part of the cache"):
